@@ -79,7 +79,7 @@ def draw(rng):
                     hk=hk, d=d, block=block, dtype=rng.choice(["bf16", "fp16", "fp32"]), seed=seed)
     if kind == "decode":
         rows = _log_int(rng, 1, 256)
-        high = _log_int(rng, 1, min(131072, (1 << 19) * 8 * 128 // (rows * hk * d)))
+        high = _log_int(rng, 1, min(131072, (1 << 18) * 12 * 128 // (rows * hk * d)))
         return dict(kind=kind, rows=rows, low=rng.choice([0, 1, high // 2, high]), high=high, h=hk * g, hk=hk, d=d, block=block,
                     dtype=rng.choice(["bf16", "fp16", "bf16", "fp32"]), seed=seed)
     rows = _log_int(rng, 1, 40)
