@@ -303,6 +303,68 @@ int nvfp4_window_attention(const void* q, int dtype, int64_t s_qz, int64_t s_qh,
                            nvfp4_stream_t stream);
 
 /*
+ * Paged 8-bit KV cache (no counterpart in the reference, whose cache is one dense batch).  Keys and values are e4m3 codes
+ * in blocks of block_size (16, 32, 64 or 128) tokens, [blocks, Hk, block_size, D] with dense heads (`*_block`: bytes
+ * from block to block), and one fp32 scale for each block and head, [blocks, Hk] (`*s_block`: floats from block to
+ * block): value = code * scale.  A request is a row of `table` [requests, width] (int32 block ids, `table_row` entries
+ * from row to row) and a length; token p of request r has slot table[r][p / block_size] * block_size + p % block_size.
+ * Free blocks are a stack: free_blocks[0 .. *free_count) with its top at the end.
+ *
+ * nvfp4_paged_reserve: new_lens[r] (< 0 counts as 0) more tokens for every request.  Pops the blocks that they need in
+ * request order, enters them in the table, adds to the lengths, and writes for token t of the call (request by request)
+ * slot_map[t] and positions[t], -1 and 0 behind the last one, for t < slots; cu_seqlens [requests + 1] are the
+ * prefix sums of the new lengths.  Where blocks, table columns or slots do not suffice nothing is reserved: *shortage is
+ * 1 (else 0), every slot -1, cu_seqlens 0 and the state unchanged.
+ * nvfp4_paged_trim: request r keeps its first keep_lens[r] tokens (all of them if it has no more, none for <= 0).  Blocks
+ * that hold none of them go back on the stack, their table entries become -1.  A trim to the lengths in front of a
+ * reservation restores the stack and the table.
+ * workspace: requests + 2 words.  Both change the state in place, on the device: calls on one state follow one another
+ * on one stream.
+ */
+int nvfp4_paged_reserve(const int32_t* new_lens, int32_t* lengths, int32_t* table,
+                        int64_t table_row, const int32_t* free_blocks, int32_t* free_count,
+                        int64_t requests, int64_t width, int64_t blocks, int block_size,
+                        int64_t slots, int64_t* slot_map, int32_t* positions, int32_t* cu_seqlens,
+                        int32_t* shortage, int32_t* workspace, nvfp4_stream_t stream);
+int nvfp4_paged_trim(const int32_t* keep_lens, int32_t* lengths, int32_t* table, int64_t table_row,
+                     int32_t* free_blocks, int32_t* free_count, int64_t requests, int64_t width,
+                     int64_t blocks, int block_size, int32_t* workspace, nvfp4_stream_t stream);
+
+/*
+ * Keys and values of new tokens into the cache.  key / value [tokens, hk, d] in `dtype` (element strides of token and
+ * head, unit stride along d, rows 16-byte aligned); token t goes to slot_map[t], tokens with a slot < 0 or behind the
+ * cache are skipped.  Per block and head e is the smallest integer with max|x| <= 448 * 2^e over the block's new values (at
+ * least -110; values that are not finite do not count), the scale 2^e and the codes e4m3 of x * 2^-e (round to nearest even;
+ * infinities saturate, NaN stays).  Where the call's first token of a block is not at its offset 0 the tokens in front of
+ * it stay: the scale becomes the larger of the old and the new one, and where that raised it, their codes are rounded
+ * again.  Tokens of one block stand next to each other in the call, their slots ascending by one, as
+ * nvfp4_paged_reserve gives them; of a block that a call names in two places the codes are unspecified.
+ */
+int nvfp4_kv8_write(const void* key, const void* value, int dtype, int64_t tokens, int64_t hk,
+                    int d, int64_t skt, int64_t skh, int64_t svt, int64_t svh,
+                    const int64_t* slot_map, uint8_t* k_cache, int64_t k_block, uint8_t* v_cache,
+                    int64_t v_block, float* k_scale, int64_t ks_block, float* v_scale,
+                    int64_t vs_block, int64_t blocks, int block_size, nvfp4_stream_t stream);
+
+/*
+ * Attention over that cache.  q [tokens, hk * g, d] in `q_dtype` (element strides of token and head, unit stride along d);
+ * request r owns query tokens cu_seqlens[r] .. cu_seqlens[r + 1] (cu_seqlens NULL: token r, tokens == requests), the last ones
+ * of its lengths[r] keys: token i of n sees keys 0 .. lengths[r] - n + i.  out [tokens, hk * g, d] in `q_dtype` and lse
+ * [tokens, hk * g] (natural log, or NULL) are contiguous; tokens that see no key, and tokens of no request, get zeros and
+ * -inf.  Table entries that are no block hide their keys; lengths are cut to width * block_size.
+ * workspace: nvfp4_kv8_attention_plan bytes, 16-byte aligned.
+ */
+int nvfp4_kv8_attention_plan(int d, int sm_count, size_t* workspace_bytes);
+int nvfp4_kv8_attention(const void* q, int q_dtype, int64_t s_qt, int64_t s_qh,
+                        const int32_t* cu_seqlens, int64_t tokens, const uint8_t* k_cache,
+                        int64_t k_block, const uint8_t* v_cache, int64_t v_block,
+                        const float* k_scale, int64_t ks_block, const float* v_scale,
+                        int64_t vs_block, int64_t blocks, int block_size, const int32_t* table,
+                        int64_t table_row, int64_t width, const int32_t* lengths, int64_t requests,
+                        int64_t hk, int g, int d, float scaling, void* out, float* lse,
+                        void* workspace, size_t workspace_bytes, nvfp4_stream_t stream);
+
+/*
  * Flash-attention forward over packed operands.  Replaces `_flash_fwd_kernel` and its host
  * drivers `_run_flash_packed` / `nvfp4_flash_attention_packed` (flash.py:739-933, 2560-2766).
  *   qnv/qsc  [Z*H,  s_q,  D/2 | D/16]  contiguous

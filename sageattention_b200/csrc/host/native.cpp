@@ -667,6 +667,168 @@ bool kv_prefill(const Tensor& key, const Tensor& value, const Tensor& knv, const
   return true;
 }
 
+// ---------------------------------------------------------------- paged 8-bit KV cache
+void require_words(const Call& c, const Tensor& t, int64_t n, at::ScalarType type, const char* msg) {
+  c.same(t);
+  if (t.scalar_type() != type) throw UnsupportedType(msg);
+  require(t.numel() == n && t.is_contiguous(), msg);
+}
+
+// A block table [requests, width]: rows may be views of a wider one, but not overlap.
+void require_table(const Call& c, const Tensor& table) {
+  c.same(table);
+  if (table.scalar_type() != at::kInt) throw UnsupportedType("block_table must be int32 [requests, width]");
+  require_dims(table, 2, "block_table must be [requests, width]");
+  require(table.size(0) >= 1 && table.size(1) >= 1, "block_table must have a row and a column");
+  require((table.stride(1) == 1 || table.size(1) == 1) && (table.size(0) == 1 || table.stride(0) >= table.size(1)),
+          "block_table rows must be contiguous and apart");
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> paged_reserve(const Tensor& new_lens, const Tensor& lengths, const Tensor& table,
+                                                         const Tensor& free_blocks, const Tensor& free_count, int64_t slots,
+                                                         int64_t block_size) {
+  require_cuda(lengths, "lengths");
+  Call c(lengths);
+  require_table(c, table);
+  const int64_t r = table.size(0), n = free_blocks.numel();
+  require_words(c, new_lens, r, at::kInt, "new_lens must be contiguous int32 [requests]");
+  require_words(c, lengths, r, at::kInt, "lengths must be contiguous int32 [requests]");
+  require_words(c, free_blocks, n, at::kInt, "free_blocks must be contiguous int32 [blocks]");
+  require_words(c, free_count, 1, at::kInt, "free_count must be one int32");
+  require(slots >= 0, "num_slots must not be negative");
+  Tensor slot_map = c.empty({slots}, at::kLong), positions = c.empty({slots}, at::kInt);
+  // cu_seqlens and shortage are results, the rest of the words is scratch: one allocation
+  Tensor words = c.empty({2 * r + 4}, at::kInt);
+  Tensor cu = words.narrow(0, 0, r + 1), shortage = words.narrow(0, r + 1, 1);
+  int32_t* w = words.data_ptr<int32_t>();
+  c.done(nvfp4_paged_reserve(new_lens.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), table.data_ptr<int32_t>(),
+                             table.stride(0), free_blocks.data_ptr<int32_t>(), free_count.data_ptr<int32_t>(), r, table.size(1),
+                             n, (int)block_size, slots, slot_map.data_ptr<int64_t>(), positions.data_ptr<int32_t>(), w, w + r + 1,
+                             w + r + 2, c.stream),
+         "nvfp4_paged_reserve");
+  return {slot_map, positions, cu, shortage};
+}
+
+void paged_trim(const Tensor& keep_lens, const Tensor& lengths, const Tensor& table, const Tensor& free_blocks,
+                const Tensor& free_count, int64_t block_size) {
+  require_cuda(lengths, "lengths");
+  Call c(lengths);
+  require_table(c, table);
+  const int64_t r = table.size(0), n = free_blocks.numel();
+  require_words(c, keep_lens, r, at::kInt, "keep_lens must be contiguous int32 [requests]");
+  require_words(c, lengths, r, at::kInt, "lengths must be contiguous int32 [requests]");
+  require_words(c, free_blocks, n, at::kInt, "free_blocks must be contiguous int32 [blocks]");
+  require_words(c, free_count, 1, at::kInt, "free_count must be one int32");
+  Tensor words = c.empty({r + 2}, at::kInt);
+  c.done(nvfp4_paged_trim(keep_lens.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), table.data_ptr<int32_t>(), table.stride(0),
+                          free_blocks.data_ptr<int32_t>(), free_count.data_ptr<int32_t>(), r, table.size(1), n, (int)block_size,
+                          words.data_ptr<int32_t>(), c.stream),
+         "nvfp4_paged_trim");
+}
+
+// Codes [blocks, Hk, block_size, D] and scales [blocks, Hk] of keys and values.
+struct PagedCache {
+  int64_t blocks, hk, bs, d;
+  uint8_t *k, *v;
+  float *ks, *vs;
+  int64_t k_block, v_block, ks_block, vs_block;
+};
+PagedCache paged_cache(const Call& c, const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs) {
+  require_dims(k, 4, "k_cache must be [blocks, Hk, block_size, D]");
+  const int64_t n = k.size(0), hk = k.size(1), bs = k.size(2), d = k.size(3);
+  require(d == 128 || d == 256, "D must be 128 or 256");
+  require(bs == 16 || bs == 32 || bs == 64 || bs == 128, "block_size must be 16, 32, 64 or 128");
+  for (const Tensor* t : {&k, &v}) {
+    c.same(*t);
+    if (t->scalar_type() != at::kFloat8_e4m3fn && t->scalar_type() != at::kByte)
+      throw UnsupportedType("k_cache and v_cache must be float8_e4m3fn (or its bytes as uint8)");
+    require(t->sizes() == k.sizes(), "k_cache and v_cache must have the same shape");
+    require(t->stride(3) == 1 && t->stride(2) == d && (hk == 1 || t->stride(1) == bs * d), "heads of a cache block must be dense");
+    require(n <= 1 || (t->stride(0) >= hk * bs * d && t->stride(0) % 16 == 0),
+            "cache blocks must not overlap, and start on 16 bytes");
+  }
+  for (const Tensor* t : {&ks, &vs}) {
+    c.same(*t);
+    if (t->scalar_type() != at::kFloat) throw UnsupportedType("k_scale and v_scale must be float32 [blocks, Hk]");
+    require(t->dim() == 2 && t->size(0) == n && t->size(1) == hk, "k_scale and v_scale must be [blocks, Hk]");
+    require((hk == 1 || t->stride(1) == 1) && (n <= 1 || t->stride(0) >= hk), "scales of a block must be contiguous");
+  }
+  return {n, hk, bs, d, u8(k), u8(v), ks.data_ptr<float>(), vs.data_ptr<float>(), k.stride(0), v.stride(0), ks.stride(0),
+          vs.stride(0)};
+}
+
+// [T, Hk, D], or one token a request as [Z, Hk, 1, D]: rows of unit stride on 16 bytes
+Tensor token_rows(const Tensor& t, const char* msg) {
+  Tensor x = t;
+  if (t.dim() == 4) {
+    require(t.size(2) == 1, msg);
+    x = t.select(2, 0);
+  }
+  require_dims(x, 3, msg);
+  const int64_t unit = 16 / t.element_size();
+  const bool aligned = x.stride(2) == 1 && x.stride(0) % unit == 0 && x.stride(1) % unit == 0 &&
+                       reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  return aligned ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+void kv8_write(const Tensor& key, const Tensor& value, const Tensor& slot_map, const Tensor& k_cache, const Tensor& v_cache,
+               const Tensor& k_scale, const Tensor& v_scale) {
+  require_cuda(key, "key");
+  Call c(key);
+  c.same(value);
+  const PagedCache p = paged_cache(c, k_cache, v_cache, k_scale, v_scale);
+  if (key.scalar_type() != value.scalar_type()) throw UnsupportedType("key and value must have the same dtype");
+  const int dt = dtype_code(key.scalar_type());
+  require(key.sizes() == value.sizes(), "key and value must have the same shape");
+  const Tensor k = token_rows(key, "key and value must be [T, Hk, D] or [Z, Hk, 1, D]");
+  const Tensor v = token_rows(value, "key and value must be [T, Hk, D] or [Z, Hk, 1, D]");
+  require(k.size(1) == p.hk && k.size(2) == p.d, "key and value must have the cache's heads and head dim");
+  require_words(c, slot_map, k.size(0), at::kLong, "slot_map must be contiguous int64 with one slot a token");
+  c.done(nvfp4_kv8_write(k.data_ptr(), v.data_ptr(), dt, k.size(0), p.hk, (int)p.d, k.stride(0), k.stride(1), v.stride(0),
+                         v.stride(1), slot_map.data_ptr<int64_t>(), p.k, p.k_block, p.v, p.v_block, p.ks, p.ks_block, p.vs,
+                         p.vs_block, p.blocks, (int)p.bs, c.stream),
+         "nvfp4_kv8_write");
+}
+
+// query [Z, H, 1, D] without cu_seqlens, [T, H, D] with
+std::tuple<Tensor, OptTensor> kv8_attention(const Tensor& query, const OptTensor& cu, const Tensor& k_cache,
+                                            const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale,
+                                            const Tensor& table, const Tensor& lengths, double scaling, int64_t g, bool want_lse) {
+  require_cuda(query, "query");
+  Call c(query);
+  const PagedCache p = paged_cache(c, k_cache, v_cache, k_scale, v_scale);
+  require_table(c, table);
+  const int64_t r = table.size(0);
+  require_words(c, lengths, r, at::kInt, "lengths must be contiguous int32 [requests]");
+  const int dt = dtype_code(query.scalar_type());
+  const bool one = !cu.has_value();
+  if (one) {
+    require_dims(query, 4, "query must be [Z, H, 1, D]");
+    require(query.size(2) == 1, "fp8_paged_decode is for seqlen_q == 1 (decode)");
+    require(query.size(0) == r, "query must have a row for every row of block_table");
+  } else {
+    require_dims(query, 3, "query must be [T, H, D]");
+    require_words(c, *cu, r + 1, at::kInt, "cu_seqlens must be contiguous int32 [requests + 1]");
+  }
+  const int64_t t = query.size(0), h = query.size(1), d = query.size(-1);
+  require(d == p.d, "query must have the cache's head dim");
+  require(g >= 1 && h == p.hk * g, "num_key_value_groups must equal H // Hk");
+  const Tensor q = query.stride(-1) == 1 ? query : query.contiguous();
+  Tensor out = c.empty(query.sizes(), query.scalar_type());
+  OptTensor lse;
+  if (want_lse) lse = c.empty({t, h}, at::kFloat);
+  size_t bytes = 0;
+  c.done(nvfp4_kv8_attention_plan((int)d, at::cuda::getDeviceProperties(c.dev.index())->multiProcessorCount, &bytes),
+         "nvfp4_kv8_attention_plan");
+  Tensor ws = c.empty({(int64_t)bytes}, at::kByte);
+  c.done(nvfp4_kv8_attention(q.data_ptr(), dt, q.stride(0), q.stride(1), opt_ptr<int32_t>(cu), t, p.k, p.k_block, p.v, p.v_block,
+                             p.ks, p.ks_block, p.vs, p.vs_block, p.blocks, (int)p.bs, table.data_ptr<int32_t>(), table.stride(0),
+                             table.size(1), lengths.data_ptr<int32_t>(), r, p.hk, (int)g, (int)d, (float)scaling, out.data_ptr(),
+                             opt_ptr<float>(lse), ws.data_ptr(), bytes, c.stream),
+         "nvfp4_kv8_attention");
+  return {out, lse};
+}
+
 // ---------------------------------------------------------------- backward
 struct Prep {
   OptTensor copy, delta, amax;
@@ -995,6 +1157,10 @@ PYBIND11_MODULE(_native, m) {
   m.def("packed_views", &packed_views, nogil());
   m.def("append_token", &append_token, nogil());
   m.def("kv_prefill", &kv_prefill, nogil());
+  m.def("paged_reserve", &paged_reserve, nogil());
+  m.def("paged_trim", &paged_trim, nogil());
+  m.def("kv8_write", &kv8_write, nogil());
+  m.def("kv8_attention", &kv8_attention, nogil());
   m.def("bwd_prep", &bwd_prep, nogil());
   m.def("bf16_rows", &bf16_rows, nogil());
   m.def("bwd_hp", &bwd_hp, nogil());

@@ -25,6 +25,15 @@ from .flash import (  # noqa: F401
     nvfp4_quant_kv_decode,
 )
 from .kv_cache import NVFP4KVCache  # noqa: F401
+from .paged_cache import (  # noqa: F401
+    FP8PagedKVCache,
+    PagedStep,
+    fp8_kv_write,
+    fp8_paged_attention,
+    fp8_paged_decode,
+    paged_kv_reserve,
+    paged_kv_trim,
+)
 
 __all__ = [
     "nvfp4_flash_attn_func",
@@ -35,4 +44,10 @@ __all__ = [
     "nvfp4_quant_kv_decode",
     "NVFP4KVCache",
     "convert_fp32_to_fp4_packed",
+    "FP8PagedKVCache",
+    "fp8_kv_write",
+    "fp8_paged_attention",
+    "fp8_paged_decode",
+    "paged_kv_reserve",
+    "paged_kv_trim",
 ]

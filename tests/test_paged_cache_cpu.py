@@ -1,0 +1,115 @@
+"""Paged 8-bit KV cache without a GPU: refusals of the C ABI and of the Python entries, and the rules the GPU tests compare
+with (scales, rounding, tables)."""
+
+import ctypes
+import math
+import os
+
+import pytest
+import torch
+
+from paged_reference import nearest_e4m3, reserve, scale_of, trim, write
+
+
+def _lib():
+    from sageattention_b200 import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    return _lib.lib()
+
+
+def test_rounding_of_the_reference_is_that_of_the_type():
+    every = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
+    every = every[torch.isfinite(every)].double()
+    assert torch.equal(nearest_e4m3(every), every)
+    x = torch.cat([every, (every[1:] + every[:-1]) / 2, torch.randn(4096, dtype=torch.float64) * 2.0 ** torch.randint(-9, 8, (4096,))])
+    x = x.float().clamp(-448, 448)
+    assert torch.equal(nearest_e4m3(x.double()).float(), x.to(torch.float8_e4m3fn).float())
+
+
+def test_scales_are_the_smallest_powers_of_two():
+    for amax in (1.0, 448.0, 448.5, 1.75, 1.7500001, 3e38, 1e-20, 0.0, 7.0 * 2.0 ** -30):
+        s = scale_of(torch.tensor([amax], dtype=torch.float64))[0].item()
+        assert math.frexp(s)[0] == 0.5 and (448 * s >= amax)
+        assert s == 2.0 ** -110 or 448 * s / 2 < amax
+
+
+def test_a_trim_undoes_a_reservation():
+    g = torch.Generator().manual_seed(0)
+    for _ in range(50):
+        rows, block = int(torch.randint(1, 9, (1,), generator=g)), 16
+        held = torch.randint(0, 80, (rows,), generator=g)
+        new = torch.randint(0, 50, (rows,), generator=g)
+        state = dict(lengths=held.clone(), table=torch.full((rows, 10), -1), free=torch.randperm(90, generator=g), count=90)
+        empty = dict(state, lengths=torch.zeros_like(held))
+        reserve(held, empty, 10 ** 6, block)
+        before = {k: (v.clone() if torch.is_tensor(v) else v) for k, v in empty.items()}
+        _, _, _, short = reserve(new, empty, 10 ** 6, block)
+        assert short == 0
+        trim(held, empty, block)
+        assert all(torch.equal(before[k], empty[k]) if torch.is_tensor(before[k]) else before[k] == empty[k] for k in before)
+
+
+def test_blocks_written_token_by_token_stay_near_the_one_shot_block():
+    """A code that is rounded again when the scale grows is off by half a step of each rounding; only codes below
+    2^-6 of the scale move at all."""
+    x = torch.randn(16, 2, 128, generator=torch.Generator().manual_seed(3)).double()
+    x *= torch.exp2(torch.arange(16).double() - 8)[:, None, None]
+    one, one_s = torch.zeros(1, 2, 16, 128).double(), torch.zeros(1, 2).double()
+    write(x, torch.arange(16), one, one_s, 16)
+    many, many_s = torch.zeros(1, 2, 16, 128).double(), torch.zeros(1, 2).double()
+    for t in range(16):
+        write(x[t:t + 1], torch.tensor([t]), many, many_s, 16)
+    assert torch.equal(one_s, many_s)
+    diff = (one - many).abs()
+    assert diff.max() <= 2.0 ** -9              # one step of the codes that move
+    assert torch.equal(one[one.abs() >= 2.0 ** -5], many[one.abs() >= 2.0 ** -5])
+
+
+def test_c_entries_refuse_bad_sizes():
+    L = _lib()
+    n = None
+    assert L.nvfp4_paged_reserve(n, n, n, 1, n, n, 1, 1, 1, 24, 1, n, n, n, n, n, n) < 0 and b"block_size" in L.nvfp4_last_error()
+    assert L.nvfp4_paged_reserve(n, n, n, 1, n, n, 0, 1, 1, 16, 1, n, n, n, n, n, n) < 0 and b"sizes" in L.nvfp4_last_error()
+    assert L.nvfp4_paged_reserve(n, n, n, 1, n, n, 1, 1, 1, 16, -1, n, n, n, n, n, n) < 0 and b"slot" in L.nvfp4_last_error()
+    assert L.nvfp4_paged_trim(n, n, n, 1, n, n, 1, 1, 1, 8, n, n) < 0 and b"block_size" in L.nvfp4_last_error()
+    assert L.nvfp4_paged_trim(n, n, n, 1, n, n, 1 << 20, 1 << 20, 1, 16, n, n) < 0 and b"entries" in L.nvfp4_last_error()
+    w = lambda **k: L.nvfp4_kv8_write(k.get("key", 0), 0, k.get("dt", 0), k.get("t", 1), 1, k.get("d", 128), k.get("st", 128), 128, 128,
+                                      128, n, 0, 2048, 0, 2048, n, 1, n, 1, 1, k.get("bs", 16), n)
+    for bad, text in ((dict(bs=17), b"block_size"), (dict(d=64), b"D must"), (dict(st=129), b"aligned"), (dict(key=2), b"aligned"),
+                      (dict(t=-1), b"sizes"), (dict(dt=7), b"dtype")):
+        assert w(**bad) < 0 and text in L.nvfp4_last_error(), bad
+    assert w(t=0) == 0
+    size = ctypes.c_size_t()
+    assert L.nvfp4_kv8_attention_plan(96, 148, ctypes.byref(size)) < 0
+    assert L.nvfp4_kv8_attention_plan(128, 148, ctypes.byref(size)) == 0 and size.value == 2 * 148 * (2 * 16 * 130 * 4 + 16)
+    a = lambda **k: L.nvfp4_kv8_attention(0, 0, 128, 128, k.get("cu", n), k.get("t", 1), k.get("kc", 0), 2048, 0, 2048, n, 1, n, 1, 1,
+                                          k.get("bs", 16), n, 1, k.get("w", 1), n, 1, 1, k.get("g", 1), k.get("d", 128), 1.0, 0, n, 0,
+                                          k.get("ws", 0), n)
+    for bad, text in ((dict(bs=48), b"block_size"), (dict(d=80), b"D must"), (dict(t=2), b"cu_seqlens"), (dict(kc=8), b"aligned"),
+                      (dict(g=0), b"sizes"), (dict(w=1 << 28), b"sizes"), (dict(t=-1, cu=16), b"sizes")):
+        assert a(**bad) < 0 and text in L.nvfp4_last_error(), bad
+    assert a(t=0, cu=16) == 0
+
+
+def test_python_entries_refuse_cpu_tensors():
+    import sageattention_b200.nvfp4 as nv
+    _lib()
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        nv.paged_kv_reserve(i(1), i(1), i(1, 1), i(1), i(1), 1, 16)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        nv.paged_kv_trim(i(1), i(1), i(1, 1), i(1), i(1), 16)
+    x = torch.zeros(1, 1, 128)
+    c, s = torch.zeros(1, 1, 16, 128, dtype=torch.float8_e4m3fn), torch.zeros(1, 1)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        nv.fp8_kv_write(x, x, torch.zeros(1, dtype=torch.int64), c, c, s, s)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        nv.fp8_paged_decode(x[:, :, None], c, c, s, s, i(1, 1), i(1), 1.0)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        nv.fp8_paged_attention(x, None, c, c, s, s, i(1, 1), i(1), 1.0)
+    with pytest.raises(AssertionError, match="block_size"):
+        nv.FP8PagedKVCache(1, 4, 1, 128, 1, 64, "cpu", block_size=24)
+    cache = nv.FP8PagedKVCache(2, 5, 3, 128, 2, 65, "cpu", block_size=32)
+    assert cache.block_table.shape == (2, 3) and int(cache.free_count) == 5 and cache.free_blocks.tolist() == [4, 3, 2, 1, 0]
+    assert cache.cache_bytes() == sum(t.numel() * t.element_size() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale))
