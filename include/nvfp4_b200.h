@@ -352,9 +352,11 @@ int nvfp4_kv8_write(const void* key, const void* value, int dtype, int64_t token
  * of its lengths[r] keys: token i of n sees keys 0 .. lengths[r] - n + i.  out [tokens, hk * g, d] in `q_dtype` and lse
  * [tokens, hk * g] (natural log, or NULL) are contiguous; tokens that see no key, and tokens of no request, get zeros and
  * -inf.  Table entries that are no block hide their keys; lengths are cut to width * block_size.
- * workspace: nvfp4_kv8_attention_plan bytes, 16-byte aligned.
+ * workspace: nvfp4_kv8_attention_plan bytes for the same call, 16-byte aligned.  status: device int, written non-zero if a
+ * bounded wait expired; may be NULL.
  */
-int nvfp4_kv8_attention_plan(int d, int sm_count, size_t* workspace_bytes);
+int nvfp4_kv8_attention_plan(int q_dtype, int64_t tokens, int64_t requests, int g, int d,
+                             int sm_count, size_t* workspace_bytes);
 int nvfp4_kv8_attention(const void* q, int q_dtype, int64_t s_qt, int64_t s_qh,
                         const int32_t* cu_seqlens, int64_t tokens, const uint8_t* k_cache,
                         int64_t k_block, const uint8_t* v_cache, int64_t v_block,
@@ -362,7 +364,8 @@ int nvfp4_kv8_attention(const void* q, int q_dtype, int64_t s_qt, int64_t s_qh,
                         int64_t vs_block, int64_t blocks, int block_size, const int32_t* table,
                         int64_t table_row, int64_t width, const int32_t* lengths, int64_t requests,
                         int64_t hk, int g, int d, float scaling, void* out, float* lse,
-                        void* workspace, size_t workspace_bytes, nvfp4_stream_t stream);
+                        void* workspace, size_t workspace_bytes, int* status,
+                        nvfp4_stream_t stream);
 
 /*
  * Flash-attention forward over packed operands.  Replaces `_flash_fwd_kernel` and its host

@@ -75,10 +75,10 @@ SIGNATURES = {
     "nvfp4_kv8_write": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p,
                                 c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int,
                                 c_void_p]),
-    "nvfp4_kv8_attention_plan": (c_int, [c_int, c_int, POINTER(c_size_t)]),
+    "nvfp4_kv8_attention_plan": (c_int, [c_int, c_int64, c_int64, c_int, c_int, c_int, POINTER(c_size_t)]),
     "nvfp4_kv8_attention": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                     c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p,
-                                    c_int64, c_int64, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+                                    c_int64, c_int64, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "nvfp4_rope_pack": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p,
                                 c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                 c_void_p]),

@@ -818,13 +818,13 @@ std::tuple<Tensor, OptTensor> kv8_attention(const Tensor& query, const OptTensor
   OptTensor lse;
   if (want_lse) lse = c.empty({t, h}, at::kFloat);
   size_t bytes = 0;
-  c.done(nvfp4_kv8_attention_plan((int)d, at::cuda::getDeviceProperties(c.dev.index())->multiProcessorCount, &bytes),
+  c.done(nvfp4_kv8_attention_plan(dt, t, r, (int)g, (int)d, at::cuda::getDeviceProperties(c.dev.index())->multiProcessorCount, &bytes),
          "nvfp4_kv8_attention_plan");
   Tensor ws = c.empty({(int64_t)bytes}, at::kByte);
   c.done(nvfp4_kv8_attention(q.data_ptr(), dt, q.stride(0), q.stride(1), opt_ptr<int32_t>(cu), t, p.k, p.k_block, p.v, p.v_block,
                              p.ks, p.ks_block, p.vs, p.vs_block, p.blocks, (int)p.bs, table.data_ptr<int32_t>(), table.stride(0),
                              table.size(1), lengths.data_ptr<int32_t>(), r, p.hk, (int)g, (int)d, (float)scaling, out.data_ptr(),
-                             opt_ptr<float>(lse), ws.data_ptr(), bytes, c.stream),
+                             opt_ptr<float>(lse), ws.data_ptr(), bytes, c.status, c.stream),
          "nvfp4_kv8_attention");
   return {out, lse};
 }

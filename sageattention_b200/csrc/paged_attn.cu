@@ -18,6 +18,7 @@
 #include "common/fp4.cuh"
 #include "common/kv8.cuh"
 #include "common/launch.cuh"
+#include "common/paged.cuh"
 #include "common/sm100.cuh"
 
 namespace nvfp4 {
@@ -26,84 +27,12 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 3;
 constexpr int kRowTile = 16;
 constexpr int kStageBytes = 8192;             // K and V of a warp's keys of a tile
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int D>
 struct Cfg {
   static constexpr int kSub = kStageBytes / (2 * D);       // keys of a warp in a tile: 32, or 16 at D = 256
   static constexpr int kTile = kSub * kWarps;
 };
-
-struct AttnParams {
-  const void* q;
-  int64_t sqt, sqh;                           // element strides of token and head
-  const int32_t* cu;                          // [requests + 1] first query token, or null: one token a request
-  int64_t tokens;
-  const uint8_t *k, *v;
-  int64_t k_block, v_block;                   // bytes from block to block
-  const float *ks, *vs;
-  int64_t ks_block, vs_block;
-  const int32_t* table;
-  int64_t table_row;
-  const int32_t* lengths;
-  int requests, width, blocks, log_block, hk, g;
-  float scale_log2;                           // scaling * log2(e)
-  void* out;                                  // [tokens, H, D]
-  float* lse;                                 // [tokens, H] or null
-  int4* cut;                                  // [grid] the unit that a CTA began and did not finish: first token row, head, rows, pieces
-  float *ws_m, *ws_l, *ws_acc;                // [2 * grid] partial results
-};
-
-// What a request asks for: its query tokens [t0, t0 + n), keys, and its units and key tiles.
-struct Request {
-  int t0, n, len, row_tiles, key_tiles;
-};
-template <int D>
-__device__ __forceinline__ Request request_of(const AttnParams& p, int r) {
-  Request q;
-  if (p.cu == nullptr) {
-    q.t0 = r;
-    q.n = 1;
-  } else {
-    const int64_t a = min(max((int64_t)p.cu[r], (int64_t)0), p.tokens), b = min((int64_t)p.cu[r + 1], p.tokens);
-    q.t0 = (int)a;
-    q.n = (int)max(b - a, (int64_t)0);
-  }
-  q.len = (int)min((int64_t)max(p.lengths[r], 0), (int64_t)p.width << p.log_block);
-  q.row_tiles = (int)(((int64_t)q.n * p.g + kRowTile - 1) / kRowTile);
-  q.key_tiles = (q.len + Cfg<D>::kTile - 1) / Cfg<D>::kTile;
-  return q;
-}
-__device__ __forceinline__ int64_t tiles_of(const AttnParams& p, const Request& q) {
-  return (int64_t)p.hk * q.row_tiles * q.key_tiles;
-}
-
-// A place in the list of all tiles.
-struct Cursor {
-  Request q;
-  int r, head, row_tile, tile;
-};
-template <int D>
-__device__ __forceinline__ void next_request(const AttnParams& p, Cursor& c) {
-  do {
-    if (++c.r >= p.requests) return;
-    c.q = request_of<D>(p, c.r);
-  } while (c.q.row_tiles == 0 || c.q.key_tiles == 0);
-}
-template <int D>
-__device__ __forceinline__ void next_unit(const AttnParams& p, Cursor& c) {
-  c.tile = 0;
-  if (++c.row_tile < c.q.row_tiles) return;
-  c.row_tile = 0;
-  if (++c.head < p.hk) return;
-  c.head = 0;
-  next_request<D>(p, c);
-}
-// keys that the last row of the unit sees; row i of the request's n * g sees len - n + 1 + i / g
-__device__ __forceinline__ int unit_limit(const AttnParams& p, const Cursor& c) {
-  const int rows = min(c.q.n * p.g, (c.row_tile + 1) * kRowTile);
-  return min(c.q.len, c.q.len - c.q.n + 1 + (rows - 1) / p.g);
-}
 
 __device__ __forceinline__ void cp_async_16(uint32_t saddr, const void* gptr, uint32_t src_bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(saddr), "l"(gptr), "r"(src_bytes) : "memory");
@@ -124,11 +53,7 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint4& a, uint32_
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+__device__ __forceinline__ float ex2(float x) { return ex2_approx(x); }
 // Key of column i of a product of eight: 0 4 1 5 2 6 3 7.  The rows that one phase of a 16-byte load touches then differ in
 // bit 2, and with the swizzle (chunk ^ row) in their banks.
 __device__ __forceinline__ int key_of_column(int i) { return (i >> 1) | ((i & 1) << 2); }
@@ -136,15 +61,6 @@ __device__ __forceinline__ int key_of_column(int i) { return (i >> 1) | ((i & 1)
 // Exponent of a scale, as log2 of what weights are kept relative to.
 __device__ __forceinline__ float scale_exponent(float s) {
   return fmaxf((float)((int)(__float_as_uint(s) >> 23 & 0xFF) - 127), -112.0f);
-}
-
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-  } else {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_16x2<T>(x[0], x[1]), pack_16x2<T>(x[2], x[3]));
-  }
 }
 
 template <typename T, int D>
@@ -157,92 +73,31 @@ struct Smem {
   static constexpr int kBytes = kRing + kShared;
 };
 
-// Rows of no key at all, and rows of no request, get zeros and -inf.
 template <typename T, int D>
-__device__ __forceinline__ void clear_rows(const AttnParams& p, int64_t t0, int64_t t1) {
-  const int h = p.hk * p.g;
-  T* out = static_cast<T*>(p.out);
-  for (int64_t i = t0 * h * D + threadIdx.x * 4; i < t1 * h * D; i += kThreads * 4) {
-    const float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    store4<T>(out + i, z);
-  }
-  if (p.lse != nullptr)
-    for (int64_t i = t0 * h + threadIdx.x; i < t1 * h; i += kThreads) p.lse[i] = -INFINITY;
-}
-
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(AttnParams p) {
+__global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(PagedParams p) {
   using S = Smem<T, D>;
   constexpr int kSub = Cfg<D>::kSub, kTile = Cfg<D>::kTile;
   constexpr int kNt = kSub / 8, kHalves = kSub / 16;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t list_s[kWarps + 2];
-  __shared__ int found_s;
   __shared__ float q_inv[kRowTile];                        // undoes the power of two that a query row was scaled by
   __shared__ float m_s[kWarps][kRowTile], l_s[kWarps][kRowTile];
   __shared__ float scale_s[kWarps][kStages][4];            // K and V scales of the stage's two halves
   __shared__ int keys_s[kWarps][kStages][2];               // keys of each half that are there
   const int tid = threadIdx.x, lane = tid & 31, warp = warp_index();
-  const int grid = gridDim.x, cta = blockIdx.x;
+  const int cta = blockIdx.x;
   griddep_wait();
   griddep_launch();
 
-  // ---- the share of this CTA: tiles [begin, end) of the list, and the request that `begin` lies in
-  auto block_sum = [&](int64_t x, int64_t& before) -> int64_t {
-    int64_t inc = x;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += y;
-    }
-    if (lane == 31) list_s[warp] = inc;
-    __syncthreads();
-    int64_t base = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) base += list_s[w];
-      all += list_s[w];
-    }
-    __syncthreads();
-    before = base + inc - x;
-    return all;
-  };
-  int64_t mine = 0, unused;
-  for (int r = tid; r < p.requests; r += kThreads) mine += tiles_of(p, request_of<D>(p, r));
-  const int64_t total = block_sum(mine, unused);
-  const int64_t share = (total + grid - 1) / grid;
-  const int64_t begin = (int64_t)cta * share, end = min(total, begin + share);
+  using Place = Cursor<kRowTile, kTile>;
+  Place use;
+  const auto [begin, end, share] = deal_tiles<kThreads>(p, list_s, use);
   if (tid == 0) p.cut[cta] = make_int4(0, 0, 0, 0);
   if (begin < end) {
-    int64_t base = 0, before;
-    if (tid == 0) found_s = -1;
-    for (int r0 = 0;; r0 += kThreads) {
-      const int r = r0 + tid;
-      const int64_t w = r < p.requests ? tiles_of(p, request_of<D>(p, r)) : 0;
-      const int64_t all = block_sum(w, before);
-      if (begin >= base + before && begin < base + before + w) {
-        found_s = r;
-        list_s[kWarps] = begin - base - before;
-      }
-      __syncthreads();
-      if (found_s >= 0) break;
-      base += all;
-    }
-    Cursor use;
-    use.r = found_s;
-    use.q = request_of<D>(p, use.r);
-    {
-      const int64_t in = list_s[kWarps];
-      const int64_t unit = in / use.q.key_tiles;
-      use.tile = (int)(in % use.q.key_tiles);
-      use.head = (int)(unit / use.q.row_tiles);
-      use.row_tile = (int)(unit % use.q.row_tiles);
-    }
-
     // ---- the ring of this warp: copies of tile `ahead` go into stage `fill`
     const uint32_t ring = smem_u32(smem) + warp * kStages * kStageBytes;
     const uint32_t shared = smem_u32(smem) + S::kRing;
-    Cursor ahead = use;
+    Place ahead = use;
     int64_t left = end - begin;                            // tiles still to be asked for
     int id[kHalves];
     auto look_up = [&]() {                                 // blocks of the keys of `ahead`, a tile before they are needed
@@ -255,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(AttnParams p) {
     };
     auto ask = [&](int stage) {
       if (left > 0) {
-        const int key = ahead.tile * kTile + warp * kSub, limit = unit_limit(p, ahead);
+        const int key = ahead.tile * kTile + warp * kSub, limit = ahead.q.limit(p, ahead.row_tile);
         const uint32_t base_s = ring + stage * kStageBytes;
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
@@ -281,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(AttnParams p) {
           }
           if (lane == 0) keys_s[warp][stage][h] = keys;
         }
-        if (--left > 0 && ++ahead.tile == ahead.q.key_tiles) next_unit<D>(p, ahead);
+        if (--left > 0 && ++ahead.tile == ahead.tiles) ahead.next_unit(p);
         look_up();
       }
       cp_async_commit();
@@ -296,9 +151,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(AttnParams p) {
     int64_t at = begin;
     bool first = true;
     while (at < end) {
-      const int rows = min(use.q.n * p.g - use.row_tile * kRowTile, kRowTile);
-      const int tiles = (int)min((int64_t)(use.q.key_tiles - use.tile), end - at);
-      const bool whole = use.tile == 0 && tiles == use.q.key_tiles;
+      const int rows = use.q.rows(p, use.row_tile);
+      const int tiles = (int)min((int64_t)(use.tiles - use.tile), end - at);
+      const bool whole = use.tile == 0 && tiles == use.tiles;
 
       // query rows as fragments of the products: row tid / 8, elements 16 e .. 16 e + 15 for e = tid % 8 (+ 8)
       {
@@ -348,10 +203,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(AttnParams p) {
       const float inv0 = q_inv[g8] * p.scale_log2, inv1 = q_inv[g8 + 8] * p.scale_log2;
       // keys that this thread's two rows see; rows of no query see all (they are not stored)
       auto limit_of = [&](int row) {
-        return row < rows ? use.q.len - use.q.n + 1 + (use.row_tile * kRowTile + row) / p.g : INT_MAX;
+        return row < rows ? use.q.seen(p, use.row_tile * kRowTile + row) : INT_MAX;
       };
       const int lim0 = limit_of(g8), lim1 = limit_of(g8 + 8);
-      const int lim_first = use.q.len - use.q.n + 1 + use.row_tile * kRowTile / p.g;    // the smallest of all rows
+      const int lim_first = use.q.seen(p, use.row_tile * kRowTile);    // the smallest of all rows
 
       float o[D / 16][2][4];
 #pragma unroll
@@ -577,13 +432,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(AttnParams p) {
               }
               if (whole) {
                 const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
-                const int i = use.row_tile * kRowTile + row;
-                const int64_t out_row = (int64_t)(use.q.t0 + i / p.g) * (p.hk * p.g) + use.head * p.g + i % p.g;
+                const int64_t to = out_row(p, (int64_t)use.q.t0 * p.g + use.row_tile * kRowTile + row, use.head);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) sum[k] *= inv;
-                store4<T>(static_cast<T*>(p.out) + out_row * D + cols * 128 + lane * 4, sum);
+                store4<T>(static_cast<T*>(p.out) + to * D + cols * 128 + lane * 4, sum);
                 if (cols == 0 && lane == 0 && p.lse != nullptr)
-                  p.lse[out_row] = total_l == 0.0f ? -INFINITY : (top + log2f(total_l)) * kLn2;
+                  p.lse[to] = lse_of(top, total_l);
               } else {
                 store4<float>(p.ws_acc + ((int64_t)slot * kRowTile + row) * D + cols * 128 + lane * 4, sum);
                 if (cols == 0 && lane == 0) {
@@ -598,93 +452,43 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(AttnParams p) {
       }
       if (!whole && use.tile == 0 && tid == 0) {
         // begun here, finished by the CTAs behind this one
-        const int64_t rest = use.q.key_tiles - tiles;
-        p.cut[cta] = make_int4(use.q.t0 * p.g + use.row_tile * kRowTile, use.head, rows,
-                               1 + (int)((rest + share - 1) / share) + (first ? 1 << 30 : 0));
+        p.cut[cta] = cut_unit(p, use, tiles, share, first);
       }
       at += tiles;
       first = false;
-      if (at < end) next_unit<D>(p, use);
+      if (at < end) use.next_unit(p);
     }
   }
-  // ---- what no tile belongs to
-  for (int r = cta; r < p.requests; r += grid) {
-    const Request q = request_of<D>(p, r);
-    if (q.key_tiles == 0) clear_rows<T, D>(p, q.t0, q.t0 + q.n);
-  }
-  if (p.cu != nullptr && cta == grid - 1) {
-    auto inside = [&](int t) { return min(max((int64_t)t, (int64_t)0), p.tokens); };
-    clear_rows<T, D>(p, 0, inside(p.cu[0]));
-    clear_rows<T, D>(p, inside(p.cu[p.requests]), p.tokens);
-  }
-}
-
-// Exact merge of the pieces of a cut unit, one warp a row, in the order of the keys.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_combine_kernel(AttnParams p) {
-  griddep_wait();
-  griddep_launch();
-  const int lane = threadIdx.x & 31, row = blockIdx.y * 4 + (threadIdx.x >> 5);
-  const int4 u = p.cut[blockIdx.x];
-  if (row >= u.z) return;
-  const int pieces = u.w & ((1 << 30) - 1), first = 2 * (int)blockIdx.x + (u.w >> 30 ? 0 : 1);
-  auto slot_of = [&](int i) { return i == 0 ? first : 2 * ((int)blockIdx.x + i); };
-  float top = -INFINITY;
-  for (int i = lane; i < pieces; i += 32) top = fmaxf(top, p.ws_m[slot_of(i) * kRowTile + row]);
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float sum[D / 128][4], total = 0.0f;
-#pragma unroll
-  for (int c = 0; c < D / 128; ++c)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) sum[c][k] = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < pieces; ++i) {
-    const int slot = slot_of(i);
-    const float f = top == -INFINITY ? 1.0f : ex2(p.ws_m[slot * kRowTile + row] - top);   // no key: zeros, or NaN
-    total += f * p.ws_l[slot * kRowTile + row];
-#pragma unroll
-    for (int c = 0; c < D / 128; ++c) {
-      const float4 v = *reinterpret_cast<const float4*>(p.ws_acc + ((int64_t)slot * kRowTile + row) * D + c * 128 + lane * 4);
-      sum[c][0] += f * v.x;
-      sum[c][1] += f * v.y;
-      sum[c][2] += f * v.z;
-      sum[c][3] += f * v.w;
-    }
-  }
-  const int i = u.x + row;                     // token * g + head of the group
-  const int64_t out_row = (int64_t)(i / p.g) * (p.hk * p.g) + u.y * p.g + i % p.g;
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-  for (int c = 0; c < D / 128; ++c) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) sum[c][k] *= inv;
-    store4<T>(static_cast<T*>(p.out) + out_row * D + c * 128 + lane * 4, sum[c]);
-  }
-  if (lane == 0 && p.lse != nullptr) p.lse[out_row] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
+  clear_untouched<T, D, kRowTile, kTile>(p);
 }
 
 template <typename T, int D>
-int run_attention(const AttnParams& p, int grid, cudaStream_t st) {
+int run_attention(const PagedParams& p, int grid, cudaStream_t st) {
   using S = Smem<T, D>;
   if (int rc = allow_smem("nvfp4_kv8_attention", reinterpret_cast<const void*>(paged_attn_kernel<T, D>), S::kBytes)) return rc;
   if (int rc = launch("nvfp4_kv8_attention", paged_attn_kernel<T, D>, dim3(grid), kThreads, S::kBytes, st, p)) return rc;
-  const int64_t rows = p.cu == nullptr ? p.g : p.tokens * p.g;
-  return launch("nvfp4_kv8_attention combine", paged_combine_kernel<T, D>, dim3(grid, (unsigned)((rows < 16 ? rows : 16) + 3) / 4),
-                128, 0, st, p);
+  return launch_combine<T, D, kRowTile>(p, grid, st);
 }
 
-constexpr int64_t cta_bytes(int d) { return 2 * kRowTile * ((int64_t)d + 2) * 4 + 16; }
+// Which kernel: tensor-memory products take 128 or 256 rows at a time and are worth it from kChunkRows query rows a request
+// on, on average (the lengths themselves are on the device); fp32 queries, whose products need two halves, stay here.
+constexpr int kChunkRows = 32;
+bool takes_chunk_kernel(int q_dtype, int64_t tokens, int64_t requests, int64_t g) {
+  return q_dtype != NVFP4_DT_FP32 && tokens * g > kChunkRows * requests;
+}
 
 }  // namespace
 }  // namespace nvfp4
 
 using namespace nvfp4;
 
-extern "C" int nvfp4_kv8_attention_plan(int d, int sm_count, size_t* workspace_bytes) {
+extern "C" int nvfp4_kv8_attention_plan(int q_dtype, int64_t tokens, int64_t requests, int g, int d, int sm_count,
+                                        size_t* workspace_bytes) {
   NVFP4_REQUIRE(d == 128 || d == 256, "nvfp4_kv8_attention_plan: D must be 128 or 256");
-  NVFP4_REQUIRE(sm_count >= 1 && workspace_bytes != nullptr, "nvfp4_kv8_attention_plan: bad argument");
-  *workspace_bytes = (size_t)(2 * sm_count * cta_bytes(d));
+  NVFP4_REQUIRE(tokens >= 0 && requests >= 1 && g >= 1 && sm_count >= 1 && workspace_bytes != nullptr,
+                "nvfp4_kv8_attention_plan: bad argument");
+  *workspace_bytes = (size_t)(takes_chunk_kernel(q_dtype, tokens, requests, g) ? sm_count * paged_slot_bytes(paged_chunk_rows(d), d)
+                                                                               : 2 * sm_count * paged_slot_bytes(kRowTile, d));
   return 0;
 }
 
@@ -694,7 +498,7 @@ extern "C" int nvfp4_kv8_attention(const void* q, int q_dtype, int64_t s_qt, int
                                    int64_t vs_block, int64_t blocks, int block_size, const int32_t* table, int64_t table_row,
                                    int64_t width, const int32_t* lengths, int64_t requests, int64_t hk, int g, int d,
                                    float scaling, void* out, float* lse, void* workspace, size_t workspace_bytes,
-                                   nvfp4_stream_t stream) {
+                                   int* status, nvfp4_stream_t stream) {
   NVFP4_REQUIRE(d == 128 || d == 256, "nvfp4_kv8_attention: D must be 128 or 256");
   int lb = 4;
   while (lb < 7 && (1 << lb) != block_size) ++lb;
@@ -709,20 +513,23 @@ extern "C" int nvfp4_kv8_attention(const void* q, int q_dtype, int64_t s_qt, int
   if (tokens == 0) return 0;
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int grid = 2 * sms;
-  NVFP4_REQUIRE(workspace_bytes >= (size_t)(grid * cta_bytes(d)), "nvfp4_kv8_attention: workspace too small");
-  AttnParams p{q, s_qt, s_qh, cu_seqlens, tokens, k_cache, v_cache, k_block, v_block, k_scale, v_scale, ks_block, vs_block, table,
-               table_row, lengths, (int)requests, (int)width, (int)blocks, lb, (int)hk, g, scaling * kLog2e, out, lse,
-               nullptr, nullptr, nullptr, nullptr};
+  const bool chunk = takes_chunk_kernel(q_dtype, tokens, requests, g);
+  const int grid = chunk ? sms : 2 * sms;
+  const int64_t rows = chunk ? paged_chunk_rows(d) : kRowTile;
+  NVFP4_REQUIRE(workspace_bytes >= (size_t)(grid * paged_slot_bytes(rows, d)), "nvfp4_kv8_attention: workspace too small");
+  NVFP4_REQUIRE(q_dtype >= NVFP4_DT_BF16 && q_dtype <= NVFP4_DT_FP32, "nvfp4_kv8_attention: unknown dtype %d", q_dtype);
+  PagedParams p{q, s_qt, s_qh, cu_seqlens, tokens, k_cache, v_cache, k_block, v_block, k_scale, v_scale, ks_block, vs_block, table,
+                table_row, lengths, (int)requests, (int)width, (int)blocks, lb, (int)hk, g, scaling * kLog2e, out, lse,
+                nullptr, nullptr, nullptr, nullptr, status};
   p.ws_acc = static_cast<float*>(workspace);
-  p.cut = reinterpret_cast<int4*>(p.ws_acc + (int64_t)2 * grid * kRowTile * d);
+  p.cut = reinterpret_cast<int4*>(p.ws_acc + 2 * grid * rows * d);
   p.ws_m = reinterpret_cast<float*>(p.cut + grid);
-  p.ws_l = p.ws_m + 2 * grid * kRowTile;
+  p.ws_l = p.ws_m + 2 * grid * rows;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (chunk) return launch_paged_chunk(p, q_dtype, d, grid, st);
   switch (q_dtype) {
     case NVFP4_DT_BF16: return d == 128 ? run_attention<__nv_bfloat16, 128>(p, grid, st) : run_attention<__nv_bfloat16, 256>(p, grid, st);
     case NVFP4_DT_FP16: return d == 128 ? run_attention<__half, 128>(p, grid, st) : run_attention<__half, 256>(p, grid, st);
-    case NVFP4_DT_FP32: return d == 128 ? run_attention<float, 128>(p, grid, st) : run_attention<float, 256>(p, grid, st);
+    default: return d == 128 ? run_attention<float, 128>(p, grid, st) : run_attention<float, 256>(p, grid, st);
   }
-  return fail(-1, "nvfp4_kv8_attention: unknown dtype %d", q_dtype);
 }

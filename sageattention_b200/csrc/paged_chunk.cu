@@ -1,0 +1,637 @@
+// Attention over the paged 8-bit KV cache for many query rows a request: chunks of prompts, drafts to verify.
+//
+// The mathematics of paged_attn.cu on the tensor cores of sm_100: S = Q K^T and O += P V as tcgen05.mma kind::f16 of halves, 128
+// rows an instruction, accumulators in tensor memory.  Codes become halves on their way into shared memory (exact; blocks of
+// a tile with smaller scales by a factor of at most 1), q enters as halves scaled by a power of two per row.
+//
+// Warps: two softmax groups (a thread a row; at D = 256 one group), four converting warps, one that issues the products.
+// Work goes through "jobs": one 128-row product pair with one key tile of 128 keys.
+//   rows > 128 (D = 128): job 2 t + g = rows of group g, key tile t; both groups use the converted tile
+//   rows <= 128 (D = 128): job t = key tile t, of group t & 1; the groups keep results of their own, merged at the end
+//   D = 256: job t = key tile t, one group; S alternates between two places
+// Job j has S in place j & 1, P overlays the S it came from, and the order of issue -- S(j + 2) behind P V (j) -- is what keeps
+// one place's products and its softmax apart: a completed S(j + 2) tells that P V (j) is complete as well.
+//
+// What bounds it (D = 128): a key tile of 256 rows is 2080 clocks of products and 2048 of ex2 on an SM; a place's own cycle is
+// product, softmax, product one after the other, with the other place's products in between.
+#include <cuda_fp16.h>
+#include "common/abi.cuh"
+#include "common/bwd_util.cuh"
+#include "common/kv8.cuh"
+#include "common/launch.cuh"
+#include "common/paged.cuh"
+#include "common/sm100.cuh"
+
+namespace nvfp4 {
+namespace {
+
+constexpr int kTile = 128;                    // keys of a tile
+constexpr int kSub = 128 * 128;               // bytes of a 128-row sub-tile of 64 halves
+constexpr int kInfo = 8;                      // tiles whose scales are kept: more than can be under way
+// P is held times 2^kLift relative to a reference that may lag behind the running maximum by 2^kLag
+constexpr float kLift = 8.0f, kLag = 7.0f;
+
+template <int D>
+struct Cfg {
+  static constexpr int kGroups = D == 128 ? 2 : 1;
+  static constexpr int kRows = 128 * kGroups;
+  static constexpr int kStages = D == 128 ? 2 : 1;
+  static constexpr int kSoft = 4 * kGroups;                // softmax warps
+  static constexpr int kThreads = 32 * (kSoft + 8);         // whole warpgroups: registers move between them
+  static constexpr int kRegsSoft = D == 128 ? 144 : 168, kRegsConvert = D == 128 ? 144 : 248, kRegsIssue = 80;
+  static constexpr int kOperand = D / 64 * kSub;           // 128 rows of q, or a tile of keys or values
+  static constexpr int kQ = 0, kK = kGroups * kOperand, kV = kK + kStages * kOperand, kOut = kV + kStages * kOperand;
+  static constexpr int kBytes = kOut + kSoft * 2048 + 1024;
+  static constexpr int kO = 256;                           // tensor memory: S at 0 and 128, O behind
+};
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Registers of a warpgroup.  The shares add up to what the launch has (512 threads of 128, or 384 of 168).
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// 16 bytes, or zeros without a load: predicated, so that the loads of a thread stay together
+__device__ __forceinline__ uint4 load_or_zero(const uint8_t* src, bool there) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}\n"
+      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+      : "l"(src), "r"((int)there)
+      : "memory");
+  return v;
+}
+
+// What a tile's softmax has to know: factor of its scores, log2 of what its values were divided by, which 16-key groups are there.
+struct TileInfo {
+  float k_factor, v_log2;
+  uint32_t there;
+};
+
+// exponent (floor of log2) of a scale
+__device__ __forceinline__ int scale_exp(float s) { return min(max((int)(__float_as_uint(s) >> 23 & 0xFF) - 127, -112), 126); }
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedParams p) {
+  using C = Cfg<D>;
+  using Place = Cursor<C::kRows, kTile>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], o_full[2], o_free[2], q_full, pv_done;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int expired;                                  // a wait ran out: site, else 0
+  __shared__ int64_t list_s[C::kThreads / 32 + 2];
+  __shared__ Place place_s;
+  __shared__ Share share_s;
+  __shared__ TileInfo info_s[kInfo];
+  __shared__ float m_s[2][128], l_s[128], c_s[128];
+  const int tid = threadIdx.x, lane = tid & 31, warp = warp_index();
+  volatile int* err = &expired;
+
+  if (tid == 0) {
+    expired = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 4);
+      mbar_init(&k_free[i], 1);
+      mbar_init(&v_full[i], 4);
+      mbar_init(&v_free[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_free[i], 4);
+    }
+    mbar_init(&q_full, C::kSoft);
+    mbar_init(&pv_done, 1);
+    mbar_fence_init();
+  }
+  if (warp == C::kSoft + 4) tmem_alloc(&tmem_base_s, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  griddep_launch();
+  griddep_wait();
+  const uint32_t tmem = tmem_base_s;
+  {
+    Place from;
+    const Share mine = deal_tiles<C::kThreads>(p, list_s, from);
+    if (tid == 0) {
+      place_s = from;
+      share_s = mine;
+      p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
+  }
+  __syncthreads();                                         // every role has its own copy from here on
+
+  if (warp >= C::kSoft && warp < C::kSoft + 4) {
+    more_registers<C::kRegsConvert>();
+    Place ahead = place_s;
+    int64_t left = share_s.end - share_s.begin;            // tiles to be asked for, and to be converted
+    int64_t rest = left;
+    // ------------------------------------------------------------------ codes to halves
+    const int w = warp - C::kSoft, t = w * 32 + lane;
+    // 16-byte pieces of a tile: eight lanes take 64 bytes of two neighbouring keys, whose halves then lie in different banks
+    constexpr int kPieces = D / 16;                        // per thread and operand
+    const int in_key = (lane >> 2) & 1, in_chunk = lane & 3, pair = w * 4 + (lane >> 3);
+    auto key_of = [&](int i) { return (i / (D / 64)) * 32 + pair * 2 + in_key; };
+    auto chunk_of = [&](int i) { return (i % (D / 64)) * 4 + in_chunk; };
+    int id = -1;                                           // block of keys 16 lane .. of the tile to come (lanes 0 to 7)
+    float ksc = 0.0f, vsc = 0.0f;
+    uint4 kr[kPieces], vr[kPieces];
+    // `ahead`: the tile whose blocks are looked up, one behind the tile (key0, limit, head) whose codes are asked for
+    int key0 = 0, limit = 0, head = 0, id_ahead = -1;
+    bool starts = true, starts_ahead = true;               // the tile is the first one of its unit, as far as this CTA sees
+    auto look_up = [&]() {
+      id_ahead = -1;
+      const int key = ahead.tile * kTile + lane * 16;
+      if (left > 0 && lane < 8 && key < ahead.q.limit(p, ahead.row_tile))
+        id_ahead = p.table[ahead.r * p.table_row + (key >> p.log_block)];
+    };
+    auto next = [&]() {
+      id = (unsigned)id_ahead < (unsigned)p.blocks ? id_ahead : -1;
+      key0 = ahead.tile * kTile;
+      limit = left > 0 ? ahead.q.limit(p, ahead.row_tile) : 0;
+      head = ahead.head;
+      starts = starts_ahead;
+      starts_ahead = false;
+      if (--left > 0 && ++ahead.tile == ahead.tiles) {
+        ahead.next_unit(p);
+        starts_ahead = true;
+      }
+      look_up();
+      ksc = id >= 0 ? p.ks[id * p.ks_block + head] : 0.0f;
+      vsc = id >= 0 ? p.vs[id * p.vs_block + head] : 0.0f;
+    };
+    auto ask = [&](const uint8_t* base, int64_t block, uint4 (&r)[kPieces]) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int key = key_of(i), b = __shfl_sync(0xffffffffu, id, key >> 4);
+        const int at_key = (key0 + key) & ((1 << p.log_block) - 1);
+        r[i] = load_or_zero(base + b * block + (((int64_t)head << p.log_block) + at_key) * D + chunk_of(i) * 16,
+                            b >= 0 && key0 + key < limit);
+      }
+    };
+    // pieces to halves times `scale` (of the key's block) * down, into a tile in shared memory
+    auto convert = [&](const uint4 (&r)[kPieces], float scale, float down, uint32_t dst) {
+      const float mine_f = scale * down;
+      const bool plain = __all_sync(0xffffffffu, lane >= 8 || id < 0 || mine_f == 1.0f);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int key = key_of(i), chunk = chunk_of(i);
+        const uint32_t words[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+        uint32_t h[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) half4_of_e4m3x4(words[k], h[2 * k], h[2 * k + 1]);
+        if (!plain) {
+          const float f = __shfl_sync(0xffffffffu, mine_f, key >> 4);
+          const __half2 f2 = __float2half2_rn(f);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h[k]), f2);
+            h[k] = *reinterpret_cast<const uint32_t*>(&v);
+          }
+        }
+        const uint32_t row = dst + (chunk >> 2) * kSub + key * 128;
+        const int c = (chunk & 3) * 2;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((c ^ (key & 7)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]),
+                     "r"(h[3])
+                     : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (((c + 1) ^ (key & 7)) << 4)), "r"(h[4]), "r"(h[5]),
+                     "r"(h[6]), "r"(h[7])
+                     : "memory");
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    if (left > 0) {
+      look_up();
+      next();
+      ask(p.k, p.k_block, kr);
+      ask(p.v, p.v_block, vr);
+    }
+    int v_run = -200;                                      // largest exponent of the unit's value scales so far
+    uint32_t n = 0;
+    for (; rest > 0; --rest, ++n) {
+      // scales of the tile, and its factors
+      const int st = n % C::kStages;
+      const uint32_t ph = (n / C::kStages) & 1;
+      if (starts) v_run = -200;
+      int ke = id >= 0 ? scale_exp(ksc) : -112, ve = id >= 0 ? scale_exp(vsc) : -112;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        ke = max(ke, __shfl_xor_sync(0xffffffffu, ke, o));
+        ve = max(ve, __shfl_xor_sync(0xffffffffu, ve, o));
+      }
+      ke = __shfl_sync(0xffffffffu, ke, 0);
+      ve = __shfl_sync(0xffffffffu, ve, 0);
+      v_run = max(v_run, ve);
+      ve = max(ve, v_run - 60);                            // smaller ones do not count beside what the unit has seen
+      const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
+      const uint32_t kdst = smem_u32(smem + C::kK + st * C::kOperand), vdst = smem_u32(smem + C::kV + st * C::kOperand);
+      const int id_now = id;
+      const float vsc_now = vsc;
+      // K of this tile; then the next tile's ids, scales and K codes are asked for
+      mbar_wait_warp(&k_free[st], ph ^ 1, err, 60);
+      if (t == 0) info_s[n % kInfo] = {exp2_int(ke), (float)ve, there};
+      convert(kr, ksc, exp2_int(-ke), kdst);
+      if (lane == 0) mbar_arrive(&k_full[st]);
+      next();
+      ask(p.k, p.k_block, kr);
+      // V of this tile: its own ids and scales
+      const int id_next = id;
+      id = id_now;
+      mbar_wait_warp(&v_free[st], ph ^ 1, err, 61);
+      convert(vr, vsc_now, exp2_int(-ve), vdst);
+      if (lane == 0) mbar_arrive(&v_full[st]);
+      id = id_next;
+      ask(p.v, p.v_block, vr);
+    }
+  } else if (warp >= C::kSoft + 4) {
+    fewer_registers<C::kRegsIssue>();
+    if (warp == C::kSoft + 4) {
+    // ------------------------------------------------------------------ issue of the products
+    Place at = place_s;
+    int64_t rest = share_s.end - share_s.begin;
+    const bool leader = elect_one();
+    const uint32_t id_s = make_idesc_bf16(128, 128, false, true), id_o = make_idesc_bf16(128, 128, true, true);
+    const uint64_t b_q = desc_sw128(smem + C::kQ, 0), b_k = desc_sw128(smem + C::kK, 0);
+    const uint64_t b_v = desc_sw128_mn(smem + C::kV, 0, kSub);
+    uint32_t n = 0, seg = 0;                               // tiles and segments so far
+    uint32_t jobs_of[2] = {0, 0};                          // jobs of each place so far
+    uint32_t results[2] = {0, 0};                          // results of each O so far
+    while (rest > 0) {
+      const int tiles = (int)min((int64_t)(at.tiles - at.tile), rest);
+      const bool both = C::kGroups == 2 && at.q.rows(p, at.row_tile) > 128;
+      const int jobs = both ? 2 * tiles : tiles;
+      mbar_wait_warp(&q_full, seg & 1, err, 62);
+      auto issue_s = [&](int j) {
+        const int tile = both ? j >> 1 : j, g = j & 1;
+        const int st = (n + tile) % C::kStages;
+        if (!both || g == 0) mbar_wait(&k_full[st], ((n + tile) / C::kStages) & 1, err, 63);
+        __syncwarp();
+        tc_fence_after();
+        if (leader) {
+          const uint64_t x_q = b_q + (both && g ? C::kOperand >> 4 : 0), x_k = b_k + (uint64_t)(st * (C::kOperand >> 4));
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16(tmem + g * 128, x_q + (k >> 2) * (kSub >> 4) + (k & 3) * 2, x_k + (k >> 2) * (kSub >> 4) + (k & 3) * 2, id_s,
+                      k > 0);
+          umma_commit(&s_full[g]);
+          if (!both || g == 1) umma_commit(&k_free[st]);
+        }
+        __syncwarp();
+      };
+      issue_s(0);
+      if (jobs > 1) issue_s(1);
+#pragma unroll 1
+      for (int j = 0; j < jobs; ++j) {
+        const int tile = both ? j >> 1 : j, g = j & 1, o = C::kGroups == 2 ? g : 0;
+        const int st = (n + tile) % C::kStages;
+        const bool first = C::kGroups == 2 ? j < 2 : j == 0;
+        if (first && results[o] > 0) mbar_wait(&o_free[o], (results[o] - 1) & 1, err, 64);
+        if (!both || g == 0) mbar_wait(&v_full[st], ((n + tile) / C::kStages) & 1, err, 65);
+        mbar_wait_warp(&p_full[g], jobs_of[g] & 1, err, 66);
+        ++jobs_of[g];
+        tc_fence_after();
+        if (leader) {
+          const uint64_t x_v = b_v + (uint64_t)(st * (C::kOperand >> 4));
+#pragma unroll
+          for (int c = 0; c < D / 128; ++c)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              umma_bf16_ta(tmem + C::kO + o * 128 + c * 128, tmem + g * 128 + k * 8, x_v + c * (2 * kSub >> 4) + k * 128, id_o,
+                           (k > 0 || !first) ? 1u : 0u);
+          if (!both || g == 1) umma_commit(&v_free[st]);
+          if (C::kGroups == 1) umma_commit(&pv_done);
+          if (j + C::kGroups >= jobs) umma_commit(&o_full[o]);
+        }
+        __syncwarp();
+        if (first) ++results[o];
+        if (j + 2 < jobs) issue_s(j + 2);
+      }
+      n += tiles;
+      ++seg;
+      rest -= tiles;
+      if (rest > 0) at.next_unit(p);
+    }
+    }
+  } else {
+    if (D == 128) more_registers<C::kRegsSoft>();
+    Place at = place_s;
+    int64_t rest = share_s.end - share_s.begin;
+    // ------------------------------------------------------------------ softmax, a thread a row
+    const int group = warp >> 2, wq = warp & 3, row_in = wq * 32 + lane;
+    const uint32_t lane_addr = (uint32_t)(wq * 32) << 16;
+    uint8_t* stg = smem + C::kOut + warp * 2048;
+    uint32_t n = 0;                                        // tiles so far
+    uint32_t seen_s[2] = {0, 0}, results = 0, pv = 0;      // phases of s_full, o_full, pv_done so far
+    bool first_segment = true;
+    while (rest > 0) {
+      const int tiles = (int)min((int64_t)(at.tiles - at.tile), rest);
+      const int rows = at.q.rows(p, at.row_tile);
+      const bool both = C::kGroups == 2 && rows > 128;
+      const bool whole = at.tile == 0 && tiles == at.tiles;
+      const int row = (both ? group * 128 : 0) + row_in;   // of the unit
+      const bool live = row < rows;
+      const int i_row = at.row_tile * C::kRows + row;      // of the request
+      // ---- query rows: all products of the segment before are complete (each group has seen its last S)
+      named_bar_sync(1, 32 * C::kSoft);
+      float c_row = 0.0f;
+      if (both || group == 0) {
+        const T* pq = static_cast<const T*>(p.q) + (int64_t)(at.q.t0 + (live ? i_row : 0) / p.g) * p.sqt +
+                      (int64_t)(at.head * p.g + (live ? i_row : 0) % p.g) * p.sqh;
+        float big = 0.0f;
+        if (live) {
+#pragma unroll 4
+          for (int e = 0; e < D / 8; ++e) {
+            float v[8];
+            load8<T>(pq + e * 8, v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) big = fmaxf(big, fabsf(v[k]));
+          }
+        }
+        // largest element in [2^12, 2^13); scaling below zero turns q
+        const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -110), 127);
+        const float up = copysignf(exp2_int(12 - ex), p.scale_log2);
+        c_row = big == 0.0f ? 0.0f : ldexpf(fabsf(p.scale_log2), ex - 12);
+        const uint32_t dst = smem_u32(smem + C::kQ) + (both ? group : 0) * C::kOperand + row_in * 128;
+#pragma unroll 4
+        for (int e = 0; e < D / 8; ++e) {
+          float v[8];
+          uint32_t h[4] = {0, 0, 0, 0};
+          if (live) {
+            load8<T>(pq + e * 8, v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) h[k] = pack_16x2<__half>(v[2 * k] * up, v[2 * k + 1] * up);
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (e >> 3) * kSub + (((e & 7) ^ (row_in & 7)) << 4)), "r"(h[0]),
+                       "r"(h[1]), "r"(h[2]), "r"(h[3])
+                       : "memory");
+        }
+        if (C::kGroups == 2 && !both) c_s[row_in] = c_row;
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+      if (C::kGroups == 2 && !both) {                      // both groups work on the same rows
+        named_bar_sync(1, 32 * C::kSoft);
+        c_row = c_s[row_in];
+      }
+      const int limit = live ? at.q.seen(p, i_row) : 0;    // keys that this row sees
+      float m = -INFINITY, ref = -INFINITY, l = 0.0f;
+
+      const int step = both || C::kGroups == 1 ? 1 : 2, start = both || C::kGroups == 1 ? 0 : group;
+#pragma unroll 1
+      for (int tile = start; tile < tiles; tile += step) {
+        const int place = C::kGroups == 2 ? group : tile & 1;
+        const uint32_t s_at = tmem + lane_addr + place * 128;
+        const int key0 = (at.tile + tile) * kTile;
+        mbar_wait(&s_full[place], seen_s[place] & 1, err, 67);
+        ++seen_s[place];
+        tc_fence_after();
+        __syncwarp();
+        const TileInfo info = info_s[(n + tile) % kInfo];
+        const bool masked = __any_sync(0xffffffffu, live && limit < key0 + kTile) || (info.there & 0xFF) != 0xFF;
+        const int visible = limit - key0;
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s0[32], s1[32];
+          tmem_ld32(s_at + c * 64, s0);
+          tmem_ld32(s_at + c * 64 + 32, s1);
+          tmem_ld_wait();
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              if (c * 64 + e >= visible || !(info.there >> ((c * 64 + e) >> 4) & 1)) s0[e] = 0xFF800000u;
+              if (c * 64 + 32 + e >= visible || !(info.there >> ((c * 64 + 32 + e) >> 4) & 1)) s1[e] = 0xFF800000u;
+            }
+          }
+          float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            t0 = fmaxf(t0, fmaxf(__uint_as_float(s0[e]), __uint_as_float(s0[e + 1])));
+            t1 = fmaxf(t1, fmaxf(__uint_as_float(s1[e]), __uint_as_float(s1[e + 1])));
+          }
+          top = fmaxf(top, fmaxf(t0, t1));
+        }
+        const float c = c_row * info.k_factor;
+        top = top == -INFINITY ? -INFINITY : top * c;
+        const float m_new = fmaxf(m, top);
+        l *= m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
+        m = m_new;
+        // reference of the weights: moves only where the maximum has left it behind
+        const float want = top + info.v_log2;
+        const bool move = want > ref + kLag;
+        if (__any_sync(0xffffffffu, move)) {
+          const float ref_new = move ? want : ref;
+          const float f = move ? ex2_approx(ref - ref_new) : 1.0f;
+          ref = ref_new;
+          if (tile > start) {
+            if (C::kGroups == 1) {                         // the product before has to be complete
+              mbar_wait(&pv_done, (pv - 1) & 1, err, 68);
+              tc_fence_after();
+              __syncwarp();
+            }
+#pragma unroll 1
+            for (int cc = 0; cc < D / 32; ++cc) {
+              uint32_t o[32];
+              const uint32_t o_at = tmem + lane_addr + C::kO + (C::kGroups == 2 ? group * 128 : 0) + cc * 32;
+              tmem_ld32(o_at, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(o_at, o);
+            }
+          }
+        }
+        const float minus = ref == -INFINITY ? 0.0f : info.v_log2 - ref + kLift;
+        float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t s[32], w[16];
+          tmem_ld32(s_at + cc * 32, s);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(fmaf(__uint_as_float(s[e]), c, minus));
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (cc * 32 + e >= visible || !(info.there >> ((cc * 32 + e) >> 4) & 1)) s[e] = 0xFF800000u;
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float x0 = ex2_approx(__uint_as_float(s[2 * e])), x1 = ex2_approx(__uint_as_float(s[2 * e + 1]));
+            sum0 += x0;
+            sum1 += x1;
+            w[e] = pack_16x2<__half>(x0, x1);
+          }
+          tmem_st16(s_at + cc * 16, w);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[place]);
+        ++pv;
+        // the sum is of weights times 2^(v_log2 - ref + lift)
+        l += m == -INFINITY ? sum0 + sum1 : (sum0 + sum1) * ex2_approx(ref - info.v_log2 - kLift - m);
+      }
+
+      // ---- result of the segment
+      const int slot = 2 * (int)blockIdx.x + (first_segment ? 0 : 1);
+      const bool has = start < tiles;
+      float f = ref == -INFINITY ? 1.0f : ex2_approx(ref - kLift - m);      // brings O to 2^-m (no key: zeros, or NaN)
+      if (has) {
+        mbar_wait(&o_full[C::kGroups == 2 ? group : 0], results & 1, err, 69);
+        ++results;
+        tc_fence_after();
+        __syncwarp();
+      }
+      const uint32_t o_at = tmem + lane_addr + C::kO + (C::kGroups == 2 ? group * 128 : 0);
+      bool writes = true;
+      if (C::kGroups == 2 && !both) {
+        // the groups' results of the same rows: the second one's goes through shared memory, where q was
+        m_s[group][row_in] = m;
+        if (group == 1) l_s[row_in] = l;
+        named_bar_sync(1, 32 * C::kSoft);
+        const float m_all = fmaxf(m_s[0][row_in], m_s[1][row_in]);
+        f *= m_all == -INFINITY ? 1.0f : ex2_approx(m - m_all);
+        const uint32_t buf = smem_u32(smem + C::kQ) + row_in * 512;
+        if (group == 1 && has) {
+#pragma unroll 1
+          for (int cc = 0; cc < 4; ++cc) {
+            uint32_t o[32];
+            tmem_ld32(o_at + cc * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(buf + (((cc * 8 + e) ^ lane) << 4)),
+                           "f"(__uint_as_float(o[4 * e]) * f), "f"(__uint_as_float(o[4 * e + 1]) * f),
+                           "f"(__uint_as_float(o[4 * e + 2]) * f), "f"(__uint_as_float(o[4 * e + 3]) * f)
+                           : "memory");
+          }
+        }
+        named_bar_sync(1, 32 * C::kSoft);
+        writes = group == 0;
+        if (writes && tiles > 1) {
+          const float m1 = m_s[1][row_in], l1 = l_s[row_in];
+          l = m_all == -INFINITY ? l + l1 : l * ex2_approx(m - m_all) + l1 * ex2_approx(m1 - m_all);
+        }
+        m = m_all;
+      }
+      const bool add = C::kGroups == 2 && !both && tiles > 1;
+      const int rows_warp = min(max(rows - (both ? group * 128 : 0) - wq * 32, 0), 32);    // of this warp that exist
+      if (writes && rows_warp > 0) {
+        const int row0 = (both ? group * 128 : 0) + wq * 32;
+        const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+        if (whole) {
+          if (live && p.lse != nullptr) p.lse[out_row(p, (int64_t)at.q.t0 * p.g + i_row, at.head)] = lse_of(m, l);
+        } else if (live) {
+          p.ws_m[(int64_t)slot * C::kRows + row] = m;
+          p.ws_l[(int64_t)slot * C::kRows + row] = l;
+        }
+#pragma unroll 1
+        for (int cc = 0; cc < D / 32; ++cc) {
+          uint32_t o[32];
+          tmem_ld32(o_at + cc * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          if (add) {
+            const uint32_t buf = smem_u32(smem + C::kQ) + row_in * 512;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float x[4];
+              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(
+                               buf + (((cc * 8 + e) ^ lane) << 4))
+                           : "memory");
+#pragma unroll
+              for (int k = 0; k < 4; ++k) o[4 * e + k] = __float_as_uint(__uint_as_float(o[4 * e + k]) + x[k]);
+            }
+          }
+          // 64 bytes of a row at a time, four lanes a row: a lane's own row would be 16 bytes of 32 rows an instruction
+          auto segment = [&](const uint32_t (&w)[16], auto address) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(stg + sw64_offset(lane, e * 16)) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = 8 * e + (lane >> 2), ch = lane & 3;
+              const uint4 v = *reinterpret_cast<const uint4*>(stg + sw64_offset(r, ch * 16));
+              if (r < rows_warp) *reinterpret_cast<uint4*>(address(r) + ch * 16) = v;
+            }
+            __syncwarp();
+          };
+          if (whole) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              w[e] = pack_16x2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            segment(w, [&](int r) {
+              const int64_t to = out_row(p, (int64_t)at.q.t0 * p.g + at.row_tile * C::kRows + row0 + r, at.head);
+              return reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) + to * D + cc * 32);
+            });
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t w[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) w[e] = o[16 * h + e];
+              segment(w, [&](int r) {
+                return reinterpret_cast<uint8_t*>(p.ws_acc + ((int64_t)slot * C::kRows + row0 + r) * D + cc * 32 + h * 16);
+              });
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (has && lane == 0) mbar_arrive(&o_free[C::kGroups == 2 ? group : 0]);
+      if (!whole && at.tile == 0 && tid == 0) p.cut[blockIdx.x] = cut_unit(p, at, tiles, share_s.share, first_segment);
+      n += tiles;
+      first_segment = false;
+      rest -= tiles;
+      if (rest > 0) at.next_unit(p);
+    }
+  }
+  clear_untouched<T, D, C::kRows, kTile>(p);
+  tc_fence_before();
+  __syncthreads();
+  report_error(&expired, p.status);
+  if (warp == C::kSoft + 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int D>
+int run_chunk(const PagedParams& p, int ctas, cudaStream_t st) {
+  using C = Cfg<D>;
+  if (int rc = allow_smem("nvfp4_kv8_attention", reinterpret_cast<const void*>(paged_chunk_kernel<T, D>), C::kBytes)) return rc;
+  if (int rc = launch("nvfp4_kv8_attention", paged_chunk_kernel<T, D>, dim3(ctas), C::kThreads, C::kBytes, st, p)) return rc;
+  return launch_combine<T, D, C::kRows>(p, ctas, st);
+}
+
+}  // namespace
+
+int launch_paged_chunk(const PagedParams& p, int q_dtype, int d, int ctas, cudaStream_t st) {
+  if (q_dtype == NVFP4_DT_BF16) return d == 128 ? run_chunk<__nv_bfloat16, 128>(p, ctas, st) : run_chunk<__nv_bfloat16, 256>(p, ctas, st);
+  return d == 128 ? run_chunk<__half, 128>(p, ctas, st) : run_chunk<__half, 256>(p, ctas, st);
+}
+
+}  // namespace nvfp4

@@ -81,11 +81,14 @@ def test_c_entries_refuse_bad_sizes():
         assert w(**bad) < 0 and text in L.nvfp4_last_error(), bad
     assert w(t=0) == 0
     size = ctypes.c_size_t()
-    assert L.nvfp4_kv8_attention_plan(96, 148, ctypes.byref(size)) < 0
-    assert L.nvfp4_kv8_attention_plan(128, 148, ctypes.byref(size)) == 0 and size.value == 2 * 148 * (2 * 16 * 130 * 4 + 16)
+    plan = lambda dt, t, r, g, d: L.nvfp4_kv8_attention_plan(dt, t, r, g, d, 148, ctypes.byref(size))
+    assert plan(0, 1, 1, 1, 96) < 0 and plan(0, 1, 0, 1, 128) < 0
+    assert plan(0, 7, 7, 16, 128) == 0 and size.value == 2 * 148 * (2 * 16 * 130 * 4 + 16)
+    assert plan(1, 80, 7, 4, 256) == 0 and size.value == 148 * (2 * 128 * 258 * 4 + 16)
+    assert plan(2, 80, 7, 4, 256) == 0 and size.value == 2 * 148 * (2 * 16 * 258 * 4 + 16)
     a = lambda **k: L.nvfp4_kv8_attention(0, 0, 128, 128, k.get("cu", n), k.get("t", 1), k.get("kc", 0), 2048, 0, 2048, n, 1, n, 1, 1,
                                           k.get("bs", 16), n, 1, k.get("w", 1), n, 1, 1, k.get("g", 1), k.get("d", 128), 1.0, 0, n, 0,
-                                          k.get("ws", 0), n)
+                                          k.get("ws", 0), n, n)
     for bad, text in ((dict(bs=48), b"block_size"), (dict(d=80), b"D must"), (dict(t=2), b"cu_seqlens"), (dict(kc=8), b"aligned"),
                       (dict(g=0), b"sizes"), (dict(w=1 << 28), b"sizes"), (dict(t=-1, cu=16), b"sizes")):
         assert a(**bad) < 0 and text in L.nvfp4_last_error(), bad
