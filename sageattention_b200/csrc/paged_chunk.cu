@@ -9,7 +9,7 @@
 //   rows > 128 (D = 128): job 2 t + g = rows of group g, key tile t; both groups use the converted tile
 //   rows <= 128 (D = 128): job t = key tile t, of group t & 1; the groups keep results of their own, merged at the end
 //   D = 256: job t = key tile t, one group; S alternates between two places
-// Job j has S in place j & 1, P overlays the S it came from, and the order of issue -- S(j + 2) behind P V (j) -- is what keeps
+// Job j has S in place j & 1, P overlays the upper half of the S it came from, and the order of issue -- S(j + 2) behind P V (j) -- is what keeps
 // one place's products and its softmax apart: a completed S(j + 2) tells that P V (j) is complete as well.
 //
 // What bounds it (D = 128): a key tile of 256 rows is 2080 clocks of products and 2048 of ex2 on an SM; a place's own cycle is
@@ -29,7 +29,7 @@ constexpr int kTile = 128;                    // keys of a tile
 constexpr int kSub = 128 * 128;               // bytes of a 128-row sub-tile of 64 halves
 constexpr int kInfo = 8;                      // tiles whose scales are kept: more than can be under way
 // P is held times 2^kLift relative to a reference that may lag behind the running maximum by 2^kLag
-constexpr float kLift = 8.0f, kLag = 7.0f;
+constexpr float kLift = 3.0f, kLag = 12.0f;
 
 template <int D>
 struct Cfg {
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
           for (int c = 0; c < D / 128; ++c)
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              umma_bf16_ta(tmem + C::kO + o * 128 + c * 128, tmem + g * 128 + k * 8, x_v + c * (2 * kSub >> 4) + k * 128, id_o,
+              umma_bf16_ta(tmem + C::kO + o * 128 + c * 128, tmem + g * 128 + 64 + k * 8, x_v + c * (2 * kSub >> 4) + k * 128, id_o,
                            (k > 0 || !first) ? 1u : 0u);
           if (!both || g == 1) umma_commit(&v_free[st]);
           if (C::kGroups == 1) umma_commit(&pv_done);
@@ -407,33 +407,33 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         const TileInfo info = info_s[(n + tile) % kInfo];
         const bool masked = __any_sync(0xffffffffu, live && limit < key0 + kTile) || (info.there & 0xFF) != 0xFF;
         const int visible = limit - key0;
+        // columns 32 x .. of S: the next ones are on their way while the present ones are used, and the last ones stay for
+        // the exponentials, which therefore run from the end
         float top = -INFINITY;
+        uint32_t s[2][32];
+        auto hide = [&](uint32_t (&v)[32], int x) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t s0[32], s1[32];
-          tmem_ld32(s_at + c * 64, s0);
-          tmem_ld32(s_at + c * 64 + 32, s1);
-          tmem_ld_wait();
-          if (masked) {
+          for (int e = 0; e < 32; ++e)
+            if (x * 32 + e >= visible || !(info.there >> (x * 2 + (e >> 4)) & 1)) v[e] = 0xFF800000u;
+        };
+        tmem_ld32(s_at, s[0]);
+        tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              if (c * 64 + e >= visible || !(info.there >> ((c * 64 + e) >> 4) & 1)) s0[e] = 0xFF800000u;
-              if (c * 64 + 32 + e >= visible || !(info.there >> ((c * 64 + 32 + e) >> 4) & 1)) s1[e] = 0xFF800000u;
-            }
-          }
+        for (int x = 0; x < 4; ++x) {
+          uint32_t (&now)[32] = s[x & 1];
+          if (x < 3) tmem_ld32(s_at + (x + 1) * 32, s[(x + 1) & 1]);
+          if (masked) hide(now, x);
           float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            t0 = fmaxf(t0, fmaxf(__uint_as_float(s0[e]), __uint_as_float(s0[e + 1])));
-            t1 = fmaxf(t1, fmaxf(__uint_as_float(s1[e]), __uint_as_float(s1[e + 1])));
+          for (int e = 0; e < 32; e += 4) {
+            t0 = fmaxf(t0, fmaxf(__uint_as_float(now[e]), __uint_as_float(now[e + 1])));
+            t1 = fmaxf(t1, fmaxf(__uint_as_float(now[e + 2]), __uint_as_float(now[e + 3])));
           }
           top = fmaxf(top, fmaxf(t0, t1));
+          if (x < 3) tmem_ld_wait();
         }
         const float c = c_row * info.k_factor;
         top = top == -INFINITY ? -INFINITY : top * c;
-        const float m_new = fmaxf(m, top);
-        l *= m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
-        m = m_new;
         // reference of the weights: moves only where the maximum has left it behind
         const float want = top + info.v_log2;
         const bool move = want > ref + kLag;
@@ -462,31 +462,31 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         const float minus = ref == -INFINITY ? 0.0f : info.v_log2 - ref + kLift;
         float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
-          uint32_t s[32], w[16];
-          tmem_ld32(s_at + cc * 32, s);
-          tmem_ld_wait();
+        for (int x = 3; x >= 0; --x) {
+          uint32_t (&now)[32] = s[x & 1];
+          if (x > 0) tmem_ld32(s_at + (x - 1) * 32, s[(x - 1) & 1]);
+          uint32_t w[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(fmaf(__uint_as_float(s[e]), c, minus));
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (cc * 32 + e >= visible || !(info.there >> ((cc * 32 + e) >> 4) & 1)) s[e] = 0xFF800000u;
-          }
+          for (int e = 0; e < 32; ++e) now[e] = __float_as_uint(fmaf(__uint_as_float(now[e]), c, minus));
+          if (masked) hide(now, x);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float x0 = ex2_approx(__uint_as_float(s[2 * e])), x1 = ex2_approx(__uint_as_float(s[2 * e + 1]));
+            const float x0 = ex2_approx(__uint_as_float(now[2 * e])), x1 = ex2_approx(__uint_as_float(now[2 * e + 1]));
             sum0 += x0;
             sum1 += x1;
             w[e] = pack_16x2<__half>(x0, x1);
           }
-          tmem_st16(s_at + cc * 16, w);
+          if (x > 0) tmem_ld_wait();
+          tmem_st16(s_at + 64 + x * 16, w);                // over columns that have been read
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[place]);
         ++pv;
+        const float m_new = fmaxf(m, top);
+        l *= m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
+        m = m_new;
         // the sum is of weights times 2^(v_log2 - ref + lift)
         l += m == -INFINITY ? sum0 + sum1 : (sum0 + sum1) * ex2_approx(ref - info.v_log2 - kLift - m);
       }
