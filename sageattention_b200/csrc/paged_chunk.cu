@@ -5,15 +5,15 @@
 // a tile with smaller scales by a factor of at most 1), q enters as halves scaled by a power of two per row.
 //
 // Warps: two softmax groups (a thread a row; at D = 256 one group), four converting warps, one that issues the products.
-// Work goes through "jobs": one 128-row product pair with one key tile of 128 keys.
-//   rows > 128 (D = 128): job 2 t + g = rows of group g, key tile t; both groups use the converted tile
-//   rows <= 128 (D = 128): job t = key tile t, of group t & 1; the groups keep results of their own, merged at the end
-//   D = 256: job t = key tile t, one group; S alternates between two places
-// Job j has S in place j & 1, P overlays the upper half of the S it came from, and the order of issue -- S(j + 2) behind P V (j) -- is what keeps
-// one place's products and its softmax apart: a completed S(j + 2) tells that P V (j) is complete as well.
+// A job is 128 rows against 64 keys (128 at D = 256); a group goes through its jobs one after the other, S of job j in place
+// j & 1 of the group's two, P over the upper half of the S it came from.
+//   rows > 128 (D = 128): group g has rows 128 g .., both go through every key tile
+//   rows <= 128 (D = 128): the groups take turns at the key tiles and keep results of their own, merged at the end
+// Products are issued in the order PV(j), S(j + 2): S(j + 1) is there when the softmax of job j ends, and a completed S(j + 2)
+// tells that PV(j) is complete as well.
 //
-// What bounds it (D = 128): a key tile of 256 rows is 2080 clocks of products and 2048 of ex2 on an SM; a place's own cycle is
-// product, softmax, product one after the other, with the other place's products in between.
+// What bounds it (D = 128): a key tile of 256 rows is 2580 clocks of products on an SM (S with 64 keys reads its operands
+// from shared memory at 48 clocks an instruction instead of 32) and 2048 of ex2.
 #include <cuda_fp16.h>
 #include "common/abi.cuh"
 #include "common/bwd_util.cuh"
@@ -42,7 +42,10 @@ struct Cfg {
   static constexpr int kOperand = D / 64 * kSub;           // 128 rows of q, or a tile of keys or values
   static constexpr int kQ = 0, kK = kGroups * kOperand, kV = kK + kStages * kOperand, kOut = kV + kStages * kOperand;
   static constexpr int kBytes = kOut + kSoft * 2048 + 1024;
-  static constexpr int kO = 256;                           // tensor memory: S at 0 and 128, O behind
+  static constexpr int kN = D == 128 ? 64 : 128;           // keys of a job
+  static constexpr int kJobs = kTile / kN;                 // jobs of a tile
+  static constexpr int kO = 256;                           // tensor memory: S of (group, place), O behind
+  static __device__ __forceinline__ uint32_t s_at(int group, int place) { return (group * 2 + place) * kN; }
 };
 
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -92,7 +95,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
   using Place = Cursor<C::kRows, kTile>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], o_full[2], o_free[2], q_full, pv_done;
+  __shared__ uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2][2], p_full[2][2], o_full[2], o_free[2], pv_done[2], q_full;
   __shared__ uint32_t tmem_base_s;
   __shared__ int expired;                                  // a wait ran out: site, else 0
   __shared__ int64_t list_s[C::kThreads / 32 + 2];
@@ -110,13 +113,15 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       mbar_init(&k_free[i], 1);
       mbar_init(&v_full[i], 4);
       mbar_init(&v_free[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&s_full[i][k], 1);
+        mbar_init(&p_full[i][k], 4);
+      }
+      mbar_init(&pv_done[i], 1);
       mbar_init(&o_full[i], 1);
       mbar_init(&o_free[i], 4);
     }
     mbar_init(&q_full, C::kSoft);
-    mbar_init(&pv_done, 1);
     mbar_fence_init();
   }
   if (warp == C::kSoft + 4) tmem_alloc(&tmem_base_s, 512);
@@ -267,61 +272,72 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     Place at = place_s;
     int64_t rest = share_s.end - share_s.begin;
     const bool leader = elect_one();
-    const uint32_t id_s = make_idesc_bf16(128, 128, false, true), id_o = make_idesc_bf16(128, 128, true, true);
+    const uint32_t id_s = make_idesc_bf16(128, C::kN, false, true), id_o = make_idesc_bf16(128, 128, true, true);
     const uint64_t b_q = desc_sw128(smem + C::kQ, 0), b_k = desc_sw128(smem + C::kK, 0);
     const uint64_t b_v = desc_sw128_mn(smem + C::kV, 0, kSub);
     uint32_t n = 0, seg = 0;                               // tiles and segments so far
-    uint32_t jobs_of[2] = {0, 0};                          // jobs of each place so far
-    uint32_t results[2] = {0, 0};                          // results of each O so far
+    uint32_t p_phase[2] = {0, 0};                          // of p_full, a bit a place
+    uint32_t results[2] = {0, 0};                          // results of each group so far
     while (rest > 0) {
       const int tiles = (int)min((int64_t)(at.tiles - at.tile), rest);
       const bool both = C::kGroups == 2 && at.q.rows(p, at.row_tile) > 128;
-      const int jobs = both ? 2 * tiles : tiles;
+      const int turn = both || C::kGroups == 1 ? 1 : 2;    // a group takes every turn-th tile
+      auto jobs_of = [&](int g) { return (turn == 1 ? tiles : (tiles + 1 - g) / 2) * C::kJobs; };
+      auto tile_of = [&](int g, int j) { return j / C::kJobs * turn + (turn == 2 ? g : 0); };
       mbar_wait_warp(&q_full, seg & 1, err, 62);
-      auto issue_s = [&](int j) {
-        const int tile = both ? j >> 1 : j, g = j & 1;
-        const int st = (n + tile) % C::kStages;
-        if (!both || g == 0) mbar_wait(&k_full[st], ((n + tile) / C::kStages) & 1, err, 63);
+      auto issue_s = [&](int g, int j) {
+        const uint32_t tile = n + tile_of(g, j), st = tile % C::kStages;
+        const int sub = j % C::kJobs;
+        if (sub == 0 && (!both || g == 0)) mbar_wait(&k_full[st], (tile / C::kStages) & 1, err, 63);
         __syncwarp();
         tc_fence_after();
         if (leader) {
-          const uint64_t x_q = b_q + (both && g ? C::kOperand >> 4 : 0), x_k = b_k + (uint64_t)(st * (C::kOperand >> 4));
+          const uint64_t x_q = b_q + (both && g ? C::kOperand >> 4 : 0);
+          const uint64_t x_k = b_k + (uint64_t)(st * (C::kOperand >> 4) + sub * (C::kN * 128 >> 4));
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tmem + g * 128, x_q + (k >> 2) * (kSub >> 4) + (k & 3) * 2, x_k + (k >> 2) * (kSub >> 4) + (k & 3) * 2, id_s,
-                      k > 0);
-          umma_commit(&s_full[g]);
-          if (!both || g == 1) umma_commit(&k_free[st]);
+            umma_bf16(tmem + C::s_at(g, j & 1), x_q + (k >> 2) * (kSub >> 4) + (k & 3) * 2, x_k + (k >> 2) * (kSub >> 4) + (k & 3) * 2,
+                      id_s, k > 0);
+          umma_commit(&s_full[g][j & 1]);
+          if (sub == C::kJobs - 1 && (!both || g == 1)) umma_commit(&k_free[st]);
         }
         __syncwarp();
       };
-      issue_s(0);
-      if (jobs > 1) issue_s(1);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int g = 0; g < C::kGroups; ++g)
+          if (j < jobs_of(g)) issue_s(g, j);
+      const int most = jobs_of(0);
 #pragma unroll 1
-      for (int j = 0; j < jobs; ++j) {
-        const int tile = both ? j >> 1 : j, g = j & 1, o = C::kGroups == 2 ? g : 0;
-        const int st = (n + tile) % C::kStages;
-        const bool first = C::kGroups == 2 ? j < 2 : j == 0;
-        if (first && results[o] > 0) mbar_wait(&o_free[o], (results[o] - 1) & 1, err, 64);
-        if (!both || g == 0) mbar_wait(&v_full[st], ((n + tile) / C::kStages) & 1, err, 65);
-        mbar_wait_warp(&p_full[g], jobs_of[g] & 1, err, 66);
-        ++jobs_of[g];
-        tc_fence_after();
-        if (leader) {
-          const uint64_t x_v = b_v + (uint64_t)(st * (C::kOperand >> 4));
+      for (int j = 0; j < most; ++j) {
 #pragma unroll
-          for (int c = 0; c < D / 128; ++c)
+        for (int g = 0; g < C::kGroups; ++g) {
+          const int jobs = jobs_of(g);
+          if (j >= jobs) continue;
+          const uint32_t tile = n + tile_of(g, j), st = tile % C::kStages;
+          const int sub = j % C::kJobs;
+          if (j == 0 && results[g] > 0) mbar_wait(&o_free[g], (results[g] - 1) & 1, err, 64);
+          if (sub == 0 && (!both || g == 0)) mbar_wait(&v_full[st], (tile / C::kStages) & 1, err, 65);
+          mbar_wait_warp(&p_full[g][j & 1], (p_phase[g] >> (j & 1)) & 1, err, 66);
+          p_phase[g] ^= 1u << (j & 1);
+          tc_fence_after();
+          if (leader) {
+            const uint64_t x_v = b_v + (uint64_t)(st * (C::kOperand >> 4) + sub * (C::kN * 128 >> 4));
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              umma_bf16_ta(tmem + C::kO + o * 128 + c * 128, tmem + g * 128 + 64 + k * 8, x_v + c * (2 * kSub >> 4) + k * 128, id_o,
-                           (k > 0 || !first) ? 1u : 0u);
-          if (!both || g == 1) umma_commit(&v_free[st]);
-          if (C::kGroups == 1) umma_commit(&pv_done);
-          if (j + C::kGroups >= jobs) umma_commit(&o_full[o]);
+            for (int c = 0; c < D / 128; ++c)
+#pragma unroll
+              for (int k = 0; k < C::kN / 16; ++k)
+                umma_bf16_ta(tmem + C::kO + g * 128 + c * 128, tmem + C::s_at(g, j & 1) + C::kN / 2 + k * 8,
+                             x_v + c * (2 * kSub >> 4) + k * 128, id_o, (k > 0 || j > 0) ? 1u : 0u);
+            if (sub == C::kJobs - 1 && (!both || g == 1)) umma_commit(&v_free[st]);
+            umma_commit(&pv_done[g]);
+            if (j + 1 == jobs) umma_commit(&o_full[g]);
+          }
+          __syncwarp();
+          if (j == 0) ++results[g];
+          if (j + 2 < jobs) issue_s(g, j + 2);
         }
-        __syncwarp();
-        if (first) ++results[o];
-        if (j + 2 < jobs) issue_s(j + 2);
       }
       n += tiles;
       ++seg;
@@ -338,7 +354,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     const uint32_t lane_addr = (uint32_t)(wq * 32) << 16;
     uint8_t* stg = smem + C::kOut + warp * 2048;
     uint32_t n = 0;                                        // tiles so far
-    uint32_t seen_s[2] = {0, 0}, results = 0, pv = 0;      // phases of s_full, o_full, pv_done so far
+    uint32_t s_phase = 0, results = 0, pv = 0;             // phases of s_full (a bit a place), o_full and pv_done so far
     bool first_segment = true;
     while (rest > 0) {
       const int tiles = (int)min((int64_t)(at.tiles - at.tile), rest);
@@ -394,34 +410,38 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       const int limit = live ? at.q.seen(p, i_row) : 0;    // keys that this row sees
       float m = -INFINITY, ref = -INFINITY, l = 0.0f;
 
-      const int step = both || C::kGroups == 1 ? 1 : 2, start = both || C::kGroups == 1 ? 0 : group;
+      const int turn = both || C::kGroups == 1 ? 1 : 2, my = turn == 2 ? group : 0;
+      const int jobs = (turn == 1 ? tiles : (tiles + 1 - my) / 2) * C::kJobs;
 #pragma unroll 1
-      for (int tile = start; tile < tiles; tile += step) {
-        const int place = C::kGroups == 2 ? group : tile & 1;
-        const uint32_t s_at = tmem + lane_addr + place * 128;
-        const int key0 = (at.tile + tile) * kTile;
-        mbar_wait(&s_full[place], seen_s[place] & 1, err, 67);
-        ++seen_s[place];
+      for (int j = 0; j < jobs; ++j) {
+        constexpr int kChunks = C::kN / 32;
+        const int place = j & 1, tile = j / C::kJobs * turn + my, sub = j % C::kJobs;
+        const uint32_t s_at = tmem + lane_addr + C::s_at(group, place);
+        const int key0 = (at.tile + tile) * kTile + sub * C::kN;
+        mbar_wait(&s_full[group][place], (s_phase >> place) & 1, err, 67);
+        s_phase ^= 1u << place;
         tc_fence_after();
         __syncwarp();
         const TileInfo info = info_s[(n + tile) % kInfo];
-        const bool masked = __any_sync(0xffffffffu, live && limit < key0 + kTile) || (info.there & 0xFF) != 0xFF;
+        const uint32_t there = info.there >> (sub * (C::kN / 16));
+        const bool masked = __any_sync(0xffffffffu, live && limit < key0 + C::kN) ||
+                            (there & ((1u << (C::kN / 16)) - 1)) != (1u << (C::kN / 16)) - 1;
         const int visible = limit - key0;
-        // columns 32 x .. of S: the next ones are on their way while the present ones are used, and the last ones stay for
+        // columns 32 x .. of S: the next ones are on their way while the present ones are used, and the last two stay for
         // the exponentials, which therefore run from the end
         float top = -INFINITY;
         uint32_t s[2][32];
         auto hide = [&](uint32_t (&v)[32], int x) {
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (x * 32 + e >= visible || !(info.there >> (x * 2 + (e >> 4)) & 1)) v[e] = 0xFF800000u;
+            if (x * 32 + e >= visible || !(there >> (x * 2 + (e >> 4)) & 1)) v[e] = 0xFF800000u;
         };
         tmem_ld32(s_at, s[0]);
         tmem_ld_wait();
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < kChunks; ++x) {
           uint32_t (&now)[32] = s[x & 1];
-          if (x < 3) tmem_ld32(s_at + (x + 1) * 32, s[(x + 1) & 1]);
+          if (x < kChunks - 1) tmem_ld32(s_at + (x + 1) * 32, s[(x + 1) & 1]);
           if (masked) hide(now, x);
           float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
@@ -430,7 +450,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
             t1 = fmaxf(t1, fmaxf(__uint_as_float(now[e + 2]), __uint_as_float(now[e + 3])));
           }
           top = fmaxf(top, fmaxf(t0, t1));
-          if (x < 3) tmem_ld_wait();
+          if (x < kChunks - 1) tmem_ld_wait();
         }
         const float c = c_row * info.k_factor;
         top = top == -INFINITY ? -INFINITY : top * c;
@@ -441,16 +461,14 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
           const float ref_new = move ? want : ref;
           const float f = move ? ex2_approx(ref - ref_new) : 1.0f;
           ref = ref_new;
-          if (tile > start) {
-            if (C::kGroups == 1) {                         // the product before has to be complete
-              mbar_wait(&pv_done, (pv - 1) & 1, err, 68);
-              tc_fence_after();
-              __syncwarp();
-            }
+          if (j > 0) {                                     // the product before has to be complete
+            mbar_wait(&pv_done[group], (pv - 1) & 1, err, 68);
+            tc_fence_after();
+            __syncwarp();
 #pragma unroll 1
             for (int cc = 0; cc < D / 32; ++cc) {
               uint32_t o[32];
-              const uint32_t o_at = tmem + lane_addr + C::kO + (C::kGroups == 2 ? group * 128 : 0) + cc * 32;
+              const uint32_t o_at = tmem + lane_addr + C::kO + group * 128 + cc * 32;
               tmem_ld32(o_at, o);
               tmem_ld_wait();
 #pragma unroll
@@ -462,9 +480,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         const float minus = ref == -INFINITY ? 0.0f : info.v_log2 - ref + kLift;
         float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-        for (int x = 3; x >= 0; --x) {
+        for (int x = kChunks - 1; x >= 0; --x) {
           uint32_t (&now)[32] = s[x & 1];
-          if (x > 0) tmem_ld32(s_at + (x - 1) * 32, s[(x - 1) & 1]);
+          if (x <= kChunks - 3) tmem_ld_wait();
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 32; ++e) now[e] = __float_as_uint(fmaf(__uint_as_float(now[e]), c, minus));
@@ -476,13 +494,13 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
             sum1 += x1;
             w[e] = pack_16x2<__half>(x0, x1);
           }
-          if (x > 0) tmem_ld_wait();
-          tmem_st16(s_at + 64 + x * 16, w);                // over columns that have been read
+          if (x >= 2) tmem_ld32(s_at + (x - 2) * 32, now);
+          tmem_st16(s_at + C::kN / 2 + x * 16, w);         // over columns that have been read
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[place]);
+        if (lane == 0) mbar_arrive(&p_full[group][place]);
         ++pv;
         const float m_new = fmaxf(m, top);
         l *= m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
@@ -493,15 +511,15 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
 
       // ---- result of the segment
       const int slot = 2 * (int)blockIdx.x + (first_segment ? 0 : 1);
-      const bool has = start < tiles;
+      const bool has = jobs > 0;
       float f = ref == -INFINITY ? 1.0f : ex2_approx(ref - kLift - m);      // brings O to 2^-m (no key: zeros, or NaN)
       if (has) {
-        mbar_wait(&o_full[C::kGroups == 2 ? group : 0], results & 1, err, 69);
+        mbar_wait(&o_full[group], results & 1, err, 69);
         ++results;
         tc_fence_after();
         __syncwarp();
       }
-      const uint32_t o_at = tmem + lane_addr + C::kO + (C::kGroups == 2 ? group * 128 : 0);
+      const uint32_t o_at = tmem + lane_addr + C::kO + group * 128;
       bool writes = true;
       if (C::kGroups == 2 && !both) {
         // the groups' results of the same rows: the second one's goes through shared memory, where q was
@@ -601,7 +619,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       }
       tc_fence_before();
       __syncwarp();
-      if (has && lane == 0) mbar_arrive(&o_free[C::kGroups == 2 ? group : 0]);
+      if (has && lane == 0) mbar_arrive(&o_free[group]);
       if (!whole && at.tile == 0 && tid == 0) p.cut[blockIdx.x] = cut_unit(p, at, tiles, share_s.share, first_segment);
       n += tiles;
       first_segment = false;
