@@ -154,46 +154,57 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     const int in_key = (lane >> 2) & 1, in_chunk = lane & 3, pair = w * 4 + (lane >> 3);
     auto key_of = [&](int i) { return (i / (D / 64)) * 32 + pair * 2 + in_key; };
     auto chunk_of = [&](int i) { return (i % (D / 64)) * 4 + in_chunk; };
-    int id = -1;                                           // block of keys 16 lane .. of the tile to come (lanes 0 to 7)
-    float ksc = 0.0f, vsc = 0.0f;
+    // Codes wait in registers, from the time that their tile's predecessor is converted on.  A load in flight holds a line of
+    // L1, of which this kernel's shared memory leaves 28 KB, less than a tile of K and V: piece i of the next tile is asked
+    // for when piece i of the present one has been converted, not all at once.
     uint4 kr[kPieces], vr[kPieces];
-    // `ahead`: the tile whose blocks are looked up, one behind the tile (key0, limit, head) whose codes are asked for
-    int key0 = 0, limit = 0, head = 0, id_ahead = -1;
-    bool starts = true, starts_ahead = true;               // the tile is the first one of its unit, as far as this CTA sees
+    // lanes 0 to 7: block of keys 16 lane .. of the tile being converted (`now`), asked for (`next`), and of the one behind
+    int id_now = -1, id_next = -1, id_ahead = -1;
+    float ks_now = 0.0f, vs_now = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
+    int key0 = 0, limit = 0, head = 0;                     // of the tile asked for
+    bool starts = true, starts_next = true, starts_ahead = true;   // first tile of its unit, as far as this CTA sees
     auto look_up = [&]() {
       id_ahead = -1;
       const int key = ahead.tile * kTile + lane * 16;
       if (left > 0 && lane < 8 && key < ahead.q.limit(p, ahead.row_tile))
         id_ahead = p.table[ahead.r * p.table_row + (key >> p.log_block)];
     };
+    // the tile asked for becomes the one converted, the one looked up the one asked for
     auto next = [&]() {
-      id = (unsigned)id_ahead < (unsigned)p.blocks ? id_ahead : -1;
+      id_now = id_next;
+      ks_now = ks_next;
+      vs_now = vs_next;
+      starts = starts_next;
+      id_next = (unsigned)id_ahead < (unsigned)p.blocks ? id_ahead : -1;
+      starts_next = starts_ahead;
+      starts_ahead = false;
       key0 = ahead.tile * kTile;
       limit = left > 0 ? ahead.q.limit(p, ahead.row_tile) : 0;
       head = ahead.head;
-      starts = starts_ahead;
-      starts_ahead = false;
       if (--left > 0 && ++ahead.tile == ahead.tiles) {
         ahead.next_unit(p);
         starts_ahead = true;
       }
       look_up();
-      ksc = id >= 0 ? p.ks[id * p.ks_block + head] : 0.0f;
-      vsc = id >= 0 ? p.vs[id * p.vs_block + head] : 0.0f;
+      ks_next = id_next >= 0 ? p.ks[id_next * p.ks_block + head] : 0.0f;
+      vs_next = id_next >= 0 ? p.vs[id_next * p.vs_block + head] : 0.0f;
     };
-    auto ask = [&](const uint8_t* base, int64_t block, uint4 (&r)[kPieces]) {
+    // a warp's keys lie in every other 16-key group: block of its u-th one (shuffles share a queue with the stores below)
+    constexpr int kOwn = 4, kEach = kPieces / kOwn;
+    auto group_of = [&](int u) { return 2 * u + (w >> 1); };
+    int own_id[kOwn];
+    auto ask = [&](const uint8_t* base, int64_t block, int i) -> uint4 {
+      const int key = key_of(i), b = own_id[i / kEach];
+      const int at_key = (key0 + key) & ((1 << p.log_block) - 1);
+      return load_or_zero(base + b * block + (((int64_t)head << p.log_block) + at_key) * D + chunk_of(i) * 16,
+                          b >= 0 && key0 + key < limit);
+    };
+    // pieces to halves times `factor` (lane h: of keys 16 h ..), into a tile in shared memory; then the next tile's are asked for
+    auto convert = [&](uint4 (&r)[kPieces], float factor, uint32_t dst, const uint8_t* base, int64_t block) {
+      const bool plain = __all_sync(0xffffffffu, lane >= 8 || id_now < 0 || factor == 1.0f);
+      __half2 own[kOwn];
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int key = key_of(i), b = __shfl_sync(0xffffffffu, id, key >> 4);
-        const int at_key = (key0 + key) & ((1 << p.log_block) - 1);
-        r[i] = load_or_zero(base + b * block + (((int64_t)head << p.log_block) + at_key) * D + chunk_of(i) * 16,
-                            b >= 0 && key0 + key < limit);
-      }
-    };
-    // pieces to halves times `scale` (of the key's block) * down, into a tile in shared memory
-    auto convert = [&](const uint4 (&r)[kPieces], float scale, float down, uint32_t dst) {
-      const float mine_f = scale * down;
-      const bool plain = __all_sync(0xffffffffu, lane >= 8 || id < 0 || mine_f == 1.0f);
+      for (int u = 0; u < kOwn; ++u) own[u] = __float2half2_rn(__shfl_sync(0xffffffffu, factor, group_of(u)));
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         const int key = key_of(i), chunk = chunk_of(i);
@@ -201,12 +212,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         uint32_t h[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) half4_of_e4m3x4(words[k], h[2 * k], h[2 * k + 1]);
+        r[i] = ask(base, block, i);
         if (!plain) {
-          const float f = __shfl_sync(0xffffffffu, mine_f, key >> 4);
-          const __half2 f2 = __float2half2_rn(f);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h[k]), f2);
+            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h[k]), own[i / kEach]);
             h[k] = *reinterpret_cast<const uint32_t*>(&v);
           }
         }
@@ -225,45 +235,36 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     if (left > 0) {
       look_up();
       next();
-      ask(p.k, p.k_block, kr);
-      ask(p.v, p.v_block, vr);
+#pragma unroll
+      for (int u = 0; u < kOwn; ++u) own_id[u] = __shfl_sync(0xffffffffu, id_next, group_of(u));
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) kr[i] = ask(p.k, p.k_block, i);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) vr[i] = ask(p.v, p.v_block, i);
     }
     int v_run = -200;                                      // largest exponent of the unit's value scales so far
     uint32_t n = 0;
     for (; rest > 0; --rest, ++n) {
-      // scales of the tile, and its factors
       const int st = n % C::kStages;
       const uint32_t ph = (n / C::kStages) & 1;
+      next();
+      // factors of the tile
       if (starts) v_run = -200;
-      int ke = id >= 0 ? scale_exp(ksc) : -112, ve = id >= 0 ? scale_exp(vsc) : -112;
+      int ke = id_now >= 0 ? scale_exp(ks_now) : -112, ve = id_now >= 0 ? scale_exp(vs_now) : -112;
+      ke = __reduce_max_sync(0xffffffffu, lane < 8 ? ke : -112);
+      ve = __reduce_max_sync(0xffffffffu, lane < 8 ? ve : -112);
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) {
-        ke = max(ke, __shfl_xor_sync(0xffffffffu, ke, o));
-        ve = max(ve, __shfl_xor_sync(0xffffffffu, ve, o));
-      }
-      ke = __shfl_sync(0xffffffffu, ke, 0);
-      ve = __shfl_sync(0xffffffffu, ve, 0);
+      for (int u = 0; u < kOwn; ++u) own_id[u] = __shfl_sync(0xffffffffu, id_next, group_of(u));
       v_run = max(v_run, ve);
       ve = max(ve, v_run - 60);                            // smaller ones do not count beside what the unit has seen
-      const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
-      const uint32_t kdst = smem_u32(smem + C::kK + st * C::kOperand), vdst = smem_u32(smem + C::kV + st * C::kOperand);
-      const int id_now = id;
-      const float vsc_now = vsc;
-      // K of this tile; then the next tile's ids, scales and K codes are asked for
+      const uint32_t there = __ballot_sync(0xffffffffu, id_now >= 0);
       mbar_wait_warp(&k_free[st], ph ^ 1, err, 60);
       if (t == 0) info_s[n % kInfo] = {exp2_int(ke), (float)ve, there};
-      convert(kr, ksc, exp2_int(-ke), kdst);
+      convert(kr, ks_now * exp2_int(-ke), smem_u32(smem + C::kK + st * C::kOperand), p.k, p.k_block);
       if (lane == 0) mbar_arrive(&k_full[st]);
-      next();
-      ask(p.k, p.k_block, kr);
-      // V of this tile: its own ids and scales
-      const int id_next = id;
-      id = id_now;
       mbar_wait_warp(&v_free[st], ph ^ 1, err, 61);
-      convert(vr, vsc_now, exp2_int(-ve), vdst);
+      convert(vr, vs_now * exp2_int(-ve), smem_u32(smem + C::kV + st * C::kOperand), p.v, p.v_block);
       if (lane == 0) mbar_arrive(&v_full[st]);
-      id = id_next;
-      ask(p.v, p.v_block, vr);
     }
   } else if (warp >= C::kSoft + 4) {
     fewer_registers<C::kRegsIssue>();
