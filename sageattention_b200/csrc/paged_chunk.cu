@@ -57,6 +57,24 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
+// two fp32 operations an instruction
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  return d;
+}
+
 // Registers of a warpgroup.  The shares add up to what the launch has (512 threads of 128, or 384 of 168).
 template <int N>
 __device__ __forceinline__ void more_registers() {
@@ -151,8 +169,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     const int w = warp - C::kSoft, t = w * 32 + lane;
     // 16-byte pieces of a tile: eight lanes take 64 bytes of two neighbouring keys, whose halves then lie in different banks
     constexpr int kPieces = D / 16;                        // per thread and operand
-    const int in_key = (lane >> 2) & 1, in_chunk = lane & 3, pair = w * 4 + (lane >> 3);
-    auto key_of = [&](int i) { return (i / (D / 64)) * 32 + pair * 2 + in_key; };
+    const int in_key = (lane >> 2) & 1, in_chunk = lane & 3, pair8 = w * 4 + (lane >> 3);
+    auto key_of = [&](int i) { return (i / (D / 64)) * 32 + pair8 * 2 + in_key; };
     auto chunk_of = [&](int i) { return (i % (D / 64)) * 4 + in_chunk; };
     // Codes wait in registers, from the time that their tile's predecessor is converted on.  A load in flight holds a line of
     // L1, of which this kernel's shared memory leaves 28 KB, less than a tile of K and V: piece i of the next tile is asked
@@ -192,15 +210,25 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     // a warp's keys lie in every other 16-key group: block of its u-th one (shuffles share a queue with the stores below)
     constexpr int kOwn = 4, kEach = kPieces / kOwn;
     auto group_of = [&](int u) { return 2 * u + (w >> 1); };
-    int own_id[kOwn];
-    auto ask = [&](const uint8_t* base, int64_t block, int i) -> uint4 {
-      const int key = key_of(i), b = own_id[i / kEach];
-      const int at_key = (key0 + key) & ((1 << p.log_block) - 1);
-      return load_or_zero(base + b * block + (((int64_t)head << p.log_block) + at_key) * D + chunk_of(i) * 16,
-                          b >= 0 && key0 + key < limit);
+    // this thread's first key of each: its codes, and how many keys of the group are there
+    const uint8_t *k_from[kOwn], *v_from[kOwn];
+    int count[kOwn];
+    const int first_key = (pair8 & 7) * 2 + in_key;         // of a group
+    auto find = [&]() {
+#pragma unroll
+      for (int u = 0; u < kOwn; ++u) {
+        const int b = __shfl_sync(0xffffffffu, id_next, group_of(u)), key = key0 + group_of(u) * 16;
+        const int64_t row = (((int64_t)head << p.log_block) + (key & ((1 << p.log_block) - 1)) + first_key) * D + in_chunk * 16;
+        k_from[u] = p.k + b * p.k_block + row;
+        v_from[u] = p.v + b * p.v_block + row;
+        count[u] = b >= 0 ? limit - key : 0;
+      }
+    };
+    auto ask = [&](const uint8_t* const (&from)[kOwn], int i) -> uint4 {
+      return load_or_zero(from[i / kEach] + i % kEach * 64, first_key < count[i / kEach]);
     };
     // pieces to halves times `factor` (lane h: of keys 16 h ..), into a tile in shared memory; then the next tile's are asked for
-    auto convert = [&](uint4 (&r)[kPieces], float factor, uint32_t dst, const uint8_t* base, int64_t block) {
+    auto convert = [&](uint4 (&r)[kPieces], float factor, uint32_t dst, const uint8_t* const (&from)[kOwn]) {
       const bool plain = __all_sync(0xffffffffu, lane >= 8 || id_now < 0 || factor == 1.0f);
       __half2 own[kOwn];
 #pragma unroll
@@ -212,7 +240,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         uint32_t h[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) half4_of_e4m3x4(words[k], h[2 * k], h[2 * k + 1]);
-        r[i] = ask(base, block, i);
+        r[i] = ask(from, i);
         if (!plain) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
@@ -235,12 +263,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     if (left > 0) {
       look_up();
       next();
+      find();
 #pragma unroll
-      for (int u = 0; u < kOwn; ++u) own_id[u] = __shfl_sync(0xffffffffu, id_next, group_of(u));
+      for (int i = 0; i < kPieces; ++i) kr[i] = ask(k_from, i);
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) kr[i] = ask(p.k, p.k_block, i);
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i) vr[i] = ask(p.v, p.v_block, i);
+      for (int i = 0; i < kPieces; ++i) vr[i] = ask(v_from, i);
     }
     int v_run = -200;                                      // largest exponent of the unit's value scales so far
     uint32_t n = 0;
@@ -253,17 +280,16 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       int ke = id_now >= 0 ? scale_exp(ks_now) : -112, ve = id_now >= 0 ? scale_exp(vs_now) : -112;
       ke = __reduce_max_sync(0xffffffffu, lane < 8 ? ke : -112);
       ve = __reduce_max_sync(0xffffffffu, lane < 8 ? ve : -112);
-#pragma unroll
-      for (int u = 0; u < kOwn; ++u) own_id[u] = __shfl_sync(0xffffffffu, id_next, group_of(u));
+      find();
       v_run = max(v_run, ve);
       ve = max(ve, v_run - 60);                            // smaller ones do not count beside what the unit has seen
       const uint32_t there = __ballot_sync(0xffffffffu, id_now >= 0);
       mbar_wait_warp(&k_free[st], ph ^ 1, err, 60);
       if (t == 0) info_s[n % kInfo] = {exp2_int(ke), (float)ve, there};
-      convert(kr, ks_now * exp2_int(-ke), smem_u32(smem + C::kK + st * C::kOperand), p.k, p.k_block);
+      convert(kr, ks_now * exp2_int(-ke), smem_u32(smem + C::kK + st * C::kOperand), k_from);
       if (lane == 0) mbar_arrive(&k_full[st]);
       mbar_wait_warp(&v_free[st], ph ^ 1, err, 61);
-      convert(vr, vs_now * exp2_int(-ve), smem_u32(smem + C::kV + st * C::kOperand), p.v, p.v_block);
+      convert(vr, vs_now * exp2_int(-ve), smem_u32(smem + C::kV + st * C::kOperand), v_from);
       if (lane == 0) mbar_arrive(&v_full[st]);
     }
   } else if (warp >= C::kSoft + 4) {
@@ -447,8 +473,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
           float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            t0 = fmaxf(t0, fmaxf(__uint_as_float(now[e]), __uint_as_float(now[e + 1])));
-            t1 = fmaxf(t1, fmaxf(__uint_as_float(now[e + 2]), __uint_as_float(now[e + 3])));
+            t0 = max3(t0, now[e], now[e + 1]);
+            t1 = max3(t1, now[e + 2], now[e + 3]);
           }
           top = fmaxf(top, fmaxf(t0, t1));
           if (x < kChunks - 1) tmem_ld_wait();
@@ -479,20 +505,26 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
           }
         }
         const float minus = ref == -INFINITY ? 0.0f : info.v_log2 - ref + kLift;
-        float sum0 = 0.0f, sum1 = 0.0f;
+        const uint64_t c2 = pair(__float_as_uint(c), __float_as_uint(c)), minus2 = pair(__float_as_uint(minus), __float_as_uint(minus));
+        uint64_t sum_a = 0, sum_b = 0;
 #pragma unroll
         for (int x = kChunks - 1; x >= 0; --x) {
           uint32_t (&now)[32] = s[x & 1];
           if (x <= kChunks - 3) tmem_ld_wait();
           uint32_t w[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) now[e] = __float_as_uint(fmaf(__uint_as_float(now[e]), c, minus));
+          for (int e = 0; e < 16; ++e) {
+            const uint64_t y = fma_pair(pair(now[2 * e], now[2 * e + 1]), c2, minus2);
+            now[2 * e] = (uint32_t)y;
+            now[2 * e + 1] = (uint32_t)(y >> 32);
+          }
           if (masked) hide(now, x);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float x0 = ex2_approx(__uint_as_float(now[2 * e])), x1 = ex2_approx(__uint_as_float(now[2 * e + 1]));
-            sum0 += x0;
-            sum1 += x1;
+            const uint64_t y = pair(__float_as_uint(x0), __float_as_uint(x1));
+            if (e & 1) sum_b = add_pair(sum_b, y);
+            else sum_a = add_pair(sum_a, y);
             w[e] = pack_16x2<__half>(x0, x1);
           }
           if (x >= 2) tmem_ld32(s_at + (x - 2) * 32, now);
@@ -507,7 +539,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         l *= m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
         m = m_new;
         // the sum is of weights times 2^(v_log2 - ref + lift)
-        l += m == -INFINITY ? sum0 + sum1 : (sum0 + sum1) * ex2_approx(ref - info.v_log2 - kLift - m);
+        sum_a = add_pair(sum_a, sum_b);
+        const float sum = __uint_as_float((uint32_t)sum_a) + __uint_as_float((uint32_t)(sum_a >> 32));
+        l += m == -INFINITY ? sum : sum * ex2_approx(ref - info.v_log2 - kLift - m);
       }
 
       // ---- result of the segment
