@@ -2,17 +2,20 @@
 //
 //   s_j = scaling * (q . k_j),  out = sum_j softmax(s)_j v_j,  k_j = ks_b * code, v_j = vs_b * code (b the block of key j)
 //
-// A unit is (request, KV head, 16 query rows): the heads of a group, for each of the request's query tokens.  Its keys are
-// cut into tiles, all tiles of all units are one list (request by request), and every CTA streams an equal share of it, so
-// ragged lengths need no plan on the host.  HBM bounds it: each code is read once by cp.async into a ring of its warp's own
-// (no barrier in the stream), turned into halves (exact) and multiplied by mma.sync m16n8k16, whose 16 rows are the unit's.
-// At 6.5 TB/s an SM gets 23 bytes a clock; the products of those bytes are 370 of the 1024 multiplications a clock of the
-// legacy tensor path, so tcgen05 would have nothing to give here.
+// A unit's rows are 8 NT at most; every warp of a CTA streams keys of its own (kSub of each tile) through a ring of its own,
+// filled by cp.async, so nothing in the stream waits for another warp.  Codes become halves (exact) on their way from shared
+// memory into mma.sync m16n8k16 with the keys on its 16 rows: S^T = K Q^T and O^T = V^T P^T.  Eight query rows then cost
+// half of what they would on the 16-row side, in products, exponentials and registers.
+//
+// What bounds it: HBM.  At 6.5 TB/s an SM gets 23 bytes a clock; the 8 KB that a warp takes at once (D = 128: 32 keys) are
+// 32 NT products and some 400 instructions of four schedulers, a quarter of the issue slots at NT = 1; tcgen05 would need
+// its 128 rows filled, and what it saves is not what bounds.
 //
 // Precision: q enters as halves scaled by a power of two per row, so that a bf16 or fp16 q is exact unless 2^-26 of its row's
-// maximum (an fp32 q is two halves); scores, maxima, sums and outputs are fp32.  A weight p_j vs_b is a half (two for
-// fp32), relative to the largest weight so far and times 2^14: its rounding is 2^-11 of itself, and of weights below 2^-28 of
-// the largest 2^-39 of that.
+// maximum (an fp32 q is two halves); scores, sums and outputs are fp32, relative to a reference that lags behind the running
+// maximum by 2^kLag at most, so that in most tiles no lane has to know another's maximum.  A weight p_j vs_b is a half (two
+// for fp32), relative to a reference of its own and times 2^kLift: its rounding is 2^-11 of itself, and of weights below
+// 2^-(14 + kLift) of the largest 2^-(25 + kLift) of that.
 #include <limits.h>
 #include "common/abi.cuh"
 #include "common/fp4.cuh"
@@ -24,9 +27,10 @@
 namespace nvfp4 {
 namespace {
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 3;
-constexpr int kRowTile = 16;
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 2;
+constexpr int kCtas = 3;                      // of an SM
 constexpr int kStageBytes = 8192;             // K and V of a warp's keys of a tile
+constexpr float kLag = 5.0f, kLift = 9.0f;
 
 template <int D>
 struct Cfg {
@@ -42,46 +46,55 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
   return v;
 }
+__device__ __forceinline__ float2 lds_f2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ void ldmatrix_x4_t(uint32_t a, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(a)
                : "memory");
 }
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+// 8 x 8 matrix of halves, a row in four lanes: transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x) { return ex2_approx(x); }
-// Key of column i of a product of eight: 0 4 1 5 2 6 3 7.  The rows that one phase of a 16-byte load touches then differ in
-// bit 2, and with the swizzle (chunk ^ row) in their banks.
-__device__ __forceinline__ int key_of_column(int i) { return (i >> 1) | ((i & 1) << 2); }
-
+// Key of row i of eight: 0 4 1 5 2 6 3 7.  The rows that one phase of a 16-byte load touches then differ in bit 2, and with
+// the swizzle (chunk ^ row) in their banks.
+__device__ __forceinline__ int key_of_row(int i) { return (i >> 1) | ((i & 1) << 2); }
 // Exponent of a scale, as log2 of what weights are kept relative to.
 __device__ __forceinline__ float scale_exponent(float s) {
   return fmaxf((float)((int)(__float_as_uint(s) >> 23 & 0xFF) - 127), -112.0f);
 }
 
-template <typename T, int D>
+template <typename T, int D, int NT>
 struct Smem {
   static constexpr bool kTwo = sizeof(T) == 4;             // fp32: q and weights as two halves each
-  static constexpr int kQ = 16 * D * 2 * (kTwo ? 2 : 1);
-  static constexpr int kMerge = kWarps * 8 * 128 * 4;      // eight rows of 128 columns of each warp
-  static constexpr int kShared = kQ > kMerge ? kQ : kMerge;
+  static constexpr int kQ = 8 * NT * D * 2;                // one set of halves
+  static constexpr int kMerge = kWarps * 8 * 64 * 4;       // eight rows of 64 columns of each warp
+  static constexpr int kShared = kQ * (kTwo ? 2 : 1) > kMerge ? kQ * (kTwo ? 2 : 1) : kMerge;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kBytes = kRing + kShared;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(PagedParams p) {
-  using S = Smem<T, D>;
-  constexpr int kSub = Cfg<D>::kSub, kTile = Cfg<D>::kTile;
-  constexpr int kNt = kSub / 8, kHalves = kSub / 16;
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kernel(PagedParams p) {
+  using S = Smem<T, D, NT>;
+  constexpr int kSub = Cfg<D>::kSub, kTile = Cfg<D>::kTile, kRows = 8 * NT;
+  constexpr int kHalves = kSub / 16;                       // 16 keys are the rows of a product
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t list_s[kWarps + 2];
-  __shared__ float q_inv[kRowTile];                        // undoes the power of two that a query row was scaled by
-  __shared__ float m_s[kWarps][kRowTile], l_s[kWarps][kRowTile];
+  __shared__ float q_inv[kRows];                           // undoes the power of two that a query row was scaled by
+  __shared__ float m_s[kWarps][kRows], l_s[kWarps][kRows];
   __shared__ float scale_s[kWarps][kStages][4];            // K and V scales of the stage's two halves
   __shared__ int keys_s[kWarps][kStages][2];               // keys of each half that are there
   const int tid = threadIdx.x, lane = tid & 31, warp = warp_index();
@@ -89,7 +102,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(PagedParams p) 
   griddep_wait();
   griddep_launch();
 
-  using Place = Cursor<kRowTile, kTile>;
+  using Place = Cursor<kRows, kTile>;
   Place use;
   const auto [begin, end, share] = deal_tiles<kThreads>(p, list_s, use);
   if (tid == 0) p.cut[cta] = make_int4(0, 0, 0, 0);
@@ -99,44 +112,51 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(PagedParams p) 
     const uint32_t shared = smem_u32(smem) + S::kRing;
     Place ahead = use;
     int64_t left = end - begin;                            // tiles still to be asked for
+    int ahead_limit = ahead.q.limit(p, ahead.row_tile);
     int id[kHalves];
     auto look_up = [&]() {                                 // blocks of the keys of `ahead`, a tile before they are needed
       const int key = ahead.tile * kTile + warp * kSub;
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const int j = (key + h * 16) >> p.log_block;
-        id[h] = left > 0 && key + h * 16 < ahead.q.len ? p.table[ahead.r * p.table_row + j] : -1;
-      }
+      for (int h = 0; h < kHalves; ++h)
+        id[h] = left > 0 && key + h * 16 < ahead_limit ? p.table[ahead.r * p.table_row + ((key + h * 16) >> p.log_block)] : -1;
+    };
+    // where a lane's 16-byte pieces of 16 keys go: piece i is key (32 i + lane) / (D / 16), and the swizzle has a period of eight keys
+    auto piece = [&](int i) -> uint32_t {
+      const int at = i * 32 + lane, key_in = at / (D / 16), chunk = at % (D / 16);
+      return (uint32_t)(chunk >> 3) * (kSub * 128) + (uint32_t)key_in * 128 + (uint32_t)(((chunk & 7) ^ (key_in & 7)) << 4);
     };
     auto ask = [&](int stage) {
       if (left > 0) {
-        const int key = ahead.tile * kTile + warp * kSub, limit = ahead.q.limit(p, ahead.row_tile);
+        const int key = ahead.tile * kTile + warp * kSub;
         const uint32_t base_s = ring + stage * kStageBytes;
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
           const bool there = (unsigned)id[h] < (unsigned)p.blocks;
-          const int keys = there ? min(max(limit - key - h * 16, 0), 16) : 0;
-          const int64_t b = there ? id[h] : 0;
-          const int64_t row = ((int64_t)ahead.head << p.log_block) + ((key + h * 16) & ((1 << p.log_block) - 1));
-          const uint8_t* pk = p.k + b * p.k_block + row * D;
-          const uint8_t* pv = p.v + b * p.v_block + row * D;
+          const int keys = there ? min(max(ahead_limit - key - h * 16, 0), 16) : 0;
           if (keys > 0) {
+            const int64_t row = ((int64_t)ahead.head << p.log_block) + ((key + h * 16) & ((1 << p.log_block) - 1));
+            const uint8_t* pk = p.k + id[h] * p.k_block + row * D + lane * 16;
+            const uint8_t* pv = p.v + id[h] * p.v_block + row * D + lane * 16;
+            const uint32_t dst = base_s + h * 16 * 128;
+            auto copy = [&](auto bytes) {                  // codes behind the last key: zeros
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-              const int at = i * 32 + lane, key_in = at / (D / 16), chunk = at % (D / 16);
-              const uint32_t dst = (uint32_t)(chunk >> 3) * (kSub * 128) + (uint32_t)(h * 16 + key_in) * 128 +
-                                   (uint32_t)(((chunk & 7) ^ (key_in & 7)) << 4);
-              const uint32_t bytes = key_in < keys ? 16 : 0;           // codes behind the last key: zeros
-              cp_async_16(base_s + dst, pk + at * 16, bytes);
-              cp_async_16(base_s + kStageBytes / 2 + dst, pv + at * 16, bytes);
-            }
+              for (int i = 0; i < D / 32; ++i) {
+                cp_async_16(dst + piece(i), pk + i * 512, bytes(i));
+                cp_async_16(dst + kStageBytes / 2 + piece(i), pv + i * 512, bytes(i));
+              }
+            };
+            if (keys == 16) copy([](int) { return 16u; });
+            else copy([&](int i) { return (i * 32 + lane) / (D / 16) < keys ? 16u : 0u; });
             if (lane < 2)
               cp_async_4(smem_u32(&scale_s[warp][stage][lane * 2 + h]),
-                         lane == 0 ? p.ks + b * p.ks_block + ahead.head : p.vs + b * p.vs_block + ahead.head, 4);
+                         (lane == 0 ? p.ks + id[h] * p.ks_block : p.vs + id[h] * p.vs_block) + ahead.head, 4);
           }
           if (lane == 0) keys_s[warp][stage][h] = keys;
         }
-        if (--left > 0 && ++ahead.tile == ahead.tiles) ahead.next_unit(p);
+        if (--left > 0 && ++ahead.tile == ahead.tiles) {
+          ahead.next_unit(p);
+          ahead_limit = ahead.q.limit(p, ahead.row_tile);
+        }
         look_up();
       }
       cp_async_commit();
@@ -147,7 +167,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(PagedParams p) 
     int stage = 0;
 
     // ---- segments: the tiles of one unit in this share
-    const int g8 = lane >> 2, c4 = lane & 3;
+    const int g8 = lane >> 2, c4 = lane & 3;               // row (key, or pair of the head dim) and pair of query rows of a product
+    const int krow = key_of_row(g8);
     int64_t at = begin;
     bool first = true;
     while (at < end) {
@@ -155,10 +176,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(PagedParams p) 
       const int tiles = (int)min((int64_t)(use.tiles - use.tile), end - at);
       const bool whole = use.tile == 0 && tiles == use.tiles;
 
-      // query rows as fragments of the products: row tid / 8, elements 16 e .. 16 e + 15 for e = tid % 8 (+ 8)
-      {
-        const int row = tid >> 3, e0 = tid & 7;
-        const int i = use.row_tile * kRowTile + row;
+      // query rows as fragments of the products: eight threads a row, elements 16 e .. 16 e + 15 for e = tid % 8 (+ 8)
+#pragma unroll 1
+      for (int row = tid >> 3; row < kRows; row += kThreads / 8) {
+        const int e0 = tid & 7;
+        const int i = use.row_tile * kRows + row;
         const T* pq = static_cast<const T*>(p.q) + (int64_t)(use.q.t0 + i / p.g) * p.sqt +
                       (int64_t)(use.head * p.g + i % p.g) * p.sqh;
         float x[D / 128][16];
@@ -171,51 +193,64 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(PagedParams p) 
             big = fmaxf(big, fabsf(x[u][k]));
           }
         }
+        const uint32_t eight = 0xFFu << (lane & 24);
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-        // largest element in [2^12, 2^13)
+        for (int o = 1; o < 8; o <<= 1) big = fmaxf(big, __shfl_xor_sync(eight, big, o));
+        // largest element in [2^12, 2^13); scaling below zero turns q
         const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -110), 127);
-        const float up = __uint_as_float((uint32_t)(127 + 12 - ex) << 23);
-        if (e0 == 0) q_inv[row] = big == 0.0f ? 0.0f : ldexpf(1.0f, ex - 12);
-        const uint32_t dst = shared + ((row & 7) * 4) * 16 + (row >> 3) * 4;
+        const float up = copysignf(__uint_as_float((uint32_t)(127 + 12 - ex) << 23), p.scale_log2);
+        if (e0 == 0) q_inv[row] = big == 0.0f ? 0.0f : ldexpf(fabsf(p.scale_log2), ex - 12);
+        // products of 16 elements: lane (row % 8) * 4 + e % 4 has elements 4 k .. 4 k + 3 of its 16; two products' words together
+        const uint32_t dst = shared + (row >> 3) * 512;
 #pragma unroll
         for (int u = 0; u < D / 128; ++u) {
-          const int e = u * 8 + e0;                        // 64 elements are four products; e % 4 is the lane of a group
+          const int e = u * 8 + e0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t a = dst + (((e >> 2) * 4 + k) * 32 + (e & 3)) * 16;
+            const uint32_t a = dst + (((e >> 2) * 2 + (k >> 1)) * NT) * 512 + ((row & 7) * 4 + (e & 3)) * 16 + (k & 1) * 8;
             float lo[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) lo[j] = x[u][4 * k + j] * up;
             const uint32_t w0 = pack_16x2<__half>(lo[0], lo[1]), w1 = pack_16x2<__half>(lo[2], lo[3]);
-            sts_b32(a, w0);
-            sts_b32(a + 8, w1);
+            sts_v2(a, w0, w1);
             if constexpr (S::kTwo) {
               const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&w0));
               const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&w1));
-              sts_b32(a + 16 * D * 2, pack_16x2<__half>(lo[0] - f0.x, lo[1] - f0.y));
-              sts_b32(a + 16 * D * 2 + 8, pack_16x2<__half>(lo[2] - f1.x, lo[3] - f1.y));
+              sts_v2(a + S::kQ, pack_16x2<__half>(lo[0] - f0.x, lo[1] - f0.y), pack_16x2<__half>(lo[2] - f1.x, lo[3] - f1.y));
             }
           }
         }
       }
       __syncthreads();
-      const float inv0 = q_inv[g8] * p.scale_log2, inv1 = q_inv[g8 + 8] * p.scale_log2;
-      // keys that this thread's two rows see; rows of no query see all (they are not stored)
-      auto limit_of = [&](int row) {
-        return row < rows ? use.q.seen(p, use.row_tile * kRowTile + row) : INT_MAX;
-      };
-      const int lim0 = limit_of(g8), lim1 = limit_of(g8 + 8);
-      const int lim_first = use.q.seen(p, use.row_tile * kRowTile);    // the smallest of all rows
+      // this thread's query rows: 8 nt + 2 c4, + 1.  Rows of no query see all keys (they are not stored).
+      float inv[NT][2];
+      int lim[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int row = nt * 8 + 2 * c4 + k;
+          inv[nt][k] = q_inv[row];
+          lim[nt][k] = row < rows ? use.q.seen(p, use.row_tile * kRows + row) : INT_MAX;
+        }
+      const int lim_first = use.q.seen(p, use.row_tile * kRows);       // the smallest of all rows
 
-      float o[D / 16][2][4];
+      float o[D / 16][NT][4];
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[i][j][k] = 0.0f;
-      float m[2] = {-INFINITY, -INFINITY}, mw[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+          for (int k = 0; k < 4; ++k) o[i][nt][k] = 0.0f;
+      // references of the scores and of the weights, 2^(their difference + kLift), sum
+      float ref[NT][2], ref_w[NT][2], lift[NT][2], l[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          ref[nt][k] = ref_w[nt][k] = -INFINITY;
+          lift[nt][k] = l[nt][k] = 0.0f;
+        }
 
       for (int tile = use.tile; tile < use.tile + tiles; ++tile) {
         ask(stage == 0 ? kStages - 1 : stage - 1);
@@ -233,119 +268,136 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(PagedParams p) 
           any |= keys[h];
         }
         if (any != 0) {
-          float kscale[kHalves], vscale[kHalves];
+          float kscale[kHalves], vscale[kHalves], vexp[kHalves];
 #pragma unroll
           for (int h = 0; h < kHalves; ++h) {
             kscale[h] = keys[h] ? scale_s[warp][stage][h] : 0.0f;
             vscale[h] = keys[h] ? scale_s[warp][stage][2 + h] : 0.0f;
+            vexp[h] = scale_exponent(vscale[h]);
           }
-          float s[kNt][4];
+          float s[kHalves][NT][4];
 #pragma unroll
-          for (int nt = 0; nt < kNt; ++nt)
+          for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[nt][k] = 0.0f;
-          const int krow = key_of_column(g8);
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) s[h][nt][k] = 0.0f;
 #pragma unroll
           for (int e = 0; e < D / 64; ++e) {
-            uint4 a[4], a2[4];
+            // rows of a missing half may be stale codes: masked below
+            uint4 lo[kHalves], hi[kHalves];                // keys g8 and g8 + 8 of a half, 16 elements of each
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              a[k] = lds128(shared + ((e * 4 + k) * 32 + lane) * 16);
-              if constexpr (S::kTwo) a2[k] = lds128(shared + 16 * D * 2 + ((e * 4 + k) * 32 + lane) * 16);
+            for (int h = 0; h < kHalves; ++h) {
+              const uint32_t a = base_s + (e >> 1) * (kSub * 128) + (h * 16 + krow) * 128 + ((((e & 1) * 4 + c4) ^ krow) << 4);
+              lo[h] = lds128(a);
+              hi[h] = lds128(a + 8 * 128);
             }
 #pragma unroll
-            for (int nt = 0; nt < kNt; ++nt) {
-              // half a stage's keys may be stale where a block is missing: they are masked below
-              const uint4 b = lds128(base_s + (e >> 1) * (kSub * 128) + (nt * 8 + krow) * 128 +
-                                     ((((e & 1) * 4 + c4) ^ krow) << 4));
-              const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+            for (int k2 = 0; k2 < 2; ++k2) {
+              uint4 b[NT], b2[NT];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                uint32_t b0, b1;
-                half4_of_e4m3x4(w[k], b0, b1);
-                mma_16816(s[nt], a[k], b0, b1);
-                if constexpr (S::kTwo) mma_16816(s[nt], a2[k], b0, b1);
+              for (int nt = 0; nt < NT; ++nt) {
+                b[nt] = lds128(shared + ((e * 2 + k2) * NT + nt) * 512 + lane * 16);
+                if constexpr (S::kTwo) b2[nt] = lds128(shared + S::kQ + ((e * 2 + k2) * NT + nt) * 512 + lane * 16);
               }
-            }
-          }
-          float big[2] = {-INFINITY, -INFINITY};
-          const bool masks = !all || key + kSub > lim_first;
 #pragma unroll
-          for (int nt = 0; nt < kNt; ++nt) {
-            const int h = nt >> 1;
-            s[nt][0] *= inv0 * kscale[h];
-            s[nt][1] *= inv0 * kscale[h];
-            s[nt][2] *= inv1 * kscale[h];
-            s[nt][3] *= inv1 * kscale[h];
-            if (masks) {
+              for (int h = 0; h < kHalves; ++h) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int in = (nt & 1) * 8 + c4 + (k & 1) * 4;          // key within its half
-                if (in >= keys[h] || key + h * 16 + in >= (k < 2 ? lim0 : lim1)) s[nt][k] = -INFINITY;
-              }
-            }
-            big[0] = fmaxf(big[0], fmaxf(s[nt][0], s[nt][1]));
-            big[1] = fmaxf(big[1], fmaxf(s[nt][2], s[nt][3]));
-          }
+                for (int k = 0; k < 2; ++k) {
+                  uint32_t a[4];
+                  half4_of_e4m3x4(k2 == 0 ? (k == 0 ? lo[h].x : lo[h].y) : (k == 0 ? lo[h].z : lo[h].w), a[0], a[2]);
+                  half4_of_e4m3x4(k2 == 0 ? (k == 0 ? hi[h].x : hi[h].y) : (k == 0 ? hi[h].z : hi[h].w), a[1], a[3]);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], 1));
-            big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], 2));
-          }
-          float vexp = -112.0f;
-#pragma unroll
-          for (int h = 0; h < kHalves; ++h) vexp = keys[h] ? fmaxf(vexp, scale_exponent(vscale[h])) : vexp;
-          float m_new[2], shrink_o[2], c[2][kHalves];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            m_new[i] = fmaxf(m[i], big[i]);
-            const float w_new = fmaxf(mw[i], big[i] + vexp);
-            const bool none = m_new[i] == -INFINITY;
-            const float ref = none ? 0.0f : m_new[i];
-            l[i] *= ex2(m[i] - ref);
-            shrink_o[i] = none ? 1.0f : ex2(mw[i] - w_new);
-            const float f = none ? 0.0f : ex2(fminf(ref - w_new + 14.0f, 126.0f));
-#pragma unroll
-            for (int h = 0; h < kHalves; ++h) c[i][h] = f * vscale[h];
-            m[i] = m_new[i];
-            mw[i] = w_new;
-            m_new[i] = ref;
-          }
-          if (__any_sync(0xffffffffu, shrink_o[0] != 1.0f || shrink_o[1] != 1.0f)) {
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                o[i][j][0] *= shrink_o[0];
-                o[i][j][1] *= shrink_o[0];
-                o[i][j][2] *= shrink_o[1];
-                o[i][j][3] *= shrink_o[1];
-              }
-          }
-          uint4 pw[kHalves], pw2[kHalves];
-#pragma unroll
-          for (int h = 0; h < kHalves; ++h) {
-            uint32_t w[4], w2[4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                const float p0 = ex2(s[2 * h + n][2 * i] - m_new[i]), p1 = ex2(s[2 * h + n][2 * i + 1] - m_new[i]);
-                l[i] += p0 + p1;
-                const float x0 = p0 * c[i][h], x1 = p1 * c[i][h];
-                w[n * 2 + i] = pack_16x2<__half>(x0, x1);
-                if constexpr (S::kTwo) {
-                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[n * 2 + i]));
-                  w2[n * 2 + i] = pack_16x2<__half>(x0 - f.x, x1 - f.y);
+                  for (int nt = 0; nt < NT; ++nt) {
+                    mma_16816(s[h][nt], a, k == 0 ? b[nt].x : b[nt].z, k == 0 ? b[nt].y : b[nt].w);
+                    if constexpr (S::kTwo) mma_16816(s[h][nt], a, k == 0 ? b2[nt].x : b2[nt].z, k == 0 ? b2[nt].y : b2[nt].w);
+                  }
                 }
               }
-            pw[h] = make_uint4(w[0], w[1], w[2], w[3]);
-            if constexpr (S::kTwo) pw2[h] = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+            }
+          }
+          // scores in units of log2; element k of a product: key g8 + 8 (k / 2), row 2 c4 + k % 2
+          const bool masks = !all || key + kSub > lim_first;
+          float top[NT][2], top_w[NT][2];                  // largest of this thread's keys, and of them with their V scale
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) top[nt][k] = top_w[nt][k] = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float f = inv[nt][k] * kscale[h];
+                s[h][nt][k] *= f;
+                s[h][nt][2 + k] *= f;
+                if (masks) {
+                  if (krow >= keys[h] || key + h * 16 + krow >= lim[nt][k]) s[h][nt][k] = -INFINITY;
+                  if (krow + 8 >= keys[h] || key + h * 16 + krow + 8 >= lim[nt][k]) s[h][nt][2 + k] = -INFINITY;
+                }
+                const float t = fmaxf(s[h][nt][k], s[h][nt][2 + k]);
+                top[nt][k] = fmaxf(top[nt][k], t);
+                top_w[nt][k] = fmaxf(top_w[nt][k], t + vexp[h]);
+              }
+          bool move = false;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) move = move || top[nt][k] > ref[nt][k] + kLag || top_w[nt][k] > ref_w[nt][k] + kLag;
+          if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                float m = top[nt][k], w = top_w[nt][k];
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) {
+                  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+                  w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, x));
+                }
+                m = fmaxf(m, ref[nt][k]);
+                w = fmaxf(w, ref_w[nt][k]);
+                if (m != -INFINITY) {
+                  l[nt][k] *= ex2_approx(ref[nt][k] - m);
+                  const float f = ex2_approx(ref_w[nt][k] - w);
+#pragma unroll
+                  for (int i = 0; i < D / 16; ++i) {
+                    o[i][nt][k] *= f;
+                    o[i][nt][2 + k] *= f;
+                  }
+                  lift[nt][k] = ex2_approx(fminf(m - w + kLift, 126.0f));
+                }
+                ref[nt][k] = m;
+                ref_w[nt][k] = w;
+              }
           }
 #pragma unroll
           for (int h = 0; h < kHalves; ++h) {
+            uint32_t pb[NT][2], pb2[NT][2];                // weights as the other operand: eight keys a word
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float w[4];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float r = ref[nt][k] == -INFINITY ? 0.0f : ref[nt][k], c = lift[nt][k] * vscale[h];
+                const float p0 = ex2_approx(s[h][nt][k] - r), p1 = ex2_approx(s[h][nt][2 + k] - r);
+                l[nt][k] += p0 + p1;
+                w[k] = p0 * c;
+                w[2 + k] = p1 * c;
+              }
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const uint32_t v = pack_16x2<__half>(w[2 * y], w[2 * y + 1]);
+                pb[nt][y] = transposed(v);
+                if constexpr (S::kTwo) {
+                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+                  pb2[nt][y] = transposed(pack_16x2<__half>(w[2 * y] - f.x, w[2 * y + 1] - f.y));
+                }
+              }
+            }
             if (keys[h] == 0) continue;                    // nothing was copied: stale codes may be NaN
-            const int vrow = h * 16 + ((lane >> 3) & 1) * 8 + key_of_column(lane & 7);
+            const int vrow = h * 16 + ((lane >> 3) & 1) * 8 + key_of_row(lane & 7);
 #pragma unroll
             for (int dg = 0; dg < D / 32; ++dg) {
               const int chunk = dg * 2 + (lane >> 4);
@@ -355,15 +407,14 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(PagedParams p) 
                             r);
 #pragma unroll
               for (int ch = 0; ch < 2; ++ch) {
-                // bytes (d, d + 1) of two keys -> the keys of d, the keys of d + 1
-                uint32_t e0, o0, e1, o1;
-                half4_of_e4m3x4(__byte_perm(r[2 * ch], 0, 0x3120), e0, o0);
-                half4_of_e4m3x4(__byte_perm(r[2 * ch + 1], 0, 0x3120), e1, o1);
-                mma_16816(o[dg * 2 + ch][0], pw[h], e0, e1);
-                mma_16816(o[dg * 2 + ch][1], pw[h], o0, o1);
-                if constexpr (S::kTwo) {
-                  mma_16816(o[dg * 2 + ch][0], pw2[h], e0, e1);
-                  mma_16816(o[dg * 2 + ch][1], pw2[h], o0, o1);
+                // bytes (d, d + 1) of two keys -> the keys of d (row g8 of the product), the keys of d + 1 (row g8 + 8)
+                uint32_t a[4];
+                half4_of_e4m3x4(__byte_perm(r[2 * ch], 0, 0x3120), a[0], a[1]);
+                half4_of_e4m3x4(__byte_perm(r[2 * ch + 1], 0, 0x3120), a[2], a[3]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  mma_16816(o[dg * 2 + ch][nt], a, pb[nt][0], pb[nt][1]);
+                  if constexpr (S::kTwo) mma_16816(o[dg * 2 + ch][nt], a, pb2[nt][0], pb2[nt][1]);
                 }
               }
             }
@@ -375,74 +426,73 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(PagedParams p) 
 
       // ---- merge of the four warps, in warp order: final rows, or a partial result of the unit
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        if (c4 == 0) {
-          m_s[warp][g8 + 8 * i] = m[i];
-          l_s[warp][g8 + 8 * i] = l[i];
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) l[nt][k] += __shfl_xor_sync(0xffffffffu, l[nt][k], x);
+          if (g8 == 0) {
+            m_s[warp][nt * 8 + 2 * c4 + k] = ref[nt][k];
+            l_s[warp][nt * 8 + 2 * c4 + k] = l[nt][k];
+          }
         }
-      }
       __syncthreads();                                     // and nobody needs the query fragments any more
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = g8 + 8 * i;
-        float top = m_s[0][row];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][row]);
-        // weights carry 2^(14 - mw); brought to 2^-top
-        const float f = mw[i] == -INFINITY ? 0.0f : ex2(mw[i] - top) * 0x1p-14f;
+        for (int k = 0; k < 2; ++k) {
+          float top = m_s[0][nt * 8 + 2 * c4 + k];
 #pragma unroll
-        for (int a = 0; a < D / 16; ++a)
+          for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][nt * 8 + 2 * c4 + k]);
+          // weights carry 2^(kLift - ref_w); brought to 2^-top
+          const float f = ref_w[nt][k] == -INFINITY ? 0.0f : ex2_approx(ref_w[nt][k] - top - kLift);
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            o[a][b][2 * i] *= f;
-            o[a][b][2 * i + 1] *= f;
+          for (int i = 0; i < D / 16; ++i) {
+            o[i][nt][k] *= f;
+            o[i][nt][2 + k] *= f;
           }
-      }
+        }
       const int slot = first ? 2 * cta : 2 * cta + 1;
 #pragma unroll
-      for (int pass = 0; pass < 2 * (D / 128); ++pass) {
-        const int half = pass % 2, cols = pass / 2;        // rows 8 half .., columns 128 cols ..
-        if (half * 8 < rows) {
+      for (int pass = 0; pass < NT * (D / 64); ++pass) {
+        const int nt = pass % NT, cols = pass / NT;        // rows 8 nt .., columns 64 cols ..
+        if (nt * 8 < rows) {
 #pragma unroll
-          for (int a = 0; a < 8; ++a) {
-            const float* x0 = o[cols * 8 + a][0] + 2 * half;
-            const float* x1 = o[cols * 8 + a][1] + 2 * half;
-            const uint32_t dst = shared + ((warp * 8 + g8) * 128 + ((a ^ (g8 & 1)) * 16) + 4 * c4) * 4;
-            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(x0[0]), "f"(x1[0]), "f"(x0[1]), "f"(x1[1])
-                         : "memory");
-          }
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float* x = o[cols * 4 + i][nt];
+              const uint32_t dst = shared + ((warp * 8 + 2 * c4 + k) * 64 + ((i ^ c4) * 16) + 2 * g8) * 4;
+              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(dst), "f"(x[k]), "f"(x[2 + k]) : "memory");
+            }
           __syncthreads();
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const int in = warp * 2 + y, row = half * 8 + in;
+            const int in = warp * 2 + y, row = nt * 8 + in;
             if (row < rows) {
-              float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, top = m_s[0][row], total_l = 0.0f;
+              float2 sum = make_float2(0.0f, 0.0f);
+              float top = m_s[0][row], total_l = 0.0f;
 #pragma unroll
               for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][row]);
 #pragma unroll
               for (int w = 0; w < kWarps; ++w) {
-                const uint4 v = lds128(shared + ((w * 8 + in) * 128 + (((lane >> 2) ^ (in & 1)) * 16) + 4 * (lane & 3)) * 4);
-                sum[0] += __uint_as_float(v.x);
-                sum[1] += __uint_as_float(v.y);
-                sum[2] += __uint_as_float(v.z);
-                sum[3] += __uint_as_float(v.w);
-                total_l += top == -INFINITY ? l_s[w][row] : l_s[w][row] * ex2(m_s[w][row] - top);   // no key: 0, or NaN
+                const float2 v = lds_f2(shared + ((w * 8 + in) * 64 + (((lane >> 3) ^ (in >> 1)) * 16) + 2 * (lane & 7)) * 4);
+                sum.x += v.x;
+                sum.y += v.y;
+                total_l += top == -INFINITY ? l_s[w][row] : l_s[w][row] * ex2_approx(m_s[w][row] - top);   // no key: 0, or NaN
               }
               if (whole) {
-                const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
-                const int64_t to = out_row(p, (int64_t)use.q.t0 * p.g + use.row_tile * kRowTile + row, use.head);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) sum[k] *= inv;
-                store4<T>(static_cast<T*>(p.out) + to * D + cols * 128 + lane * 4, sum);
-                if (cols == 0 && lane == 0 && p.lse != nullptr)
-                  p.lse[to] = lse_of(top, total_l);
+                const float f = total_l == 0.0f ? 0.0f : 1.0f / total_l;
+                const int64_t to = out_row(p, (int64_t)use.q.t0 * p.g + use.row_tile * kRows + row, use.head);
+                T* dst = static_cast<T*>(p.out) + to * D + cols * 64 + lane * 2;
+                if constexpr (S::kTwo) *reinterpret_cast<float2*>(dst) = make_float2(sum.x * f, sum.y * f);
+                else *reinterpret_cast<uint32_t*>(dst) = pack_16x2<T>(sum.x * f, sum.y * f);
+                if (cols == 0 && lane == 0 && p.lse != nullptr) p.lse[to] = lse_of(top, total_l);
               } else {
-                store4<float>(p.ws_acc + ((int64_t)slot * kRowTile + row) * D + cols * 128 + lane * 4, sum);
+                *reinterpret_cast<float2*>(p.ws_acc + ((int64_t)slot * kRows + row) * D + cols * 64 + lane * 2) = sum;
                 if (cols == 0 && lane == 0) {
-                  p.ws_m[slot * kRowTile + row] = top;
-                  p.ws_l[slot * kRowTile + row] = total_l;
+                  p.ws_m[slot * kRows + row] = top;
+                  p.ws_l[slot * kRows + row] = total_l;
                 }
               }
             }
@@ -450,31 +500,45 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(PagedParams p) 
           __syncthreads();
         }
       }
-      if (!whole && use.tile == 0 && tid == 0) {
-        // begun here, finished by the CTAs behind this one
-        p.cut[cta] = cut_unit(p, use, tiles, share, first);
-      }
+      // begun here, finished by the CTAs behind this one
+      if (!whole && use.tile == 0 && tid == 0) p.cut[cta] = cut_unit(p, use, tiles, share, first);
       at += tiles;
       first = false;
       if (at < end) use.next_unit(p);
     }
   }
-  clear_untouched<T, D, kRowTile, kTile>(p);
+  clear_untouched<T, D, kRows, kTile>(p);
 }
 
+template <typename T, int D, int NT>
+int run_attention(const PagedParams& p, int sms, cudaStream_t st) {
+  using S = Smem<T, D, NT>;
+  const int grid = (NT == 1 ? kCtas : 2) * sms;
+  if (int rc = allow_smem("nvfp4_kv8_attention", reinterpret_cast<const void*>(paged_attn_kernel<T, D, NT>), S::kBytes)) return rc;
+  if (int rc = launch("nvfp4_kv8_attention", paged_attn_kernel<T, D, NT>, dim3(grid), kThreads, S::kBytes, st, p)) return rc;
+  return launch_combine<T, D, 8 * NT>(p, grid, st);
+}
+
+// Which kernel, by query rows a request on average (their numbers are on the device): eight, sixteen or (D = 128) 24 rows of
+// this file's, rounded up; above them the one whose tensor-memory products take 128 or 256 rows at a time.  fp32
+// queries, whose products need two halves, stay here, sixteen rows at a time.
+struct Choice {
+  bool chunk;
+  int nt, ctas;
+  int64_t rows;
+};
+Choice choose(int q_dtype, int64_t tokens, int64_t requests, int64_t g, int d, int sms) {
+  const int64_t rows = (tokens * g + requests - 1) / requests, most = d == 128 ? 24 : 16;
+  if (q_dtype != NVFP4_DT_FP32 && rows > most) return {true, 0, sms, paged_chunk_rows(d)};
+  const int nt = rows <= 8 ? 1 : rows <= 16 || q_dtype == NVFP4_DT_FP32 ? 2 : 3;
+  return {false, nt, (nt == 1 ? kCtas : 2) * sms, 8 * nt};
+}
 template <typename T, int D>
-int run_attention(const PagedParams& p, int grid, cudaStream_t st) {
-  using S = Smem<T, D>;
-  if (int rc = allow_smem("nvfp4_kv8_attention", reinterpret_cast<const void*>(paged_attn_kernel<T, D>), S::kBytes)) return rc;
-  if (int rc = launch("nvfp4_kv8_attention", paged_attn_kernel<T, D>, dim3(grid), kThreads, S::kBytes, st, p)) return rc;
-  return launch_combine<T, D, kRowTile>(p, grid, st);
-}
-
-// Which kernel: tensor-memory products take 128 or 256 rows at a time and are worth it from kChunkRows query rows a request
-// on, on average (the lengths themselves are on the device); fp32 queries, whose products need two halves, stay here.
-constexpr int kChunkRows = 32;
-bool takes_chunk_kernel(int q_dtype, int64_t tokens, int64_t requests, int64_t g) {
-  return q_dtype != NVFP4_DT_FP32 && tokens * g > kChunkRows * requests;
+int run_rows(const PagedParams& p, int nt, int sms, cudaStream_t st) {
+  if (nt == 1) return run_attention<T, D, 1>(p, sms, st);
+  if constexpr (D == 128 && sizeof(T) == 2)
+    if (nt == 3) return run_attention<T, D, 3>(p, sms, st);
+  return run_attention<T, D, 2>(p, sms, st);
 }
 
 }  // namespace
@@ -487,8 +551,8 @@ extern "C" int nvfp4_kv8_attention_plan(int q_dtype, int64_t tokens, int64_t req
   NVFP4_REQUIRE(d == 128 || d == 256, "nvfp4_kv8_attention_plan: D must be 128 or 256");
   NVFP4_REQUIRE(tokens >= 0 && requests >= 1 && g >= 1 && sm_count >= 1 && workspace_bytes != nullptr,
                 "nvfp4_kv8_attention_plan: bad argument");
-  *workspace_bytes = (size_t)(takes_chunk_kernel(q_dtype, tokens, requests, g) ? sm_count * paged_slot_bytes(paged_chunk_rows(d), d)
-                                                                               : 2 * sm_count * paged_slot_bytes(kRowTile, d));
+  const Choice c = choose(q_dtype, tokens, requests, g, d, sm_count);
+  *workspace_bytes = (size_t)(c.ctas * paged_slot_bytes(c.rows, d));
   return 0;
 }
 
@@ -513,9 +577,9 @@ extern "C" int nvfp4_kv8_attention(const void* q, int q_dtype, int64_t s_qt, int
   if (tokens == 0) return 0;
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const bool chunk = takes_chunk_kernel(q_dtype, tokens, requests, g);
-  const int grid = chunk ? sms : 2 * sms;
-  const int64_t rows = chunk ? paged_chunk_rows(d) : kRowTile;
+  const Choice c = choose(q_dtype, tokens, requests, g, d, sms);
+  const int grid = c.ctas;
+  const int64_t rows = c.rows;
   NVFP4_REQUIRE(workspace_bytes >= (size_t)(grid * paged_slot_bytes(rows, d)), "nvfp4_kv8_attention: workspace too small");
   NVFP4_REQUIRE(q_dtype >= NVFP4_DT_BF16 && q_dtype <= NVFP4_DT_FP32, "nvfp4_kv8_attention: unknown dtype %d", q_dtype);
   PagedParams p{q, s_qt, s_qh, cu_seqlens, tokens, k_cache, v_cache, k_block, v_block, k_scale, v_scale, ks_block, vs_block, table,
@@ -526,10 +590,10 @@ extern "C" int nvfp4_kv8_attention(const void* q, int q_dtype, int64_t s_qt, int
   p.ws_m = reinterpret_cast<float*>(p.cut + grid);
   p.ws_l = p.ws_m + 2 * grid * rows;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (chunk) return launch_paged_chunk(p, q_dtype, d, grid, st);
+  if (c.chunk) return launch_paged_chunk(p, q_dtype, d, grid, st);
   switch (q_dtype) {
-    case NVFP4_DT_BF16: return d == 128 ? run_attention<__nv_bfloat16, 128>(p, grid, st) : run_attention<__nv_bfloat16, 256>(p, grid, st);
-    case NVFP4_DT_FP16: return d == 128 ? run_attention<__half, 128>(p, grid, st) : run_attention<__half, 256>(p, grid, st);
-    default: return d == 128 ? run_attention<float, 128>(p, grid, st) : run_attention<float, 256>(p, grid, st);
+    case NVFP4_DT_BF16: return d == 128 ? run_rows<__nv_bfloat16, 128>(p, c.nt, sms, st) : run_rows<__nv_bfloat16, 256>(p, c.nt, sms, st);
+    case NVFP4_DT_FP16: return d == 128 ? run_rows<__half, 128>(p, c.nt, sms, st) : run_rows<__half, 256>(p, c.nt, sms, st);
+    default: return d == 128 ? run_rows<float, 128>(p, c.nt, sms, st) : run_rows<float, 256>(p, c.nt, sms, st);
   }
 }

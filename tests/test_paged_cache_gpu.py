@@ -218,6 +218,11 @@ def _spoil(codes, scale, table, lengths, block):
     scale[~used.any(1)] = math.nan
 
 
+def _chunk(dtype, d, tokens, g, requests):
+    """Whether a call takes the kernel for many rows."""
+    return dtype != torch.float32 and -(-tokens * g // requests) > (24 if d == 128 else 16)
+
+
 def _key_scales(scale, row, length, block):
     """[Hk, length]: the scale of every key's block."""
     return R.gather(torch.ones(scale.shape[0], scale.shape[1], block, 1), scale, row, length, block)[..., 0]
@@ -227,8 +232,8 @@ def _close(got, lse, q, k, v, vscale, limits, scaling, g, hidden=None, chunk=Fal
     """Rows of one request.  With A = sum p |v|, S = scaling * sum |q| |k|: scores are off by delta = S (D + 8) 2^-23 (products
     of exact halves summed in fp32; an fp32 q is two halves, 2^-22), a weight by its rounding to halves (2^-11, as two
     2^-22), exp2 and the sums by (keys + 8) 2^-23; the result is rounded once.  Halves end at 2^-24: a weight p vs is held times
-    2^14 / W, W = the largest p of 32 keys times their largest vs (what a warp's products of a tile are relative to), so its
-    rounding is at least 2^-39 W, and with codes of at most 448 a value is off by 2^-39 W 448 keys: all that is left of it
+    2^9 / W, W = the largest p of 32 keys times their largest vs (at least what a warp's weights are relative to), so its
+    rounding is at least 2^-34 W, and with codes of at most 448 a value is off by 2^-34 W 448 keys: all that is left of it
     where the code of the one key that counts is 0.  Calls of many rows (`chunk`) take 128 keys at once and hold weights times 2^3:
     2^-28; and K and V of a block as halves relative to the largest scale of the 128 keys, which below 2^-14 of it are off by
     2^-25 of it: in a score scaling * sum |q| 2^-25 of the largest K scale, in the result 2^-25 sum p of the largest V scale."""
@@ -256,7 +261,7 @@ def _close(got, lse, q, k, v, vscale, limits, scaling, g, hidden=None, chunk=Fal
         pad = -p.shape[2] % keys
         groups = lambda x: torch.nn.functional.pad(x, (0, pad)).unflatten(-1, (-1, keys)).amax(-1)
         w = (groups(p) * groups(vscale.double()).repeat_interleave(g, 0)).amax(2)
-        tol = tol + (2.0 ** (-28 if chunk else -39) * 448 * k.shape[1] * w)[..., None]
+        tol = tol + (2.0 ** (-28 if chunk else -34) * 448 * k.shape[1] * w)[..., None]
         if chunk:
             top_k = qd.abs().sum(2) * scaling * 2.0 ** -25 * float(k.abs().max())     # every block here has codes above 1
             delta = delta + top_k
@@ -288,7 +293,7 @@ def _decode_case(lengths, h, hk, d, block, dtype, seed=0, spread=2.0, spoil=True
     for r, n in enumerate(lengths):
         kk, vv = R.gather(k, ks, table[r], n, block), R.gather(v, vs, table[r], n, block)
         _close(out[r].transpose(0, 1), lse[r:r + 1], q[r].transpose(0, 1), kk, vv, _key_scales(vs, table[r], n, block), [n], scaling, h // hk,
-               chunk=h // hk > 32 and dtype != torch.float32)
+               chunk=_chunk(dtype, d, 1, h // hk, 1))
     return out, lse
 
 
@@ -383,7 +388,7 @@ def _attend_case(new, held, h, hk, d, block, dtype, seed=0, behind=0, spoil=True
             a, b = starts[r], starts[r + 1]
             kk, vv = R.gather(k, ks, table[r], total[r], block), R.gather(v, vs, table[r], total[r], block)
             _close(out[a:b], lse[a:b], q[a:b], kk, vv, _key_scales(vs, table[r], total[r], block), [held[r] + 1 + i for i in range(n)],
-                   scaling, h // hk, chunk=dtype != torch.float32 and tokens * (h // hk) > 32 * len(new))
+                   scaling, h // hk, chunk=_chunk(dtype, d, tokens, h // hk, len(new)))
     assert bool((out[starts[-1]:] == 0).all()) and bool((lse[starts[-1]:] == -math.inf).all())
     return out
 
@@ -484,7 +489,7 @@ def _server(dtype, capture):
                     kk, vv = (R.gather(*ref[2 * layer + i], table[r], lengths[r], block) for i in (0, 1))
                     _close(out[layer][0][at:at + n], out[layer][1][at:at + n], query[at:at + n], kk, vv,
                            _key_scales(ref[2 * layer + 1][1], table[r], lengths[r], block), [lengths[r] - n + 1 + i for i in range(n)],
-                           d ** -0.5, h // hk, chunk=sum(new) * h // hk > 32 * rows)
+                           d ** -0.5, h // hk, chunk=_chunk(dtype, d, query.shape[0], h // hk, rows))
                     at += n
 
     def inputs_of(n):
