@@ -3,7 +3,9 @@
 //
 // A unit is (request, KV head, ROWS query rows): the heads of a group, for each of the request's query tokens.  Its keys, as
 // far as its last row sees them, are cut into tiles of TILE; all tiles of all units are one list (request, head, rows, keys),
-// and CTA c takes tiles [c, c + 1) * ceil(total / CTAs) of it, so ragged lengths need no plan on the host.  A CTA can hold
+// and CTA c takes entries [c, c + 1) * ceil(total / CTAs) of it, so ragged lengths need no plan on the host.  In front of a
+// unit's tiles the list has kUnitCost entries without work, for what a unit costs besides (its query, its merge): decode of
+// 160 requests of 1 to 4100 keys, where a CTA held up to four short units.  A CTA can hold
 // the end of one unit and the beginning of another, each a partial result of its own (slots 2 c and 2 c + 1).
 #pragma once
 #include <cuda_runtime.h>
@@ -13,6 +15,7 @@
 
 namespace nvfp4 {
 
+constexpr int kUnitCost = 1;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct PagedParams {
@@ -28,6 +31,7 @@ struct PagedParams {
   int64_t table_row;
   const int32_t* lengths;
   int requests, width, blocks, log_block, hk, g;
+  uint32_t g_mul, g_shift;                    // division by g (set_group)
   float scale_log2;                           // scaling * log2(e)
   void* out;                                  // [tokens, H, D]
   float* lse;                                 // [tokens, H] or null
@@ -35,6 +39,18 @@ struct PagedParams {
   float *ws_m, *ws_l, *ws_acc;                // [2 * CTAs][ROWS] partial results
   int* status;
 };
+
+// i / g for 0 <= i < 2^31: with 2^shift the next power of two from g on, i / g = (i + hi(i * mul)) >> shift for
+// mul = floor(2^32 (2^shift - g) / g) + 1 (division by an invariant integer by multiplication).
+inline void set_group(PagedParams& p, int g) {
+  p.g = g;
+  p.g_shift = 0;
+  while ((1ll << p.g_shift) < g) ++p.g_shift;
+  p.g_mul = (uint32_t)(((1ull << 32) * ((1ull << p.g_shift) - (uint64_t)g)) / (uint64_t)g + 1);
+}
+__device__ __forceinline__ int token_of(const PagedParams& p, int i) {
+  return (int)((__umulhi((uint32_t)i, p.g_mul) + (uint32_t)i) >> p.g_shift);
+}
 
 // What a request asks for: its query tokens [t0, t0 + n), its keys, its units.
 template <int ROWS, int TILE>
@@ -56,7 +72,7 @@ struct Request {
   }
   __device__ __forceinline__ int rows(const PagedParams& p, int row_tile) const { return min(n * p.g - row_tile * ROWS, ROWS); }
   // keys that row i of the request sees
-  __device__ __forceinline__ int seen(const PagedParams& p, int i) const { return len - n + 1 + i / p.g; }
+  __device__ __forceinline__ int seen(const PagedParams& p, int i) const { return len - n + 1 + token_of(p, i); }
   // keys that the last row of a unit sees, in keys and in tiles: one at least, so that every unit is in the list
   __device__ __forceinline__ int limit(const PagedParams& p, int row_tile) const {
     return max(seen(p, row_tile * ROWS + rows(p, row_tile) - 1), 0);
@@ -64,42 +80,53 @@ struct Request {
   __device__ __forceinline__ int tiles(const PagedParams& p, int row_tile) const {
     return max((limit(p, row_tile) + TILE - 1) / TILE, 1);
   }
-  __device__ __forceinline__ int64_t head_tiles(const PagedParams& p) const {
-    int64_t sum = 0;
+  __device__ __forceinline__ int64_t head_entries(const PagedParams& p) const {
+    int64_t sum = (int64_t)kUnitCost * row_tiles;
     for (int j = 0; j < row_tiles; ++j) sum += tiles(p, j);
     return sum;
   }
 };
 
-// A place in the list: tile `tile` of the `tiles` of a unit.
+// The rest of a CTA's share, segment by segment: open() gives tiles [from, to) of a unit, close() goes on to the next one.
 template <int ROWS, int TILE>
-struct Cursor {
+struct Walk {
   Request<ROWS, TILE> q;
-  int r, head, row_tile, tile, tiles;
+  int r, head, row_tile, entry, tiles;        // entry: -kUnitCost .. -1 without work, then the unit's tiles
+  int from, to;
+  int64_t left;                               // entries
 
-  __device__ __forceinline__ void next_unit(const PagedParams& p) {
-    tile = 0;
+  __device__ __forceinline__ bool open() {
+    if (left <= 0) return false;
+    const int take = (int)min((int64_t)(tiles - entry), left);
+    left -= take;
+    from = max(entry, 0);
+    to = entry + take;
+    return to > 0;                            // else the share ends in front of the unit's tiles
+  }
+  __device__ __forceinline__ void close(const PagedParams& p) {
+    if (left <= 0) return;
+    entry = -kUnitCost;
     if (++row_tile >= q.row_tiles) {
       row_tile = 0;
       if (++head >= p.hk) {
         head = 0;
         do {
-          if (++r >= p.requests) return;
+          if (++r >= p.requests) {            // not within a share
+            left = 0;
+            return;
+          }
           q = Request<ROWS, TILE>(p, r);
         } while (q.row_tiles == 0);
       }
     }
     tiles = q.tiles(p, row_tile);
   }
+  __device__ __forceinline__ bool whole() const { return from == 0 && to == tiles; }
 };
 
-// The share of this CTA: tiles [begin, end) of the list, and the place of `begin`.  All threads; `list` has THREADS / 32 + 2
-// words of shared memory.
-struct Share {
-  int64_t begin, end, share;
-};
+// The share of this CTA; returns the entries of a full share.  All threads; `list` has THREADS / 32 + 2 words of shared memory.
 template <int THREADS, int ROWS, int TILE>
-__device__ __forceinline__ Share deal_tiles(const PagedParams& p, int64_t* list, Cursor<ROWS, TILE>& at) {
+__device__ __forceinline__ int64_t deal_tiles(const PagedParams& p, int64_t* list, Walk<ROWS, TILE>& at) {
   constexpr int kW = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   auto block_sum = [&](int64_t x, int64_t& before) -> int64_t {
@@ -122,26 +149,33 @@ __device__ __forceinline__ Share deal_tiles(const PagedParams& p, int64_t* list,
     return all;
   };
   auto weight = [&](int r) -> int64_t {
-    return r < p.requests ? p.hk * Request<ROWS, TILE>(p, r).head_tiles(p) : 0;
+    return r < p.requests ? p.hk * Request<ROWS, TILE>(p, r).head_entries(p) : 0;
   };
-  // of up to THREADS requests a thread keeps its one
+  // of up to THREADS requests a thread keeps its one, and the sum its place
   const int64_t first = weight(tid);
-  int64_t mine = first, before;
-  for (int r = tid + THREADS; r < p.requests; r += THREADS) mine += weight(r);
-  const int64_t total = block_sum(mine, before);
-  Share s;
-  s.share = (total + gridDim.x - 1) / gridDim.x;
-  s.begin = (int64_t)blockIdx.x * s.share;
-  s.end = min(total, s.begin + s.share);
-  if (s.begin >= s.end) return s;
+  int64_t more = 0, before, first_before;
+  const int64_t first_all = block_sum(first, first_before);
+  int64_t total = first_all;
+  if (p.requests > THREADS) {
+    for (int r = tid + THREADS; r < p.requests; r += THREADS) more += weight(r);
+    total += block_sum(more, before);
+  }
+  const int64_t share = (total + gridDim.x - 1) / gridDim.x, begin = (int64_t)blockIdx.x * share;
+  at.left = min(total, begin + share) - begin;
+  if (at.left <= 0) return share;
   if (tid == 0) list[kW] = -1;
+  __syncthreads();
   int64_t base = 0;
   for (int r0 = 0;; r0 += THREADS) {
-    const int64_t w = r0 == 0 ? first : weight(r0 + tid);
-    const int64_t all = block_sum(w, before);
-    if (s.begin >= base + before && s.begin < base + before + w) {
+    int64_t w = first, all = first_all;
+    before = first_before;
+    if (r0 > 0) {
+      w = weight(r0 + tid);
+      all = block_sum(w, before);
+    }
+    if (begin >= base + before && begin < base + before + w) {
       list[kW] = r0 + tid;
-      list[kW + 1] = s.begin - base - before;
+      list[kW + 1] = begin - base - before;
     }
     __syncthreads();
     if (list[kW] >= 0) break;
@@ -149,22 +183,34 @@ __device__ __forceinline__ Share deal_tiles(const PagedParams& p, int64_t* list,
   }
   at.r = (int)list[kW];
   at.q = Request<ROWS, TILE>(p, at.r);
-  const int64_t in = list[kW + 1], per_head = at.q.head_tiles(p);
-  at.head = (int)(in / per_head);
-  int64_t rest = in % per_head;
-  at.row_tile = 0;
-  while ((at.tiles = at.q.tiles(p, at.row_tile)) <= rest) {
-    rest -= at.tiles;
-    ++at.row_tile;
+  int64_t rest = list[kW + 1];
+  at.head = 0;
+  if (at.q.row_tiles == 1) {                  // the common case without a 64-bit division
+    at.row_tile = 0;
+    at.tiles = at.q.tiles(p, 0);
+    const int unit = at.tiles + kUnitCost;
+    if (rest >= unit) {
+      at.head = (int)((uint64_t)rest >> 31 ? rest / unit : (int)rest / unit);
+      rest -= (int64_t)at.head * unit;
+    }
+  } else {
+    const int64_t per_head = at.q.head_entries(p);
+    at.head = (int)(rest / per_head);
+    rest %= per_head;
+    at.row_tile = 0;
+    while ((at.tiles = at.q.tiles(p, at.row_tile)) + kUnitCost <= rest) {
+      rest -= at.tiles + kUnitCost;
+      ++at.row_tile;
+    }
   }
-  at.tile = (int)rest;
-  return s;
+  at.entry = (int)rest - kUnitCost;
+  return share;
 }
-// pieces of a unit that the CTA begins with `tiles` of its tiles, as its first segment or not
+// pieces of a unit whose first tiles are this segment, the CTA's first one or not
 template <int ROWS, int TILE>
-__device__ __forceinline__ int4 cut_unit(const PagedParams& p, const Cursor<ROWS, TILE>& u, int tiles, int64_t share, bool first) {
+__device__ __forceinline__ int4 cut_unit(const PagedParams& p, const Walk<ROWS, TILE>& u, int64_t share, bool first) {
   return make_int4(u.q.t0 * p.g + u.row_tile * ROWS, u.head, u.q.rows(p, u.row_tile),
-                   1 + (int)((u.tiles - tiles + share - 1) / share) + (first ? 1 << 30 : 0));
+                   1 + (int)((u.tiles - u.to + share - 1) / share) + (first ? 1 << 30 : 0));
 }
 
 __device__ __forceinline__ float ex2_approx(float x) {
@@ -181,8 +227,15 @@ __device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
   }
 }
 // row of `out` that row i (token * g + head of its group) of KV head `head` is
-__device__ __forceinline__ int64_t out_row(const PagedParams& p, int64_t i, int head) {
-  return (i / p.g) * (p.hk * p.g) + (int64_t)head * p.g + i % p.g;
+__device__ __forceinline__ int64_t out_row(const PagedParams& p, int i, int head) {
+  const int t = token_of(p, i);
+  return (int64_t)t * (p.hk * p.g) + head * p.g + (i - t * p.g);
+}
+// query row of row i of the request whose tokens begin at t0
+template <typename T>
+__device__ __forceinline__ const T* query_row(const PagedParams& p, int t0, int i, int head) {
+  const int t = token_of(p, i);
+  return static_cast<const T*>(p.q) + (t0 + t) * p.sqt + (head * p.g + (i - t * p.g)) * p.sqh;
 }
 // log-sum-exp of a sum relative to 2^top
 __device__ __forceinline__ float lse_of(float top, float sum) { return sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2; }
@@ -211,7 +264,8 @@ __device__ __forceinline__ void clear_untouched(const PagedParams& p) {
   }
 }
 
-// Exact merge of the pieces of a cut unit, one warp a row, in the order of the keys.
+// Exact merge of the pieces of a cut unit, one warp a row, in the order of the keys.  Bound by trips to L2: the maxima, sums
+// and rows of up to four pieces are asked for at once.
 constexpr int kCombineWarps = 4;
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(32 * kCombineWarps) paged_combine_kernel(PagedParams p) {
@@ -222,32 +276,52 @@ __global__ void __launch_bounds__(32 * kCombineWarps) paged_combine_kernel(Paged
   if (row >= u.z) return;
   const int pieces = u.w & ((1 << 30) - 1), first = 2 * (int)blockIdx.x + (u.w >> 30 ? 0 : 1);
   auto at = [&](int i) { return (int64_t)(i == 0 ? first : 2 * ((int)blockIdx.x + i)) * ROWS + row; };
-  float top = -INFINITY;
-  for (int i = lane; i < pieces; i += 32) top = fmaxf(top, p.ws_m[at(i)]);
+  constexpr int kAtOnce = 4, kC = D / 128;
+  float top = -INFINITY, total = 0.0f, sum[kC][4];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float sum[D / 128][4], total = 0.0f;
-#pragma unroll
-  for (int c = 0; c < D / 128; ++c)
+  for (int c = 0; c < kC; ++c)
 #pragma unroll
     for (int k = 0; k < 4; ++k) sum[c][k] = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < pieces; ++i) {
-    const float f = top == -INFINITY ? 1.0f : ex2_approx(p.ws_m[at(i)] - top);        // no key: zeros, or NaN
-    total += f * p.ws_l[at(i)];
+  for (int i0 = 0; i0 < pieces; i0 += kAtOnce) {
+    float m[kAtOnce], l[kAtOnce];
+    float4 v[kAtOnce][kC];
 #pragma unroll
-    for (int c = 0; c < D / 128; ++c) {
-      const float4 v = *reinterpret_cast<const float4*>(p.ws_acc + at(i) * D + c * 128 + lane * 4);
-      sum[c][0] += f * v.x;
-      sum[c][1] += f * v.y;
-      sum[c][2] += f * v.z;
-      sum[c][3] += f * v.w;
+    for (int x = 0; x < kAtOnce; ++x) {
+      const int64_t a = at(min(i0 + x, pieces - 1));       // behind the last piece: that one again, not counted
+      m[x] = p.ws_m[a];
+      l[x] = p.ws_l[a];
+#pragma unroll
+      for (int c = 0; c < kC; ++c) v[x][c] = *reinterpret_cast<const float4*>(p.ws_acc + a * D + c * 128 + lane * 4);
     }
+    float now = top;
+#pragma unroll
+    for (int x = 0; x < kAtOnce; ++x) now = fmaxf(now, m[x]);
+    const float ref = now == -INFINITY ? 0.0f : now;
+    const float f = top == -INFINITY ? 1.0f : ex2_approx(top - ref);         // no key so far: zeros, or NaN
+    total *= f;
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[c][k] *= f;
+#pragma unroll
+    for (int x = 0; x < kAtOnce; ++x) {
+      if (i0 + x >= pieces) break;
+      const float g = m[x] == -INFINITY ? 1.0f : ex2_approx(m[x] - ref);
+      total += g * l[x];
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        sum[c][0] += g * v[x][c].x;
+        sum[c][1] += g * v[x][c].y;
+        sum[c][2] += g * v[x][c].z;
+        sum[c][3] += g * v[x][c].w;
+      }
+    }
+    top = now;
   }
   const int64_t row_out = out_row(p, u.x + row, u.y);
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
-  for (int c = 0; c < D / 128; ++c) {
+  for (int c = 0; c < kC; ++c) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) sum[c][k] *= inv;
     store4<T>(static_cast<T*>(p.out) + row_out * D + c * 128 + lane * 4, sum[c]);

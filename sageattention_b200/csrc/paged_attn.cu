@@ -18,6 +18,7 @@
 // 2^-(14 + kLift) of the largest 2^-(25 + kLift) of that.
 #include <limits.h>
 #include "common/abi.cuh"
+#include "common/bwd_util.cuh"
 #include "common/fp4.cuh"
 #include "common/kv8.cuh"
 #include "common/launch.cuh"
@@ -30,7 +31,7 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 2;
 constexpr int kCtas = 3;                      // of an SM
 constexpr int kStageBytes = 8192;             // K and V of a warp's keys of a tile
-constexpr float kLag = 5.0f, kLift = 9.0f;
+constexpr float kLag = 9.0f, kLift = 5.0f;
 
 template <int D>
 struct Cfg {
@@ -102,23 +103,29 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
   griddep_wait();
   griddep_launch();
 
-  using Place = Cursor<kRows, kTile>;
+  using Place = Walk<kRows, kTile>;
   Place use;
-  const auto [begin, end, share] = deal_tiles<kThreads>(p, list_s, use);
+  const int64_t share = deal_tiles<kThreads>(p, list_s, use);
   if (tid == 0) p.cut[cta] = make_int4(0, 0, 0, 0);
-  if (begin < end) {
-    // ---- the ring of this warp: copies of tile `ahead` go into stage `fill`
+  if (use.left > 0) {
+    // ---- the ring of this warp: copies of tile `ahead_tile` of `ahead` go into stage `fill`
     const uint32_t ring = smem_u32(smem) + warp * kStages * kStageBytes;
     const uint32_t shared = smem_u32(smem) + S::kRing;
     Place ahead = use;
-    int64_t left = end - begin;                            // tiles still to be asked for
-    int ahead_limit = ahead.q.limit(p, ahead.row_tile);
+    bool more = ahead.open();
+    int ahead_tile = ahead.from, ahead_limit = ahead.q.limit(p, ahead.row_tile);
     int id[kHalves];
     auto look_up = [&]() {                                 // blocks of the keys of `ahead`, a tile before they are needed
-      const int key = ahead.tile * kTile + warp * kSub;
+      const int key = ahead_tile * kTile + warp * kSub;
 #pragma unroll
       for (int h = 0; h < kHalves; ++h)
-        id[h] = left > 0 && key + h * 16 < ahead_limit ? p.table[ahead.r * p.table_row + ((key + h * 16) >> p.log_block)] : -1;
+        id[h] = more && key + h * 16 < ahead_limit ? p.table[ahead.r * p.table_row + ((key + h * 16) >> p.log_block)] : -1;
+    };
+    auto warm = [&](const Place& u) {                      // query rows of a unit to come, into L2
+      constexpr int kLines = D * sizeof(T) / 128;
+      if (warp != 0) return;
+      for (int i = lane; i < u.q.rows(p, u.row_tile) * kLines; i += 32)
+        prefetch_l2(reinterpret_cast<const uint8_t*>(query_row<T>(p, u.q.t0, u.row_tile * kRows + i / kLines, u.head)) + i % kLines * 128);
     };
     // where a lane's 16-byte pieces of 16 keys go: piece i is key (32 i + lane) / (D / 16), and the swizzle has a period of eight keys
     auto piece = [&](int i) -> uint32_t {
@@ -126,8 +133,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
       return (uint32_t)(chunk >> 3) * (kSub * 128) + (uint32_t)key_in * 128 + (uint32_t)(((chunk & 7) ^ (key_in & 7)) << 4);
     };
     auto ask = [&](int stage) {
-      if (left > 0) {
-        const int key = ahead.tile * kTile + warp * kSub;
+      if (more) {
+        const int key = ahead_tile * kTile + warp * kSub;
         const uint32_t base_s = ring + stage * kStageBytes;
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
@@ -153,15 +160,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
           }
           if (lane == 0) keys_s[warp][stage][h] = keys;
         }
-        if (--left > 0 && ++ahead.tile == ahead.tiles) {
-          ahead.next_unit(p);
-          ahead_limit = ahead.q.limit(p, ahead.row_tile);
+        if (++ahead_tile == ahead.to) {
+          ahead.close(p);
+          more = ahead.open();
+          if (more) {
+            ahead_tile = ahead.from;
+            ahead_limit = ahead.q.limit(p, ahead.row_tile);
+            warm(ahead);
+          }
         }
         look_up();
       }
       cp_async_commit();
     };
     look_up();
+    if (more) warm(ahead);
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) ask(s);
     int stage = 0;
@@ -169,30 +182,30 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
     // ---- segments: the tiles of one unit in this share
     const int g8 = lane >> 2, c4 = lane & 3;               // row (key, or pair of the head dim) and pair of query rows of a product
     const int krow = key_of_row(g8);
-    int64_t at = begin;
     bool first = true;
-    while (at < end) {
+    for (; use.open(); use.close(p)) {
       const int rows = use.q.rows(p, use.row_tile);
-      const int tiles = (int)min((int64_t)(use.tiles - use.tile), end - at);
-      const bool whole = use.tile == 0 && tiles == use.tiles;
+      const bool whole = use.whole();
 
       // query rows as fragments of the products: eight threads a row, elements 16 e .. 16 e + 15 for e = tid % 8 (+ 8)
 #pragma unroll 1
       for (int row = tid >> 3; row < kRows; row += kThreads / 8) {
         const int e0 = tid & 7;
-        const int i = use.row_tile * kRows + row;
-        const T* pq = static_cast<const T*>(p.q) + (int64_t)(use.q.t0 + i / p.g) * p.sqt +
-                      (int64_t)(use.head * p.g + i % p.g) * p.sqh;
+        const T* pq = query_row<T>(p, use.q.t0, use.row_tile * kRows + min(row, rows - 1), use.head);
         float x[D / 128][16];
         float big = 0.0f;
 #pragma unroll
         for (int u = 0; u < D / 128; ++u) {
+          float v[2][8];
+          load8<T>(pq + (u * 8 + e0) * 16, v[0]);
+          load8<T>(pq + (u * 8 + e0) * 16 + 8, v[1]);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            x[u][k] = row < rows ? to_f32<T>(pq[(u * 8 + e0) * 16 + k]) : 0.0f;
-            big = fmaxf(big, fabsf(x[u][k]));
-          }
+          for (int k = 0; k < 16; ++k) x[u][k] = row < rows ? v[k / 8][k % 8] : 0.0f;
         }
+#pragma unroll
+        for (int u = 0; u < D / 128; ++u)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) big = fmaxf(big, fabsf(x[u][k]));
         const uint32_t eight = 0xFFu << (lane & 24);
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) big = fmaxf(big, __shfl_xor_sync(eight, big, o));
@@ -252,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
           lift[nt][k] = l[nt][k] = 0.0f;
         }
 
-      for (int tile = use.tile; tile < use.tile + tiles; ++tile) {
+      for (int tile = use.from; tile < use.to; ++tile) {
         ask(stage == 0 ? kStages - 1 : stage - 1);
         cp_async_wait<kStages - 1>();
         __syncwarp();
@@ -340,14 +353,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
                 top[nt][k] = fmaxf(top[nt][k], t);
                 top_w[nt][k] = fmaxf(top_w[nt][k], t + vexp[h]);
               }
-          bool move = false;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            bool move = false;
 #pragma unroll
             for (int k = 0; k < 2; ++k) move = move || top[nt][k] > ref[nt][k] + kLag || top_w[nt][k] > ref_w[nt][k] + kLag;
-          if (__any_sync(0xffffffffu, move)) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 float m = top[nt][k], w = top_w[nt][k];
@@ -371,6 +382,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
                 ref[nt][k] = m;
                 ref_w[nt][k] = w;
               }
+            }
           }
 #pragma unroll
           for (int h = 0; h < kHalves; ++h) {
@@ -483,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
               }
               if (whole) {
                 const float f = total_l == 0.0f ? 0.0f : 1.0f / total_l;
-                const int64_t to = out_row(p, (int64_t)use.q.t0 * p.g + use.row_tile * kRows + row, use.head);
+                const int64_t to = out_row(p, use.q.t0 * p.g + use.row_tile * kRows + row, use.head);
                 T* dst = static_cast<T*>(p.out) + to * D + cols * 64 + lane * 2;
                 if constexpr (S::kTwo) *reinterpret_cast<float2*>(dst) = make_float2(sum.x * f, sum.y * f);
                 else *reinterpret_cast<uint32_t*>(dst) = pack_16x2<T>(sum.x * f, sum.y * f);
@@ -501,10 +513,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
         }
       }
       // begun here, finished by the CTAs behind this one
-      if (!whole && use.tile == 0 && tid == 0) p.cut[cta] = cut_unit(p, use, tiles, share, first);
-      at += tiles;
+      if (!whole && use.from == 0 && tid == 0) p.cut[cta] = cut_unit(p, use, share, first);
       first = false;
-      if (at < end) use.next_unit(p);
     }
   }
   clear_untouched<T, D, kRows, kTile>(p);
@@ -583,8 +593,9 @@ extern "C" int nvfp4_kv8_attention(const void* q, int q_dtype, int64_t s_qt, int
   NVFP4_REQUIRE(workspace_bytes >= (size_t)(grid * paged_slot_bytes(rows, d)), "nvfp4_kv8_attention: workspace too small");
   NVFP4_REQUIRE(q_dtype >= NVFP4_DT_BF16 && q_dtype <= NVFP4_DT_FP32, "nvfp4_kv8_attention: unknown dtype %d", q_dtype);
   PagedParams p{q, s_qt, s_qh, cu_seqlens, tokens, k_cache, v_cache, k_block, v_block, k_scale, v_scale, ks_block, vs_block, table,
-                table_row, lengths, (int)requests, (int)width, (int)blocks, lb, (int)hk, g, scaling * kLog2e, out, lse,
+                table_row, lengths, (int)requests, (int)width, (int)blocks, lb, (int)hk, g, 0, 0, scaling * kLog2e, out, lse,
                 nullptr, nullptr, nullptr, nullptr, status};
+  set_group(p, g);
   p.ws_acc = static_cast<float*>(workspace);
   p.cut = reinterpret_cast<int4*>(p.ws_acc + 2 * grid * rows * d);
   p.ws_m = reinterpret_cast<float*>(p.cut + grid);

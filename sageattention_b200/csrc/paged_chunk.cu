@@ -110,7 +110,7 @@ __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint3
 template <typename T, int D>
 __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedParams p) {
   using C = Cfg<D>;
-  using Place = Cursor<C::kRows, kTile>;
+  using Place = Walk<C::kRows, kTile>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2][2], p_full[2][2], o_full[2], o_free[2], pv_done[2], q_full;
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
   __shared__ int expired;                                  // a wait ran out: site, else 0
   __shared__ int64_t list_s[C::kThreads / 32 + 2];
   __shared__ Place place_s;
-  __shared__ Share share_s;
+  __shared__ int64_t share_s;                              // entries of a full share
   __shared__ TileInfo info_s[kInfo];
   __shared__ float m_s[2][128], l_s[128], c_s[128];
   const int tid = threadIdx.x, lane = tid & 31, warp = warp_index();
@@ -151,10 +151,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
   const uint32_t tmem = tmem_base_s;
   {
     Place from;
-    const Share mine = deal_tiles<C::kThreads>(p, list_s, from);
+    const int64_t share = deal_tiles<C::kThreads>(p, list_s, from);
     if (tid == 0) {
       place_s = from;
-      share_s = mine;
+      share_s = share;
       p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
     }
   }
@@ -163,8 +163,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
   if (warp >= C::kSoft && warp < C::kSoft + 4) {
     more_registers<C::kRegsConvert>();
     Place ahead = place_s;
-    int64_t left = share_s.end - share_s.begin;            // tiles to be asked for, and to be converted
-    int64_t rest = left;
+    bool more = ahead.open();                              // there is a tile to be looked up: `tile` of `ahead`
+    int tile = ahead.from;
     // ------------------------------------------------------------------ codes to halves
     const int w = warp - C::kSoft, t = w * 32 + lane;
     // 16-byte pieces of a tile: eight lanes take 64 bytes of two neighbouring keys, whose halves then lie in different banks
@@ -180,11 +180,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     int id_now = -1, id_next = -1, id_ahead = -1;
     float ks_now = 0.0f, vs_now = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
     int key0 = 0, limit = 0, head = 0;                     // of the tile asked for
+    bool asked = false;                                    // there is one
     bool starts = true, starts_next = true, starts_ahead = true;   // first tile of its unit, as far as this CTA sees
     auto look_up = [&]() {
       id_ahead = -1;
-      const int key = ahead.tile * kTile + lane * 16;
-      if (left > 0 && lane < 8 && key < ahead.q.limit(p, ahead.row_tile))
+      const int key = tile * kTile + lane * 16;
+      if (more && lane < 8 && key < ahead.q.limit(p, ahead.row_tile))
         id_ahead = p.table[ahead.r * p.table_row + (key >> p.log_block)];
     };
     // the tile asked for becomes the one converted, the one looked up the one asked for
@@ -196,11 +197,14 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       id_next = (unsigned)id_ahead < (unsigned)p.blocks ? id_ahead : -1;
       starts_next = starts_ahead;
       starts_ahead = false;
-      key0 = ahead.tile * kTile;
-      limit = left > 0 ? ahead.q.limit(p, ahead.row_tile) : 0;
+      asked = more;
+      key0 = tile * kTile;
+      limit = more ? ahead.q.limit(p, ahead.row_tile) : 0;
       head = ahead.head;
-      if (--left > 0 && ++ahead.tile == ahead.tiles) {
-        ahead.next_unit(p);
+      if (more && ++tile == ahead.to) {
+        ahead.close(p);
+        more = ahead.open();
+        tile = ahead.from;
         starts_ahead = true;
       }
       look_up();
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       fence_proxy_async_smem();
       __syncwarp();
     };
-    if (left > 0) {
+    if (more) {
       look_up();
       next();
       find();
@@ -271,7 +275,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     }
     int v_run = -200;                                      // largest exponent of the unit's value scales so far
     uint32_t n = 0;
-    for (; rest > 0; --rest, ++n) {
+    for (; asked; ++n) {
       const int st = n % C::kStages;
       const uint32_t ph = (n / C::kStages) & 1;
       next();
@@ -297,7 +301,6 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     if (warp == C::kSoft + 4) {
     // ------------------------------------------------------------------ issue of the products
     Place at = place_s;
-    int64_t rest = share_s.end - share_s.begin;
     const bool leader = elect_one();
     const uint32_t id_s = make_idesc_bf16(128, C::kN, false, true), id_o = make_idesc_bf16(128, 128, true, true);
     const uint64_t b_q = desc_sw128(smem + C::kQ, 0), b_k = desc_sw128(smem + C::kK, 0);
@@ -305,8 +308,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     uint32_t n = 0, seg = 0;                               // tiles and segments so far
     uint32_t p_phase[2] = {0, 0};                          // of p_full, a bit a place
     uint32_t results[2] = {0, 0};                          // results of each group so far
-    while (rest > 0) {
-      const int tiles = (int)min((int64_t)(at.tiles - at.tile), rest);
+    for (; at.open(); at.close(p)) {
+      const int tiles = at.to - at.from;
       const bool both = C::kGroups == 2 && at.q.rows(p, at.row_tile) > 128;
       const int turn = both || C::kGroups == 1 ? 1 : 2;    // a group takes every turn-th tile
       auto jobs_of = [&](int g) { return (turn == 1 ? tiles : (tiles + 1 - g) / 2) * C::kJobs; };
@@ -368,14 +371,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       }
       n += tiles;
       ++seg;
-      rest -= tiles;
-      if (rest > 0) at.next_unit(p);
     }
     }
   } else {
     if (D == 128) more_registers<C::kRegsSoft>();
     Place at = place_s;
-    int64_t rest = share_s.end - share_s.begin;
     // ------------------------------------------------------------------ softmax, a thread a row
     const int group = warp >> 2, wq = warp & 3, row_in = wq * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(wq * 32) << 16;
@@ -383,11 +383,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     uint32_t n = 0;                                        // tiles so far
     uint32_t s_phase = 0, results = 0, pv = 0;             // phases of s_full (a bit a place), o_full and pv_done so far
     bool first_segment = true;
-    while (rest > 0) {
-      const int tiles = (int)min((int64_t)(at.tiles - at.tile), rest);
+    for (; at.open(); at.close(p)) {
+      const int tiles = at.to - at.from;
       const int rows = at.q.rows(p, at.row_tile);
       const bool both = C::kGroups == 2 && rows > 128;
-      const bool whole = at.tile == 0 && tiles == at.tiles;
+      const bool whole = at.whole();
       const int row = (both ? group * 128 : 0) + row_in;   // of the unit
       const bool live = row < rows;
       const int i_row = at.row_tile * C::kRows + row;      // of the request
@@ -395,8 +395,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       named_bar_sync(1, 32 * C::kSoft);
       float c_row = 0.0f;
       if (both || group == 0) {
-        const T* pq = static_cast<const T*>(p.q) + (int64_t)(at.q.t0 + (live ? i_row : 0) / p.g) * p.sqt +
-                      (int64_t)(at.head * p.g + (live ? i_row : 0) % p.g) * p.sqh;
+        const T* pq = query_row<T>(p, at.q.t0, live ? i_row : 0, at.head);
         float big = 0.0f;
         if (live) {
 #pragma unroll 4
@@ -444,7 +443,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         constexpr int kChunks = C::kN / 32;
         const int place = j & 1, tile = j / C::kJobs * turn + my, sub = j % C::kJobs;
         const uint32_t s_at = tmem + lane_addr + C::s_at(group, place);
-        const int key0 = (at.tile + tile) * kTile + sub * C::kN;
+        const int key0 = (at.from + tile) * kTile + sub * C::kN;
         mbar_wait(&s_full[group][place], (s_phase >> place) & 1, err, 67);
         s_phase ^= 1u << place;
         tc_fence_after();
@@ -592,7 +591,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         const int row0 = (both ? group * 128 : 0) + wq * 32;
         const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
         if (whole) {
-          if (live && p.lse != nullptr) p.lse[out_row(p, (int64_t)at.q.t0 * p.g + i_row, at.head)] = lse_of(m, l);
+          if (live && p.lse != nullptr) p.lse[out_row(p, at.q.t0 * p.g + i_row, at.head)] = lse_of(m, l);
         } else if (live) {
           p.ws_m[(int64_t)slot * C::kRows + row] = m;
           p.ws_l[(int64_t)slot * C::kRows + row] = l;
@@ -636,7 +635,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
             for (int e = 0; e < 16; ++e)
               w[e] = pack_16x2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
             segment(w, [&](int r) {
-              const int64_t to = out_row(p, (int64_t)at.q.t0 * p.g + at.row_tile * C::kRows + row0 + r, at.head);
+              const int64_t to = out_row(p, at.q.t0 * p.g + at.row_tile * C::kRows + row0 + r, at.head);
               return reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) + to * D + cc * 32);
             });
           } else {
@@ -655,11 +654,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       tc_fence_before();
       __syncwarp();
       if (has && lane == 0) mbar_arrive(&o_free[group]);
-      if (!whole && at.tile == 0 && tid == 0) p.cut[blockIdx.x] = cut_unit(p, at, tiles, share_s.share, first_segment);
+      if (!whole && at.from == 0 && tid == 0) p.cut[blockIdx.x] = cut_unit(p, at, share_s, first_segment);
       n += tiles;
       first_segment = false;
-      rest -= tiles;
-      if (rest > 0) at.next_unit(p);
     }
   }
   clear_untouched<T, D, C::kRows, kTile>(p);

@@ -232,8 +232,8 @@ def _close(got, lse, q, k, v, vscale, limits, scaling, g, hidden=None, chunk=Fal
     """Rows of one request.  With A = sum p |v|, S = scaling * sum |q| |k|: scores are off by delta = S (D + 8) 2^-23 (products
     of exact halves summed in fp32; an fp32 q is two halves, 2^-22), a weight by its rounding to halves (2^-11, as two
     2^-22), exp2 and the sums by (keys + 8) 2^-23; the result is rounded once.  Halves end at 2^-24: a weight p vs is held times
-    2^9 / W, W = the largest p of 32 keys times their largest vs (at least what a warp's weights are relative to), so its
-    rounding is at least 2^-34 W, and with codes of at most 448 a value is off by 2^-34 W 448 keys: all that is left of it
+    2^5 / W, W = the largest p of 32 keys times their largest vs (at least what a warp's weights are relative to), so its
+    rounding is at least 2^-30 W, and with codes of at most 448 a value is off by 2^-30 W 448 keys: all that is left of it
     where the code of the one key that counts is 0.  Calls of many rows (`chunk`) take 128 keys at once and hold weights times 2^3:
     2^-28; and K and V of a block as halves relative to the largest scale of the 128 keys, which below 2^-14 of it are off by
     2^-25 of it: in a score scaling * sum |q| 2^-25 of the largest K scale, in the result 2^-25 sum p of the largest V scale."""
@@ -261,7 +261,7 @@ def _close(got, lse, q, k, v, vscale, limits, scaling, g, hidden=None, chunk=Fal
         pad = -p.shape[2] % keys
         groups = lambda x: torch.nn.functional.pad(x, (0, pad)).unflatten(-1, (-1, keys)).amax(-1)
         w = (groups(p) * groups(vscale.double()).repeat_interleave(g, 0)).amax(2)
-        tol = tol + (2.0 ** (-28 if chunk else -34) * 448 * k.shape[1] * w)[..., None]
+        tol = tol + (2.0 ** (-28 if chunk else -30) * 448 * k.shape[1] * w)[..., None]
         if chunk:
             top_k = qd.abs().sum(2) * scaling * 2.0 ** -25 * float(k.abs().max())     # every block here has codes above 1
             delta = delta + top_k
