@@ -53,7 +53,7 @@ class _Tables:
         assert self.count.tolist() == [n] and self.free[:n].tolist() == self.ref["free"][:n].tolist()
 
 
-@pytest.mark.parametrize("rows,most,block,seed", [(1, 40, 16, 0), (3, 5, 16, 1), (70, 1, 64, 2), (33, 300, 32, 3), (1030, 9, 16, 4),
+@pytest.mark.parametrize("rows,most,block,seed", [(1, 40, 16, 0), (3, 5, 16, 1), (70, 1, 64, 2), (33, 300, 32, 3), (1030, 9, 16, 4), (2049, 4, 64, 7),
                                                   (4100, 3, 128, 5), (2, 9000, 16, 6)])
 def test_steps_of_reservations_and_trims(rows, most, block, seed):
     g = torch.Generator().manual_seed(seed)
