@@ -318,7 +318,7 @@ int nvfp4_window_attention(const void* q, int dtype, int64_t s_qz, int64_t s_qh,
  * nvfp4_paged_trim: request r keeps its first keep_lens[r] tokens (all of them if it has no more, none for <= 0).  Blocks
  * that hold none of them go back on the stack, their table entries become -1.  A trim to the lengths in front of a
  * reservation restores the stack and the table.
- * workspace: 2 * (requests + 1) words.  Both change the state in place, on the device: calls on one state follow one another
+ * workspace: requests + 2 words.  Both change the state in place, on the device: calls on one state follow one another
  * on one stream.
  */
 int nvfp4_paged_reserve(const int32_t* new_lens, int32_t* lengths, int32_t* table,

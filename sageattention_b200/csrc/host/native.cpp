@@ -697,7 +697,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> paged_reserve(const Tensor& new_lens,
   require_words(c, free_count, 1, at::kInt, "free_count must be one int32");
   require(slots >= 0, "num_slots must not be negative");
   Tensor slot_map = c.empty({slots}, at::kLong), positions = c.empty({slots}, at::kInt);
-  Tensor cu = c.empty({r + 1}, at::kInt), shortage = c.empty({1}, at::kInt), scratch = c.empty({2 * (r + 1)}, at::kInt);
+  Tensor cu = c.empty({r + 1}, at::kInt), shortage = c.empty({1}, at::kInt), scratch = c.empty({r + 2}, at::kInt);
   c.done(nvfp4_paged_reserve(new_lens.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), table.data_ptr<int32_t>(),
                              table.stride(0), free_blocks.data_ptr<int32_t>(), free_count.data_ptr<int32_t>(), r, table.size(1),
                              n, (int)block_size, slots, slot_map.data_ptr<int64_t>(), positions.data_ptr<int32_t>(),
@@ -716,7 +716,7 @@ void paged_trim(const Tensor& keep_lens, const Tensor& lengths, const Tensor& ta
   require_words(c, lengths, r, at::kInt, "lengths must be contiguous int32 [requests]");
   require_words(c, free_blocks, n, at::kInt, "free_blocks must be contiguous int32 [blocks]");
   require_words(c, free_count, 1, at::kInt, "free_count must be one int32");
-  Tensor words = c.empty({2 * (r + 1)}, at::kInt);
+  Tensor words = c.empty({r + 2}, at::kInt);
   c.done(nvfp4_paged_trim(keep_lens.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), table.data_ptr<int32_t>(), table.stride(0),
                           free_blocks.data_ptr<int32_t>(), free_count.data_ptr<int32_t>(), r, table.size(1), n, (int)block_size,
                           words.data_ptr<int32_t>(), c.stream),

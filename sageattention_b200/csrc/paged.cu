@@ -13,7 +13,7 @@ namespace {
 // ------------------------------------------------------------------------------------------ tables
 constexpr int kTableThreads = 1024;
 constexpr int kSearchRows = 2048;        // prefix sums of as many requests are searched in shared memory
-constexpr int64_t kAlone = 4096;         // entries that one block of threads sees to
+constexpr int64_t kAlone = 8192;         // entries that one block of threads sees to
 
 // Exclusive prefix sum over the block of two counts at once, and their totals.
 struct Sums {
@@ -77,49 +77,102 @@ struct TableParams {
   int32_t* positions;
   int32_t* cu;
   int32_t* shortage;
-  int32_t* scratch;                      // [2][requests + 1] prefix sums of more than kSearchRows requests
+  int32_t* scratch;                      // [requests + 2] prefix sums of blocks, where one kernel hands them to another
 };
 
 __device__ __forceinline__ int64_t blocks_of(int64_t tokens, int log_block) {
   return (tokens + (1 << log_block) - 1) >> log_block;
 }
 
-// Both table kernels are one cluster: every block of threads makes the prefix sums of all requests for itself, does its share of
-// the entries, and the first one updates lengths and stack when all have read them.  A launch then costs its latency, few
-// requests or many.
+// All blocks of threads of a kernel that is one cluster.
 __device__ __forceinline__ void all_blocks() {
   if (gridDim.z > 1) cluster_sync_all();
   else __syncthreads();
 }
 
+// Slots and positions, by warps `warp`, `warp` + `warps`, ...: a thread has four tokens 32 apart (four neighbours would be stores of
+// 32 sectors an instruction), whose look-ups are under way together.  A fresh block starts with the token at its offset 0,
+// whose thread also enters it in the table: fresh blocks come off the stack, so no thread reads an entry that another one
+// writes.  start_of(r): tokens that request r held.
+template <typename F>
+__device__ __forceinline__ void fill_slots(const TableParams& p, const int32_t* cu, const int32_t* off, int avail, int used, int warp,
+                                           int warps, F start_of) {
+  constexpr int kFour = 4;
+  const int slots = (int)p.slots, mask = (1 << p.log_block) - 1;
+  int r = -1, next = 0, begin = 0, had = 0;                // request of the last token: its end, position 0, blocks it had
+  const int32_t* fresh = nullptr;                          // where its block j comes from: fresh[-j]
+  int32_t* row = nullptr;
+  for (int64_t t0 = 32 * kFour * (int64_t)warp + (threadIdx.x & 31); t0 < slots; t0 += 32 * kFour * (int64_t)warps) {
+    int32_t* entry[kFour];
+    const int32_t* from[kFour];
+    int block[kFour], pos[kFour];
+#pragma unroll
+    for (int x = 0; x < kFour; ++x) {
+      const int t = (int)t0 + 32 * x;
+      from[x] = nullptr;
+      pos[x] = 0;
+      if (t < used) {
+        if (t >= next) {
+          // the request behind, mostly
+          if (r >= 0 && t < cu[r + 2 <= p.requests ? r + 2 : p.requests]) ++r;
+          else r = row_of(cu, p.requests, t);
+          const int start = start_of(r);
+          next = cu[r + 1];
+          begin = start - cu[r];
+          had = (int)blocks_of(start, p.log_block);
+          row = p.table + r * p.table_row;
+          fresh = p.free_blocks + ((int64_t)avail - 1 - (off[r] - had));
+        }
+        pos[x] = begin + t;
+        const int j = pos[x] >> p.log_block;
+        entry[x] = row + j;
+        from[x] = j < had ? entry[x] : fresh - j;
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < kFour; ++x) block[x] = from[x] != nullptr ? *from[x] : -1;
+#pragma unroll
+    for (int x = 0; x < kFour; ++x) {
+      const int t = (int)t0 + 32 * x;
+      if (t >= slots) break;
+      const int in = pos[x] & mask;
+      if (from[x] != nullptr && in == 0) *entry[x] = block[x];
+      p.slot_map[t] = from[x] != nullptr ? ((int64_t)block[x] << p.log_block) + in : -1;
+      p.positions[t] = pos[x];
+    }
+  }
+}
+
 // New tokens n_r of every request: cu_seqlens = prefix sums of n_r; blocks needed = ceil((len + n) / B) - ceil(len / B),
 // popped from the stack in request order.  All or nothing: a short pool, a narrow table or too few slots change nothing.
-__global__ void __launch_bounds__(kTableThreads) reserve_kernel(TableParams p) {
+// One block of threads, whose latency is what it costs; a long list of slots is filled by reserve_fill_kernel behind it.  (As
+// one cluster of eight, 200000 slots of 512 requests took 22 us: 90 instructions a token on eight SMs.)
+__global__ void __launch_bounds__(kTableThreads) reserve_kernel(TableParams p, int fill) {
   __shared__ Sums warp_sums[33];
-  __shared__ int32_t cu_s[kSearchRows + 1], off_s[kSearchRows + 1];
+  __shared__ int32_t cu_s[kSearchRows + 1], off_s[kSearchRows + 1], len_s[kSearchRows];
   __shared__ int too_wide;
   const int tid = threadIdx.x, threads = blockDim.x;
-  const bool first = blockIdx.z == 0;
   if (tid == 0) too_wide = 0;
   griddep_wait();
   griddep_launch();
   __syncthreads();
-  const int64_t avail = min(max(*p.free_count, 0), p.blocks);
+  const int avail = min(max(*p.free_count, 0), p.blocks);
+  const bool in_smem = p.requests <= kSearchRows;
   auto counts = [&](int r) -> Sums {
     if (r >= p.requests) return {0, 0};
     const int64_t len = max(p.lengths[r], 0), n = max(p.wanted[r], 0), want = blocks_of(len + n, p.log_block);
+    if (in_smem) len_s[r] = (int)len;
     if (want > p.width || len + n > INT32_MAX) too_wide = 1;
     return {n, want - blocks_of(len, p.log_block)};
   };
   // prefix sums of tokens and of blocks
-  const bool in_smem = p.requests <= kSearchRows;
-  int32_t* cu = in_smem ? cu_s : p.scratch;
-  int32_t* off = in_smem ? off_s : p.scratch + p.requests + 1;
+  int32_t* cu = in_smem ? cu_s : p.cu;
+  int32_t* off = in_smem ? off_s : p.scratch + 1;
   Sums total{0, 0};
   for (int r0 = 0; r0 < p.requests; r0 += threads) {
     Sums part;
     const Sums at = block_exclusive(counts(r0 + tid), warp_sums, part);
-    if (r0 + tid < p.requests && (in_smem || first)) {
+    if (r0 + tid < p.requests) {
       cu[r0 + tid] = (int32_t)min(total.a + at.a, (int64_t)INT32_MAX);
       off[r0 + tid] = (int32_t)min(total.b + at.b, (int64_t)INT32_MAX);
     }
@@ -127,59 +180,51 @@ __global__ void __launch_bounds__(kTableThreads) reserve_kernel(TableParams p) {
     total.b += part.b;
   }
   const bool ok = total.a <= p.slots && total.b <= avail && !too_wide;
-  if (tid == 0 && (in_smem || first)) cu[p.requests] = (int32_t)min(total.a, (int64_t)INT32_MAX);
-  if (in_smem) __syncthreads();
-  else all_blocks();
-  // slots and positions, four tokens in a row a thread: they are mostly of one request and one block, whose look-ups they
-  // share.  A fresh block starts with the token at its offset 0, whose thread also enters it in the table: fresh blocks
-  // come off the stack, so no thread reads an entry that another one writes.
-  const int64_t used = ok ? total.a : 0;
-  for (int64_t t0 = 4 * ((int64_t)blockIdx.z * threads + tid); t0 < p.slots; t0 += 4 * (int64_t)gridDim.z * threads) {
-    int r = -1, block = 0;
-    int64_t start = 0, had = 0, seen = -1;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int64_t t = t0 + x;
-      if (t >= p.slots) break;
-      int64_t slot = -1, pos = 0;
-      if (t < used) {
-        if (r < 0 || t >= cu[r + 1]) {
-          r = row_of(cu, p.requests, t);
-          start = max(p.lengths[r], 0);
-          had = blocks_of(start, p.log_block);
-          seen = -1;
-        }
-        pos = start + (t - cu[r]);
-        const int64_t j = pos >> p.log_block, in = pos & ((1 << p.log_block) - 1);
-        if (j != seen) {
-          int32_t* entry = p.table + r * p.table_row + j;
-          block = j < had ? *entry : p.free_blocks[avail - 1 - (off[r] + (j - had))];
-          if (in == 0) *entry = block;                     // at offset 0 the block is a fresh one
-          seen = j;
-        }
-        slot = ((int64_t)block << p.log_block) + in;
-      }
-      p.slot_map[t] = slot;
-      p.positions[t] = (int32_t)pos;
-    }
+  if (tid == 0) cu[p.requests] = (int32_t)min(total.a, (int64_t)INT32_MAX);
+  __syncthreads();
+  if (fill)
+    fill_slots(p, cu, off, avail, ok ? (int)total.a : 0, tid >> 5, threads >> 5,
+               [&](int r) { return in_smem ? len_s[r] : max(p.lengths[r], 0); });
+  __syncthreads();                       // lengths and, of many requests, p.cu have been read
+  for (int r = tid; r <= p.requests; r += threads) {
+    p.cu[r] = ok ? cu[r] : 0;
+    if (r == p.requests) break;
+    if (!fill) p.scratch[1 + r] = off[r];
+    if (ok) p.lengths[r] = max(p.lengths[r], 0) + max(p.wanted[r], 0);
   }
-  if (first)
-    for (int r = tid; r <= p.requests; r += threads) p.cu[r] = ok ? cu[r] : 0;
-  all_blocks();                          // lengths and free_count have been read by all
-  if (!first) return;
-  if (ok)
-    for (int r = tid; r < p.requests; r += threads) p.lengths[r] = max(p.lengths[r], 0) + max(p.wanted[r], 0);
   if (tid == 0) {
     *p.shortage = ok ? 0 : 1;
     if (ok) *p.free_count = (int32_t)(avail - total.b);
+    if (!fill) p.scratch[0] = avail;
   }
 }
 
-// Every request keeps its first tokens.  Freed blocks go on the stack with the last one popped first, so a trim to the lengths
+__global__ void __launch_bounds__(256) reserve_fill_kernel(TableParams p) {
+  __shared__ int32_t cu_s[kSearchRows + 1], off_s[kSearchRows + 1];
+  griddep_wait();
+  griddep_launch();
+  const int32_t* cu = p.cu;
+  const int32_t* off = p.scratch + 1;
+  if (p.requests <= kSearchRows) {
+    for (int i = threadIdx.x; i <= p.requests; i += blockDim.x) {
+      cu_s[i] = cu[i];
+      if (i < p.requests) off_s[i] = off[i];
+    }
+    __syncthreads();
+    cu = cu_s;
+    off = off_s;
+  }
+  const int warps = blockDim.x >> 5;
+  fill_slots(p, cu, off, p.scratch[0], cu[p.requests], (int)blockIdx.x * warps + (threadIdx.x >> 5), (int)gridDim.x * warps,
+             [&](int r) { return p.lengths[r] - (cu[r + 1] - cu[r]); });
+}
+
+// Every request keeps its first tokens.  A cluster: every block of threads makes the prefix sums for itself and does its share of
+// the entries, the first one updates lengths and stack when all have read them.  Freed blocks go on the stack with the last one popped first, so a trim to the lengths
 // before a reservation leaves the stack as that found it.
 __global__ void __launch_bounds__(kTableThreads) trim_kernel(TableParams p) {
   __shared__ Sums warp_sums[33];
-  __shared__ int32_t off_s[kSearchRows + 1];
+  __shared__ int32_t off_s[kSearchRows + 1], stay_s[kSearchRows];
   const int tid = threadIdx.x, threads = blockDim.x;
   const bool first = blockIdx.z == 0;
   griddep_wait();
@@ -194,7 +239,12 @@ __global__ void __launch_bounds__(kTableThreads) trim_kernel(TableParams p) {
   for (int r0 = 0; r0 < p.requests; r0 += threads) {
     const int r = r0 + tid;
     Sums part;
-    const int64_t mine = r < p.requests ? blocks_of(held(r), p.log_block) - blocks_of(kept(r), p.log_block) : 0;
+    int64_t mine = 0;
+    if (r < p.requests) {
+      const int64_t stay = blocks_of(kept(r), p.log_block);
+      if (in_smem) stay_s[r] = (int)stay;
+      mine = blocks_of(held(r), p.log_block) - stay;
+    }
     const Sums at = block_exclusive({mine, 0}, warp_sums, part);
     if (r < p.requests && (in_smem || first)) off[r] = (int32_t)(gone + at.a);
     gone += part.a;
@@ -205,7 +255,7 @@ __global__ void __launch_bounds__(kTableThreads) trim_kernel(TableParams p) {
   const int64_t top = avail + gone - 1;
   for (int64_t f = (int64_t)blockIdx.z * threads + tid; f < gone; f += (int64_t)gridDim.z * threads) {
     const int r = row_of(off, p.requests, f);
-    int32_t* entry = p.table + r * p.table_row + blocks_of(kept(r), p.log_block) + (f - off[r]);
+    int32_t* entry = p.table + r * p.table_row + (in_smem ? stay_s[r] : blocks_of(kept(r), p.log_block)) + (f - off[r]);
     if (top - f < p.blocks) p.free_blocks[top - f] = *entry;
     *entry = -1;
   }
@@ -215,13 +265,11 @@ __global__ void __launch_bounds__(kTableThreads) trim_kernel(TableParams p) {
   if (tid == 0) *p.free_count = (int32_t)min(avail + gone, (int64_t)p.blocks);
 }
 
-// one block of threads where a few rounds of it do, else a cluster of eight
-int launch_tables(const char* what, void (*kern)(TableParams), const TableParams& p, int64_t entries, cudaStream_t st) {
-  const int64_t most = entries > p.requests ? entries : p.requests;
+unsigned table_threads(int64_t entries, int64_t requests) {
+  const int64_t most = entries > requests ? entries : requests;
   unsigned threads = 128;
   while (threads < kTableThreads && threads < most) threads *= 2;
-  const unsigned cluster = entries > kAlone ? 8 : 1;
-  return launch_cluster(what, kern, dim3(1, 1, cluster), cluster, threads, 0, st, p);
+  return threads;
 }
 
 // ------------------------------------------------------------------------------------------ write
@@ -314,7 +362,15 @@ __global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(WriteParams p)
     const int64_t t = t0 - 1 + tid;
     if (t >= 0 && t < p.tokens) my_slot = p.slot_map[t];
   }
-  if (kSmall) fetch(first, 0);
+  if (kSmall) {
+    fetch(first, 0);
+  } else {                                                   // into L2, while it is found out which of them are this block's
+    constexpr int kLines = D * (int)sizeof(T) / 128;
+    for (int x = tid; x < W * kLines; x += kWriteThreads)
+      if (t0 + x / kLines < p.tokens)
+        prefetch_l2(reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.x[first & 1]) + (first >> 1) * p.sh[first & 1] +
+                                                     (t0 + x / kLines) * p.st[first & 1]) + x % kLines * 128);
+  }
   if (tid <= kSpan) slot_s[tid] = my_slot < p.slots ? my_slot : -1;
   if (tid == 0) {
     begin_s = W;
@@ -590,10 +646,15 @@ extern "C" int nvfp4_paged_reserve(const int32_t* new_lens, int32_t* lengths, in
   NVFP4_REQUIRE(lb >= 0, "nvfp4_paged_reserve: block_size must be 16, 32, 64 or 128");
   NVFP4_REQUIRE(requests >= 1 && requests < (1 << 30) && width >= 1 && width < (1 << 30) && blocks >= 0 && blocks < INT32_MAX,
                 "nvfp4_paged_reserve: sizes out of range");
-  NVFP4_REQUIRE(slots >= 0 && slots < INT32_MAX, "nvfp4_paged_reserve: slot count out of range");
+  NVFP4_REQUIRE(slots >= 0 && slots < (1ll << 30), "nvfp4_paged_reserve: slot count out of range");
   const TableParams p{new_lens, lengths, table, table_row, const_cast<int32_t*>(free_blocks), free_count, (int)requests, (int)width,
                       (int)blocks, lb, slots, slot_map, positions, cu_seqlens, shortage, workspace};
-  return launch_tables("nvfp4_paged_reserve", reserve_kernel, p, slots, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool alone = slots <= kAlone;
+  const int rc = launch("nvfp4_paged_reserve", reserve_kernel, dim3(1), table_threads(alone ? slots : 0, requests), 0, st, p, alone ? 1 : 0);
+  if (rc != 0 || alone) return rc;
+  const int64_t grid = (slots + 1023) / 1024;
+  return launch("nvfp4_paged_reserve", reserve_fill_kernel, dim3((unsigned)(grid < 592 ? grid : 592)), 256, 0, st, p);
 }
 
 extern "C" int nvfp4_paged_trim(const int32_t* keep_lens, int32_t* lengths, int32_t* table, int64_t table_row,
@@ -606,7 +667,11 @@ extern "C" int nvfp4_paged_trim(const int32_t* keep_lens, int32_t* lengths, int3
   NVFP4_REQUIRE(requests * width < INT32_MAX, "nvfp4_paged_trim: the table has too many entries");
   const TableParams p{keep_lens, lengths, table, table_row, free_blocks, free_count, (int)requests, (int)width, (int)blocks, lb, 0,
                       nullptr, nullptr, nullptr, nullptr, workspace};
-  return launch_tables("nvfp4_paged_trim", trim_kernel, p, requests * width, static_cast<cudaStream_t>(stream));
+  // one block of threads, or a cluster of eight for wide tables; of a table's entries a call gives few back, mostly
+  const int64_t entries = requests * width / 4;
+  const unsigned cluster = entries > kAlone ? 8 : 1;
+  return launch_cluster("nvfp4_paged_trim", trim_kernel, dim3(1, 1, cluster), cluster, table_threads(entries, requests), 0,
+                        static_cast<cudaStream_t>(stream), p);
 }
 
 extern "C" int nvfp4_kv8_write(const void* key, const void* value, int dtype, int64_t tokens, int64_t hk, int d, int64_t skt,
