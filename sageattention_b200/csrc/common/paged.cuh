@@ -4,8 +4,9 @@
 // A unit is (request, KV head, ROWS query rows): the heads of a group, for each of the request's query tokens.  Its keys, as
 // far as its last row sees them, are cut into tiles of TILE; all tiles of all units are one list (request, head, rows, keys),
 // and CTA c takes entries [c, c + 1) * ceil(total / CTAs) of it, so ragged lengths need no plan on the host.  In front of a
-// unit's tiles the list has kUnitCost entries without work, for what a unit costs besides (its query, its merge): decode of
-// 160 requests of 1 to 4100 keys, where a CTA held up to four short units.  A CTA can hold
+// unit's tiles the list has unit_cost() entries without work, for what a unit costs besides (its query, its merge).  With one, two,
+// three and four of them: decode of 160 requests of 1 to 4100 keys 23.1, 22.7, 24.2, 24.3 us; drafts of 32 requests 79.5, 70.0,
+// 67.7, 69.4; chunks and single tokens in one batch at D 256 87.6, 82.7, 79.0, 79.4.  A CTA can hold
 // the end of one unit and the beginning of another, each a partial result of its own (slots 2 c and 2 c + 1).
 #pragma once
 #include <cuda_runtime.h>
@@ -15,7 +16,6 @@
 
 namespace nvfp4 {
 
-constexpr int kUnitCost = 1;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct PagedParams {
@@ -52,6 +52,8 @@ __device__ __forceinline__ int token_of(const PagedParams& p, int i) {
   return (int)((__umulhi((uint32_t)i, p.g_mul) + (uint32_t)i) >> p.g_shift);
 }
 
+__host__ __device__ constexpr int unit_cost(int rows) { return rows <= 8 ? 2 : 3; }
+
 // What a request asks for: its query tokens [t0, t0 + n), its keys, its units.
 template <int ROWS, int TILE>
 struct Request {
@@ -81,7 +83,7 @@ struct Request {
     return max((limit(p, row_tile) + TILE - 1) / TILE, 1);
   }
   __device__ __forceinline__ int64_t head_entries(const PagedParams& p) const {
-    int64_t sum = (int64_t)kUnitCost * row_tiles;
+    int64_t sum = (int64_t)unit_cost(ROWS) * row_tiles;
     for (int j = 0; j < row_tiles; ++j) sum += tiles(p, j);
     return sum;
   }
@@ -90,6 +92,7 @@ struct Request {
 // The rest of a CTA's share, segment by segment: open() gives tiles [from, to) of a unit, close() goes on to the next one.
 template <int ROWS, int TILE>
 struct Walk {
+  static constexpr int kUnitCost = unit_cost(ROWS);
   Request<ROWS, TILE> q;
   int r, head, row_tile, entry, tiles;        // entry: -kUnitCost .. -1 without work, then the unit's tiles
   int from, to;
@@ -151,36 +154,29 @@ __device__ __forceinline__ int64_t deal_tiles(const PagedParams& p, int64_t* lis
   auto weight = [&](int r) -> int64_t {
     return r < p.requests ? p.hk * Request<ROWS, TILE>(p, r).head_entries(p) : 0;
   };
-  // of up to THREADS requests a thread keeps its one, and the sum its place
-  const int64_t first = weight(tid);
-  int64_t more = 0, before, first_before;
-  const int64_t first_all = block_sum(first, first_before);
-  int64_t total = first_all;
-  if (p.requests > THREADS) {
-    for (int r = tid + THREADS; r < p.requests; r += THREADS) more += weight(r);
-    total += block_sum(more, before);
+  constexpr int kUnitCost = unit_cost(ROWS);
+  // a thread has `each` requests in a row
+  const int each = (p.requests + THREADS - 1) / THREADS, r0 = tid * each;
+  int64_t mine = 0, before;
+  if (each == 1) {
+    mine = weight(r0);
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < each; ++i) mine += weight(r0 + i);
   }
+  const int64_t total = block_sum(mine, before);
   const int64_t share = (total + gridDim.x - 1) / gridDim.x, begin = (int64_t)blockIdx.x * share;
   at.left = min(total, begin + share) - begin;
   if (at.left <= 0) return share;
-  if (tid == 0) list[kW] = -1;
-  __syncthreads();
-  int64_t base = 0;
-  for (int r0 = 0;; r0 += THREADS) {
-    int64_t w = first, all = first_all;
-    before = first_before;
-    if (r0 > 0) {
-      w = weight(r0 + tid);
-      all = block_sum(w, before);
-    }
-    if (begin >= base + before && begin < base + before + w) {
-      list[kW] = r0 + tid;
-      list[kW + 1] = begin - base - before;
-    }
-    __syncthreads();
-    if (list[kW] >= 0) break;
-    base += all;
+  if (begin >= before && begin < before + mine) {
+    int r = r0;
+    int64_t rest = begin - before;
+    if (each > 1)
+      for (int64_t w; rest >= (w = weight(r)); ++r) rest -= w;
+    list[kW] = r;
+    list[kW + 1] = rest;
   }
+  __syncthreads();
   at.r = (int)list[kW];
   at.q = Request<ROWS, TILE>(p, at.r);
   int64_t rest = list[kW + 1];
