@@ -14,6 +14,12 @@ second compute path.
     torch.ops.sageattention_b200.nvfp4_kv_append(k_new, v_new, knv, ksc, vnv, vsc, partial, rk, rv, pos)
     out = torch.ops.sageattention_b200.nvfp4_hybrid_decode(q, knv, ksc, vnv, vsc, rk, rv, length, window,
                                                            scaling, groups)
+    slot_map, positions, cu, shortage = torch.ops.sageattention_b200.paged_kv_reserve(new, lengths, table, free, count, n, block)
+    torch.ops.sageattention_b200.paged_kv_trim(keep, lengths, table, free, count, block)
+    torch.ops.sageattention_b200.fp8_kv_write(key, value, slot_map, k_cache, v_cache, k_scale, v_scale)
+    out, lse = torch.ops.sageattention_b200.fp8_paged_decode(q, k_cache, v_cache, k_scale, v_scale, table, lengths, scaling, groups)
+    out, lse = torch.ops.sageattention_b200.fp8_paged_attention(q, cu, k_cache, v_cache, k_scale, v_scale, table, lengths,
+                                                                scaling, groups)
 """
 
 from __future__ import annotations
@@ -24,6 +30,7 @@ import torch
 
 from . import flash
 from . import kv_cache as _kvc
+from . import paged_cache as _paged
 
 _NS = "sageattention_b200"
 
@@ -209,3 +216,66 @@ def nvfp4_hybrid_decode(q: torch.Tensor, knv: torch.Tensor, ksc: torch.Tensor, v
 @nvfp4_hybrid_decode.register_fake
 def _(q, knv, ksc, vnv, vsc, rk, rv, length, recent_window, scaling, groups):
     return q.new_empty(q.shape)
+
+
+# ---------------------------------------------------------------- paged 8-bit KV cache
+@torch.library.custom_op(f"{_NS}::paged_kv_reserve", mutates_args=("lengths", "block_table", "free_count"))
+def paged_kv_reserve(new_lens: torch.Tensor, lengths: torch.Tensor, block_table: torch.Tensor, free_blocks: torch.Tensor,
+                     free_count: torch.Tensor, num_slots: int,
+                     block_size: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``paged_kv_reserve``: (slot_map, positions, cu_seqlens, shortage)."""
+    return tuple(_paged.paged_kv_reserve(new_lens, lengths, block_table, free_blocks, free_count, num_slots, block_size))
+
+
+@paged_kv_reserve.register_fake
+def _(new_lens, lengths, block_table, free_blocks, free_count, num_slots, block_size):
+    i32 = lambda n: new_lens.new_empty(n, dtype=torch.int32)
+    return new_lens.new_empty(num_slots, dtype=torch.int64), i32(num_slots), i32(new_lens.shape[0] + 1), i32(1)
+
+
+@torch.library.custom_op(f"{_NS}::paged_kv_trim", mutates_args=("lengths", "block_table", "free_blocks", "free_count"))
+def paged_kv_trim(keep_lens: torch.Tensor, lengths: torch.Tensor, block_table: torch.Tensor, free_blocks: torch.Tensor,
+                  free_count: torch.Tensor, block_size: int) -> None:
+    _paged.paged_kv_trim(keep_lens, lengths, block_table, free_blocks, free_count, block_size)
+
+
+@paged_kv_trim.register_fake
+def _(keep_lens, lengths, block_table, free_blocks, free_count, block_size):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::fp8_kv_write", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"))
+def fp8_kv_write(key: torch.Tensor, value: torch.Tensor, slot_map: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
+    """``fp8_kv_write`` (caches as float8_e4m3fn or uint8)."""
+    _paged.fp8_kv_write(key, value, slot_map, k_cache, v_cache, k_scale, v_scale)
+
+
+@fp8_kv_write.register_fake
+def _(key, value, slot_map, k_cache, v_cache, k_scale, v_scale):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::fp8_paged_decode", mutates_args=())
+def fp8_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                     block_table: torch.Tensor, lengths: torch.Tensor, scaling: float,
+                     groups: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _paged.fp8_paged_decode(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, scaling, groups, return_lse=True)
+
+
+@fp8_paged_decode.register_fake
+def _(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, scaling, groups):
+    return q.new_empty(q.shape), q.new_empty(q.shape[0], q.shape[1], dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_NS}::fp8_paged_attention", mutates_args=())
+def fp8_paged_attention(q: torch.Tensor, cu_seqlens: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                        v_scale: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, scaling: float,
+                        groups: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _paged.fp8_paged_attention(q, cu_seqlens, k_cache, v_cache, k_scale, v_scale, block_table, lengths, scaling, groups,
+                                      return_lse=True)
+
+
+@fp8_paged_attention.register_fake
+def _(q, cu_seqlens, k_cache, v_cache, k_scale, v_scale, block_table, lengths, scaling, groups):
+    return q.new_empty(q.shape), q.new_empty(q.shape[0], q.shape[1], dtype=torch.float32)

@@ -5,13 +5,15 @@
 Stands in for the reference's ``example/nvfp4_decode_demo.py`` (which patches a pretrained Qwen2):
 no checkpoint is assumed here, so the model is a randomly initialised pre-norm decoder with
 rotary embeddings and grouped-query attention (default 8 query heads on 2 KV heads, head dim
-128).  The prompt is prefilled once with plain bf16 attention; decoding then runs three ways from
+128).  The prompt is prefilled once with plain bf16 attention; decoding then runs four ways from
 the same prompt state --
 
   bf16    keys and values kept in bf16, ``scaled_dot_product_attention`` per step (the baseline);
   fp4     each layer appends the post-RoPE K and V to its ``NVFP4KVCache`` and attends with
           ``nvfp4_flash_decode_prequant`` over the packed cache;
-  hybrid  ``NVFP4KVCache.hybrid_decode``: recent tokens in bf16, older prefix in NVFP4 --
+  hybrid  ``NVFP4KVCache.hybrid_decode``: recent tokens in bf16, older prefix in NVFP4;
+  fp8     one ``FP8PagedKVCache`` for all layers: blocks and slots of the step's tokens reserved on the GPU, keys and
+          values in e4m3 with a scale for each block and head --
 
 and the demo reports what the reference's demo reports: greedy top-1 agreement with the bf16 run,
 the teacher-forced logit cosine per step, cache memory per mode, and the per-step latency.
@@ -26,7 +28,7 @@ import time
 import torch
 import torch.nn.functional as F
 
-from . import NVFP4KVCache, nvfp4_flash_decode_prequant
+from . import FP8PagedKVCache, NVFP4KVCache, nvfp4_flash_decode_prequant
 
 
 class TinyGQADecoder(torch.nn.Module):
@@ -93,11 +95,13 @@ def prefill(model, tokens):
 
 @torch.no_grad()
 def decode_step(model, token, position, state, mode):
-    """One decode step; ``state`` is per-layer: (K, V) bf16 tensors or an NVFP4KVCache."""
+    """One decode step; ``state`` is per-layer: (K, V) bf16 tensors or an NVFP4KVCache, or one FP8PagedKVCache."""
     x = model.emb[token][:, None]
     pos = torch.tensor([position], device=x.device)
     g = model.h // model.hk
     scaling = model.d ** -0.5
+    if mode == "fp8":
+        step = state.reserve(torch.ones_like(state.lengths), token.shape[0])
     for li, blk in enumerate(model.blocks):
         q, k, v = model.qkv(blk, x, pos)
         if mode == "bf16":
@@ -106,6 +110,9 @@ def decode_step(model, token, position, state, mode):
             state[li] = (kc, vc, n + 1)
             attn = F.scaled_dot_product_attention(q, kc[:, :, :n + 1].repeat_interleave(g, 1),
                                                   vc[:, :, :n + 1].repeat_interleave(g, 1))
+        elif mode == "fp8":
+            state.write(li, k, v, step.slot_map)
+            attn = state.decode(li, q, scaling, g)
         else:
             cache = state[li]
             cache.append(k, v)
@@ -126,6 +133,16 @@ def fresh_state(model, kv, mode, capacity, window):
             kc[:, :, :n], vc[:, :, :n] = k, v
             out.append((kc, vc, n))
         return out
+    if mode == "fp8":
+        k0 = kv[0][0]
+        s = k0.shape[2]
+        block = 64
+        cache = FP8PagedKVCache(len(kv), z * -(-capacity // block), model.hk, model.d, z, capacity, k0.device, block_size=block)
+        step = cache.reserve(torch.full_like(cache.lengths, s), z * s)
+        rows = lambda t: t.transpose(1, 2).reshape(z * s, model.hk, model.d)     # request by request
+        for li, (k, v) in enumerate(kv):
+            cache.write(li, rows(k), rows(v), step.slot_map)
+        return cache
     caches = []
     for k, v in kv:
         c = NVFP4KVCache(z, model.hk, model.d, capacity, k.device, k.dtype,
@@ -182,14 +199,18 @@ def main(argv=None):
     print(f"model: {a.layers} layers, {a.heads} heads on {a.kv_heads} KV heads, head dim {a.head_dim}; "
           f"prompt {a.prompt} tokens x batch {a.batch}, {a.new} new tokens (greedy)")
     print(f"  bf16 cache : {ref_ms:.3f} ms/step")
-    for mode in ("fp4", "hybrid"):
+    for mode in ("fp4", "hybrid", "fp8"):
         toks, _, ms, state = generate(model, kv, first, a.new, mode, cap, a.window)
         agree = float((toks == ref_toks).float().mean())
         _, forced_logits, _, _ = generate(model, kv, first, a.new, mode, cap, a.window,
                                           forced=[ref_toks[:, i] for i in range(a.new)])
         cos = float(F.cosine_similarity(forced_logits.flatten(0, 1), ref_logits.flatten(0, 1), dim=-1).mean())
-        mem = sum(c.hybrid_bytes() if mode == "hybrid" else c.fp4_bytes() for c in state)
-        bf = sum(c.bf16_bytes() for c in state)
+        if mode == "fp8":
+            mem = state.held_bytes()
+            bf = 2 * a.layers * a.batch * (a.prompt + a.new) * a.kv_heads * a.head_dim * 2
+        else:
+            mem = sum(c.hybrid_bytes() if mode == "hybrid" else c.fp4_bytes() for c in state)
+            bf = sum(c.bf16_bytes() for c in state)
         report[mode] = {"agreement": agree, "logit_cos": cos, "ms_per_step": ms, "bytes": mem, "bf16_bytes": bf}
         print(f"  {mode:<6} cache: {ms:.3f} ms/step; free-running top-1 agreement with bf16 {agree * 100:.1f} %; "
               f"teacher-forced logit cosine {cos:.4f}; cache {mem / 1e6:.2f} MB vs bf16 {bf / 1e6:.2f} MB "

@@ -145,3 +145,7 @@ class FP8PagedKVCache:
     def cache_bytes(self) -> int:
         """Bytes of codes and scales, all layers and blocks."""
         return 2 * self.num_layers * self.num_blocks * self.hk * (self.block_size * self.d + 4)
+
+    def held_bytes(self) -> int:
+        """Bytes of the blocks that requests hold, all layers (reads the stack's size: synchronises)."""
+        return self.cache_bytes() // self.num_blocks * (self.num_blocks - int(self.free_count))

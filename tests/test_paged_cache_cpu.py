@@ -116,3 +116,25 @@ def test_python_entries_refuse_cpu_tensors():
     cache = nv.FP8PagedKVCache(2, 5, 3, 128, 2, 65, "cpu", block_size=32)
     assert cache.block_table.shape == (2, 3) and int(cache.free_count) == 5 and cache.free_blocks.tolist() == [4, 3, 2, 1, 0]
     assert cache.cache_bytes() == sum(t.numel() * t.element_size() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale))
+
+
+def test_custom_ops_infer_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import sageattention_b200.nvfp4.custom_ops  # noqa: F401  (registers the ops)
+    ns = torch.ops.sageattention_b200
+    with FakeTensorMode():
+        i = lambda *s: torch.empty(*s, dtype=torch.int32)
+        slots, pos, cu, short = ns.paged_kv_reserve(i(3), i(3), i(3, 9), i(20), i(1), 50, 16)
+        assert slots.shape == (50,) and slots.dtype == torch.int64 and pos.shape == (50,) and cu.shape == (4,) and short.shape == (1,)
+        assert {pos.dtype, cu.dtype, short.dtype} == {torch.int32}
+        assert ns.paged_kv_trim(i(3), i(3), i(3, 9), i(20), i(1), 16) is None
+        c, s = torch.empty(20, 2, 16, 128, dtype=torch.float8_e4m3fn), torch.empty(20, 2)
+        x = torch.empty(50, 2, 128, dtype=torch.bfloat16)
+        assert ns.fp8_kv_write(x, x, slots, c, c, s, s) is None
+        q = torch.empty(3, 8, 1, 128, dtype=torch.bfloat16)
+        out, lse = ns.fp8_paged_decode(q, c, c, s, s, i(3, 9), i(3), 0.1, 4)
+        assert out.shape == q.shape and out.dtype == q.dtype and lse.shape == (3, 8) and lse.dtype == torch.float32
+        q = torch.empty(50, 8, 128, dtype=torch.float16)
+        out, lse = ns.fp8_paged_attention(q, cu, c, c, s, s, i(3, 9), i(3), 0.1, 4)
+        assert out.shape == q.shape and out.dtype == q.dtype and lse.shape == (50, 8)

@@ -574,6 +574,54 @@ def test_two_captured_decodes_replayed_in_turn_and_on_other_streams():
     assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
 
 
+def test_registered_operators_are_the_same_calls():
+    import sageattention_b200.nvfp4.custom_ops  # noqa: F401
+    ns, nv = torch.ops.sageattention_b200, _nv()
+    a, b = (nv.FP8PagedKVCache(1, 12, 2, 128, 3, 64, "cuda", block_size=16) for _ in range(2))
+    new = _i32([5, 0, 20])
+    step = a.reserve(new, 27)
+    got = ns.paged_kv_reserve(new, b.lengths, b.block_table, b.free_blocks, b.free_count, 27, 16)
+    for x, y in zip(step, got):
+        assert torch.equal(x, y)
+    key, value = _rows((27, 2, 128), 1, torch.bfloat16).cuda(), _rows((27, 2, 128), 2, torch.bfloat16).cuda()
+    a.write(0, key, value, step.slot_map)
+    ns.fp8_kv_write(key, value, got[0], b.k[0], b.v[0], b.k_scale[0], b.v_scale[0])
+    q = _rows((27, 8, 128), 3, torch.bfloat16).cuda()
+    for x, y in zip(a.attend(0, q, step.cu_seqlens, 0.1, 4, True),
+                    ns.fp8_paged_attention(q, got[2], b.k[0], b.v[0], b.k_scale[0], b.v_scale[0], b.block_table, b.lengths, 0.1, 4)):
+        assert torch.equal(x, y)
+    for x, y in zip(a.decode(0, q[:3, :, None], 0.1, 4, True),
+                    ns.fp8_paged_decode(q[:3, :, None], b.k[0], b.v[0], b.k_scale[0], b.v_scale[0], b.block_table, b.lengths, 0.1, 4)):
+        assert torch.equal(x, y)
+    a.trim(_i32([1, 0, 17]))
+    ns.paged_kv_trim(_i32([1, 0, 17]), b.lengths, b.block_table, b.free_blocks, b.free_count, 16)
+    assert torch.equal(a.block_table, b.block_table) and torch.equal(a.free_blocks, b.free_blocks) and torch.equal(a.lengths, b.lengths)
+
+
+def test_positions_feed_the_rotary_pack():
+    """A step's positions are what ``rope_quant_nvfp4`` takes."""
+    nv = _nv()
+    cache = nv.FP8PagedKVCache(1, 12, 1, 128, 2, 64, "cuda", block_size=16)
+    cache.reserve(_i32([7, 30]), 37)
+    step = cache.reserve(_i32([2, 1]), 5)
+    assert step.positions.tolist() == [7, 8, 30, 0, 0]
+    ang = torch.arange(64, device="cuda")[:, None] * 0.01 * torch.arange(64, device="cuda")[None]
+    x = _rows((1, 5, 128), 3, torch.bfloat16).cuda()
+    packed = nv.rope_quant_nvfp4(x, ang.cos(), ang.sin(), positions=step.positions)
+    one = nv.rope_quant_nvfp4(x[:, 2:3], ang.cos(), ang.sin(), pos0=30)
+    assert torch.equal(packed[0][:, 2], one[0][:, 0])
+
+
+def test_the_demo_runs_with_the_paged_cache():
+    from sageattention_b200 import _lib
+    from sageattention_b200.nvfp4 import demo_decode
+    rep = demo_decode.main(["--layers", "2", "--hidden", "512", "--heads", "4", "--kv-heads", "2", "--vocab", "512", "--batch", "2",
+                            "--prompt", "150", "--new", "4", "--window", "64"])
+    assert math.isfinite(rep["fp8"]["logit_cos"])
+    assert rep["fp8"]["bytes"] == 2 * 2 * 2 * 3 * 2 * (64 * 128 + 4)      # layers, K and V, requests, blocks, heads
+    assert _lib.read_status("cuda:0") == 0
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals():
     nv = _nv()
