@@ -15,6 +15,7 @@
 // What bounds it (D = 128): a key tile of 256 rows is 2580 clocks of products on an SM (S with 64 keys reads its operands
 // from shared memory at 48 clocks an instruction instead of 32) and 2048 of ex2.
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "common/abi.cuh"
 #include "common/bwd_util.cuh"
 #include "common/kv8.cuh"
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
   __shared__ Place place_s;
   __shared__ int64_t share_s;                              // entries of a full share
   __shared__ TileInfo info_s[kInfo];
-  __shared__ float m_s[2][128], l_s[128], c_s[128];
+  __shared__ float m_s[2][128], l_s[128], c_s[2][128];
   const int tid = threadIdx.x, lane = tid & 31, warp = warp_index();
   volatile int* err = &expired;
 
@@ -298,6 +299,16 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     }
   } else if (warp >= C::kSoft + 4) {
     fewer_registers<C::kRegsIssue>();
+    if (warp == C::kSoft + 5) {
+      // query rows of all units of this CTA into L2: a unit's softmax begins with them, and from HBM they were 5 us
+      constexpr int kLines = D * (int)sizeof(T) / 128;
+      for (Place at = place_s; at.open(); at.close(p)) {
+        const int rows = at.q.rows(p, at.row_tile);
+        for (int i = lane; i < rows * kLines; i += 32)
+          prefetch_l2(reinterpret_cast<const uint8_t*>(query_row<T>(p, at.q.t0, at.row_tile * C::kRows + i / kLines, at.head)) +
+                      i % kLines * 128);
+      }
+    }
     if (warp == C::kSoft + 4) {
     // ------------------------------------------------------------------ issue of the products
     Place at = place_s;
@@ -393,46 +404,73 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       const int i_row = at.row_tile * C::kRows + row;      // of the request
       // ---- query rows: all products of the segment before are complete (each group has seen its last S)
       named_bar_sync(1, 32 * C::kSoft);
-      float c_row = 0.0f;
+      // A warp loads its 32 rows together, D / 8 lanes a row: a thread's own row would be 32 lines an instruction, and took
+      // 9 to 12 us a unit.
       if (both || group == 0) {
-        const T* pq = query_row<T>(p, at.q.t0, live ? i_row : 0, at.head);
-        float big = 0.0f;
-        if (live) {
-#pragma unroll 4
-          for (int e = 0; e < D / 8; ++e) {
-            float v[8];
-            load8<T>(pq + e * 8, v);
+        constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kBatch = 8;       // of a row; rows an instruction; loads in flight
+        const int base = (both ? group * 128 : 0) + wq * 32;
+        const uint32_t dst = smem_u32(smem + C::kQ) + (both ? group : 0) * C::kOperand;
+        const int e = lane % kLanes;                       // piece of eight elements
+        const bool aligned = ((reinterpret_cast<uintptr_t>(p.q) | (uint64_t)(p.sqt * 2) | (uint64_t)(p.sqh * 2)) & 15) == 0;
+#pragma unroll 1
+        for (int x0 = 0; x0 < 32 / kAtOnce; x0 += kBatch) {
+          uint4 raw[kBatch];
+          auto piece = [&](int x) {
+            const int r = base + (x0 + x) * kAtOnce + lane / kLanes;
+            return query_row<T>(p, at.q.t0, at.row_tile * C::kRows + min(r, rows - 1), at.head) + e * 8;
+          };
+          if (aligned) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) big = fmaxf(big, fabsf(v[k]));
+            for (int x = 0; x < kBatch; ++x) raw[x] = *reinterpret_cast<const uint4*>(piece(x));
+          } else {
+#pragma unroll 1
+            for (int x = 0; x < kBatch; ++x) {
+              const uint16_t* t = reinterpret_cast<const uint16_t*>(piece(x));
+              const uint4 w = make_uint4(t[0] | (uint32_t)t[1] << 16, t[2] | (uint32_t)t[3] << 16, t[4] | (uint32_t)t[5] << 16,
+                                         t[6] | (uint32_t)t[7] << 16);
+#pragma unroll
+              for (int y = 0; y < kBatch; ++y)
+                if (y == x) raw[y] = w;
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < kBatch; ++x) {
+            const int in = wq * 32 + (x0 + x) * kAtOnce + lane / kLanes;
+            const bool there = (both ? group * 128 : 0) + in < rows;
+            // the row's largest magnitude, two values at a time
+            using T2 = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>::type;
+            auto two = [](uint32_t w) { return *reinterpret_cast<const T2*>(&w); };
+            T2 top = __hmax2(__hmax2(__habs2(two(raw[x].x)), __habs2(two(raw[x].y))),
+                             __hmax2(__habs2(two(raw[x].z)), __habs2(two(raw[x].w))));
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) {
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&top), o);
+              top = __hmax2(top, two(other));
+            }
+            const float big = fmaxf(to_f32<T>(top.x), to_f32<T>(top.y));
+            // largest element in [2^12, 2^13); scaling below zero turns q
+            const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -110), 127);
+            const float up = there ? copysignf(exp2_int(12 - ex), p.scale_log2) : 0.0f;
+            if (e == 0) c_s[both ? group : 0][in] = big == 0.0f ? 0.0f : fabsf(p.scale_log2) * exp2_int(ex - 12);
+            uint32_t h[4];
+            const uint32_t words[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const T2 t = two(words[k]);
+              h[k] = there ? pack_16x2<__half>(to_f32<T>(t.x) * up, to_f32<T>(t.y) * up) : 0u;
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + in * 128 + (e >> 3) * kSub + (((e & 7) ^ (in & 7)) << 4)),
+                         "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
+                         : "memory");
           }
         }
-        // largest element in [2^12, 2^13); scaling below zero turns q
-        const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -110), 127);
-        const float up = copysignf(exp2_int(12 - ex), p.scale_log2);
-        c_row = big == 0.0f ? 0.0f : ldexpf(fabsf(p.scale_log2), ex - 12);
-        const uint32_t dst = smem_u32(smem + C::kQ) + (both ? group : 0) * C::kOperand + row_in * 128;
-#pragma unroll 4
-        for (int e = 0; e < D / 8; ++e) {
-          float v[8];
-          uint32_t h[4] = {0, 0, 0, 0};
-          if (live) {
-            load8<T>(pq + e * 8, v);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) h[k] = pack_16x2<__half>(v[2 * k] * up, v[2 * k + 1] * up);
-          }
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (e >> 3) * kSub + (((e & 7) ^ (row_in & 7)) << 4)), "r"(h[0]),
-                       "r"(h[1]), "r"(h[2]), "r"(h[3])
-                       : "memory");
-        }
-        if (C::kGroups == 2 && !both) c_s[row_in] = c_row;
         fence_proxy_async_smem();
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full);
-      if (C::kGroups == 2 && !both) {                      // both groups work on the same rows
-        named_bar_sync(1, 32 * C::kSoft);
-        c_row = c_s[row_in];
-      }
+      // where both groups work on the same rows, the first one has loaded them
+      if (C::kGroups == 2 && !both) named_bar_sync(1, 32 * C::kSoft);
+      const float c_row = c_s[both ? group : 0][row_in];
       const int limit = live ? at.q.seen(p, i_row) : 0;    // keys that this row sees
       float m = -INFINITY, ref = -INFINITY, l = 0.0f;
 
