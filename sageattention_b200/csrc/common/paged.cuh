@@ -84,6 +84,7 @@ struct Request {
   }
   __device__ __forceinline__ int64_t head_entries(const PagedParams& p) const {
     int64_t sum = (int64_t)unit_cost(ROWS) * row_tiles;
+#pragma unroll 1
     for (int j = 0; j < row_tiles; ++j) sum += tiles(p, j);
     return sum;
   }
@@ -161,7 +162,7 @@ __device__ __forceinline__ int64_t deal_tiles(const PagedParams& p, int64_t* lis
   if (each == 1) {
     mine = weight(r0);
   } else {
-#pragma unroll 4
+#pragma unroll 1
     for (int i = 0; i < each; ++i) mine += weight(r0 + i);
   }
   const int64_t total = block_sum(mine, before);
@@ -171,8 +172,10 @@ __device__ __forceinline__ int64_t deal_tiles(const PagedParams& p, int64_t* lis
   if (begin >= before && begin < before + mine) {
     int r = r0;
     int64_t rest = begin - before;
-    if (each > 1)
+    if (each > 1) {
+#pragma unroll 1
       for (int64_t w; rest >= (w = weight(r)); ++r) rest -= w;
+    }
     list[kW] = r;
     list[kW + 1] = rest;
   }
@@ -194,6 +197,7 @@ __device__ __forceinline__ int64_t deal_tiles(const PagedParams& p, int64_t* lis
     at.head = (int)(rest / per_head);
     rest %= per_head;
     at.row_tile = 0;
+#pragma unroll 1
     while ((at.tiles = at.q.tiles(p, at.row_tile)) + kUnitCost <= rest) {
       rest -= at.tiles + kUnitCost;
       ++at.row_tile;
@@ -242,21 +246,28 @@ __device__ __forceinline__ void clear_untouched(const PagedParams& p) {
   const int h = p.hk * p.g;
   auto clear = [&](int64_t t0, int64_t t1) {
     T* out = static_cast<T*>(p.out);
+#pragma unroll 1
     for (int64_t i = t0 * h * D + threadIdx.x * 4; i < t1 * h * D; i += blockDim.x * 4) {
       const float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       store4<T>(out + i, z);
     }
-    if (p.lse != nullptr)
+    if (p.lse != nullptr) {
+#pragma unroll 1
       for (int64_t i = t0 * h + threadIdx.x; i < t1 * h; i += blockDim.x) p.lse[i] = -INFINITY;
+    }
   };
-  for (int r = blockIdx.x; r < p.requests; r += gridDim.x) {
+  // in turn: requests of this CTA, then (the last CTA) the tokens in front of the first one's and behind the last one's
+  auto inside = [&](int t) { return min(max((int64_t)t, (int64_t)0), p.tokens); };
+  const int extra = p.cu != nullptr && blockIdx.x == gridDim.x - 1 ? 2 : 0;
+#pragma unroll 1
+  for (int r = (int)blockIdx.x - (int)gridDim.x * extra; r < p.requests; r += gridDim.x) {
+    if (r < 0) {
+      const bool front = r < -(int)gridDim.x;
+      clear(front ? 0 : inside(p.cu[p.requests]), front ? inside(p.cu[0]) : p.tokens);
+      continue;
+    }
     const Request<ROWS, TILE> q(p, r);
     if (q.len == 0) clear(q.t0, q.t0 + q.n);
-  }
-  if (p.cu != nullptr && blockIdx.x == gridDim.x - 1) {
-    auto inside = [&](int t) { return min(max((int64_t)t, (int64_t)0), p.tokens); };
-    clear(0, inside(p.cu[0]));
-    clear(inside(p.cu[p.requests]), p.tokens);
   }
 }
 

@@ -810,7 +810,7 @@ std::tuple<Tensor, OptTensor> kv8_attention(const Tensor& query, const OptTensor
   const int64_t t = query.size(0), h = query.size(1), d = query.size(-1);
   require(d == p.d, "query must have the cache's head dim");
   require(g >= 1 && h == p.hk * g, "num_key_value_groups must equal H // Hk");
-  const Tensor q = query.stride(-1) == 1 ? query : query.contiguous();
+  const Tensor q = token_rows(query, "query must be [T, H, D] or [Z, H, 1, D]");
   Tensor out = c.empty(query.sizes(), query.scalar_type());
   OptTensor lse;
   if (want_lse) lse = c.empty({t, h}, at::kFloat);

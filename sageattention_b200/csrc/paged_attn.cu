@@ -18,7 +18,6 @@
 // 2^-(14 + kLift) of the largest 2^-(25 + kLift) of that.
 #include <limits.h>
 #include "common/abi.cuh"
-#include "common/bwd_util.cuh"
 #include "common/fp4.cuh"
 #include "common/kv8.cuh"
 #include "common/launch.cuh"
@@ -196,11 +195,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
         float big = 0.0f;
 #pragma unroll
         for (int u = 0; u < D / 128; ++u) {
-          float v[2][8];
-          load8<T>(pq + (u * 8 + e0) * 16, v[0]);
-          load8<T>(pq + (u * 8 + e0) * 16 + 8, v[1]);
+          constexpr int kPer = 16 / (int)sizeof(T);
+          uint4 raw[16 / kPer];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) x[u][k] = row < rows ? v[k / 8][k % 8] : 0.0f;
+          for (int w = 0; w < 16 / kPer; ++w) raw[w] = reinterpret_cast<const uint4*>(pq + (u * 8 + e0) * 16)[w];
+          const T* t = reinterpret_cast<const T*>(raw);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) x[u][k] = row < rows ? to_f32<T>(t[k]) : 0.0f;
         }
 #pragma unroll
         for (int u = 0; u < D / 128; ++u)
@@ -465,52 +466,54 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
           }
         }
       const int slot = first ? 2 * cta : 2 * cta + 1;
-#pragma unroll
+#pragma unroll 1
       for (int pass = 0; pass < NT * (D / 64); ++pass) {
         const int nt = pass % NT, cols = pass / NT;        // rows 8 nt .., columns 64 cols ..
-        if (nt * 8 < rows) {
+        if (nt * 8 >= rows) continue;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+        for (int x = 0; x < NT * (D / 64); ++x)
+          if (x == pass) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float* x = o[cols * 4 + i][nt];
-              const uint32_t dst = shared + ((warp * 8 + 2 * c4 + k) * 64 + ((i ^ c4) * 16) + 2 * g8) * 4;
-              asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(dst), "f"(x[k]), "f"(x[2 + k]) : "memory");
-            }
-          __syncthreads();
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int in = warp * 2 + y, row = nt * 8 + in;
-            if (row < rows) {
-              float2 sum = make_float2(0.0f, 0.0f);
-              float top = m_s[0][row], total_l = 0.0f;
-#pragma unroll
-              for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][row]);
-#pragma unroll
-              for (int w = 0; w < kWarps; ++w) {
-                const float2 v = lds_f2(shared + ((w * 8 + in) * 64 + (((lane >> 3) ^ (in >> 1)) * 16) + 2 * (lane & 7)) * 4);
-                sum.x += v.x;
-                sum.y += v.y;
-                total_l += top == -INFINITY ? l_s[w][row] : l_s[w][row] * ex2_approx(m_s[w][row] - top);   // no key: 0, or NaN
+              for (int k = 0; k < 2; ++k) {
+                const float* v = o[x / NT * 4 + i][x % NT];
+                const uint32_t dst = shared + ((warp * 8 + 2 * c4 + k) * 64 + ((i ^ c4) * 16) + 2 * g8) * 4;
+                asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(dst), "f"(v[k]), "f"(v[2 + k]) : "memory");
               }
-              if (whole) {
-                const float f = total_l == 0.0f ? 0.0f : 1.0f / total_l;
-                const int64_t to = out_row(p, use.q.t0 * p.g + use.row_tile * kRows + row, use.head);
-                T* dst = static_cast<T*>(p.out) + to * D + cols * 64 + lane * 2;
-                if constexpr (S::kTwo) *reinterpret_cast<float2*>(dst) = make_float2(sum.x * f, sum.y * f);
-                else *reinterpret_cast<uint32_t*>(dst) = pack_16x2<T>(sum.x * f, sum.y * f);
-                if (cols == 0 && lane == 0 && p.lse != nullptr) p.lse[to] = lse_of(top, total_l);
-              } else {
-                *reinterpret_cast<float2*>(p.ws_acc + ((int64_t)slot * kRows + row) * D + cols * 64 + lane * 2) = sum;
-                if (cols == 0 && lane == 0) {
-                  p.ws_m[slot * kRows + row] = top;
-                  p.ws_l[slot * kRows + row] = total_l;
-                }
-              }
+          }
+        __syncthreads();
+#pragma unroll 1
+        for (int in = warp * 2; in < warp * 2 + 2; ++in) {
+          const int row = nt * 8 + in;
+          if (row >= rows) break;
+          float2 sum = make_float2(0.0f, 0.0f);
+          float top = m_s[0][row], total_l = 0.0f;
+#pragma unroll
+          for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][row]);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float2 v = lds_f2(shared + ((w * 8 + in) * 64 + (((lane >> 3) ^ (in >> 1)) * 16) + 2 * (lane & 7)) * 4);
+            sum.x += v.x;
+            sum.y += v.y;
+            total_l += top == -INFINITY ? l_s[w][row] : l_s[w][row] * ex2_approx(m_s[w][row] - top);   // no key: 0, or NaN
+          }
+          if (whole) {
+            const float f = total_l == 0.0f ? 0.0f : __frcp_rn(total_l);
+            const int64_t to = out_row(p, use.q.t0 * p.g + use.row_tile * kRows + row, use.head);
+            T* dst = static_cast<T*>(p.out) + to * D + cols * 64 + lane * 2;
+            if constexpr (S::kTwo) *reinterpret_cast<float2*>(dst) = make_float2(sum.x * f, sum.y * f);
+            else *reinterpret_cast<uint32_t*>(dst) = pack_16x2<T>(sum.x * f, sum.y * f);
+            if (cols == 0 && lane == 0 && p.lse != nullptr) p.lse[to] = lse_of(top, total_l);
+          } else {
+            *reinterpret_cast<float2*>(p.ws_acc + ((int64_t)slot * kRows + row) * D + cols * 64 + lane * 2) = sum;
+            if (cols == 0 && lane == 0) {
+              p.ws_m[slot * kRows + row] = top;
+              p.ws_l[slot * kRows + row] = total_l;
             }
           }
-          __syncthreads();
         }
+        __syncthreads();
       }
       // begun here, finished by the CTAs behind this one
       if (!whole && use.from == 0 && tid == 0) p.cut[cta] = cut_unit(p, use, share, first);
@@ -584,6 +587,8 @@ extern "C" int nvfp4_kv8_attention(const void* q, int q_dtype, int64_t s_qt, int
   NVFP4_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0 &&
                     ((k_block | v_block) & 15) == 0,
                 "nvfp4_kv8_attention: cache blocks, out and workspace must be 16-byte aligned");
+  NVFP4_REQUIRE(((uintptr_t)q & 15) == 0 && ((s_qt | s_qh) * (q_dtype == NVFP4_DT_FP32 ? 4 : 2) & 15) == 0,
+                "nvfp4_kv8_attention: query rows must be 16-byte aligned");
   if (tokens == 0) return 0;
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

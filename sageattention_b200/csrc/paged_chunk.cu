@@ -38,13 +38,20 @@ struct Cfg {
   static constexpr int kRows = 128 * kGroups;
   static constexpr int kStages = D == 128 ? 2 : 1;
   static constexpr int kSoft = 4 * kGroups;                // softmax warps
-  static constexpr int kThreads = 32 * (kSoft + 8);         // whole warpgroups: registers move between them
-  static constexpr int kRegsSoft = D == 128 ? 144 : 168, kRegsConvert = D == 128 ? 144 : 248, kRegsIssue = 80;
+  // converting warpgroups: one for K and V, or (D = 256, where one took 3600 clocks a tile) one for each
+  static constexpr int kConvert = D == 128 ? 1 : 2;
+  static constexpr int kIssue = kSoft + 4 * kConvert;      // first warp of the last warpgroup, which issues the products
+  static constexpr int kThreads = 32 * (kIssue + 4);       // whole warpgroups: registers move between them
+  static constexpr int kRegsSoft = D == 128 ? 144 : 168, kRegsConvert = D == 128 ? 144 : 128, kRegsIssue = 80;
   static constexpr int kOperand = D / 64 * kSub;           // 128 rows of q, or a tile of keys or values
   static constexpr int kQ = 0, kK = kGroups * kOperand, kV = kK + kStages * kOperand, kOut = kV + kStages * kOperand;
   static constexpr int kBytes = kOut + kSoft * 2048 + 1024;
   static constexpr int kN = D == 128 ? 64 : 128;           // keys of a job
   static constexpr int kJobs = kTile / kN;                 // jobs of a tile
+  // Products issued from straight code or (1) from loops: an instruction per 64 halves' step at D = 128, where the straight
+  // code took 351 us of the 2048-row chunk and loops 372; at D = 256 products are longer and the straight code larger than
+  // the instruction cache keeps (mixed batch 77 us straight, 70 in loops).
+  static constexpr int kIssueUnroll = D == 128 ? 2 : 1;
   static constexpr int kO = 256;                           // tensor memory: S of (group, place), O behind
   static __device__ __forceinline__ uint32_t s_at(int group, int place) { return (group * 2 + place) * kN; }
 };
@@ -76,7 +83,7 @@ __device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
   return d;
 }
 
-// Registers of a warpgroup.  The shares add up to what the launch has (512 threads of 128, or 384 of 168).
+// Registers of a warpgroup.  The shares are at most what the launch has (512 threads of 128).
 template <int N>
 __device__ __forceinline__ void more_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -143,7 +150,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     mbar_init(&q_full, C::kSoft);
     mbar_fence_init();
   }
-  if (warp == C::kSoft + 4) tmem_alloc(&tmem_base_s, 512);
+  if (warp == C::kIssue) tmem_alloc(&tmem_base_s, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -161,13 +168,14 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
   }
   __syncthreads();                                         // every role has its own copy from here on
 
-  if (warp >= C::kSoft && warp < C::kSoft + 4) {
-    more_registers<C::kRegsConvert>();
+  if (warp >= C::kSoft && warp < C::kIssue) {
+    if (C::kRegsConvert > 128) more_registers<C::kRegsConvert>();
     Place ahead = place_s;
     bool more = ahead.open();                              // there is a tile to be looked up: `tile` of `ahead`
     int tile = ahead.from;
     // ------------------------------------------------------------------ codes to halves
-    const int w = warp - C::kSoft, t = w * 32 + lane;
+    const int w = warp & 3, t = w * 32 + lane;
+    const bool does_k = C::kConvert == 1 || warp < C::kSoft + 4, does_v = C::kConvert == 1 || !does_k;
     // 16-byte pieces of a tile: eight lanes take 64 bytes of two neighbouring keys, whose halves then lie in different banks
     constexpr int kPieces = D / 16;                        // per thread and operand
     const int in_key = (lane >> 2) & 1, in_chunk = lane & 3, pair8 = w * 4 + (lane >> 3);
@@ -176,7 +184,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     // Codes wait in registers, from the time that their tile's predecessor is converted on.  A load in flight holds a line of
     // L1, of which this kernel's shared memory leaves 28 KB, less than a tile of K and V: piece i of the next tile is asked
     // for when piece i of the present one has been converted, not all at once.
-    uint4 kr[kPieces], vr[kPieces];
+    uint4 kr[kPieces], vr[C::kConvert == 1 ? kPieces : 1];   // where a warp does one operand, its codes are in the first
     // lanes 0 to 7: block of keys 16 lane .. of the tile being converted (`now`), asked for (`next`), and of the one behind
     int id_now = -1, id_next = -1, id_ahead = -1;
     float ks_now = 0.0f, vs_now = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
@@ -216,7 +224,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     constexpr int kOwn = 4, kEach = kPieces / kOwn;
     auto group_of = [&](int u) { return 2 * u + (w >> 1); };
     // this thread's first key of each: its codes, and how many keys of the group are there
-    const uint8_t *k_from[kOwn], *v_from[kOwn];
+    const uint8_t *k_from[kOwn], *v_from[kOwn];              // (one of them where a warp does one operand)
     int count[kOwn];
     const int first_key = (pair8 & 7) * 2 + in_key;         // of a group
     auto find = [&]() {
@@ -224,8 +232,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       for (int u = 0; u < kOwn; ++u) {
         const int b = __shfl_sync(0xffffffffu, id_next, group_of(u)), key = key0 + group_of(u) * 16;
         const int64_t row = (((int64_t)head << p.log_block) + (key & ((1 << p.log_block) - 1)) + first_key) * D + in_chunk * 16;
-        k_from[u] = p.k + b * p.k_block + row;
-        v_from[u] = p.v + b * p.v_block + row;
+        if (does_k) k_from[u] = p.k + b * p.k_block + row;
+        if (does_v) (C::kConvert == 1 ? v_from : k_from)[u] = p.v + b * p.v_block + row;
         count[u] = b >= 0 ? limit - key : 0;
       }
     };
@@ -271,8 +279,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       find();
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) kr[i] = ask(k_from, i);
+      if constexpr (C::kConvert == 1) {
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) vr[i] = ask(v_from, i);
+        for (int i = 0; i < kPieces; ++i) vr[i] = ask(v_from, i);
+      }
     }
     int v_run = -200;                                      // largest exponent of the unit's value scales so far
     uint32_t n = 0;
@@ -289,17 +299,23 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       v_run = max(v_run, ve);
       ve = max(ve, v_run - 60);                            // smaller ones do not count beside what the unit has seen
       const uint32_t there = __ballot_sync(0xffffffffu, id_now >= 0);
-      mbar_wait_warp(&k_free[st], ph ^ 1, err, 60);
-      if (t == 0) info_s[n % kInfo] = {exp2_int(ke), (float)ve, there};
-      convert(kr, ks_now * exp2_int(-ke), smem_u32(smem + C::kK + st * C::kOperand), k_from);
-      if (lane == 0) mbar_arrive(&k_full[st]);
-      mbar_wait_warp(&v_free[st], ph ^ 1, err, 61);
-      convert(vr, vs_now * exp2_int(-ve), smem_u32(smem + C::kV + st * C::kOperand), v_from);
-      if (lane == 0) mbar_arrive(&v_full[st]);
+      if (does_k) {
+        mbar_wait_warp(&k_free[st], ph ^ 1, err, 60);
+        if (t == 0) info_s[n % kInfo] = {exp2_int(ke), (float)ve, there};
+        convert(kr, ks_now * exp2_int(-ke), smem_u32(smem + C::kK + st * C::kOperand), k_from);
+        if (lane == 0) mbar_arrive(&k_full[st]);
+      }
+      if (does_v) {
+        mbar_wait_warp(&v_free[st], ph ^ 1, err, 61);
+        const uint32_t dst = smem_u32(smem + C::kV + st * C::kOperand);
+        if constexpr (C::kConvert == 1) convert(vr, vs_now * exp2_int(-ve), dst, v_from);
+        else convert(kr, vs_now * exp2_int(-ve), dst, k_from);
+        if (lane == 0) mbar_arrive(&v_full[st]);
+      }
     }
-  } else if (warp >= C::kSoft + 4) {
+  } else if (warp >= C::kIssue) {
     fewer_registers<C::kRegsIssue>();
-    if (warp == C::kSoft + 5) {
+    if (warp == C::kIssue + 1) {
       // query rows of all units of this CTA into L2: a unit's softmax begins with them, and from HBM they were 5 us
       constexpr int kLines = D * (int)sizeof(T) / 128;
       for (Place at = place_s; at.open(); at.close(p)) {
@@ -309,7 +325,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
                       i % kLines * 128);
       }
     }
-    if (warp == C::kSoft + 4) {
+    if (warp == C::kIssue) {
     // ------------------------------------------------------------------ issue of the products
     Place at = place_s;
     const bool leader = elect_one();
@@ -317,8 +333,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     const uint64_t b_q = desc_sw128(smem + C::kQ, 0), b_k = desc_sw128(smem + C::kK, 0);
     const uint64_t b_v = desc_sw128_mn(smem + C::kV, 0, kSub);
     uint32_t n = 0, seg = 0;                               // tiles and segments so far
-    uint32_t p_phase[2] = {0, 0};                          // of p_full, a bit a place
-    uint32_t results[2] = {0, 0};                          // results of each group so far
+    uint32_t p_phase = 0;                                  // of p_full, a bit a group and place
+    uint32_t used = 0, o_phase = 0;                        // groups that have had a result, and how many, a bit a group
     for (; at.open(); at.close(p)) {
       const int tiles = at.to - at.from;
       const bool both = C::kGroups == 2 && at.q.rows(p, at.row_tile) > 128;
@@ -335,48 +351,49 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         if (leader) {
           const uint64_t x_q = b_q + (both && g ? C::kOperand >> 4 : 0);
           const uint64_t x_k = b_k + (uint64_t)(st * (C::kOperand >> 4) + sub * (C::kN * 128 >> 4));
+#pragma unroll C::kIssueUnroll
+          for (int c = 0; c < D / 64; ++c)
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tmem + C::s_at(g, j & 1), x_q + (k >> 2) * (kSub >> 4) + (k & 3) * 2, x_k + (k >> 2) * (kSub >> 4) + (k & 3) * 2,
-                      id_s, k > 0);
+            for (int k = 0; k < 4; ++k)
+              umma_bf16(tmem + C::s_at(g, j & 1), x_q + c * (kSub >> 4) + k * 2, x_k + c * (kSub >> 4) + k * 2, id_s, (c > 0 || k > 0) ? 1u : 0u);
           umma_commit(&s_full[g][j & 1]);
           if (sub == C::kJobs - 1 && (!both || g == 1)) umma_commit(&k_free[st]);
         }
         __syncwarp();
       };
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int g = 0; g < C::kGroups; ++g)
-          if (j < jobs_of(g)) issue_s(g, j);
       const int most = jobs_of(0);
 #pragma unroll 1
-      for (int j = 0; j < most; ++j) {
-#pragma unroll
+      for (int j = -2; j < most; ++j) {                    // PV of job j behind S of job j + 1, S of job j + 2 behind that
+#pragma unroll C::kIssueUnroll
         for (int g = 0; g < C::kGroups; ++g) {
           const int jobs = jobs_of(g);
-          if (j >= jobs) continue;
-          const uint32_t tile = n + tile_of(g, j), st = tile % C::kStages;
-          const int sub = j % C::kJobs;
-          if (j == 0 && results[g] > 0) mbar_wait(&o_free[g], (results[g] - 1) & 1, err, 64);
-          if (sub == 0 && (!both || g == 0)) mbar_wait(&v_full[st], (tile / C::kStages) & 1, err, 65);
-          mbar_wait_warp(&p_full[g][j & 1], (p_phase[g] >> (j & 1)) & 1, err, 66);
-          p_phase[g] ^= 1u << (j & 1);
-          tc_fence_after();
-          if (leader) {
-            const uint64_t x_v = b_v + (uint64_t)(st * (C::kOperand >> 4) + sub * (C::kN * 128 >> 4));
+          if (j >= 0 && j < jobs) {
+            const uint32_t tile = n + tile_of(g, j), st = tile % C::kStages;
+            const int sub = j % C::kJobs;
+            if (j == 0 && (used >> g & 1)) mbar_wait(&o_free[g], (o_phase >> g & 1) ^ 1, err, 64);
+            if (sub == 0 && (!both || g == 0)) mbar_wait(&v_full[st], (tile / C::kStages) & 1, err, 65);
+            mbar_wait_warp(&p_full[g][j & 1], p_phase >> (2 * g + (j & 1)) & 1, err, 66);
+            p_phase ^= 1u << (2 * g + (j & 1));
+            tc_fence_after();
+            if (leader) {
+              const uint64_t x_v = b_v + (uint64_t)(st * (C::kOperand >> 4) + sub * (C::kN * 128 >> 4));
+              const uint32_t x_p = tmem + C::s_at(g, j & 1) + C::kN / 2;
+#pragma unroll C::kIssueUnroll
+              for (int c = 0; c < D / 128; ++c)
 #pragma unroll
-            for (int c = 0; c < D / 128; ++c)
-#pragma unroll
-              for (int k = 0; k < C::kN / 16; ++k)
-                umma_bf16_ta(tmem + C::kO + g * 128 + c * 128, tmem + C::s_at(g, j & 1) + C::kN / 2 + k * 8,
-                             x_v + c * (2 * kSub >> 4) + k * 128, id_o, (k > 0 || j > 0) ? 1u : 0u);
-            if (sub == C::kJobs - 1 && (!both || g == 1)) umma_commit(&v_free[st]);
-            umma_commit(&pv_done[g]);
-            if (j + 1 == jobs) umma_commit(&o_full[g]);
+                for (int k = 0; k < C::kN / 16; ++k)
+                  umma_bf16_ta(tmem + C::kO + g * 128 + c * 128, x_p + k * 8, x_v + c * (2 * kSub >> 4) + k * 128, id_o,
+                               (k > 0 || j > 0) ? 1u : 0u);
+              if (sub == C::kJobs - 1 && (!both || g == 1)) umma_commit(&v_free[st]);
+              umma_commit(&pv_done[g]);
+              if (j + 1 == jobs) umma_commit(&o_full[g]);
+            }
+            __syncwarp();
+            if (j == 0) {
+              used |= 1u << g;
+              o_phase ^= 1u << g;
+            }
           }
-          __syncwarp();
-          if (j == 0) ++results[g];
           if (j + 2 < jobs) issue_s(g, j + 2);
         }
       }
@@ -385,7 +402,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     }
     }
   } else {
-    if (D == 128) more_registers<C::kRegsSoft>();
+    more_registers<C::kRegsSoft>();
     Place at = place_s;
     // ------------------------------------------------------------------ softmax, a thread a row
     const int group = warp >> 2, wq = warp & 3, row_in = wq * 32 + lane;
@@ -411,27 +428,14 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         const int base = (both ? group * 128 : 0) + wq * 32;
         const uint32_t dst = smem_u32(smem + C::kQ) + (both ? group : 0) * C::kOperand;
         const int e = lane % kLanes;                       // piece of eight elements
-        const bool aligned = ((reinterpret_cast<uintptr_t>(p.q) | (uint64_t)(p.sqt * 2) | (uint64_t)(p.sqh * 2)) & 15) == 0;
 #pragma unroll 1
         for (int x0 = 0; x0 < 32 / kAtOnce; x0 += kBatch) {
           uint4 raw[kBatch];
-          auto piece = [&](int x) {
+#pragma unroll
+          for (int x = 0; x < kBatch; ++x) {
             const int r = base + (x0 + x) * kAtOnce + lane / kLanes;
-            return query_row<T>(p, at.q.t0, at.row_tile * C::kRows + min(r, rows - 1), at.head) + e * 8;
-          };
-          if (aligned) {
-#pragma unroll
-            for (int x = 0; x < kBatch; ++x) raw[x] = *reinterpret_cast<const uint4*>(piece(x));
-          } else {
-#pragma unroll 1
-            for (int x = 0; x < kBatch; ++x) {
-              const uint16_t* t = reinterpret_cast<const uint16_t*>(piece(x));
-              const uint4 w = make_uint4(t[0] | (uint32_t)t[1] << 16, t[2] | (uint32_t)t[3] << 16, t[4] | (uint32_t)t[5] << 16,
-                                         t[6] | (uint32_t)t[7] << 16);
-#pragma unroll
-              for (int y = 0; y < kBatch; ++y)
-                if (y == x) raw[y] = w;
-            }
+            raw[x] = *reinterpret_cast<const uint4*>(
+                query_row<T>(p, at.q.t0, at.row_tile * C::kRows + min(r, rows - 1), at.head) + e * 8);
           }
 #pragma unroll
           for (int x = 0; x < kBatch; ++x) {
@@ -495,18 +499,26 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         // the exponentials, which therefore run from the end
         float top = -INFINITY;
         uint32_t s[2][32];
-        auto hide = [&](uint32_t (&v)[32], int x) {
+        if (masked) {                                      // a few tiles of a unit: S is edited where it is
+#pragma unroll 1
+          for (int x = 0; x < kChunks; ++x) {
+            tmem_ld32(s_at + x * 32, s[0]);
+            tmem_ld_wait();
+            const int left = visible - x * 32;
+            uint32_t seen = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1;
+            seen &= ((there >> (2 * x) & 1) ? 0xFFFFu : 0u) | ((there >> (2 * x + 1) & 1) ? 0xFFFF0000u : 0u);
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (x * 32 + e >= visible || !(there >> (x * 2 + (e >> 4)) & 1)) v[e] = 0xFF800000u;
-        };
+            for (int e = 0; e < 32; ++e) s[0][e] = (seen >> e & 1) ? s[0][e] : 0xFF800000u;
+            tmem_st32(s_at + x * 32, s[0]);
+          }
+          tmem_st_wait();
+        }
         tmem_ld32(s_at, s[0]);
         tmem_ld_wait();
 #pragma unroll
         for (int x = 0; x < kChunks; ++x) {
           uint32_t (&now)[32] = s[x & 1];
           if (x < kChunks - 1) tmem_ld32(s_at + (x + 1) * 32, s[(x + 1) & 1]);
-          if (masked) hide(now, x);
           float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
@@ -516,7 +528,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
           top = fmaxf(top, fmaxf(t0, t1));
           if (x < kChunks - 1) tmem_ld_wait();
         }
-        const float c = c_row * info.k_factor;
+        const float c = fmaxf(c_row * info.k_factor, 0x1p-126f);   // never 0: hidden keys are -inf
         top = top == -INFINITY ? -INFINITY : top * c;
         // reference of the weights: moves only where the maximum has left it behind
         const float want = top + info.v_log2;
@@ -555,7 +567,6 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
             now[2 * e] = (uint32_t)y;
             now[2 * e + 1] = (uint32_t)(y >> 32);
           }
-          if (masked) hide(now, x);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float x0 = ex2_approx(__uint_as_float(now[2 * e])), x1 = ex2_approx(__uint_as_float(now[2 * e + 1]));
@@ -627,7 +638,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       const int rows_warp = min(max(rows - (both ? group * 128 : 0) - wq * 32, 0), 32);    // of this warp that exist
       if (writes && rows_warp > 0) {
         const int row0 = (both ? group * 128 : 0) + wq * 32;
-        const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+        const float inv = whole && l != 0.0f ? __frcp_rn(l) : 0.0f;
         if (whole) {
           if (live && p.lse != nullptr) p.lse[out_row(p, at.q.t0 * p.g + i_row, at.head)] = lse_of(m, l);
         } else if (live) {
@@ -654,7 +665,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
             }
           }
           // 64 bytes of a row at a time, four lanes a row: a lane's own row would be 16 bytes of 32 rows an instruction
-          auto segment = [&](const uint32_t (&w)[16], auto address) {
+#pragma unroll 1
+          for (int h = 0; h < (whole ? 1 : 2); ++h) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              w[e] = whole ? pack_16x2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv) : h ? o[16 + e] : o[e];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               *reinterpret_cast<uint4*>(stg + sw64_offset(lane, e * 16)) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
@@ -663,29 +679,15 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
             for (int e = 0; e < 4; ++e) {
               const int r = 8 * e + (lane >> 2), ch = lane & 3;
               const uint4 v = *reinterpret_cast<const uint4*>(stg + sw64_offset(r, ch * 16));
-              if (r < rows_warp) *reinterpret_cast<uint4*>(address(r) + ch * 16) = v;
+              if (r < rows_warp) {
+                uint8_t* to = whole ? reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) +
+                                                                 out_row(p, at.q.t0 * p.g + at.row_tile * C::kRows + row0 + r, at.head) * D +
+                                                                 cc * 32)
+                                    : reinterpret_cast<uint8_t*>(p.ws_acc + ((int64_t)slot * C::kRows + row0 + r) * D + cc * 32 + h * 16);
+                *reinterpret_cast<uint4*>(to + ch * 16) = v;
+              }
             }
             __syncwarp();
-          };
-          if (whole) {
-            uint32_t w[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              w[e] = pack_16x2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-            segment(w, [&](int r) {
-              const int64_t to = out_row(p, at.q.t0 * p.g + at.row_tile * C::kRows + row0 + r, at.head);
-              return reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) + to * D + cc * 32);
-            });
-          } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t w[16];
-#pragma unroll
-              for (int e = 0; e < 16; ++e) w[e] = o[16 * h + e];
-              segment(w, [&](int r) {
-                return reinterpret_cast<uint8_t*>(p.ws_acc + ((int64_t)slot * C::kRows + row0 + r) * D + cc * 32 + h * 16);
-              });
-            }
           }
         }
       }
@@ -701,7 +703,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
   tc_fence_before();
   __syncthreads();
   report_error(&expired, p.status);
-  if (warp == C::kSoft + 4) {
+  if (warp == C::kIssue) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
