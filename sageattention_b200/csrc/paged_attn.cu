@@ -589,6 +589,7 @@ extern "C" int nvfp4_kv8_attention(const void* q, int q_dtype, int64_t s_qt, int
                 "nvfp4_kv8_attention: cache blocks, out and workspace must be 16-byte aligned");
   NVFP4_REQUIRE(((uintptr_t)q & 15) == 0 && ((s_qt | s_qh) * (q_dtype == NVFP4_DT_FP32 ? 4 : 2) & 15) == 0,
                 "nvfp4_kv8_attention: query rows must be 16-byte aligned");
+  NVFP4_REQUIRE(isfinite(scaling), "nvfp4_kv8_attention: scaling must be finite");
   if (tokens == 0) return 0;
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

@@ -43,13 +43,15 @@ struct Cfg {
   static constexpr int kIssue = kSoft + 4 * kConvert;      // first warp of the last warpgroup, which issues the products
   static constexpr int kThreads = 32 * (kIssue + 4);       // whole warpgroups: registers move between them
   static constexpr int kRegsSoft = D == 128 ? 144 : 168, kRegsConvert = D == 128 ? 144 : 128, kRegsIssue = 80;
+  // an increase waits for registers of this launch, which has 128 a thread (65536 / 512): more than those would wait forever
+  static_assert(kThreads == 512 && kSoft * kRegsSoft + 4 * kConvert * kRegsConvert + 4 * kRegsIssue <= kThreads / 32 * 128, "registers");
   static constexpr int kOperand = D / 64 * kSub;           // 128 rows of q, or a tile of keys or values
   static constexpr int kQ = 0, kK = kGroups * kOperand, kV = kK + kStages * kOperand, kOut = kV + kStages * kOperand;
   static constexpr int kBytes = kOut + kSoft * 2048 + 1024;
   static constexpr int kN = D == 128 ? 64 : 128;           // keys of a job
   static constexpr int kJobs = kTile / kN;                 // jobs of a tile
   // Products issued from straight code or (1) from loops: an instruction per 64 halves' step at D = 128, where the straight
-  // code took 351 us of the 2048-row chunk and loops 372; at D = 256 products are longer and the straight code larger than
+  // code took 359 us of the 2048-row chunk and loops 380; at D = 256 products are longer and the straight code larger than
   // the instruction cache keeps (mixed batch 77 us straight, 70 in loops).
   static constexpr int kIssueUnroll = D == 128 ? 2 : 1;
   static constexpr int kO = 256;                           // tensor memory: S of (group, place), O behind

@@ -8,8 +8,10 @@ be captured in a CUDA graph.  (No counterpart in the reference.)
 Layout, shared by every function here:
 
   k_cache, v_cache   [blocks, Hk, block_size, D] float8_e4m3fn: codes; heads dense, any stride between blocks
-  k_scale, v_scale   [blocks, Hk] float32: value = code * scale
-  block_table        [requests, width] int32: block of tokens j * block_size .. of a request, -1 where it has none
+  k_scale, v_scale   [blocks, Hk] float32: value = code * scale (a power of two; attention also reads others, which calls of
+                     more than 24 query rows a request round to eleven bits)
+  block_table        [requests, width] int32: block of tokens j * block_size .. of a request, -1 where it has none.
+                     Attention may read a block for several requests; reserve, write and trim take it to be one's own
   lengths            [requests] int32: tokens that a request holds
   free_blocks        [blocks] int32, free_count [1] int32: a stack of block ids, its top at free_count - 1
 
@@ -61,7 +63,7 @@ def fp8_kv_write(key, value, slot_map, k_cache, v_cache, k_scale, v_scale) -> No
     ones need a larger scale, their codes are rounded again to it.  Infinities saturate and do not count for the scale,
     nor do NaN, which stay.  Slots below 0 are skipped.  A block's tokens stand next to each other in ``slot_map``,
     ascending by one, as ``paged_kv_reserve`` lists them; a block named in two places of one call is left with
-    unspecified codes.
+    unspecified codes.  Two calls that write the same block are ordered by the caller (one stream, or events).
     """
     _lib.native().kv8_write(key, value, slot_map, k_cache, v_cache, k_scale, v_scale)
 
@@ -84,8 +86,9 @@ def fp8_paged_attention(query, cu_seqlens, k_cache, v_cache, k_scale, v_scale, b
     """Causal attention of several query tokens a request: drafts to verify, chunks of a prompt, or both in one batch.
 
     ``query`` ``[T, H, D]``; request r owns tokens ``cu_seqlens[r] .. cu_seqlens[r + 1]``, the last ones of its
-    ``lengths[r]`` keys (written before the call): token i of n sees keys ``0 .. lengths[r] - n + i``.  Returns
-    ``[T, H, D]``, with ``return_lse`` also ``[T, H]``; tokens without a key, or behind the last request's, get zeros and -inf.
+    ``lengths[r]`` keys (written before the call): token i of n sees keys ``0 .. lengths[r] - n + i``.  A value that is NaN
+    reaches the call's tokens in front of it too (their weight 0 times NaN), as in a masked softmax; keys, and what is
+    behind ``lengths[r]`` in a block, reach nothing that does not see them.  Returns ``[T, H, D]``, with ``return_lse`` also ``[T, H]``; tokens without a key, or behind the last request's, get zeros and -inf.
     """
     if cu_seqlens is None:
         raise ValueError("fp8_paged_attention needs cu_seqlens (one token a request: fp8_paged_decode)")

@@ -95,6 +95,13 @@ def test_c_entries_refuse_bad_sizes():
     assert a(t=0, cu=16) == 0
 
 
+def test_scaling_has_to_be_finite():
+    L, n = _lib(), None
+    for scaling in (math.inf, -math.inf, math.nan):
+        assert L.nvfp4_kv8_attention(0, 0, 128, 128, 16, 0, 0, 2048, 0, 2048, n, 1, n, 1, 1, 16, n, 1, 1, n, 1, 1, 1, 128, scaling, 0, n, 0,
+                                     0, n, n) < 0 and b"scaling" in L.nvfp4_last_error()
+
+
 def test_python_entries_refuse_cpu_tensors():
     import sageattention_b200.nvfp4 as nv
     _lib()

@@ -574,6 +574,96 @@ def test_two_captured_decodes_replayed_in_turn_and_on_other_streams():
     assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
 
 
+# several tokens a request, one set for each kernel: 8, 16, 24 and more query rows
+_KERNELS = [([1, 1, 1], torch.bfloat16, 128), ([2, 3, 2], torch.float16, 128), ([5, 6, 5], torch.bfloat16, 128),
+            ([7, 40, 150], torch.bfloat16, 128), ([7, 40, 150], torch.float16, 256), ([5, 6, 5], torch.float32, 256)]
+
+
+def _set(new, dtype, d, seed, h=8, hk=2, block=16, held=(90, 0, 21)):
+    """Operands on the GPU of a batch whose requests have `new` tokens behind `held` others."""
+    total = [a + b for a, b in zip(new, held)]
+    blocks = sum(-(-n // block) for n in total) + 2
+    k, ks = _cache(blocks, hk, block, d, seed)
+    v, vs = _cache(blocks, hk, block, d, seed + 50)
+    table = _table(total, block, blocks, seed)
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    q = torch.randn(starts[-1], h, d, generator=torch.Generator().manual_seed(seed + 7)).to(dtype)
+    cache = [x.cuda() for x in (k, v, ks, vs, table)]
+    return q.cuda(), _i32(starts), cache, _i32(total), (k, v, ks, vs, table, total, block)
+
+
+@pytest.mark.parametrize("new,dtype,d", _KERNELS)
+def test_scaling_of_zero_and_below(new, dtype, d):
+    q, cu, cache, lengths, (k, v, ks, vs, table, total, block) = _set(new, dtype, d, 1)
+    call = lambda q, s: _nv().fp8_paged_attention(q, cu, *cache, lengths, s, 4, return_lse=True)
+    for a, b in zip(call(q, -0.1), call(-q, 0.1)):
+        assert torch.equal(a, b)
+    out, lse = call(q, 0.0)                                            # the mean of what a row sees
+    for r, n in enumerate(new):
+        a = int(cu[r])
+        kk, vv = R.gather(k, ks, table[r], total[r], block), R.gather(v, vs, table[r], total[r], block)
+        _close(out[a:a + n], lse[a:a + n], q[a:a + n].cpu(), kk, vv, _key_scales(vs, table[r], total[r], block),
+               [total[r] - n + 1 + i for i in range(n)], 0.0, 4, chunk=_chunk(dtype, d, q.shape[0], 4, 3))
+
+
+@pytest.mark.parametrize("new,dtype,d", _KERNELS)
+def test_attention_of_rows_that_are_not_aligned(new, dtype, d):
+    q, cu, cache, lengths, _ = _set(new, dtype, d, 2)
+    want = _nv().fp8_paged_attention(q, cu, *cache, lengths, 0.1, 4)
+    flat = torch.empty(q.numel() + 1, dtype=dtype, device="cuda")[1:].view(q.shape)
+    flat.copy_(q)
+    wide = torch.empty(q.shape[0], 8, d + 3, dtype=dtype, device="cuda")[..., :d]
+    wide.copy_(q)
+    last = torch.empty(d, 8, q.shape[0], dtype=dtype, device="cuda").permute(2, 1, 0)
+    last.copy_(q)
+    for x in (flat, wide, last):
+        assert torch.equal(_nv().fp8_paged_attention(x, cu, *cache, lengths, 0.1, 4), want)
+
+
+@pytest.mark.parametrize("new,dtype,d", _KERNELS)
+def test_two_captured_batches_replayed_at_once(new, dtype, d):
+    graphs, outs, want = [], [], []
+    for seed in (1, 2):
+        q, cu, cache, lengths, _ = _set(new, dtype, d, seed)
+        call = lambda q=q, cu=cu, cache=cache, lengths=lengths: _nv().fp8_paged_attention(q, cu, *cache, lengths, 0.1, 4)
+        want.append(call().clone())
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call())
+        graphs.append((graph, call))                                   # the operands live as long as the graph
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for (graph, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+@pytest.mark.parametrize("tokens", [20, 3000])
+def test_a_block_named_twice_spoils_no_other(tokens):
+    """Its codes are anybody's; those of the call's other blocks, and of blocks that it does not name, are as ever."""
+    block, blocks = 16, 400
+    slots = torch.arange(tokens) + 3 * block
+    twice = slots.clone()
+    twice[tokens // 2 // block * block] = 5                            # inside block 0, as the last token is
+    twice[-1] = 5
+    key, value = _rows((tokens, 2, 128), 1, torch.bfloat16).cuda(), _rows((tokens, 2, 128), 2, torch.bfloat16).cuda()
+    got = []
+    for s in (slots, twice):
+        codes = [torch.zeros(blocks, 2, block, 128, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        scales = [torch.zeros(blocks, 2, device="cuda") for _ in range(2)]
+        _nv().fp8_kv_write(key, value, s.cuda(), *codes, *scales)
+        got.append((codes, scales))
+    touched = {0} | {int(s) // block for s, t in zip(slots, twice) if s != t}
+    others = torch.tensor([b for b in range(blocks) if b not in touched]).cuda()
+    for a, b in zip(sum(map(list, got[0]), []), sum(map(list, got[1]), [])):
+        assert torch.equal(a[others], b[others])
+
+
 def test_registered_operators_are_the_same_calls():
     import sageattention_b200.nvfp4.custom_ops  # noqa: F401
     ns, nv = torch.ops.sageattention_b200, _nv()
