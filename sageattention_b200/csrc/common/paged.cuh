@@ -271,19 +271,21 @@ __device__ __forceinline__ void clear_untouched(const PagedParams& p) {
   }
 }
 
-// Exact merge of the pieces of a cut unit, one warp a row, in the order of the keys.  Bound by trips to L2: the maxima, sums
-// and rows of up to four pieces are asked for at once.
+// Exact merge of the pieces of a cut unit, L lanes a row, in the order of the keys.  Bound by trips to L2: the maxima, sums
+// and rows of up to four pieces are asked for at once.  Pieces lie row by row, a warp a row; or (kColumns) four columns of
+// all rows behind each other, as threads that have a row each store them, two rows a warp, so that sectors are whole.
 constexpr int kCombineWarps = 4;
-template <typename T, int D, int ROWS>
+template <typename T, int D, int ROWS, bool kColumns>
 __global__ void __launch_bounds__(32 * kCombineWarps) paged_combine_kernel(PagedParams p) {
   griddep_wait();
   griddep_launch();
-  const int lane = threadIdx.x & 31, row = blockIdx.y * kCombineWarps + (threadIdx.x >> 5);
+  constexpr int L = kColumns ? 16 : 32;
+  const int lane = threadIdx.x % L, row = (int)(blockIdx.y * blockDim.x + threadIdx.x) / L;
   const int4 u = p.cut[blockIdx.x];
   if (row >= u.z) return;
   const int pieces = u.w & ((1 << 30) - 1), first = 2 * (int)blockIdx.x + (u.w >> 30 ? 0 : 1);
-  auto at = [&](int i) { return (int64_t)(i == 0 ? first : 2 * ((int)blockIdx.x + i)) * ROWS + row; };
-  constexpr int kAtOnce = 4, kC = D / 128;
+  auto slot = [&](int i) { return (int64_t)(i == 0 ? first : 2 * ((int)blockIdx.x + i)); };
+  constexpr int kAtOnce = 4, kC = D / (4 * L);
   float top = -INFINITY, total = 0.0f, sum[kC][4];
 #pragma unroll
   for (int c = 0; c < kC; ++c)
@@ -294,11 +296,14 @@ __global__ void __launch_bounds__(32 * kCombineWarps) paged_combine_kernel(Paged
     float4 v[kAtOnce][kC];
 #pragma unroll
     for (int x = 0; x < kAtOnce; ++x) {
-      const int64_t a = at(min(i0 + x, pieces - 1));       // behind the last piece: that one again, not counted
-      m[x] = p.ws_m[a];
-      l[x] = p.ws_l[a];
+      const int64_t a = slot(min(i0 + x, pieces - 1)) * ROWS;                // behind the last piece: that one again, not counted
+      m[x] = p.ws_m[a + row];
+      l[x] = p.ws_l[a + row];
 #pragma unroll
-      for (int c = 0; c < kC; ++c) v[x][c] = *reinterpret_cast<const float4*>(p.ws_acc + a * D + c * 128 + lane * 4);
+      for (int c = 0; c < kC; ++c) {
+        const int four = c * L + lane;
+        v[x][c] = *(reinterpret_cast<const float4*>(p.ws_acc + a * D) + (kColumns ? four * ROWS + row : row * (D / 4) + four));
+      }
     }
     float now = top;
 #pragma unroll
@@ -331,15 +336,16 @@ __global__ void __launch_bounds__(32 * kCombineWarps) paged_combine_kernel(Paged
   for (int c = 0; c < kC; ++c) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) sum[c][k] *= inv;
-    store4<T>(static_cast<T*>(p.out) + row_out * D + c * 128 + lane * 4, sum[c]);
+    store4<T>(static_cast<T*>(p.out) + row_out * D + (c * L + lane) * 4, sum[c]);
   }
   if (lane == 0 && p.lse != nullptr) p.lse[row_out] = lse_of(top, total);
 }
-template <typename T, int D, int ROWS>
+template <typename T, int D, int ROWS, bool kColumns>
 int launch_combine(const PagedParams& p, int grid, cudaStream_t st) {
   const int64_t rows = p.cu == nullptr ? p.g : p.tokens * p.g;
-  return launch("nvfp4_kv8_attention combine", paged_combine_kernel<T, D, ROWS>,
-                dim3(grid, (unsigned)(((rows < ROWS ? rows : ROWS) + kCombineWarps - 1) / kCombineWarps)), 32 * kCombineWarps, 0, st, p);
+  constexpr int kRowsBlock = kCombineWarps * (kColumns ? 2 : 1);
+  return launch("nvfp4_kv8_attention combine", paged_combine_kernel<T, D, ROWS, kColumns>,
+                dim3(grid, (unsigned)(((rows < ROWS ? rows : ROWS) + kRowsBlock - 1) / kRowsBlock)), 32 * kCombineWarps, 0, st, p);
 }
 
 // ---- the kernel for long chunks (paged_chunk.cu)

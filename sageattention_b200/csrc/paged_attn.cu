@@ -529,7 +529,7 @@ int run_attention(const PagedParams& p, int sms, cudaStream_t st) {
   const int grid = (NT == 1 ? kCtas : 2) * sms;
   if (int rc = allow_smem("nvfp4_kv8_attention", reinterpret_cast<const void*>(paged_attn_kernel<T, D, NT>), S::kBytes)) return rc;
   if (int rc = launch("nvfp4_kv8_attention", paged_attn_kernel<T, D, NT>, dim3(grid), kThreads, S::kBytes, st, p)) return rc;
-  return launch_combine<T, D, 8 * NT>(p, grid, st);
+  return launch_combine<T, D, 8 * NT, false>(p, grid, st);
 }
 
 // Which kernel, by query rows a request on average (their numbers are on the device): eight, sixteen or (D = 128) 24 rows of

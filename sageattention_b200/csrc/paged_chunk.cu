@@ -28,6 +28,7 @@ namespace {
 
 constexpr int kTile = 128;                    // keys of a tile
 constexpr int kSub = 128 * 128;               // bytes of a 128-row sub-tile of 64 halves
+constexpr int kLoaders = 3;                   // warps that fetch query rows
 constexpr int kInfo = 8;                      // tiles whose scales are kept: more than can be under way
 // P is held times 2^kLift relative to a reference that may lag behind the running maximum by 2^kLag
 constexpr float kLift = 3.0f, kLag = 12.0f;
@@ -123,14 +124,14 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
   using Place = Walk<C::kRows, kTile>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2][2], p_full[2][2], o_full[2], o_free[2], pv_done[2], q_full;
+  __shared__ uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2][2], p_full[2][2], o_full[2], o_free[2], pv_done[2], q_full, q_free;
   __shared__ uint32_t tmem_base_s;
   __shared__ int expired;                                  // a wait ran out: site, else 0
   __shared__ int64_t list_s[C::kThreads / 32 + 2];
   __shared__ Place place_s;
   __shared__ int64_t share_s;                              // entries of a full share
   __shared__ TileInfo info_s[kInfo];
-  __shared__ float m_s[2][128], l_s[128], c_s[2][128];
+  __shared__ float m_s[2][128], l_s[128], c_s[C::kRows];
   const int tid = threadIdx.x, lane = tid & 31, warp = warp_index();
   volatile int* err = &expired;
 
@@ -149,7 +150,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       mbar_init(&o_full[i], 1);
       mbar_init(&o_free[i], 4);
     }
-    mbar_init(&q_full, C::kSoft);
+    mbar_init(&q_full, kLoaders);
+    mbar_init(&q_free, C::kSoft + 1);
     mbar_fence_init();
   }
   if (warp == C::kIssue) tmem_alloc(&tmem_base_s, 512);
@@ -317,17 +319,86 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     }
   } else if (warp >= C::kIssue) {
     fewer_registers<C::kRegsIssue>();
-    if (warp == C::kIssue + 1) {
-      // query rows of all units of this CTA into L2: a unit's softmax begins with them, and from HBM they were 5 us
-      constexpr int kLines = D * (int)sizeof(T) / 128;
-      for (Place at = place_s; at.open(); at.close(p)) {
-        const int rows = at.q.rows(p, at.row_tile);
-        for (int i = lane; i < rows * kLines; i += 32)
-          prefetch_l2(reinterpret_cast<const uint8_t*>(query_row<T>(p, at.q.t0, at.row_tile * C::kRows + i / kLines, at.head)) +
-                      i % kLines * 128);
+    if (warp > C::kIssue) {
+    // ------------------------------------------------------------------ query rows
+    // L lanes a row, eight 16-byte pieces a lane: copied as they are, all rows of a warp at once, as soon as the last S of the
+    // segment before is complete (its softmax and its result are still to come), then halves in their place.  A row of bf16 is
+    // scaled by the power of two that brings its largest element to [2^12, 2^13): exact, but for elements below 2^-26 of
+    // that one.  fp16 rows are taken as they are.  A scaling below zero turns q.
+    constexpr int L = D / 64, kPass = 32 / L, kPasses = C::kRows / kPass;
+    const int piece = lane % L, sub = lane >> 3, in8 = (lane & 7) / L;
+    // eight lanes in a row of them touch every bank once
+    const int row_in = L == 4 ? sub + 4 * in8 : 2 * in8 + (sub & 1) + 8 * (sub >> 1);
+    Place at = place_s;
+    uint32_t seg = 0;
+    for (; at.open(); at.close(p), ++seg) {
+      const int rows = at.q.rows(p, at.row_tile), passes = rows > 128 ? kPasses : 128 / kPass;
+      mbar_wait_warp(&q_free, (seg & 1) ^ 1, err, 70);
+      auto place_of = [&](int row, int j) {                // of piece L j + piece
+        const int c = L * j + piece;
+        return smem_u32(smem + C::kQ) + (row >> 7) * C::kOperand + (c >> 3) * kSub + (row & 127) * 128 + (((c & 7) ^ (row & 7)) << 4);
+      };
+#pragma unroll 1
+      for (int x = warp - C::kIssue - 1; x < passes; x += kLoaders) {
+        const int row = x * kPass + row_in;
+        const T* src = query_row<T>(p, at.q.t0, at.row_tile * C::kRows + min(row, rows - 1), at.head) + piece * 8;
+        const uint32_t bytes = row < rows ? 16 : 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place_of(row, j)), "l"(src + j * L * 8), "r"(bytes) : "memory");
       }
+      cp_async_commit();
+      cp_async_wait<0>();
+      const bool as_is = std::is_same<T, __half>::value && p.scale_log2 >= 0.0f;
+#pragma unroll 1
+      for (int x = warp - C::kIssue - 1; x < passes; x += kLoaders) {
+        const int row = x * kPass + row_in;
+        if (as_is) {
+          if (piece == 0) c_s[row] = p.scale_log2;
+          continue;
+        }
+        uint4 raw[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[j].x), "=r"(raw[j].y), "=r"(raw[j].z), "=r"(raw[j].w)
+                       : "r"(place_of(row, j)) : "memory");
+        float up = -1.0f, c = fabsf(p.scale_log2);
+        if constexpr (!std::is_same<T, __half>::value) {
+          auto two = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+          __nv_bfloat162 top = two(0u);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            top = __hmax2(top, __hmax2(__hmax2(__habs2(two(raw[j].x)), __habs2(two(raw[j].y))),
+                                       __hmax2(__habs2(two(raw[j].z)), __habs2(two(raw[j].w)))));
+#pragma unroll
+          for (int o = L / 2; o > 0; o >>= 1) {
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&top), o);
+            top = __hmax2(top, two(other));
+          }
+          const float big = fmaxf(__low2float(top), __high2float(top));
+          const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -110), 127);
+          up = copysignf(exp2_int(12 - ex), p.scale_log2);
+          c = big == 0.0f ? 0.0f : c * exp2_int(ex - 12);
+        }
+        if (piece == 0) c_s[row] = c;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t words[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+          uint32_t h[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            using T2 = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>::type;
+            const T2 t = *reinterpret_cast<const T2*>(&words[k]);
+            h[k] = pack_16x2<__half>(to_f32<T>(t.x) * up, to_f32<T>(t.y) * up);
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place_of(row, j)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
     }
-    if (warp == C::kIssue) {
+    } else {
     // ------------------------------------------------------------------ issue of the products
     Place at = place_s;
     const bool leader = elect_one();
@@ -344,7 +415,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       auto jobs_of = [&](int g) { return (turn == 1 ? tiles : (tiles + 1 - g) / 2) * C::kJobs; };
       auto tile_of = [&](int g, int j) { return j / C::kJobs * turn + (turn == 2 ? g : 0); };
       mbar_wait_warp(&q_full, seg & 1, err, 62);
+      int s_left = jobs_of(0) + (C::kGroups == 2 ? jobs_of(1) : 0);
       auto issue_s = [&](int g, int j) {
+        const bool last = --s_left == 0;
         const uint32_t tile = n + tile_of(g, j), st = tile % C::kStages;
         const int sub = j % C::kJobs;
         if (sub == 0 && (!both || g == 0)) mbar_wait(&k_full[st], (tile / C::kStages) & 1, err, 63);
@@ -360,6 +433,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
               umma_bf16(tmem + C::s_at(g, j & 1), x_q + c * (kSub >> 4) + k * 2, x_k + c * (kSub >> 4) + k * 2, id_s, (c > 0 || k > 0) ? 1u : 0u);
           umma_commit(&s_full[g][j & 1]);
           if (sub == C::kJobs - 1 && (!both || g == 1)) umma_commit(&k_free[st]);
+          if (last) umma_commit(&q_free);
         }
         __syncwarp();
       };
@@ -411,6 +485,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     const uint32_t lane_addr = (uint32_t)(wq * 32) << 16;
     uint8_t* stg = smem + C::kOut + warp * 2048;
     uint32_t n = 0;                                        // tiles so far
+    uint32_t seg = 0;                                      // segments so far
     uint32_t s_phase = 0, results = 0, pv = 0;             // phases of s_full (a bit a place), o_full and pv_done so far
     bool first_segment = true;
     for (; at.open(); at.close(p)) {
@@ -421,62 +496,13 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       const int row = (both ? group * 128 : 0) + row_in;   // of the unit
       const bool live = row < rows;
       const int i_row = at.row_tile * C::kRows + row;      // of the request
-      // ---- query rows: all products of the segment before are complete (each group has seen its last S)
-      named_bar_sync(1, 32 * C::kSoft);
-      // A warp loads its 32 rows together, D / 8 lanes a row: a thread's own row would be 32 lines an instruction, and took
-      // 9 to 12 us a unit.
-      if (both || group == 0) {
-        constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kBatch = 8;       // of a row; rows an instruction; loads in flight
-        const int base = (both ? group * 128 : 0) + wq * 32;
-        const uint32_t dst = smem_u32(smem + C::kQ) + (both ? group : 0) * C::kOperand;
-        const int e = lane % kLanes;                       // piece of eight elements
-#pragma unroll 1
-        for (int x0 = 0; x0 < 32 / kAtOnce; x0 += kBatch) {
-          uint4 raw[kBatch];
-#pragma unroll
-          for (int x = 0; x < kBatch; ++x) {
-            const int r = base + (x0 + x) * kAtOnce + lane / kLanes;
-            raw[x] = *reinterpret_cast<const uint4*>(
-                query_row<T>(p, at.q.t0, at.row_tile * C::kRows + min(r, rows - 1), at.head) + e * 8);
-          }
-#pragma unroll
-          for (int x = 0; x < kBatch; ++x) {
-            const int in = wq * 32 + (x0 + x) * kAtOnce + lane / kLanes;
-            const bool there = (both ? group * 128 : 0) + in < rows;
-            // the row's largest magnitude, two values at a time
-            using T2 = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>::type;
-            auto two = [](uint32_t w) { return *reinterpret_cast<const T2*>(&w); };
-            T2 top = __hmax2(__hmax2(__habs2(two(raw[x].x)), __habs2(two(raw[x].y))),
-                             __hmax2(__habs2(two(raw[x].z)), __habs2(two(raw[x].w))));
-#pragma unroll
-            for (int o = kLanes / 2; o > 0; o >>= 1) {
-              const uint32_t other = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&top), o);
-              top = __hmax2(top, two(other));
-            }
-            const float big = fmaxf(to_f32<T>(top.x), to_f32<T>(top.y));
-            // largest element in [2^12, 2^13); scaling below zero turns q
-            const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -110), 127);
-            const float up = there ? copysignf(exp2_int(12 - ex), p.scale_log2) : 0.0f;
-            if (e == 0) c_s[both ? group : 0][in] = big == 0.0f ? 0.0f : fabsf(p.scale_log2) * exp2_int(ex - 12);
-            uint32_t h[4];
-            const uint32_t words[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const T2 t = two(words[k]);
-              h[k] = there ? pack_16x2<__half>(to_f32<T>(t.x) * up, to_f32<T>(t.y) * up) : 0u;
-            }
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + in * 128 + (e >> 3) * kSub + (((e & 7) ^ (in & 7)) << 4)),
-                         "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
-                         : "memory");
-          }
-        }
-        fence_proxy_async_smem();
-      }
+      mbar_wait(&q_full, seg & 1, err, 71);
+      ++seg;
+      const float c_row = c_s[both ? row : row_in];
+      // where both groups work on the same rows, they exchange results where q is
+      const bool merge = C::kGroups == 2 && !both;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full);
-      // where both groups work on the same rows, the first one has loaded them
-      if (C::kGroups == 2 && !both) named_bar_sync(1, 32 * C::kSoft);
-      const float c_row = c_s[both ? group : 0][row_in];
+      if (!merge && lane == 0) mbar_arrive(&q_free);
       const int limit = live ? at.q.seen(p, i_row) : 0;    // keys that this row sees
       float m = -INFINITY, ref = -INFINITY, l = 0.0f;
 
@@ -606,7 +632,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       }
       const uint32_t o_at = tmem + lane_addr + C::kO + group * 128;
       bool writes = true;
-      if (C::kGroups == 2 && !both) {
+      if (merge) {
         // the groups' results of the same rows: the second one's goes through shared memory, where q was
         m_s[group][row_in] = m;
         if (group == 1) l_s[row_in] = l;
@@ -636,24 +662,32 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         }
         m = m_all;
       }
-      const bool add = C::kGroups == 2 && !both && tiles > 1;
+      const bool add = merge && tiles > 1;
       const int rows_warp = min(max(rows - (both ? group * 128 : 0) - wq * 32, 0), 32);    // of this warp that exist
       if (writes && rows_warp > 0) {
         const int row0 = (both ? group * 128 : 0) + wq * 32;
-        const float inv = whole && l != 0.0f ? __frcp_rn(l) : 0.0f;
+        const float inv = !whole ? 1.0f : l != 0.0f ? __frcp_rn(l) : 0.0f;
         if (whole) {
           if (live && p.lse != nullptr) p.lse[out_row(p, at.q.t0 * p.g + i_row, at.head)] = lse_of(m, l);
         } else if (live) {
           p.ws_m[(int64_t)slot * C::kRows + row] = m;
           p.ws_l[(int64_t)slot * C::kRows + row] = l;
         }
+        // a result goes out 64 bytes of a row at a time, four lanes a row; a partial one four columns at a time, a lane a row
+        T* to[4];
+        if (whole) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = min(8 * e + (lane >> 2), rows_warp - 1);
+            to[e] = static_cast<T*>(p.out) + out_row(p, at.q.t0 * p.g + at.row_tile * C::kRows + row0 + r, at.head) * D + (lane & 3) * 8;
+          }
+        }
+        float4* part = reinterpret_cast<float4*>(p.ws_acc + (int64_t)slot * C::kRows * D) + row;
 #pragma unroll 1
         for (int cc = 0; cc < D / 32; ++cc) {
           uint32_t o[32];
           tmem_ld32(o_at + cc * 32, o);
           tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
           if (add) {
             const uint32_t buf = smem_u32(smem + C::kQ) + row_in * 512;
 #pragma unroll
@@ -663,39 +697,40 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
                                buf + (((cc * 8 + e) ^ lane) << 4))
                            : "memory");
 #pragma unroll
-              for (int k = 0; k < 4; ++k) o[4 * e + k] = __float_as_uint(__uint_as_float(o[4 * e + k]) + x[k]);
+              for (int k = 0; k < 4; ++k) o[4 * e + k] = __float_as_uint((__uint_as_float(o[4 * e + k]) * f + x[k]) * inv);
             }
+          } else {
+            const float f_inv = f * inv;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f_inv);
           }
-          // 64 bytes of a row at a time, four lanes a row: a lane's own row would be 16 bytes of 32 rows an instruction
-#pragma unroll 1
-          for (int h = 0; h < (whole ? 1 : 2); ++h) {
-            uint32_t w[16];
+          if (whole) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              w[e] = whole ? pack_16x2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv) : h ? o[16 + e] : o[e];
+            for (int e = 0; e < 4; ++e) {
+              uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<uint4*>(stg + sw64_offset(lane, e * 16)) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+              for (int k = 0; k < 4; ++k) w[k] = pack_16x2<T>(__uint_as_float(o[8 * e + 2 * k]), __uint_as_float(o[8 * e + 2 * k + 1]));
+              *reinterpret_cast<uint4*>(stg + sw64_offset(lane, e * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
             __syncwarp();
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int r = 8 * e + (lane >> 2), ch = lane & 3;
-              const uint4 v = *reinterpret_cast<const uint4*>(stg + sw64_offset(r, ch * 16));
-              if (r < rows_warp) {
-                uint8_t* to = whole ? reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) +
-                                                                 out_row(p, at.q.t0 * p.g + at.row_tile * C::kRows + row0 + r, at.head) * D +
-                                                                 cc * 32)
-                                    : reinterpret_cast<uint8_t*>(p.ws_acc + ((int64_t)slot * C::kRows + row0 + r) * D + cc * 32 + h * 16);
-                *reinterpret_cast<uint4*>(to + ch * 16) = v;
-              }
+              const int r = 8 * e + (lane >> 2);
+              const uint4 v = *reinterpret_cast<const uint4*>(stg + sw64_offset(r, (lane & 3) * 16));
+              if (r < rows_warp) *reinterpret_cast<uint4*>(to[e] + cc * 32) = v;
             }
             __syncwarp();
+          } else if (live) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(part + (cc * 8 + e) * C::kRows) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
       }
       tc_fence_before();
       __syncwarp();
       if (has && lane == 0) mbar_arrive(&o_free[group]);
+      if (merge && lane == 0) mbar_arrive(&q_free);
       if (!whole && at.from == 0 && tid == 0) p.cut[blockIdx.x] = cut_unit(p, at, share_s, first_segment);
       n += tiles;
       first_segment = false;
@@ -716,7 +751,7 @@ int run_chunk(const PagedParams& p, int ctas, cudaStream_t st) {
   using C = Cfg<D>;
   if (int rc = allow_smem("nvfp4_kv8_attention", reinterpret_cast<const void*>(paged_chunk_kernel<T, D>), C::kBytes)) return rc;
   if (int rc = launch("nvfp4_kv8_attention", paged_chunk_kernel<T, D>, dim3(ctas), C::kThreads, C::kBytes, st, p)) return rc;
-  return launch_combine<T, D, C::kRows>(p, ctas, st);
+  return launch_combine<T, D, C::kRows, true>(p, ctas, st);
 }
 
 }  // namespace
