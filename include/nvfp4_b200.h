@@ -348,10 +348,11 @@ int nvfp4_kv8_write(const void* key, const void* value, int dtype, int64_t token
 
 /*
  * Attention over that cache.  q [tokens, hk * g, d] in `q_dtype` (element strides of token and head, unit stride along d,
- * rows 16-byte aligned), `scaling` finite; request r owns query tokens cu_seqlens[r] .. cu_seqlens[r + 1] (cu_seqlens NULL: token r, tokens == requests), the last ones
- * of its lengths[r] keys: token i of n sees keys 0 .. lengths[r] - n + i.  out [tokens, hk * g, d] in `q_dtype` and lse
- * [tokens, hk * g] (natural log, or NULL) are contiguous; tokens that see no key, and tokens of no request, get zeros and
- * -inf.  Table entries that are no block hide their keys; lengths are cut to width * block_size.
+ * rows 16-byte aligned), `scaling` finite; request r owns query tokens cu_seqlens[r] .. cu_seqlens[r + 1] (cu_seqlens NULL:
+ * token r, tokens == requests), the last ones of its lengths[r] keys: token i of n sees keys 0 .. lengths[r] - n + i.  out
+ * [tokens, hk * g, d] in `q_dtype` (32-byte aligned) and lse [tokens, hk * g] (natural log, or NULL) are contiguous; tokens that
+ * see no key, and tokens of no request, get zeros and -inf.  Table entries that are no block hide their keys; lengths are
+ * cut to width * block_size.
  * workspace: nvfp4_kv8_attention_plan bytes for the same call, 16-byte aligned.  status: device int, written non-zero if a
  * bounded wait expired; may be NULL.
  */

@@ -85,8 +85,8 @@ inline int allow_smem(const char* what, const void* kern, int bytes) {
 // forward, whose 202 KB leave 28 of L1, the packs of a prompt Z4 S8192 took 119 us instead of 92 (prompt S12289 D256 in all
 // 675 -> 663).  A hint, not checked.
 constexpr int kStreamSmem = 45;
-inline void prefer_l1(const void* kern) {
-  if (kernel_attribute<cudaFuncAttributePreferredSharedMemoryCarveout>(kern, kStreamSmem) != cudaSuccess) cudaGetLastError();
+inline void prefer_l1(const void* kern, int smem_percent = kStreamSmem) {
+  if (kernel_attribute<cudaFuncAttributePreferredSharedMemoryCarveout>(kern, smem_percent) != cudaSuccess) cudaGetLastError();
 }
 
 // Clusters of `size` CTAs (1 to 8, else 0) of a kernel that are resident at once.  Of kernels whose shared memory leaves room

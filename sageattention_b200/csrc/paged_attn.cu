@@ -584,9 +584,9 @@ extern "C" int nvfp4_kv8_attention(const void* q, int q_dtype, int64_t s_qt, int
                     hk * g < (1 << 20) && blocks >= 0 && blocks < INT32_MAX && width >= 0 && width * block_size < INT32_MAX - 256,
                 "nvfp4_kv8_attention: sizes out of range");
   NVFP4_REQUIRE(cu_seqlens != nullptr || tokens == requests, "nvfp4_kv8_attention: one token a request without cu_seqlens");
-  NVFP4_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)workspace) & 15) == 0 &&
+  NVFP4_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)workspace) & 15) == 0 && ((uintptr_t)out & 31) == 0 &&
                     ((k_block | v_block) & 15) == 0,
-                "nvfp4_kv8_attention: cache blocks, out and workspace must be 16-byte aligned");
+                "nvfp4_kv8_attention: cache blocks and workspace must be 16-byte aligned, out 32-byte aligned");
   NVFP4_REQUIRE(((uintptr_t)q & 15) == 0 && ((s_qt | s_qh) * (q_dtype == NVFP4_DT_FP32 ? 4 : 2) & 15) == 0,
                 "nvfp4_kv8_attention: query rows must be 16-byte aligned");
   NVFP4_REQUIRE(isfinite(scaling), "nvfp4_kv8_attention: scaling must be finite");

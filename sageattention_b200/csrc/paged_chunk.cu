@@ -47,8 +47,7 @@ struct Cfg {
   // an increase waits for registers of this launch, which has 128 a thread (65536 / 512): more than those would wait forever
   static_assert(kThreads == 512 && kSoft * kRegsSoft + 4 * kConvert * kRegsConvert + 4 * kRegsIssue <= kThreads / 32 * 128, "registers");
   static constexpr int kOperand = D / 64 * kSub;           // 128 rows of q, or a tile of keys or values
-  static constexpr int kQ = 0, kK = kGroups * kOperand, kV = kK + kStages * kOperand, kOut = kV + kStages * kOperand;
-  static constexpr int kBytes = kOut + kSoft * 2048 + 1024;
+  static constexpr int kQ = 0, kK = kGroups * kOperand, kV = kK + kStages * kOperand, kTail = kV + kStages * kOperand;
   static constexpr int kN = D == 128 ? 64 : 128;           // keys of a job
   static constexpr int kJobs = kTile / kN;                 // jobs of a tile
   // Products issued from straight code or (1) from loops: an instruction per 64 halves' step at D = 128, where the straight
@@ -66,6 +65,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+
+__device__ __forceinline__ void store_sector(void* dst, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
 // two fp32 operations an instruction
@@ -118,23 +123,49 @@ struct TileInfo {
 __device__ __forceinline__ int scale_exp(float s) { return min(max((int)(__float_as_uint(s) >> 23 & 0xFF) - 127, -112), 126); }
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// Shared memory behind the tiles.  All of it is dynamic, and within 195 KB: with that the SM's split leaves 60 KB of L1, whose
+// lines hold what the converting warps have asked for, and with more than 195 KB 28.
+template <int D>
+struct Tail {
+  using C = Cfg<D>;
+  uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2][2], p_full[2][2], o_full[2], o_free[2], pv_done[2], q_full, q_free;
+  int64_t list[C::kThreads / 32 + 2];
+  Walk<C::kRows, kTile> place;
+  int64_t share;                                           // entries of a full share
+  uint32_t tmem_base;
+  int expired;
+  TileInfo info[kInfo];
+  float c[C::kRows];
+  float m[C::kGroups][128];
+  __device__ __forceinline__ float* l() { return c + C::kRows - 128; }       // of rows that a unit of one group's rows does not have
+};
+constexpr int kSmemPercent = 85;
+template <int D>
+constexpr int smem_bytes() {
+  static_assert(Cfg<D>::kTail + sizeof(Tail<D>) <= 195 * 1024, "L1");
+  return Cfg<D>::kTail + (int)sizeof(Tail<D>);
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedParams p) {
   using C = Cfg<D>;
   using Place = Walk<C::kRows, kTile>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2][2], p_full[2][2], o_full[2], o_free[2], pv_done[2], q_full, q_free;
-  __shared__ uint32_t tmem_base_s;
-  __shared__ int expired;                                  // a wait ran out: site, else 0
-  __shared__ int64_t list_s[C::kThreads / 32 + 2];
-  __shared__ Place place_s;
-  __shared__ int64_t share_s;                              // entries of a full share
-  __shared__ TileInfo info_s[kInfo];
-  __shared__ float m_s[2][128], l_s[128], c_s[C::kRows];
+  extern __shared__ __align__(1024) uint8_t smem[];        // at 1024 without static shared memory in front of it, see below
+  Tail<D>& sh = *reinterpret_cast<Tail<D>*>(smem + C::kTail);
+  auto &k_full = sh.k_full, &k_free = sh.k_free, &v_full = sh.v_full, &v_free = sh.v_free, &pv_done = sh.pv_done, &o_full = sh.o_full,
+       &o_free = sh.o_free;
+  auto &s_full = sh.s_full, &p_full = sh.p_full;
+  uint64_t &q_full = sh.q_full, &q_free = sh.q_free;
+  int& expired = sh.expired;                               // a wait ran out: site, else 0
+  auto& info_s = sh.info;
+  auto& c_s = sh.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = warp_index();
   volatile int* err = &expired;
 
+  if (smem_u32(smem) & 1023) {                             // what the products' descriptors take for granted
+    if (tid == 0 && p.status != nullptr) atomicExch(p.status, 72);
+    return;
+  }
   if (tid == 0) {
     expired = 0;
     for (int i = 0; i < 2; ++i) {
@@ -154,19 +185,19 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     mbar_init(&q_free, C::kSoft + 1);
     mbar_fence_init();
   }
-  if (warp == C::kIssue) tmem_alloc(&tmem_base_s, 512);
+  if (warp == C::kIssue) tmem_alloc(&sh.tmem_base, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   griddep_launch();
   griddep_wait();
-  const uint32_t tmem = tmem_base_s;
+  const uint32_t tmem = sh.tmem_base;
   {
     Place from;
-    const int64_t share = deal_tiles<C::kThreads>(p, list_s, from);
+    const int64_t share = deal_tiles<C::kThreads>(p, sh.list, from);
     if (tid == 0) {
-      place_s = from;
-      share_s = share;
+      sh.place = from;
+      sh.share = share;
       p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
     }
   }
@@ -174,7 +205,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
 
   if (warp >= C::kSoft && warp < C::kIssue) {
     if (C::kRegsConvert > 128) more_registers<C::kRegsConvert>();
-    Place ahead = place_s;
+    Place ahead = sh.place;
     bool more = ahead.open();                              // there is a tile to be looked up: `tile` of `ahead`
     int tile = ahead.from;
     // ------------------------------------------------------------------ codes to halves
@@ -329,7 +360,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     const int piece = lane % L, sub = lane >> 3, in8 = (lane & 7) / L;
     // eight lanes in a row of them touch every bank once
     const int row_in = L == 4 ? sub + 4 * in8 : 2 * in8 + (sub & 1) + 8 * (sub >> 1);
-    Place at = place_s;
+    Place at = sh.place;
     uint32_t seg = 0;
     for (; at.open(); at.close(p), ++seg) {
       const int rows = at.q.rows(p, at.row_tile), passes = rows > 128 ? kPasses : 128 / kPass;
@@ -400,7 +431,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     }
     } else {
     // ------------------------------------------------------------------ issue of the products
-    Place at = place_s;
+    Place at = sh.place;
     const bool leader = elect_one();
     const uint32_t id_s = make_idesc_bf16(128, C::kN, false, true), id_o = make_idesc_bf16(128, 128, true, true);
     const uint64_t b_q = desc_sw128(smem + C::kQ, 0), b_k = desc_sw128(smem + C::kK, 0);
@@ -479,11 +510,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     }
   } else {
     more_registers<C::kRegsSoft>();
-    Place at = place_s;
+    Place at = sh.place;
     // ------------------------------------------------------------------ softmax, a thread a row
     const int group = warp >> 2, wq = warp & 3, row_in = wq * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(wq * 32) << 16;
-    uint8_t* stg = smem + C::kOut + warp * 2048;
     uint32_t n = 0;                                        // tiles so far
     uint32_t seg = 0;                                      // segments so far
     uint32_t s_phase = 0, results = 0, pv = 0;             // phases of s_full (a bit a place), o_full and pv_done so far
@@ -634,10 +664,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       bool writes = true;
       if (merge) {
         // the groups' results of the same rows: the second one's goes through shared memory, where q was
-        m_s[group][row_in] = m;
-        if (group == 1) l_s[row_in] = l;
+        sh.m[group][row_in] = m;
+        if (group == 1) sh.l()[row_in] = l;
         named_bar_sync(1, 32 * C::kSoft);
-        const float m_all = fmaxf(m_s[0][row_in], m_s[1][row_in]);
+        const float m_all = fmaxf(sh.m[0][row_in], sh.m[1][row_in]);
         f *= m_all == -INFINITY ? 1.0f : ex2_approx(m - m_all);
         const uint32_t buf = smem_u32(smem + C::kQ) + row_in * 512;
         if (group == 1 && has) {
@@ -657,7 +687,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         named_bar_sync(1, 32 * C::kSoft);
         writes = group == 0;
         if (writes && tiles > 1) {
-          const float m1 = m_s[1][row_in], l1 = l_s[row_in];
+          const float m1 = sh.m[1][row_in], l1 = sh.l()[row_in];
           l = m_all == -INFINITY ? l + l1 : l * ex2_approx(m - m_all) + l1 * ex2_approx(m1 - m_all);
         }
         m = m_all;
@@ -673,15 +703,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
           p.ws_m[(int64_t)slot * C::kRows + row] = m;
           p.ws_l[(int64_t)slot * C::kRows + row] = l;
         }
-        // a result goes out 64 bytes of a row at a time, four lanes a row; a partial one four columns at a time, a lane a row
-        T* to[4];
-        if (whole) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = min(8 * e + (lane >> 2), rows_warp - 1);
-            to[e] = static_cast<T*>(p.out) + out_row(p, at.q.t0 * p.g + at.row_tile * C::kRows + row0 + r, at.head) * D + (lane & 3) * 8;
-          }
-        }
+        // a lane a row: of a result a sector at a time, of a partial one four columns, which lie row by row
+        T* to = static_cast<T*>(p.out) + out_row(p, at.q.t0 * p.g + min(i_row, at.row_tile * C::kRows + rows - 1), at.head) * D;
         float4* part = reinterpret_cast<float4*>(p.ws_acc + (int64_t)slot * C::kRows * D) + row;
 #pragma unroll 1
         for (int cc = 0; cc < D / 32; ++cc) {
@@ -704,34 +727,27 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f_inv);
           }
-          if (whole) {
+          if (live && whole) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t w[4];
+            for (int e = 0; e < 2; ++e) {
+              uint32_t w[8];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) w[k] = pack_16x2<T>(__uint_as_float(o[8 * e + 2 * k]), __uint_as_float(o[8 * e + 2 * k + 1]));
-              *reinterpret_cast<uint4*>(stg + sw64_offset(lane, e * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int k = 0; k < 8; ++k) w[k] = pack_16x2<T>(__uint_as_float(o[16 * e + 2 * k]), __uint_as_float(o[16 * e + 2 * k + 1]));
+              store_sector(to + cc * 32 + e * 16, w);
             }
-            __syncwarp();
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = 8 * e + (lane >> 2);
-              const uint4 v = *reinterpret_cast<const uint4*>(stg + sw64_offset(r, (lane & 3) * 16));
-              if (r < rows_warp) *reinterpret_cast<uint4*>(to[e] + cc * 32) = v;
-            }
-            __syncwarp();
           } else if (live) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               *reinterpret_cast<uint4*>(part + (cc * 8 + e) * C::kRows) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
+          __syncwarp();
         }
       }
       tc_fence_before();
       __syncwarp();
       if (has && lane == 0) mbar_arrive(&o_free[group]);
       if (merge && lane == 0) mbar_arrive(&q_free);
-      if (!whole && at.from == 0 && tid == 0) p.cut[blockIdx.x] = cut_unit(p, at, share_s, first_segment);
+      if (!whole && at.from == 0 && tid == 0) p.cut[blockIdx.x] = cut_unit(p, at, sh.share, first_segment);
       n += tiles;
       first_segment = false;
     }
@@ -749,8 +765,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
 template <typename T, int D>
 int run_chunk(const PagedParams& p, int ctas, cudaStream_t st) {
   using C = Cfg<D>;
-  if (int rc = allow_smem("nvfp4_kv8_attention", reinterpret_cast<const void*>(paged_chunk_kernel<T, D>), C::kBytes)) return rc;
-  if (int rc = launch("nvfp4_kv8_attention", paged_chunk_kernel<T, D>, dim3(ctas), C::kThreads, C::kBytes, st, p)) return rc;
+  const void* kern = reinterpret_cast<const void*>(paged_chunk_kernel<T, D>);
+  if (int rc = allow_smem("nvfp4_kv8_attention", kern, smem_bytes<D>())) return rc;
+  prefer_l1(kern, kSmemPercent);
+  if (int rc = launch("nvfp4_kv8_attention", paged_chunk_kernel<T, D>, dim3(ctas), C::kThreads, smem_bytes<D>(), st, p)) return rc;
   return launch_combine<T, D, C::kRows, true>(p, ctas, st);
 }
 
