@@ -588,12 +588,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         }
         const float c = fmaxf(c_row * info.k_factor, 0x1p-126f);   // never 0: hidden keys are -inf
         top = top == -INFINITY ? -INFINITY : top * c;
-        // reference of the weights: moves only where the maximum has left it behind
+        // reference of the weights: moves only where the maximum has left it behind, and then for all rows of the warp, whose
+        // results are all read and written anyway, so that the next move is a while away
         const float want = top + info.v_log2;
-        const bool move = want > ref + kLag;
-        if (__any_sync(0xffffffffu, move)) {
-          const float ref_new = move ? want : ref;
-          const float f = move ? ex2_approx(ref - ref_new) : 1.0f;
+        if (__any_sync(0xffffffffu, want > ref + kLag)) {
+          const float ref_new = fmaxf(ref, want);
+          const float f = want > ref ? ex2_approx(ref - ref_new) : 1.0f;
           ref = ref_new;
           if (j > 0) {                                     // the product before has to be complete
             mbar_wait(&pv_done[group], (pv - 1) & 1, err, 68);
