@@ -85,6 +85,11 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
@@ -591,25 +596,13 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         // reference of the weights: moves only where the maximum has left it behind, and then for all rows of the warp, whose
         // results are all read and written anyway, so that the next move is a while away
         const float want = top + info.v_log2;
+        bool moved = false;
+        float f = 1.0f;
         if (__any_sync(0xffffffffu, want > ref + kLag)) {
           const float ref_new = fmaxf(ref, want);
-          const float f = want > ref ? ex2_approx(ref - ref_new) : 1.0f;
+          if (want > ref) f = ex2_approx(ref - ref_new);
           ref = ref_new;
-          if (j > 0) {                                     // the product before has to be complete
-            mbar_wait(&pv_done[group], (pv - 1) & 1, err, 68);
-            tc_fence_after();
-            __syncwarp();
-#pragma unroll 1
-            for (int cc = 0; cc < D / 32; ++cc) {
-              uint32_t o[32];
-              const uint32_t o_at = tmem + lane_addr + C::kO + group * 128 + cc * 32;
-              tmem_ld32(o_at, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st32(o_at, o);
-            }
-          }
+          moved = j > 0;
         }
         const float minus = ref == -INFINITY ? 0.0f : info.v_log2 - ref + kLift;
         const uint64_t c2 = pair(__float_as_uint(c), __float_as_uint(c)), minus2 = pair(__float_as_uint(minus), __float_as_uint(minus));
@@ -635,6 +628,29 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
           }
           if (x >= 2) tmem_ld32(s_at + (x - 2) * 32, now);
           tmem_st16(s_at + C::kN / 2 + x * 16, w);         // over columns that have been read
+        }
+        if (moved) {                                       // the product before has to be complete: mostly it is by now
+          mbar_wait(&pv_done[group], (pv - 1) & 1, err, 68);
+          tc_fence_after();
+          __syncwarp();
+          const uint64_t f2 = pair(__float_as_uint(f), __float_as_uint(f));
+#pragma unroll 1
+          for (int cc = 0; cc < D / 64; ++cc) {
+            const uint32_t o_at = tmem + lane_addr + C::kO + group * 128 + cc * 64;
+            tmem_ld32(o_at, s[0]);
+            tmem_ld32(o_at + 32, s[1]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const uint64_t y = mul_pair(pair(s[h][2 * e], s[h][2 * e + 1]), f2);
+                s[h][2 * e] = (uint32_t)y;
+                s[h][2 * e + 1] = (uint32_t)(y >> 32);
+              }
+              tmem_st32(o_at + h * 32, s[h]);
+            }
+          }
         }
         tmem_st_wait();
         tc_fence_before();
