@@ -9,8 +9,7 @@
 // j & 1 of the group's two, P over the upper half of the S it came from.
 //   rows > 128 (D = 128): group g has rows 128 g .., both go through every key tile
 //   rows <= 128 (D = 128): the groups take turns at the key tiles and keep results of their own, merged at the end
-// Products are issued in the order PV(j), S(j + 2): S(j + 1) is there when the softmax of job j ends, and a completed S(j + 2)
-// tells that PV(j) is complete as well.
+// Products are issued in the order PV(j), S(j + 2): S(j + 1) is there when the softmax of job j ends.
 //
 // What bounds it (D = 128): a key tile of 256 rows is 2580 clocks of products on an SM (S with 64 keys reads its operands
 // from shared memory at 48 clocks an instruction instead of 32) and 2048 of ex2.
@@ -473,40 +472,53 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         }
         __syncwarp();
       };
-      const int most = jobs_of(0);
-#pragma unroll 1
-      for (int j = -2; j < most; ++j) {                    // PV of job j behind S of job j + 1, S of job j + 2 behind that
+      auto issue_pv = [&](int g, int j) {
+        const uint32_t tile = n + tile_of(g, j), st = tile % C::kStages;
+        const int sub = j % C::kJobs;
+        if (j == 0 && (used >> g & 1)) mbar_wait(&o_free[g], (o_phase >> g & 1) ^ 1, err, 64);
+        if (sub == 0 && (!both || g == 0)) mbar_wait(&v_full[st], (tile / C::kStages) & 1, err, 65);
+        mbar_wait_warp(&p_full[g][j & 1], p_phase >> (2 * g + (j & 1)) & 1, err, 66);
+        p_phase ^= 1u << (2 * g + (j & 1));
+        tc_fence_after();
+        if (leader) {
+          const uint64_t x_v = b_v + (uint64_t)(st * (C::kOperand >> 4) + sub * (C::kN * 128 >> 4));
+          const uint32_t x_p = tmem + C::s_at(g, j & 1) + C::kN / 2;
 #pragma unroll C::kIssueUnroll
-        for (int g = 0; g < C::kGroups; ++g) {
-          const int jobs = jobs_of(g);
-          if (j >= 0 && j < jobs) {
-            const uint32_t tile = n + tile_of(g, j), st = tile % C::kStages;
-            const int sub = j % C::kJobs;
-            if (j == 0 && (used >> g & 1)) mbar_wait(&o_free[g], (o_phase >> g & 1) ^ 1, err, 64);
-            if (sub == 0 && (!both || g == 0)) mbar_wait(&v_full[st], (tile / C::kStages) & 1, err, 65);
-            mbar_wait_warp(&p_full[g][j & 1], p_phase >> (2 * g + (j & 1)) & 1, err, 66);
-            p_phase ^= 1u << (2 * g + (j & 1));
-            tc_fence_after();
-            if (leader) {
-              const uint64_t x_v = b_v + (uint64_t)(st * (C::kOperand >> 4) + sub * (C::kN * 128 >> 4));
-              const uint32_t x_p = tmem + C::s_at(g, j & 1) + C::kN / 2;
-#pragma unroll C::kIssueUnroll
-              for (int c = 0; c < D / 128; ++c)
+          for (int c = 0; c < D / 128; ++c)
 #pragma unroll
-                for (int k = 0; k < C::kN / 16; ++k)
-                  umma_bf16_ta(tmem + C::kO + g * 128 + c * 128, x_p + k * 8, x_v + c * (2 * kSub >> 4) + k * 128, id_o,
-                               (k > 0 || j > 0) ? 1u : 0u);
-              if (sub == C::kJobs - 1 && (!both || g == 1)) umma_commit(&v_free[st]);
-              umma_commit(&pv_done[g]);
-              if (j + 1 == jobs) umma_commit(&o_full[g]);
-            }
-            __syncwarp();
-            if (j == 0) {
-              used |= 1u << g;
-              o_phase ^= 1u << g;
-            }
+            for (int k = 0; k < C::kN / 16; ++k)
+              umma_bf16_ta(tmem + C::kO + g * 128 + c * 128, x_p + k * 8, x_v + c * (2 * kSub >> 4) + k * 128, id_o,
+                           (k > 0 || j > 0) ? 1u : 0u);
+          if (sub == C::kJobs - 1 && (!both || g == 1)) umma_commit(&v_free[st]);
+          umma_commit(&pv_done[g]);
+          if (j + 1 == jobs_of(g)) umma_commit(&o_full[g]);
+        }
+        __syncwarp();
+        if (j == 0) {
+          used |= 1u << g;
+          o_phase ^= 1u << g;
+        }
+      };
+      // Where the groups take turns, S of a tile must not stand in front of the products with V of the tile three before: its K is
+      // converted behind V of the tile before it, which waits for that place.  So there group 1 is a job behind group 0, and
+      // a step has both groups' PV first.  With more than 128 rows both groups are at the same tile, and that PV is two steps old.
+      const bool turns = C::kGroups == 2 && !both;
+      const int steps = jobs_of(0) + (turns ? 1 : 0);
+#pragma unroll 1
+      for (int j = -2; j < steps; ++j) {                   // PV of job j behind S of job j + 1, S of job j + 2 behind that
+        if (turns) {
+#pragma unroll 1
+          for (int x = 0; x < 4; ++x) {
+            const int g = x & 1, at_j = j - g;
+            if (x < 2 && at_j >= 0 && at_j < jobs_of(g)) issue_pv(g, at_j);
+            if (x >= 2 && at_j >= -2 && at_j + 2 < jobs_of(g)) issue_s(g, at_j + 2);
           }
-          if (j + 2 < jobs) issue_s(g, j + 2);
+        } else {
+#pragma unroll C::kIssueUnroll
+          for (int g = 0; g < C::kGroups; ++g) {
+            if (j >= 0 && j < jobs_of(g)) issue_pv(g, j);
+            if (j + 2 < jobs_of(g)) issue_s(g, j + 2);
+          }
         }
       }
       n += tiles;

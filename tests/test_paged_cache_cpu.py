@@ -145,3 +145,49 @@ def test_custom_ops_infer_shapes():
         q = torch.empty(50, 8, 128, dtype=torch.float16)
         out, lse = ns.fp8_paged_attention(q, cu, c, c, s, s, i(3, 9), i(3), 0.1, 4)
         assert out.shape == q.shape and out.dtype == q.dtype and lse.shape == (50, 8)
+
+
+def _ends(segments, stages=2, per_tile=2):
+    """The roles of the many-row kernel at D 128 as lists of (what is waited for, what is told); True if all come to their end.
+    Segments are (tiles, rows above 128).  One converting group does K and V of tile after tile in two places; group g of two
+    has every tile, or every other one; products are issued one after the other."""
+    convert, issue, soft, done, jobs_of = [], [], [[], []], set(), []
+    n = 0
+    for at, (tiles, both) in enumerate(segments):
+        for t in range(n, n + tiles):
+            convert += [([("s of", t - stages)] if t >= stages else [], ("k", t)), ([("pv of", t - stages)] if t >= stages else [], ("v", t))]
+        jobs = [(tiles if both else (tiles + 1 - g) // 2) * per_tile for g in (0, 1)]
+        steps = [(kind, g, j + ahead) for j in range(-2, max(jobs) + 1)
+                 for kind, g, ahead in ((("pv", 0, 0), ("s", 0, 2), ("pv", 1, 0), ("s", 1, 2)) if both else
+                                        (("pv", 0, 0), ("pv", 1, -1), ("s", 0, 2), ("s", 1, 1)))]
+        for kind, g, j in steps:
+            if 0 <= j < jobs[g]:
+                tile = n + j // per_tile * (1 if both else 2) + (0 if both else g)
+                told = [(kind, at, g, j)]
+                if j % per_tile == per_tile - 1 and (not both or g == 1):
+                    told.append((kind + " of", tile))
+                issue.append(([("k", tile)] if kind == "s" else [("v", tile), ("p", at, g, j)], *told))
+        for g in (0, 1):
+            soft[g] += [([("s", at, g, j)], ("p", at, g, j)) for j in range(jobs[g])]
+        jobs_of.append(jobs)
+        n += tiles
+    assert len(issue) == 2 * sum(map(sum, jobs_of))
+    roles = [convert, issue, *soft]
+    moved = True
+    while moved:
+        moved = False
+        for role in roles:
+            while role and all(w in done for w in role[0][0]):
+                done.update(role.pop(0)[1:])
+                moved = True
+    return not any(roles)
+
+
+def test_no_role_of_the_many_row_kernel_waits_for_itself():
+    gen = torch.Generator().manual_seed(0)
+    for tiles in range(1, 40):
+        assert _ends([(tiles, False)]) and _ends([(tiles, True)])
+    for _ in range(300):
+        size = torch.randint(1, 25, (5,), generator=gen).tolist()
+        rows = (torch.rand(5, generator=gen) < 0.5).tolist()
+        assert _ends(list(zip(size, rows)))

@@ -405,6 +405,34 @@ def test_chunks_of_prompts(new, held, d):
     _attend_case(new, held, 8, 2, d, 32, torch.bfloat16, seed=3)
 
 
+@pytest.mark.parametrize("h,hk,d,most,dtype", [(32, 8, 128, 8, torch.bfloat16), (32, 8, 128, 30, torch.float16), (16, 2, 128, 20, torch.bfloat16),
+                                               (16, 4, 256, 8, torch.float16), (32, 8, 128, 5, torch.bfloat16), (32, 8, 128, 4, torch.float32)])
+def test_long_shares_of_every_kernel(h, hk, d, most, dtype):
+    """So much work that a CTA goes through many key tiles of a unit and through several units; a few requests are compared."""
+    g = torch.Generator().manual_seed(h + most)
+    block, requests = 64, 50
+    new = torch.randint(1, most + 1, (requests,), generator=g).tolist()
+    new[3], new[7] = most, 1                                           # on average above most / 2
+    held = torch.randint(1500, 4000, (requests,), generator=g).tolist()
+    total = [a + b for a, b in zip(new, held)]
+    blocks = sum(-(-n // block) for n in total) + 1
+    k, ks = _cache(blocks, hk, block, d, 1)
+    v, vs = _cache(blocks, hk, block, d, 2)
+    table = _table(total, block, blocks, 3)
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    q = torch.randn(starts[-1], h, d, generator=g).to(dtype)
+    scaling = d ** -0.5
+    out, lse = _nv().fp8_paged_attention(q.cuda(), _i32(starts), k.cuda(), v.cuda(), ks.cuda(), vs.cuda(), table.cuda(), _i32(total), scaling,
+                                         h // hk, return_lse=True)
+    for r in (0, 3, 7, 20, 33, 49):
+        a, b = starts[r], starts[r + 1]
+        kk, vv = R.gather(k, ks, table[r], total[r], block), R.gather(v, vs, table[r], total[r], block)
+        _close(out[a:b], lse[a:b], q[a:b], kk, vv, _key_scales(vs, table[r], total[r], block), [held[r] + 1 + i for i in range(new[r])],
+               scaling, h // hk, chunk=_chunk(dtype, d, starts[-1], h // hk, requests))
+
+
 def test_single_tokens_are_decode():
     """The same rows through both entries, to the bit: one schedule."""
     lengths, block = [33, 500, 1, 0, 90], 16
