@@ -533,17 +533,19 @@ int run_attention(const PagedParams& p, int sms, cudaStream_t st) {
 }
 
 // Which kernel, by query rows a request on average (their numbers are on the device): eight, sixteen or (D = 128) 24 rows of
-// this file's, rounded up; above them the one whose tensor-memory products take 128 or 256 rows at a time.  fp32
-// queries, whose products need two halves, stay here, sixteen rows at a time.
+// this file's, rounded up, or (D = 128) two row tiles of sixteen; above them the one whose tensor-memory products take 128 or
+// 256 rows at a time.  fp32 queries, whose products need two halves, stay here, sixteen rows at a time.  Measured, 32 requests
+// of 300 to 8190 keys, Hk 8 G 4, the other kernel in brackets: D 128, 24 rows 73.7 (131) us, 32 rows 96 (133), 40 rows 121 (133) but
+// of 256 requests 233 (207); Hk 4 D 256, 16 rows 59.4 (73.8), 20 rows (73.8).
 struct Choice {
   bool chunk;
   int nt, ctas;
   int64_t rows;
 };
 Choice choose(int q_dtype, int64_t tokens, int64_t requests, int64_t g, int d, int sms) {
-  const int64_t rows = (tokens * g + requests - 1) / requests, most = d == 128 ? 24 : 16;
+  const int64_t rows = (tokens * g + requests - 1) / requests, most = d == 128 ? 32 : 16;
   if (q_dtype != NVFP4_DT_FP32 && rows > most) return {true, 0, sms, paged_chunk_rows(d)};
-  const int nt = rows <= 8 ? 1 : rows <= 16 || q_dtype == NVFP4_DT_FP32 ? 2 : 3;
+  const int nt = rows <= 8 ? 1 : rows <= 16 || rows > 24 || q_dtype == NVFP4_DT_FP32 ? 2 : 3;
   return {false, nt, (nt == 1 ? kCtas : 2) * sms, 8 * nt};
 }
 template <typename T, int D>

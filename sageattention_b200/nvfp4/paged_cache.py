@@ -9,7 +9,7 @@ Layout, shared by every function here:
 
   k_cache, v_cache   [blocks, Hk, block_size, D] float8_e4m3fn: codes; heads dense, any stride between blocks
   k_scale, v_scale   [blocks, Hk] float32: value = code * scale (a power of two; attention also reads others, which calls of
-                     more than 24 query rows a request round to eleven bits)
+                     many query rows a request round to eleven bits)
   block_table        [requests, width] int32: block of tokens j * block_size .. of a request, -1 where it has none.
                      Attention may read a block for several requests; reserve, write and trim take it to be one's own
   lengths            [requests] int32: tokens that a request holds

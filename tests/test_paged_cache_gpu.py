@@ -220,7 +220,7 @@ def _spoil(codes, scale, table, lengths, block):
 
 def _chunk(dtype, d, tokens, g, requests):
     """Whether a call takes the kernel for many rows."""
-    return dtype != torch.float32 and -(-tokens * g // requests) > (24 if d == 128 else 16)
+    return dtype != torch.float32 and -(-tokens * g // requests) > (32 if d == 128 else 16)
 
 
 def _key_scales(scale, row, length, block):
