@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     int tile = ahead.from;
     // ------------------------------------------------------------------ codes to halves
     const int w = warp & 3, t = w * 32 + lane;
-    const bool does_k = C::kConvert == 1 || warp < C::kSoft + 4, does_v = C::kConvert == 1 || !does_k;
+    const bool does_k = C::kConvert == 1 || warp < C::kSoft + 4;
     // 16-byte pieces of a tile: eight lanes take 64 bytes of two neighbouring keys, whose halves then lie in different banks
     constexpr int kPieces = D / 16;                        // per thread and operand
     const int in_key = (lane >> 2) & 1, in_chunk = lane & 3, pair8 = w * 4 + (lane >> 3);
@@ -262,26 +262,24 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     // a warp's keys lie in every other 16-key group: block of its u-th one (shuffles share a queue with the stores below)
     constexpr int kOwn = 4, kEach = kPieces / kOwn;
     auto group_of = [&](int u) { return 2 * u + (w >> 1); };
-    // this thread's first key of each: its codes, and how many keys of the group are there
-    const uint8_t *k_from[kOwn], *v_from[kOwn];              // (one of them where a warp does one operand)
-    int count[kOwn];
     const int first_key = (pair8 & 7) * 2 + in_key;         // of a group
-    auto find = [&]() {
+    // this thread's first key of each in an operand of the tile asked for: its codes, and how many keys of the group are there
+    auto find = [&](const uint8_t* codes, int64_t block, const uint8_t* (&from)[kOwn], int (&count)[kOwn]) {
 #pragma unroll
       for (int u = 0; u < kOwn; ++u) {
         const int b = __shfl_sync(0xffffffffu, id_next, group_of(u)), key = key0 + group_of(u) * 16;
-        const int64_t row = (((int64_t)head << p.log_block) + (key & ((1 << p.log_block) - 1)) + first_key) * D + in_chunk * 16;
-        if (does_k) k_from[u] = p.k + b * p.k_block + row;
-        if (does_v) (C::kConvert == 1 ? v_from : k_from)[u] = p.v + b * p.v_block + row;
+        from[u] = codes + b * block + (((int64_t)head << p.log_block) + (key & ((1 << p.log_block) - 1)) + first_key) * D + in_chunk * 16;
         count[u] = b >= 0 ? limit - key : 0;
       }
     };
-    auto ask = [&](const uint8_t* const (&from)[kOwn], int i) -> uint4 {
+    const uint8_t *k_from[kOwn], *v_from[kOwn];              // (where a warp does one operand, its own in the first)
+    int k_count[kOwn], v_count[kOwn];
+    auto ask = [&](const uint8_t* const (&from)[kOwn], const int (&count)[kOwn], int i) -> uint4 {
       return load_or_zero(from[i / kEach] + i % kEach * 64, first_key < count[i / kEach]);
     };
     // pieces to halves times `factor` (lane h: of keys 16 h ..), into a tile in shared memory; then the next tile's are asked for
-    auto convert = [&](uint4 (&r)[kPieces], float factor, uint32_t dst, const uint8_t* const (&from)[kOwn]) {
-      const bool plain = __all_sync(0xffffffffu, lane >= 8 || id_now < 0 || factor == 1.0f);
+    auto convert = [&](uint4 (&r)[kPieces], float factor, int id, uint32_t dst, const uint8_t* const (&from)[kOwn], const int (&count)[kOwn]) {
+      const bool plain = __all_sync(0xffffffffu, lane >= 8 || id < 0 || factor == 1.0f);
       __half2 own[kOwn];
 #pragma unroll
       for (int u = 0; u < kOwn; ++u) own[u] = __float2half2_rn(__shfl_sync(0xffffffffu, factor, group_of(u)));
@@ -292,7 +290,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         uint32_t h[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) half4_of_e4m3x4(words[k], h[2 * k], h[2 * k + 1]);
-        r[i] = ask(from, i);
+        r[i] = ask(from, count, i);
         if (!plain) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
@@ -312,44 +310,75 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       fence_proxy_async_smem();
       __syncwarp();
     };
+    int v_run = -200;                                      // largest exponent of the unit's value scales so far
+    // factors of the tile converted now
+    int ke, ve;
+    auto factors = [&]() {
+      if (starts) v_run = -200;
+      ke = id_now >= 0 ? scale_exp(ks_now) : -112;
+      ve = id_now >= 0 ? scale_exp(vs_now) : -112;
+      ke = __reduce_max_sync(0xffffffffu, lane < 8 ? ke : -112);
+      ve = __reduce_max_sync(0xffffffffu, lane < 8 ? ve : -112);
+      v_run = max(v_run, ve);
+      ve = max(ve, v_run - 60);                            // smaller ones do not count beside what the unit has seen
+    };
+    auto do_k = [&](uint32_t n) {
+      const int st = n % C::kStages;
+      const uint32_t there = __ballot_sync(0xffffffffu, id_now >= 0);
+      mbar_wait_warp(&k_free[st], (n / C::kStages & 1) ^ 1, err, 60);
+      if (t == 0) info_s[n % kInfo] = {exp2_int(ke), (float)ve, there};
+      convert(kr, ks_now * exp2_int(-ke), id_now, smem_u32(smem + C::kK + st * C::kOperand), k_from, k_count);
+      if (lane == 0) mbar_arrive(&k_full[st]);
+    };
+    auto do_v = [&](uint32_t n, uint4 (&r)[kPieces], float factor, int id, const uint8_t* const (&from)[kOwn], const int (&count)[kOwn]) {
+      const int st = n % C::kStages;
+      mbar_wait_warp(&v_free[st], (n / C::kStages & 1) ^ 1, err, 61);
+      convert(r, factor, id, smem_u32(smem + C::kV + st * C::kOperand), from, count);
+      if (lane == 0) mbar_arrive(&v_full[st]);
+    };
     if (more) {
       look_up();
       next();
-      find();
+      find(does_k ? p.k : p.v, does_k ? p.k_block : p.v_block, k_from, k_count);
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) kr[i] = ask(k_from, i);
-      if constexpr (C::kConvert == 1) {
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) vr[i] = ask(v_from, i);
-      }
+      for (int i = 0; i < kPieces; ++i) kr[i] = ask(k_from, k_count, i);
     }
-    int v_run = -200;                                      // largest exponent of the unit's value scales so far
     uint32_t n = 0;
-    for (; asked; ++n) {
-      const int st = n % C::kStages;
-      const uint32_t ph = (n / C::kStages) & 1;
-      next();
-      // factors of the tile
-      if (starts) v_run = -200;
-      int ke = id_now >= 0 ? scale_exp(ks_now) : -112, ve = id_now >= 0 ? scale_exp(vs_now) : -112;
-      ke = __reduce_max_sync(0xffffffffu, lane < 8 ? ke : -112);
-      ve = __reduce_max_sync(0xffffffffu, lane < 8 ? ve : -112);
-      find();
-      v_run = max(v_run, ve);
-      ve = max(ve, v_run - 60);                            // smaller ones do not count beside what the unit has seen
-      const uint32_t there = __ballot_sync(0xffffffffu, id_now >= 0);
-      if (does_k) {
-        mbar_wait_warp(&k_free[st], ph ^ 1, err, 60);
-        if (t == 0) info_s[n % kInfo] = {exp2_int(ke), (float)ve, there};
-        convert(kr, ks_now * exp2_int(-ke), smem_u32(smem + C::kK + st * C::kOperand), k_from);
-        if (lane == 0) mbar_arrive(&k_full[st]);
+    if constexpr (C::kConvert == 1) {
+      // K of a tile in front of V of the tile before it: V waits until a product two tiles back is complete, and S of the next
+      // tile must not wait with it (units of 32 rows, 32 requests: 133 us the other way round)
+      find(p.v, p.v_block, v_from, v_count);
+      if (asked) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) vr[i] = ask(v_from, v_count, i);
       }
-      if (does_v) {
-        mbar_wait_warp(&v_free[st], ph ^ 1, err, 61);
-        const uint32_t dst = smem_u32(smem + C::kV + st * C::kOperand);
-        if constexpr (C::kConvert == 1) convert(vr, vs_now * exp2_int(-ve), dst, v_from);
-        else convert(kr, vs_now * exp2_int(-ve), dst, k_from);
-        if (lane == 0) mbar_arrive(&v_full[st]);
+      bool v_left = false;                                 // V of tile n - 1 is to be done
+      float v_factor = 0.0f;
+      int v_id = -1;
+      while (asked || v_left) {
+        const bool tile_there = asked;
+        if (tile_there) {
+          next();
+          factors();
+          find(p.k, p.k_block, k_from, k_count);
+          do_k(n);
+        }
+        if (v_left) do_v(n - 1, vr, v_factor, v_id, v_from, v_count);
+        v_left = tile_there;
+        if (tile_there) {
+          v_factor = vs_now * exp2_int(-ve);
+          v_id = id_now;
+          find(p.v, p.v_block, v_from, v_count);
+          ++n;
+        }
+      }
+    } else {
+      for (; asked; ++n) {
+        next();
+        factors();
+        find(does_k ? p.k : p.v, does_k ? p.k_block : p.v_block, k_from, k_count);
+        if (does_k) do_k(n);
+        else do_v(n, kr, vs_now * exp2_int(-ve), id_now, k_from, k_count);
       }
     }
   } else if (warp >= C::kIssue) {
@@ -499,9 +528,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
           o_phase ^= 1u << g;
         }
       };
-      // Where the groups take turns, S of a tile must not stand in front of the products with V of the tile three before: its K is
-      // converted behind V of the tile before it, which waits for that place.  So there group 1 is a job behind group 0, and
-      // a step has both groups' PV first.  With more than 128 rows both groups are at the same tile, and that PV is two steps old.
+      // Where the groups take turns, S of a tile must not stand in front of PV of the tile four before: its K is converted behind
+      // V of the tile two before it, which waits for that place.  So there group 1 is a job behind group 0, and a step has both
+      // groups' PV first.  With more than 128 rows both groups are at the same tile, and that PV is some steps old.
       const bool turns = C::kGroups == 2 && !both;
       const int steps = jobs_of(0) + (turns ? 1 : 0);
 #pragma unroll 1
@@ -723,7 +752,6 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       const bool add = merge && tiles > 1;
       const int rows_warp = min(max(rows - (both ? group * 128 : 0) - wq * 32, 0), 32);    // of this warp that exist
       if (writes && rows_warp > 0) {
-        const int row0 = (both ? group * 128 : 0) + wq * 32;
         const float inv = !whole ? 1.0f : l != 0.0f ? __frcp_rn(l) : 0.0f;
         if (whole) {
           if (live && p.lse != nullptr) p.lse[out_row(p, at.q.t0 * p.g + i_row, at.head)] = lse_of(m, l);

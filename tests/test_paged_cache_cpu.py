@@ -154,8 +154,6 @@ def _ends(segments, stages=2, per_tile=2):
     convert, issue, soft, done, jobs_of = [], [], [[], []], set(), []
     n = 0
     for at, (tiles, both) in enumerate(segments):
-        for t in range(n, n + tiles):
-            convert += [([("s of", t - stages)] if t >= stages else [], ("k", t)), ([("pv of", t - stages)] if t >= stages else [], ("v", t))]
         jobs = [(tiles if both else (tiles + 1 - g) // 2) * per_tile for g in (0, 1)]
         steps = [(kind, g, j + ahead) for j in range(-2, max(jobs) + 1)
                  for kind, g, ahead in ((("pv", 0, 0), ("s", 0, 2), ("pv", 1, 0), ("s", 1, 2)) if both else
@@ -171,6 +169,9 @@ def _ends(segments, stages=2, per_tile=2):
             soft[g] += [([("s", at, g, j)], ("p", at, g, j)) for j in range(jobs[g])]
         jobs_of.append(jobs)
         n += tiles
+    for t in range(n + 1):                                 # K of a tile, then V of the one before
+        convert += [([("s of", t - stages)] if t >= stages else [], ("k", t))] if t < n else []
+        convert += [([("pv of", t - 1 - stages)] if t > stages else [], ("v", t - 1))] if t else []
     assert len(issue) == 2 * sum(map(sum, jobs_of))
     roles = [convert, issue, *soft]
     moved = True
