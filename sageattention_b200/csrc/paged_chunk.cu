@@ -1,18 +1,28 @@
 // Attention over the paged 8-bit KV cache for many query rows a request: chunks of prompts, drafts to verify.
 //
 // The mathematics of paged_attn.cu on the tensor cores of sm_100: S = Q K^T and O += P V as tcgen05.mma kind::f16 of halves, 128
-// rows an instruction, accumulators in tensor memory.  Codes become halves on their way into shared memory (exact; blocks of
-// a tile with smaller scales by a factor of at most 1), q enters as halves scaled by a power of two per row.
+// rows an instruction, accumulators in tensor memory.  Codes become halves on their way into shared memory; kind::f8f6f4 would
+// take them as they are, but round q and the weights to three bits of mantissa.
 //
-// Warps: two softmax groups (a thread a row; at D = 256 one group), four converting warps, one that issues the products.
-// A job is 128 rows against 64 keys (128 at D = 256); a group goes through its jobs one after the other, S of job j in place
-// j & 1 of the group's two, P over the upper half of the S it came from.
+// Warps: two softmax groups (a thread a row; at D = 256 one group), four converting warps (at D = 256 four an operand), one that
+// issues the products, three that fetch query rows.  A job is 128 rows against 64 keys (128 at D = 256); a group goes through
+// its jobs one after the other, S of job j in place j & 1 of the group's two, P over the upper half of the S it came from.
 //   rows > 128 (D = 128): group g has rows 128 g .., both go through every key tile
 //   rows <= 128 (D = 128): the groups take turns at the key tiles and keep results of their own, merged at the end
 // Products are issued in the order PV(j), S(j + 2): S(j + 1) is there when the softmax of job j ends.
 //
-// What bounds it (D = 128): a key tile of 256 rows is 2580 clocks of products on an SM (S with 64 keys reads its operands
-// from shared memory at 48 clocks an instruction instead of 32) and 2048 of ex2.
+// Precision: scores, maxima, sums and outputs are fp32.  A bf16 row of q becomes halves times a power of two, exact unless
+// below 2^-26 of its maximum.  K and V are halves relative to the largest scale of their tile, exact unless below 2^-24 of it (a
+// scale that is no power of two is rounded to eleven bits).  A weight is a half relative to a reference that the running
+// maximum may have left behind by 2^kLag, times 2^kLift (2^15 at most): its rounding is 2^-11 of itself, and of weights below
+// 2^-(14 + kLift) of the largest 2^-(25 + kLift) of that.
+//
+// What bounds it: at D = 128 the chain of a softmax warp, 2000 clocks a job: waiting for S 300, masks 160, maximum 175, the
+// reference 110, exponentials 1040 (512 on the special-function unit, which two warps share).  A 2048-token chunk over 10240
+// keys, Hk 8 G 4: 339 us = 910 TFLOP/s, tensor pipe 0.46, issue 0.52.  With 128 rows or fewer the converting warps, 3700
+// clocks a tile: 32 requests of 36 rows and 300 to 8190 keys 120 us = 1.4 TB/s.  At D = 256 the softmax warps, one a scheduler:
+// 4000 clocks a tile; seven requests of 0 to 777 tokens over 800 to 6007 keys 45.6 us.  Turns of the two groups at the
+// exponentials changed nothing, a quarter of them as polynomials took 359 us instead of 337.
 #include <cuda_fp16.h>
 #include <type_traits>
 #include "common/abi.cuh"
@@ -220,9 +230,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     const int in_key = (lane >> 2) & 1, in_chunk = lane & 3, pair8 = w * 4 + (lane >> 3);
     auto key_of = [&](int i) { return (i / (D / 64)) * 32 + pair8 * 2 + in_key; };
     auto chunk_of = [&](int i) { return (i % (D / 64)) * 4 + in_chunk; };
-    // Codes wait in registers, from the time that their tile's predecessor is converted on.  A load in flight holds a line of
-    // L1, of which this kernel's shared memory leaves 28 KB, less than a tile of K and V: piece i of the next tile is asked
-    // for when piece i of the present one has been converted, not all at once.
+    // Codes wait in registers, from the time that their tile's predecessor is converted on: asked for when all of that one's are
+    // (piece by piece between the conversions took 343.5 us of the chunk instead of 339; before there was L1 for a tile of K
+    // and V it was the better way).
     uint4 kr[kPieces], vr[C::kConvert == 1 ? kPieces : 1];   // where a warp does one operand, its codes are in the first
     // lanes 0 to 7: block of keys 16 lane .. of the tile being converted (`now`), asked for (`next`), and of the one behind
     int id_now = -1, id_next = -1, id_ahead = -1;
@@ -277,7 +287,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     auto ask = [&](const uint8_t* const (&from)[kOwn], const int (&count)[kOwn], int i) -> uint4 {
       return load_or_zero(from[i / kEach] + i % kEach * 64, first_key < count[i / kEach]);
     };
-    // pieces to halves times `factor` (lane h: of keys 16 h ..), into a tile in shared memory; then the next tile's are asked for
+    // pieces to halves times `factor` (lane h: of keys 16 h ..), into a tile in shared memory; behind them the next tile's are asked for
     auto convert = [&](uint4 (&r)[kPieces], float factor, int id, uint32_t dst, const uint8_t* const (&from)[kOwn], const int (&count)[kOwn]) {
       const bool plain = __all_sync(0xffffffffu, lane >= 8 || id < 0 || factor == 1.0f);
       __half2 own[kOwn];
@@ -290,7 +300,6 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         uint32_t h[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) half4_of_e4m3x4(words[k], h[2 * k], h[2 * k + 1]);
-        r[i] = ask(from, count, i);
         if (!plain) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
@@ -307,6 +316,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
                      "r"(h[6]), "r"(h[7])
                      : "memory");
       }
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) r[i] = ask(from, count, i);
       fence_proxy_async_smem();
       __syncwarp();
     };
