@@ -12,10 +12,12 @@
 // Products are issued in the order PV(j), S(j + 2): S(j + 1) is there when the softmax of job j ends.
 //
 // Precision: scores, maxima, sums and outputs are fp32.  A bf16 row of q becomes halves times a power of two, exact unless
-// below 2^-26 of its maximum.  K and V are halves relative to the largest scale of their tile, exact unless below 2^-24 of it (a
-// scale that is no power of two is rounded to eleven bits).  A weight is a half relative to a reference that the running
-// maximum may have left behind by 2^kLag, times 2^kLift (2^15 at most): its rounding is 2^-11 of itself, and of weights below
-// 2^-(14 + kLift) of the largest 2^-(25 + kLift) of that.
+// below 2^-26 of its maximum.  K and V are halves relative to the largest scale of their tile where its scales are within
+// 2^kNear of each other, which keeps every code exact (a scale that is no power of two is rounded to eleven bits).  In a tile
+// whose scales lie further apart each block is relative to its own, and the softmax brings them together key by key, for what a row
+// sees: scores by their K scales, weights by their V scales relative to the largest of them.  A weight is a half relative to a
+// reference that the running maximum may have left behind by 2^kLag, times 2^kLift (2^15 at most): its rounding is 2^-11 of itself,
+// and of weights below 2^-(14 + kLift) of the largest 2^-(25 + kLift) of that.
 //
 // What bounds it: at D = 128 the chain of a softmax warp, 2000 clocks a job: waiting for S 300, masks 160, maximum 175, the
 // reference 110, exponentials 1040 (512 on the special-function unit, which two warps share).  A 2048-token chunk over 10240
@@ -41,6 +43,7 @@ constexpr int kLoaders = 3;                   // warps that fetch query rows
 constexpr int kInfo = 8;                      // tiles whose scales are kept: more than can be under way
 // P is held times 2^kLift relative to a reference that may lag behind the running maximum by 2^kLag
 constexpr float kLift = 3.0f, kLag = 12.0f;
+constexpr int kNear = 15;                     // codes are multiples of 2^-9, halves of 2^-24
 
 template <int D>
 struct Cfg {
@@ -127,10 +130,12 @@ __device__ __forceinline__ uint4 load_or_zero(const uint8_t* src, bool there) {
   return v;
 }
 
-// What a tile's softmax has to know: factor of its scores, log2 of what its values were divided by, which 16-key groups are there.
+// What a tile's softmax has to know: factor of its scores, log2 of what its values were divided by, which 16-key groups are there
+// (a bit each).  Where the scales lie apart `there` is 0, `apart` says which groups are there, and each has exponents of its own.
 struct TileInfo {
   float k_factor, v_log2;
-  uint32_t there;
+  uint32_t there, apart;
+  int8_t k_exp[8], v_exp[8];
 };
 
 // exponent (floor of log2) of a scale
@@ -322,23 +327,39 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       __syncwarp();
     };
     int v_run = -200;                                      // largest exponent of the unit's value scales so far
-    // factors of the tile converted now
-    int ke, ve;
+    // exponents of the tile converted now: what its keys and values are relative to, and (lane h) those of keys 16 h .. where apart
+    int ke, ve, ke_own, ve_own;
+    bool apart;
     auto factors = [&]() {
       if (starts) v_run = -200;
-      ke = id_now >= 0 ? scale_exp(ks_now) : -112;
-      ve = id_now >= 0 ? scale_exp(vs_now) : -112;
-      ke = __reduce_max_sync(0xffffffffu, lane < 8 ? ke : -112);
-      ve = __reduce_max_sync(0xffffffffu, lane < 8 ? ve : -112);
+      ke_own = id_now >= 0 ? scale_exp(ks_now) : -112;
+      ve_own = id_now >= 0 ? scale_exp(vs_now) : -112;
+      ke = __reduce_max_sync(0xffffffffu, ke_own);
+      ve = __reduce_max_sync(0xffffffffu, ve_own);
       v_run = max(v_run, ve);
-      ve = max(ve, v_run - 60);                            // smaller ones do not count beside what the unit has seen
+      ve = max(ve, v_run - 60);                            // the sum of weights relative to the reference stays within fp32
+      apart = __any_sync(0xffffffffu, id_now >= 0 && (ke_own < ke - kNear || ve_own < ve - kNear));
+      if (!apart) {
+        ke_own = ke;
+        ve_own = ve;
+      }
     };
     auto do_k = [&](uint32_t n) {
       const int st = n % C::kStages;
       const uint32_t there = __ballot_sync(0xffffffffu, id_now >= 0);
       mbar_wait_warp(&k_free[st], (n / C::kStages & 1) ^ 1, err, 60);
-      if (t == 0) info_s[n % kInfo] = {exp2_int(ke), (float)ve, there};
-      convert(kr, ks_now * exp2_int(-ke), id_now, smem_u32(smem + C::kK + st * C::kOperand), k_from, k_count);
+      TileInfo& info = info_s[n % kInfo];
+      if (t == 0) {
+        info.k_factor = exp2_int(ke);
+        info.v_log2 = (float)ve;
+        info.there = apart ? 0 : there;
+        info.apart = apart ? there : 0;
+      }
+      if (apart && t < 8) {
+        info.k_exp[t] = (int8_t)ke_own;
+        info.v_exp[t] = (int8_t)ve_own;
+      }
+      convert(kr, ks_now * exp2_int(-ke_own), id_now, smem_u32(smem + C::kK + st * C::kOperand), k_from, k_count);
       if (lane == 0) mbar_arrive(&k_full[st]);
     };
     auto do_v = [&](uint32_t n, uint4 (&r)[kPieces], float factor, int id, const uint8_t* const (&from)[kOwn], const int (&count)[kOwn]) {
@@ -377,7 +398,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         if (v_left) do_v(n - 1, vr, v_factor, v_id, v_from, v_count);
         v_left = tile_there;
         if (tile_there) {
-          v_factor = vs_now * exp2_int(-ve);
+          v_factor = vs_now * exp2_int(-ve_own);
           v_id = id_now;
           find(p.v, p.v_block, v_from, v_count);
           ++n;
@@ -389,7 +410,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         factors();
         find(does_k ? p.k : p.v, does_k ? p.k_block : p.v_block, k_from, k_count);
         if (does_k) do_k(n);
-        else do_v(n, kr, vs_now * exp2_int(-ve), id_now, k_from, k_count);
+        else do_v(n, kr, vs_now * exp2_int(-ve_own), id_now, k_from, k_count);
       }
     }
   } else if (warp >= C::kIssue) {
@@ -605,7 +626,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         s_phase ^= 1u << place;
         tc_fence_after();
         __syncwarp();
-        const TileInfo info = info_s[(n + tile) % kInfo];
+        const TileInfo& info = info_s[(n + tile) % kInfo];
+        const float k_factor = info.k_factor, v_log2 = info.v_log2;
         const uint32_t there = info.there >> (sub * (C::kN / 16));
         const bool masked = __any_sync(0xffffffffu, live && limit < key0 + C::kN) ||
                             (there & ((1u << (C::kN / 16)) - 1)) != (1u << (C::kN / 16)) - 1;
@@ -615,6 +637,72 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         float top = -INFINITY;
         uint32_t s[2][32];
         if (masked) {                                      // a few tiles of a unit: S is edited where it is
+          if (const uint32_t groups = info.apart; groups != 0) {
+            // Scales far apart: scores in units of log2 with each group's K scale, the reference of the weights from scores with their
+            // V scales, then two exponentials a score, for the sum and (times the V scale) for the product.
+            constexpr int kOf = C::kN / 16;                // groups of a job
+            float want = -INFINITY;
+#pragma unroll 1
+            for (int x = 0; x < kOf; ++x) {
+              uint32_t now[16];
+              tmem_ld16(s_at + x * 16, now);
+              tmem_ld_wait();
+              const int of = sub * kOf + x, left = groups >> of & 1 ? visible - x * 16 : 0;
+              const float f = c_row * exp2_int(info.k_exp[of]);
+              float t = -INFINITY;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                now[e] = e < left ? __float_as_uint(__uint_as_float(now[e]) * f) : 0xFF800000u;
+                t = fmaxf(t, __uint_as_float(now[e]));
+              }
+              top = fmaxf(top, t);
+              want = fmaxf(want, t + (float)info.v_exp[of]);
+              tmem_st16(s_at + x * 16, now);
+            }
+            const float m_new = fmaxf(m, top), less = m_new == -INFINITY ? 0.0f : m_new;
+            if (__any_sync(0xffffffffu, want > ref + kLag)) {
+              const float ref_new = fmaxf(ref, want), f = want > ref ? ex2_approx(ref - ref_new) : 1.0f;
+              ref = ref_new;
+              if (j > 0) {
+                mbar_wait(&pv_done[group], (pv - 1) & 1, err, 68);
+                tc_fence_after();
+                __syncwarp();
+#pragma unroll 1
+                for (int cc = 0; cc < D / 16; ++cc) {
+                  const uint32_t o_at = tmem + lane_addr + C::kO + group * 128 + cc * 16;
+                  uint32_t o[16];
+                  tmem_ld16(o_at, o);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                  tmem_st16(o_at, o);
+                }
+              }
+            }
+            tmem_st_wait();
+            l *= m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
+            m = m_new;
+#pragma unroll 1
+            for (int x = kOf - 1; x >= 0; --x) {           // weights over scores that have been read
+              uint32_t now[16], w[8];
+              tmem_ld16(s_at + x * 16, now);
+              tmem_ld_wait();
+              const float plus = ref == -INFINITY ? 0.0f : (float)info.v_exp[sub * kOf + x] - ref + kLift;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float y0 = __uint_as_float(now[2 * e]), y1 = __uint_as_float(now[2 * e + 1]);
+                l += ex2_approx(y0 - less) + ex2_approx(y1 - less);
+                w[e] = pack_16x2<__half>(ex2_approx(y0 + plus), ex2_approx(y1 + plus));
+              }
+              tmem_st8(s_at + C::kN / 2 + x * 8, w);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[group][place]);
+            ++pv;
+            continue;
+          }
 #pragma unroll 1
           for (int x = 0; x < kChunks; ++x) {
             tmem_ld32(s_at + x * 32, s[0]);
@@ -643,11 +731,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
           top = fmaxf(top, fmaxf(t0, t1));
           if (x < kChunks - 1) tmem_ld_wait();
         }
-        const float c = fmaxf(c_row * info.k_factor, 0x1p-126f);   // never 0: hidden keys are -inf
+        const float c = fmaxf(c_row * k_factor, 0x1p-126f);   // never 0: hidden keys are -inf
         top = top == -INFINITY ? -INFINITY : top * c;
         // reference of the weights: moves only where the maximum has left it behind, and then for all rows of the warp, whose
         // results are all read and written anyway, so that the next move is a while away
-        const float want = top + info.v_log2;
+        const float want = top + v_log2;
         bool moved = false;
         float f = 1.0f;
         if (__any_sync(0xffffffffu, want > ref + kLag)) {
@@ -656,7 +744,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
           ref = ref_new;
           moved = j > 0;
         }
-        const float minus = ref == -INFINITY ? 0.0f : info.v_log2 - ref + kLift;
+        const float minus = ref == -INFINITY ? 0.0f : v_log2 - ref + kLift;
         const uint64_t c2 = pair(__float_as_uint(c), __float_as_uint(c)), minus2 = pair(__float_as_uint(minus), __float_as_uint(minus));
         uint64_t sum_a = 0, sum_b = 0;
 #pragma unroll
@@ -715,7 +803,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         // the sum is of weights times 2^(v_log2 - ref + lift)
         sum_a = add_pair(sum_a, sum_b);
         const float sum = __uint_as_float((uint32_t)sum_a) + __uint_as_float((uint32_t)(sum_a >> 32));
-        l += m == -INFINITY ? sum : sum * ex2_approx(ref - info.v_log2 - kLift - m);
+        l += m == -INFINITY ? sum : sum * ex2_approx(ref - v_log2 - kLift - m);
       }
 
       // ---- result of the segment
