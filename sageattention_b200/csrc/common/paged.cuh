@@ -218,6 +218,12 @@ __device__ __forceinline__ float ex2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Product of a query row's scale and a key's, at most the largest float: with inf a score that is 0 would become NaN.
+__device__ __forceinline__ float scale_product(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a * b), "f"(3.402823466e38f));
+  return y;
+}
 template <typename T>
 __device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
   if constexpr (sizeof(T) == 4) {

@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                const float f = inv[nt][k] * kscale[h];
+                const float f = scale_product(inv[nt][k], kscale[h]);
                 s[h][nt][k] *= f;
                 s[h][nt][2 + k] *= f;
                 if (masks) {

@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
               tmem_ld16(s_at + x * 16, now);
               tmem_ld_wait();
               const int of = sub * kOf + x, left = groups >> of & 1 ? visible - x * 16 : 0;
-              const float f = c_row * exp2_int(info.k_exp[of]);
+              const float f = scale_product(c_row, exp2_int(info.k_exp[of]));
               float t = -INFINITY;
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
           top = fmaxf(top, fmaxf(t0, t1));
           if (x < kChunks - 1) tmem_ld_wait();
         }
-        const float c = fmaxf(c_row * k_factor, 0x1p-126f);   // never 0: hidden keys are -inf
+        const float c = fmaxf(scale_product(c_row, k_factor), 0x1p-126f);   // never 0: hidden keys are -inf
         top = top == -INFINITY ? -INFINITY : top * c;
         // reference of the weights: moves only where the maximum has left it behind, and then for all rows of the warp, whose
         // results are all read and written anyway, so that the next move is a while away

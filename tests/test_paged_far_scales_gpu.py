@@ -1,6 +1,8 @@
 """Attention over the paged 8-bit KV cache where the scales of neighbouring blocks lie far apart, with a row count for each of its
 kernels: what a row does not see, or gives no weight, leaves its result alone."""
 
+import math
+
 import pytest
 import torch
 
@@ -159,3 +161,23 @@ def test_far_scales_in_long_shares(most, d, dtype):
         kk, vv = R.gather(k, ks, table[r], total[r], block), R.gather(v, vs, table[r], total[r], block)
         _near(out[a:b], lse[a:b], q[a:b], kk, vv, _key_scales(vs, table[r], total[r], block), [held[r] + 1 + i for i in range(most)], d ** -0.5,
               h // hk)
+
+
+@pytest.mark.parametrize("new,d,dtype", [m for m in _FEW + _MANY if m[2] != torch.float16])
+def test_large_factors_of_products_that_are_zero(new, d, dtype):
+    """q and K of 2^100 in channels of their own: every score is 0, although the product of their scales is above fp32."""
+    x = _One(new, 90, d, dtype, 11)
+    x.q = torch.zeros_like(x.q)
+    x.q[..., 3] = 2.0 ** 100
+    raw = x.k.view(torch.uint8)
+    raw[:, :, :, 3] = 0
+    x.ks[:] = 2.0 ** 100
+    out, lse = x.run()
+    vv = R.gather(x.v, x.vs, x.table[0], x.total, 16)
+    for i in range(new):
+        n = x.held + 1 + i
+        want = vv[:, :n].mean(1).repeat_interleave(4, 0)
+        # weights are equal powers of two, V exact: fp32 sums of n values, the sum of weights and its reciprocal, one rounding
+        tol = vv[:, :n].abs().mean(1).repeat_interleave(4, 0) * (n + 8) * 2.0 ** -22 + want.abs() * _HALF_STEP[dtype] + 1e-30
+        assert bool(((out[i].cpu().double() - want).abs() <= tol).all())
+        assert bool(((lse[i].cpu().double() - math.log(n)).abs() <= 2.0 ** -20 * math.log(n)).all())
