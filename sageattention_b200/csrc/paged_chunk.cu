@@ -182,7 +182,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
   volatile int* err = &expired;
 
   if (smem_u32(smem) & 1023) {                             // what the products' descriptors take for granted
-    if (tid == 0 && p.status != nullptr) atomicExch(p.status, 72);
+    griddep_wait();
+    if (tid == 0) {
+      p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);           // nothing to be merged
+      if (p.status != nullptr) atomicExch(p.status, 72);
+    }
     return;
   }
   if (tid == 0) {

@@ -56,3 +56,22 @@ def test_every_other_kernel_waits_unconditionally():
     for f in {kernels[n][0] for n in with_pdl}:      # ... and all of them are launched with the attribute
         assert "<<<" not in open(os.path.join(CSRC, f)).read(), f
     assert {kernels[n][0] for n in kernels if n not in with_pdl} == {"peak.cu", "selftest.cu"}
+
+
+def test_no_kernel_returns_in_front_of_its_wait():
+    """A kernel that ended before the one in front of it would let the one behind it start too early."""
+    kernels = _kernels()
+    late = {k for k, _ in _pairs()}
+    for n, (_, body) in kernels.items():
+        if "griddep_" in body and n not in late:
+            assert not re.search(r"\breturn;", body[:body.index("griddep_wait();")]), n
+
+
+def test_no_paged_attention_returns_without_its_entry_of_the_merge():
+    """The merge reads every block's entry: one that was never written would send it anywhere."""
+    kernels = _kernels()
+    for n in ("paged_attn_kernel", "paged_chunk_kernel"):
+        body = kernels[n][1]
+        first = re.search(r"\breturn;", body)
+        if first:
+            assert "p.cut[" in body[:first.start()], n
