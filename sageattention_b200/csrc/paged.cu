@@ -305,8 +305,8 @@ __global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(WriteParams p)
   constexpr int kLanes = kLoads < 32 ? kLoads : 32, kVec = kLoads / kLanes;
   constexpr int kRows = kWriteThreads / kLanes;              // rows of a pass of the block
   constexpr int kHold = (W + kRows - 1) / kRows;             // rows of the window that a thread sees to
-  constexpr int kSpan = W + kMaxBlock;
-  static_assert(kSpan <= kWriteThreads, "one thread looks at one token");
+  constexpr int kSpan = W + kMaxBlock - 1;                   // tokens that runs of the window can reach
+  static_assert(kSpan + 1 <= kWriteThreads, "one thread fetches one slot, that in front of the window among them");
   extern __shared__ __align__(16) uint8_t values_s[];        // [2][W rows]
   struct Run {
     int64_t block;                                           // of the cache
