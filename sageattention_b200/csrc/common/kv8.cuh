@@ -27,12 +27,7 @@ __device__ __forceinline__ uint32_t kv8_magnitude(float x) {
   return u < 0x7F800000u ? u : 0u;
 }
 
-// the two e4m3 values in 16 bits as a pair of halves (exact), and both pairs of a word
-__device__ __forceinline__ uint32_t half2_of_e4m3x2(uint16_t v) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
-  return r;
-}
+// the four e4m3 values of a word as two pairs of halves (exact)
 __device__ __forceinline__ void half4_of_e4m3x4(uint32_t v, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 a, b;\n\t"
       "mov.b32 {a, b}, %2;\n\t"

@@ -19,3 +19,10 @@ def test_every_slot_that_is_looked_at_has_been_fetched():
         assert looked_at <= fetched, w
         # a run begins in the window's last token at the latest, and is a cache block at most
         assert span >= w - 1 + names["kMaxBlock"]
+
+
+def test_every_function_of_the_headers_is_called():
+    text = {f: open(os.path.join(root, f)).read() for root, _, files in os.walk(CSRC) for f in files if f.endswith((".cu", ".cuh"))}
+    for header in ("kv8.cuh", "paged.cuh"):
+        for name in re.findall(r"__forceinline__ [\w:<>* ]+? \*?(\w+)\(", text[header]):
+            assert sum(len(re.findall(rf"\b{name}\b", re.sub(r"//[^\n]*", "", t))) for t in text.values()) > 1, name
