@@ -246,34 +246,32 @@ __device__ __forceinline__ const T* query_row(const PagedParams& p, int t0, int 
 // log-sum-exp of a sum relative to 2^top
 __device__ __forceinline__ float lse_of(float top, float sum) { return sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2; }
 
-// Rows of no request, and of requests without keys: zeros and -inf.
+// Rows of no request, and of requests without keys: zeros and -inf.  The rows in front of the first request and behind the
+// last one may be most of a captured step's, so all CTAs take part: a call of 32 single tokens and 8160 such rows
+// of H 32 D 128 (67 MB) takes 66 us, and took 1078 with one.
 template <typename T, int D, int ROWS, int TILE>
 __device__ __forceinline__ void clear_untouched(const PagedParams& p) {
   const int h = p.hk * p.g;
-  auto clear = [&](int64_t t0, int64_t t1) {
-    T* out = static_cast<T*>(p.out);
+  auto clear = [&](int64_t t0, int64_t t1, int64_t first, int64_t step) {    // tokens t0 .. t1 - 1 by threads first, first + step, ...
+    constexpr int kRow = D * sizeof(T) / 16;
 #pragma unroll 1
-    for (int64_t i = t0 * h * D + threadIdx.x * 4; i < t1 * h * D; i += blockDim.x * 4) {
-      const float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      store4<T>(out + i, z);
-    }
+    for (int64_t i = t0 * h * kRow + first; i < t1 * h * kRow; i += step) static_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
     if (p.lse != nullptr) {
 #pragma unroll 1
-      for (int64_t i = t0 * h + threadIdx.x; i < t1 * h; i += blockDim.x) p.lse[i] = -INFINITY;
+      for (int64_t i = t0 * h + first; i < t1 * h; i += step) p.lse[i] = -INFINITY;
     }
   };
-  // in turn: requests of this CTA, then (the last CTA) the tokens in front of the first one's and behind the last one's
-  auto inside = [&](int t) { return min(max((int64_t)t, (int64_t)0), p.tokens); };
-  const int extra = p.cu != nullptr && blockIdx.x == gridDim.x - 1 ? 2 : 0;
+  if (p.cu != nullptr) {
+    auto inside = [&](int t) { return min(max((int64_t)t, (int64_t)0), p.tokens); };
+    const int64_t front = inside(p.cu[0]), behind = inside(p.cu[p.requests]);
+    const int64_t first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
 #pragma unroll 1
-  for (int r = (int)blockIdx.x - (int)gridDim.x * extra; r < p.requests; r += gridDim.x) {
-    if (r < 0) {
-      const bool front = r < -(int)gridDim.x;
-      clear(front ? 0 : inside(p.cu[p.requests]), front ? inside(p.cu[0]) : p.tokens);
-      continue;
-    }
+    for (int x = 0; x < 2; ++x) clear(x == 0 ? 0 : behind, x == 0 ? front : p.tokens, first, step);
+  }
+#pragma unroll 1
+  for (int r = (int)blockIdx.x; r < p.requests; r += gridDim.x) {
     const Request<ROWS, TILE> q(p, r);
-    if (q.len == 0) clear(q.t0, q.t0 + q.n);
+    if (q.len == 0) clear(q.t0, q.t0 + q.n, threadIdx.x, blockDim.x);
   }
 }
 

@@ -790,3 +790,50 @@ def test_refusals():
         nv.paged_kv_reserve(*good, 4, 24)
     with pytest.raises(AssertionError):
         nv.paged_kv_reserve(*good, -1, 16)
+
+
+# ------------------------------------------------------------------------------------------------ padding
+def _padded(front, behind, dtype, d, h=32, hk=8, requests=32, held=200):
+    """A captured step's batch: one token for each request, and thousands of rows that are nobody's around them."""
+    q, _, cache, lengths, _ = _set([1] * requests, dtype, d, 3, h=h, hk=hk, held=[held] * requests)
+    cu = _i32([front + i for i in range(requests + 1)])
+    rows = torch.randn(front + requests + behind, h, d, device="cuda").to(dtype)
+    rows[front:front + requests] = q
+    return rows, cu, cache, lengths
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 256), (torch.float32, 128)])
+@pytest.mark.parametrize("front,behind", [(0, 3000), (3000, 0), (1501, 777)])
+def test_thousands_of_padded_rows_are_zeros(front, behind, dtype, d):
+    rows, cu, cache, lengths = _padded(front, behind, dtype, d)
+    out, lse = _nv().fp8_paged_attention(rows, cu, *cache, lengths, 0.1, 4, return_lse=True)
+    want, want_lse = _nv().fp8_paged_decode(rows[front:front + 32, :, None], *cache, lengths, 0.1, 4, return_lse=True)
+    for x, y in ((slice(0, front), 0), (slice(front + 32, None), 0)):
+        assert bool((out[x] == y).all()) and bool((lse[x] == -math.inf).all())
+    # the other kernel, maybe: weights and the result rounded apart
+    size = float(want.float().abs().max())
+    assert float((out[front:front + 32].float() - want[:, :, 0].float()).abs().max()) <= size * 4 * _HALF_STEP[torch.bfloat16]
+    assert float((lse[front:front + 32] - want_lse).abs().max()) <= 1e-3
+
+
+def test_padded_rows_are_cleared_by_the_whole_chip():
+    """8160 padded rows, 67 MB: at most what the call takes without them, the few rows through the kernel for many, and ten plain fills of as
+    many bytes.  (By one block of threads it was a hundred.)"""
+    def time_of(f):
+        f()
+        times = []
+        for _ in range(7):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda.synchronize()
+            a.record()
+            f()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return sorted(times)[3]
+
+    rows, cu, cache, lengths = _padded(0, 8160, torch.bfloat16, 128)
+    call = lambda rows: time_of(lambda: _nv().fp8_paged_attention(rows, cu, *cache, lengths, 0.1, 4))
+    fill = time_of(lambda: torch.zeros_like(rows))
+    few, padded = call(rows[:32]), call(rows)
+    assert padded <= 4 * few + 10 * fill
