@@ -55,7 +55,7 @@ struct Cfg {
   static constexpr int kConvert = D == 128 ? 1 : 2;
   static constexpr int kIssue = kSoft + 4 * kConvert;      // first warp of the last warpgroup, which issues the products
   static constexpr int kThreads = 32 * (kIssue + 4);       // whole warpgroups: registers move between them
-  static constexpr int kRegsSoft = D == 128 ? 144 : 168, kRegsConvert = D == 128 ? 144 : 128, kRegsIssue = 80;
+  static constexpr int kRegsSoft = D == 128 ? 144 : 168, kRegsConvert = D == 128 ? 152 : 128, kRegsIssue = D == 128 ? 72 : 80;
   // an increase waits for registers of this launch, which has 128 a thread (65536 / 512): more than those would wait forever
   static_assert(kThreads == 512 && kSoft * kRegsSoft + 4 * kConvert * kRegsConvert + 4 * kRegsIssue <= kThreads / 32 * 128, "registers");
   static constexpr int kOperand = D / 64 * kSub;           // 128 rows of q, or a tile of keys or values
@@ -247,6 +247,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     int id_now = -1, id_next = -1, id_ahead = -1;
     float ks_now = 0.0f, vs_now = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
     int key0 = 0, limit = 0, head = 0;                     // of the tile asked for
+    int key0_now = 0, limit_now = 0, head_now = 0;         // and of the one converted
     bool asked = false;                                    // there is one
     bool starts = true, starts_next = true, starts_ahead = true;   // first tile of its unit, as far as this CTA sees
     auto look_up = [&]() {
@@ -265,6 +266,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       starts_next = starts_ahead;
       starts_ahead = false;
       asked = more;
+      key0_now = key0;
+      limit_now = limit;
+      head_now = head;
       key0 = tile * kTile;
       limit = more ? ahead.q.limit(p, ahead.row_tile) : 0;
       head = ahead.head;
@@ -282,23 +286,29 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     constexpr int kOwn = 4, kEach = kPieces / kOwn;
     auto group_of = [&](int u) { return 2 * u + (w >> 1); };
     const int first_key = (pair8 & 7) * 2 + in_key;         // of a group
-    // this thread's first key of each in an operand of the tile asked for: its codes, and how many keys of the group are there
-    auto find = [&](const uint8_t* codes, int64_t block, const uint8_t* (&from)[kOwn], int (&count)[kOwn]) {
+    // this thread's first key of each in an operand of a tile (blocks `id`, keys from `key0` to `limit` of a head): its codes, and how
+    // many keys of the group are there
+    auto find = [&](const uint8_t* codes, int64_t block, int id, int key0, int limit, int head, const uint8_t* (&from)[kOwn], int (&count)[kOwn]) {
 #pragma unroll
       for (int u = 0; u < kOwn; ++u) {
-        const int b = __shfl_sync(0xffffffffu, id_next, group_of(u)), key = key0 + group_of(u) * 16;
+        const int b = __shfl_sync(0xffffffffu, id, group_of(u)), key = key0 + group_of(u) * 16;
         from[u] = codes + b * block + (((int64_t)head << p.log_block) + (key & ((1 << p.log_block) - 1)) + first_key) * D + in_chunk * 16;
         count[u] = b >= 0 ? limit - key : 0;
       }
     };
-    const uint8_t *k_from[kOwn], *v_from[kOwn];              // (where a warp does one operand, its own in the first)
-    int k_count[kOwn], v_count[kOwn];
+    auto find_next = [&](bool k, const uint8_t* (&from)[kOwn], int (&count)[kOwn]) {       // of the tile asked for
+      find(k ? p.k : p.v, k ? p.k_block : p.v_block, id_next, key0, limit, head, from, count);
+    };
+    const uint8_t* from[kOwn];
+    int count[kOwn];
     auto ask = [&](const uint8_t* const (&from)[kOwn], const int (&count)[kOwn], int i) -> uint4 {
       return load_or_zero(from[i / kEach] + i % kEach * 64, first_key < count[i / kEach]);
     };
     // pieces to halves times `factor` (lane h: of keys 16 h ..), into a tile in shared memory; behind them the next tile's are asked for
     auto convert = [&](uint4 (&r)[kPieces], float factor, int id, uint32_t dst, const uint8_t* const (&from)[kOwn], const int (&count)[kOwn]) {
-      const bool plain = __all_sync(0xffffffffu, lane >= 8 || id < 0 || factor == 1.0f);
+      // Factors of 1 are tested for at D = 256 alone, whose warps spill without the test (mixed batch 55 us instead of 45.7); at D = 128 they
+      // have no registers to spare for it (32 requests of 36 rows 118 us instead of 112).
+      const bool plain = C::kConvert == 2 && __all_sync(0xffffffffu, lane >= 8 || id < 0 || factor == 1.0f);
       __half2 own[kOwn];
 #pragma unroll
       for (int u = 0; u < kOwn; ++u) own[u] = __float2half2_rn(__shfl_sync(0xffffffffu, factor, group_of(u)));
@@ -363,10 +373,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         info.k_exp[t] = (int8_t)ke_own;
         info.v_exp[t] = (int8_t)ve_own;
       }
-      convert(kr, ks_now * exp2_int(-ke_own), id_now, smem_u32(smem + C::kK + st * C::kOperand), k_from, k_count);
+      convert(kr, ks_now * exp2_int(-ke_own), id_now, smem_u32(smem + C::kK + st * C::kOperand), from, count);
       if (lane == 0) mbar_arrive(&k_full[st]);
     };
-    auto do_v = [&](uint32_t n, uint4 (&r)[kPieces], float factor, int id, const uint8_t* const (&from)[kOwn], const int (&count)[kOwn]) {
+    auto do_v = [&](uint32_t n, uint4 (&r)[kPieces], float factor, int id) {
       const int st = n % C::kStages;
       mbar_wait_warp(&v_free[st], (n / C::kStages & 1) ^ 1, err, 61);
       convert(r, factor, id, smem_u32(smem + C::kV + st * C::kOperand), from, count);
@@ -375,18 +385,18 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     if (more) {
       look_up();
       next();
-      find(does_k ? p.k : p.v, does_k ? p.k_block : p.v_block, k_from, k_count);
+      find_next(does_k, from, count);
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) kr[i] = ask(k_from, k_count, i);
+      for (int i = 0; i < kPieces; ++i) kr[i] = ask(from, count, i);
     }
     uint32_t n = 0;
     if constexpr (C::kConvert == 1) {
       // K of a tile in front of V of the tile before it: V waits until a product two tiles back is complete, and S of the next
       // tile must not wait with it (units of 32 rows, 32 requests: 133 us the other way round)
-      find(p.v, p.v_block, v_from, v_count);
       if (asked) {
+        find_next(false, from, count);
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) vr[i] = ask(v_from, v_count, i);
+        for (int i = 0; i < kPieces; ++i) vr[i] = ask(from, count, i);
       }
       bool v_left = false;                                 // V of tile n - 1 is to be done
       float v_factor = 0.0f;
@@ -396,15 +406,17 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         if (tile_there) {
           next();
           factors();
-          find(p.k, p.k_block, k_from, k_count);
+          find_next(true, from, count);
           do_k(n);
         }
-        if (v_left) do_v(n - 1, vr, v_factor, v_id, v_from, v_count);
+        if (v_left) {                                      // behind it, the values of this tile are asked for
+          find(p.v, p.v_block, tile_there ? id_now : -1, key0_now, limit_now, head_now, from, count);
+          do_v(n - 1, vr, v_factor, v_id);
+        }
         v_left = tile_there;
         if (tile_there) {
           v_factor = vs_now * exp2_int(-ve_own);
           v_id = id_now;
-          find(p.v, p.v_block, v_from, v_count);
           ++n;
         }
       }
@@ -412,9 +424,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       for (; asked; ++n) {
         next();
         factors();
-        find(does_k ? p.k : p.v, does_k ? p.k_block : p.v_block, k_from, k_count);
+        find_next(does_k, from, count);
         if (does_k) do_k(n);
-        else do_v(n, kr, vs_now * exp2_int(-ve_own), id_now, k_from, k_count);
+        else do_v(n, kr, vs_now * exp2_int(-ve_own), id_now);
       }
     }
   } else if (warp >= C::kIssue) {
