@@ -13,7 +13,7 @@
 //
 // Measured with the merge: one query row of 839 MB of cache 142 to 152 us (the kernel alone 131 to 135, 0.95 of the copy
 // rate); 160 requests of 1 to 4100 keys, 51.7 MB, 22.5 us and D = 256, 87.7 MB, 28.7 us, of which 3 are the deal, 3 to 5 the
-// merge, and the rest units of few tiles each; 20 rows a request, 169 MB, 67.5 us: 1290 instructions a warp and 32 keys at two
+// merge, and the rest units of few tiles each; 20 rows a request, 169 MB, 68.2 us: 1290 instructions a warp and 32 keys at two
 // warps a scheduler, which registers allow no more of.
 //
 // Precision: q enters as halves scaled by a power of two per row, so that a bf16 or fp16 q is exact unless 2^-26 of its row's
@@ -541,7 +541,9 @@ int run_attention(const PagedParams& p, int sms, cudaStream_t st) {
 // this file's, rounded up, or (D = 128) two row tiles of sixteen; above them the one whose tensor-memory products take 128 or
 // 256 rows at a time.  fp32 queries, whose products need two halves, stay here, sixteen rows at a time.  Measured, 32 requests
 // of 300 to 8190 keys, Hk 8 G 4, the other kernel in brackets: D 128, 24 rows 73.7 (131) us, 32 rows 96 (133), 40 rows 121 (133) but
-// of 256 requests 233 (207); Hk 4 D 256, 16 rows 59.4 (73.8), 20 rows (73.8).
+// of 256 requests 233 (207); Hk 4 D 256, 16 rows 59.4 (73.8), 20 rows (73.8).  The average is over all rows of the table and all
+// query tokens, padded ones too, as the host knows no others: a chunk of 2048 tokens over 12288 keys takes 0.39 ms in a table of 32 rows and,
+// in tiles of sixteen rows, 2.4 in one of 256 whose other rows are idle.
 struct Choice {
   bool chunk;
   int nt, ctas;

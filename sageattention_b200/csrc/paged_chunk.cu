@@ -21,10 +21,11 @@
 //
 // What bounds it: at D = 128 the chain of a softmax warp, 2000 clocks a job: waiting for S 300, masks 160, maximum 175, the
 // reference 110, exponentials 1040 (512 on the special-function unit, which two warps share).  A 2048-token chunk over 10240
-// keys, Hk 8 G 4: 339 us = 910 TFLOP/s, tensor pipe 0.46, issue 0.52.  With 128 rows or fewer the converting warps, 3700
-// clocks a tile: 32 requests of 36 rows and 300 to 8190 keys 120 us = 1.4 TB/s.  At D = 256 the softmax warps, one a scheduler:
-// 4000 clocks a tile; seven requests of 0 to 777 tokens over 800 to 6007 keys 45.6 us.  Turns of the two groups at the
-// exponentials changed nothing, a quarter of them as polynomials took 359 us instead of 337.
+// keys, Hk 8 G 4: 342 us = 900 TFLOP/s, tensor pipe 0.46, issue 0.53.  With 128 rows or fewer the converting warps, 3700
+// clocks a tile: 32 requests of 36 rows and 300 to 8190 keys 112 us = 1.5 TB/s.  At D = 256 the softmax warps, one a scheduler:
+// 4000 clocks a tile; seven requests of 0 to 777 tokens over 800 to 6007 keys 45.7 us.  Where all tiles hold
+// scales far apart the chunk takes 1.8 times as long (two exponentials a score, one after the other), 32 requests of 36 rows
+// 1.1 times.  Turns of the two groups at the exponentials changed nothing, a quarter of them as polynomials took 359 us instead of 337.
 #include <cuda_fp16.h>
 #include <type_traits>
 #include "common/abi.cuh"
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
     auto key_of = [&](int i) { return (i / (D / 64)) * 32 + pair8 * 2 + in_key; };
     auto chunk_of = [&](int i) { return (i % (D / 64)) * 4 + in_chunk; };
     // Codes wait in registers, from the time that their tile's predecessor is converted on: asked for when all of that one's are
-    // (piece by piece between the conversions took 343.5 us of the chunk instead of 339; before there was L1 for a tile of K
+    // (piece by piece between the conversions the chunk took 4 us more; before there was L1 for a tile of K
     // and V it was the better way).
     uint4 kr[kPieces], vr[C::kConvert == 1 ? kPieces : 1];   // where a warp does one operand, its codes are in the first
     // lanes 0 to 7: block of keys 16 lane .. of the tile being converted (`now`), asked for (`next`), and of the one behind

@@ -33,7 +33,7 @@ class PagedStep(NamedTuple):
     """New tokens of one step, request by request: where each goes, its position, and where each request's begin."""
 
     slot_map: torch.Tensor      # [num_slots] int64: block * block_size + offset, -1 behind the last token
-    positions: torch.Tensor     # [num_slots] int32: position in the request (what ``rope_quant_nvfp4`` takes), 0 behind
+    positions: torch.Tensor     # [num_slots] int32: position in the request (for the caller's rotary embedding), 0 behind
     cu_seqlens: torch.Tensor    # [requests + 1] int32
     shortage: torch.Tensor      # [1] int32: 1 where nothing was reserved
 
@@ -51,7 +51,8 @@ def paged_kv_reserve(new_lens, lengths, block_table, free_blocks, free_count, nu
 
 def paged_kv_trim(keep_lens, lengths, block_table, free_blocks, free_count, block_size: int) -> None:
     """Every request r keeps its first ``keep_lens[r]`` tokens (0: it ends); blocks that hold none of them go back on
-    the stack.  In place.  Trimmed to the lengths in front of a reservation, stack and table are what they were."""
+    the stack.  In place.  Trimmed to the lengths in front of a reservation, stack and table are what they were; codes and scales are not
+    touched, so a block that stays keeps the scale that a token taken away may have raised (see ``fp8_kv_write``)."""
     _lib.native().paged_trim(keep_lens, lengths, block_table, free_blocks, free_count, block_size)
 
 
@@ -86,7 +87,9 @@ def fp8_paged_attention(query, cu_seqlens, k_cache, v_cache, k_scale, v_scale, b
     """Causal attention of several query tokens a request: drafts to verify, chunks of a prompt, or both in one batch.
 
     ``query`` ``[T, H, D]``; request r owns tokens ``cu_seqlens[r] .. cu_seqlens[r + 1]``, the last ones of its
-    ``lengths[r]`` keys (written before the call): token i of n sees keys ``0 .. lengths[r] - n + i``.  A value that is NaN
+    ``lengths[r]`` keys (written before the call): token i of n sees keys ``0 .. lengths[r] - n + i``.  The kernel is chosen by the query
+    tokens a row of the table, idle rows among them: a long chunk is called with the rows of the table that it needs
+    (``block_table[r:r + 1]``, ``lengths[r:r + 1]``) rather than with hundreds of idle ones.  A value that is NaN
     reaches the call's tokens in front of it too (their weight 0 times NaN), as in a masked softmax; keys, and what is
     behind ``lengths[r]`` in a block, reach nothing that does not see them.  Returns ``[T, H, D]``, with ``return_lse`` also ``[T, H]``; tokens without a key, or behind the last request's, get zeros and -inf.
     """

@@ -98,3 +98,23 @@ def test_nan_and_infinite_operands_reach_their_rows_only(new, d, dtype):
     sees[last, 2:4] = True
     assert torch.equal(torch.isnan(out).any(2), sees) and torch.equal(torch.isnan(out).all(2), sees)
     assert torch.equal(torch.isnan(lse), sees)
+
+
+@pytest.mark.parametrize("d", [128, 256])
+def test_a_chunk_by_itself_and_among_idle_rows(d):
+    """The rows of the table that a chunk needs, or all of it: other kernels, the same attention."""
+    rows, n, total, block = 40, 60, [0] * 17 + [300] + [0] * 22, 16
+    k, ks = _cache(25, 2, block, d, 3)
+    v, vs = _cache(25, 2, block, d, 53)
+    table = _table(total, block, 25, 1)
+    _spoil(k, ks, table, total, block)
+    _spoil(v, vs, table, total, block)
+    q = torch.randn(n, 8, d, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    kk, vv = R.gather(k, ks, table[17], 300, block), R.gather(v, vs, table[17], 300, block)
+    cu = [0] * 18 + [n] * 23
+    for a, b, chunk in ((0, rows, False), (17, 18, True)):
+        assert _chunk(torch.bfloat16, d, n, 4, b - a) == chunk
+        whole, lengths = table.cuda(), _i32(total)
+        out, lse = _nv().fp8_paged_attention(q.cuda(), _i32(cu[a:b + 1]), k.cuda(), v.cuda(), ks.cuda(), vs.cuda(), whole[a:b], lengths[a:b], 0.1, 4,
+                                             return_lse=True)
+        _close(out, lse, q, kk, vv, _key_scales(vs, table[17], 300, block), [241 + i for i in range(n)], 0.1, 4, chunk=chunk)
