@@ -118,3 +118,41 @@ def test_a_chunk_by_itself_and_among_idle_rows(d):
         out, lse = _nv().fp8_paged_attention(q.cuda(), _i32(cu[a:b + 1]), k.cuda(), v.cuda(), ks.cuda(), vs.cuda(), whole[a:b], lengths[a:b], 0.1, 4,
                                              return_lse=True)
         _close(out, lse, q, kk, vv, _key_scales(vs, table[17], 300, block), [241 + i for i in range(n)], 0.1, 4, chunk=chunk)
+
+
+@pytest.mark.parametrize("new,d,dtype", [([3, 1, 2], 128, torch.bfloat16), ([2, 3, 1], 256, torch.float32), _MANY[0], _MANY[3]])
+def test_blocks_whose_offsets_pass_32_bits(new, d, dtype):
+    """A view of a wider buffer, half a gigabyte from block to block: written and read through both kernels."""
+    hk, block, apart = 2, 64, (1 << 29) + 4096
+    total = [130, 61, 90]
+    blocks = sum(-(-n // block) for n in total) + 4                  # 4.5 GB and more
+    assert (blocks - 1) * apart > 1 << 32
+    flat = torch.empty(blocks * apart, dtype=torch.uint8, device="cuda")
+    view = lambda at: flat.as_strided((blocks, hk, block, d), (apart, block * d, d, 1), at)
+    k, v = view(0), view(1 << 20)
+    k.zero_(), v.zero_()
+    ks, vs = torch.zeros(blocks, hk, device="cuda"), torch.zeros(blocks, hk, device="cuda")
+    table = _table(total, block, blocks, 2)
+    g = torch.Generator().manual_seed(4)
+    assert int(table.max()) * apart > 1 << 32
+    slots = [int(table[r, p // block]) * block + p % block for r, n in enumerate(total) for p in range(n)]
+    key, value = (torch.randn(len(slots), hk, d, generator=g) for _ in range(2))
+    _nv().fp8_kv_write(key.cuda(), value.cuda(), torch.tensor(slots).cuda(), k, v, ks, vs)
+    wk, wv = torch.zeros(blocks, hk, block, d).double(), torch.zeros(blocks, hk, block, d).double()
+    wks, wvs = torch.zeros(blocks, hk).double(), torch.zeros(blocks, hk).double()
+    R.write(key.double(), slots, wk, wks, block)
+    R.write(value.double(), slots, wv, wvs, block)
+    for got, s, want, ws in ((k, ks, wk, wks), (v, vs, wv, wvs)):
+        assert torch.equal(s.cpu().double(), ws)
+        assert torch.equal(got.cpu().view(torch.float8_e4m3fn).double(), want)
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    q = torch.randn(starts[-1], 4 * hk, d, generator=g).to(dtype)
+    out, lse = _nv().fp8_paged_attention(q.cuda(), _i32(starts), k, v, ks, vs, table.cuda(), _i32(total), 0.1, 4, return_lse=True)
+    for r, n in enumerate(new):
+        if n:
+            a, b = starts[r], starts[r + 1]
+            kk, vv = R.gather(wk, wks, table[r], total[r], block), R.gather(wv, wvs, table[r], total[r], block)
+            _close(out[a:b], lse[a:b], q[a:b], kk, vv, _key_scales(wvs, table[r], total[r], block), [total[r] - n + 1 + i for i in range(n)], 0.1, 4,
+                   chunk=_chunk(dtype, d, starts[-1], 4, 3))
