@@ -473,6 +473,86 @@ int nvfp4_bwd_fp4(const uint8_t* qnv, const uint8_t* qsc, const uint8_t* knv, co
                   int* status, nvfp4_stream_t stream);
 
 /*
+ * Trees of drafted tokens over the paged 8-bit cache (no counterpart in the reference).  A request's tokens cu_seqlens[r] ..
+ * cu_seqlens[r + 1] are a tree of at most 1024 nodes: parents[t] is the number, within the request, of the earlier token that t hangs
+ * on; anything else (-1) makes it a root.
+ *   nvfp4_draft_tree: mask [tokens, ceil(max_tokens / 64)], bit j of a token's row: node j is the token itself or above it;
+ *   positions [tokens] = lengths[r] - n + depth (lengths: int32 [requests], the n tokens of the call among them).  Nodes from
+ *   max_tokens (1 to 1024) on have no bits and depth 0; tokens of no request zeros.
+ */
+int nvfp4_draft_tree(const int32_t* parents, const int32_t* cu_seqlens, const int32_t* lengths, int64_t tokens, int64_t requests,
+                     int64_t max_tokens, uint64_t* mask, int32_t* positions, nvfp4_stream_t stream);
+
+/*
+ * nvfp4_kv8_attention (workspace: nvfp4_kv8_attention_plan) where token i of a request's n sees keys 0 .. lengths[r] - n - 1 and
+ * those keys lengths[r] - n + j whose bit j its row of tree_mask [tokens, tree_words] has; bits j >= n do not count.
+ */
+int nvfp4_kv8_tree_attention(const void* q, int q_dtype, int64_t s_qt, int64_t s_qh, const int32_t* cu_seqlens, int64_t tokens,
+                             const uint64_t* tree_mask, int64_t tree_words, const uint8_t* k_cache, int64_t k_block,
+                             const uint8_t* v_cache, int64_t v_block, const float* k_scale, int64_t ks_block,
+                             const float* v_scale, int64_t vs_block, int64_t blocks, int block_size, const int32_t* table,
+                             int64_t table_row, int64_t width, const int32_t* lengths, int64_t requests, int64_t hk, int g,
+                             int d, float scaling, void* out, float* lse, void* workspace, size_t workspace_bytes, int* status,
+                             nvfp4_stream_t stream);
+
+/*
+ * Which drafted tokens the target's probabilities keep, from given random numbers, and the token that comes next.  At node x (node 0
+ * first) with its row p of target_probs and its children in order, R = p, M = 1:
+ *   with draft_probs (its row q: what the children of x were drawn from)  a child passes where u q(c) M < R(c), else
+ *       R <- max(R / M - q, 0), M <- sum R;
+ *   without (NULL)                                                        where u M < R(c), else M <- M - R(c), R(c) <- 0.
+ * The first child that passes is the next node; where none does, the next token is the first v with R(0) + .. + R(v) > w sum R (of p,
+ * where nothing is left).  u = uniforms[t] of the child, w that of node 0; sums in 64 bits; what is no finite number above zero counts
+ * as 0, a token id outside the vocabulary has probability 0.
+ *   target_probs, draft_probs [num_tokens, vocab] of `dtype`, element strides of rows; tokens [num_tokens] int32 or int64
+ *   accepted [num_tokens]: a request's path as node numbers, node 0 first, then -1;  num_accepted [requests];
+ *   next_tokens [requests] (-1 for a request without tokens)
+ */
+int nvfp4_verify_drafts(const void* target_probs, int64_t target_row, const void* draft_probs, int64_t draft_row, int dtype,
+                        int64_t vocab, const void* tokens, int tokens_int64, const int32_t* parents, const int32_t* cu_seqlens,
+                        const float* uniforms, int64_t num_tokens, int64_t requests, int32_t* accepted, int32_t* num_accepted,
+                        int64_t* next_tokens, nvfp4_stream_t stream);
+
+/*
+ * The tokens of an accepted path moved together: of a request's n newest tokens, token accepted[cu[r] + j] (ascending in j <
+ * num_accepted[r]; the path ends in front of an entry that is not) goes to position lengths[r] - n + j, keys and values of all layers
+ * and heads.  A block that receives codes of larger scales takes the smallest power of two that holds them, and its older codes are
+ * rounded again to it.  keep_lens [requests]: what nvfp4_paged_trim is to keep.  Caches [layers, blocks, Hk, block_size, D] in bytes,
+ * scales [layers, blocks, Hk], strides of layer and block in elements.
+ */
+int nvfp4_paged_keep_path(const int32_t* accepted, const int32_t* num_accepted, const int32_t* cu_seqlens, int64_t tokens,
+                          const int32_t* lengths, const int32_t* table, int64_t table_row, int64_t requests, int64_t width,
+                          uint8_t* k_cache, int64_t k_layer, int64_t k_block, uint8_t* v_cache, int64_t v_layer,
+                          int64_t v_block, float* k_scale, int64_t ks_layer, int64_t ks_block, float* v_scale,
+                          int64_t vs_layer, int64_t vs_block, int64_t layers, int64_t blocks, int64_t hk, int block_size, int d,
+                          int32_t* keep_lens, nvfp4_stream_t stream);
+
+/*
+ * RMS norm of every head's queries and keys and their rotation by position, in one launch: y = rot(x w / sqrt(mean(x^2) + eps)), in
+ * fp32, rounded once.  (No counterpart in the reference; the rotation is that of nvfp4_rope_pack.)
+ *   q [z, s, h, d], k [z, s, hk, d] of `dtype`, d 128 or 256, unit stride along d, rows 16-byte aligned; strides[3]: elements from
+ *   batch entry to entry, token to token, head to head (host arrays), the results' likewise
+ *   wq, wk [d] of `dtype` or fp32;  cos_tab / sin_tab [table_rows, d/2] fp32
+ *   positions: int32, token s of entry b at positions[b * pos_batch + s], or NULL: pos0 + s.  Rows outside the tables become NaN.
+ * nvfp4_qk_norm_rope_bwd: gradients of q and k in their type, and (NULL: not wanted) of the weights in theirs, from operands and
+ * incoming gradients; sums in an order that depends on the sizes and the device alone.  workspace: nvfp4_qk_norm_rope_bwd_plan
+ * bytes where a weight's gradient is wanted.
+ */
+int nvfp4_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype, int64_t z,
+                       int64_t s, int64_t h, int64_t hk, int d, const void* wq, const void* wk, int w_dtype,
+                       const float* cos_tab, const float* sin_tab, int64_t table_rows, const int32_t* positions,
+                       int64_t pos_batch, int64_t pos0, float eps, void* out_q, const int64_t* oq_strides, void* out_k,
+                       const int64_t* ok_strides, nvfp4_stream_t stream);
+int nvfp4_qk_norm_rope_bwd_plan(int d, int sm_count, size_t* workspace_bytes);
+int nvfp4_qk_norm_rope_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* grad_q,
+                           const int64_t* gq_strides, const void* grad_k, const int64_t* gk_strides, int dtype, int64_t z,
+                           int64_t s, int64_t h, int64_t hk, int d, const void* wq, const void* wk, int w_dtype,
+                           const float* cos_tab, const float* sin_tab, int64_t table_rows, const int32_t* positions,
+                           int64_t pos_batch, int64_t pos0, float eps, void* dq, const int64_t* dq_strides, void* dk,
+                           const int64_t* dk_strides, void* dwq, void* dwk, void* workspace, size_t workspace_bytes,
+                           nvfp4_stream_t stream);
+
+/*
  * Measured pipe rates (no counterpart in the reference): launches a resident-operand micro-kernel
  * on every SM -- what = 0: tcgen05.mma kind::mxf4nvf4 M128 N128 K64; 1: kind::f16 (bf16) M128 N128
  * K16; 2: ex2.approx.f32; 3: cvt e2m1x2; 4: fma.f32; 5: ex2 + cvt e2m1x2 pairs; 6: cvt e4m3x2.f32;

@@ -79,6 +79,22 @@ SIGNATURES = {
     "nvfp4_kv8_attention": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                     c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p,
                                     c_int64, c_int64, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "nvfp4_draft_tree": (c_int, [c_void_p] * 3 + [c_int64] * 3 + [c_void_p] * 3),
+    "nvfp4_kv8_tree_attention": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                         c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64,
+                                         c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p,
+                                         c_size_t, c_void_p, c_void_p]),
+    "nvfp4_verify_drafts": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                    c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nvfp4_paged_keep_path": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64]
+                              + [c_void_p, c_int64, c_int64] * 4 + [c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p]),
+    "nvfp4_qk_norm_rope": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p,
+                                   c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_float, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nvfp4_qk_norm_rope_bwd_plan": (c_int, [c_int, c_int, POINTER(c_size_t)]),
+    "nvfp4_qk_norm_rope_bwd": (c_int, [c_void_p] * 8 + [c_int, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int,
+                                       c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_float] + [c_void_p] * 7
+                               + [c_size_t, c_void_p]),
     "nvfp4_rope_pack": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p,
                                 c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                 c_void_p]),

@@ -38,6 +38,8 @@ struct PagedParams {
   int4* cut;                                  // [CTAs] the unit that a CTA began and did not finish: first row, head, rows, pieces
   float *ws_m, *ws_l, *ws_acc;                // [2 * CTAs][ROWS] partial results
   int* status;
+  const uint32_t* tree;                       // [tokens, tree_words]: bit j of a token's row: it sees the request's token j; or null (causal)
+  int tree_words;
 };
 
 // i / g for 0 <= i < 2^31: with 2^shift the next power of two from g on, i / g = (i + hi(i * mul)) >> shift for
@@ -54,8 +56,9 @@ __device__ __forceinline__ int token_of(const PagedParams& p, int i) {
 
 __host__ __device__ constexpr int unit_cost(int rows) { return rows <= 8 ? 2 : 3; }
 
-// What a request asks for: its query tokens [t0, t0 + n), its keys, its units.
-template <int ROWS, int TILE>
+// What a request asks for: its query tokens [t0, t0 + n), its keys, its units.  TREE: what its tokens see of each other is in
+// bits, so that all of them go through all keys.
+template <int ROWS, int TILE, bool TREE>
 struct Request {
   int t0, n, len, row_tiles;
 
@@ -73,11 +76,11 @@ struct Request {
     row_tiles = len == 0 ? 0 : (int)(((int64_t)n * p.g + ROWS - 1) / ROWS);
   }
   __device__ __forceinline__ int rows(const PagedParams& p, int row_tile) const { return min(n * p.g - row_tile * ROWS, ROWS); }
-  // keys that row i of the request sees
-  __device__ __forceinline__ int seen(const PagedParams& p, int i) const { return len - n + 1 + token_of(p, i); }
+  // keys that row i of the request sees, or (TREE) that all rows see
+  __device__ __forceinline__ int seen(const PagedParams& p, int i) const { return TREE ? len - n : len - n + 1 + token_of(p, i); }
   // keys that the last row of a unit sees, in keys and in tiles: one at least, so that every unit is in the list
   __device__ __forceinline__ int limit(const PagedParams& p, int row_tile) const {
-    return max(seen(p, row_tile * ROWS + rows(p, row_tile) - 1), 0);
+    return TREE ? len : max(seen(p, row_tile * ROWS + rows(p, row_tile) - 1), 0);
   }
   __device__ __forceinline__ int tiles(const PagedParams& p, int row_tile) const {
     return max((limit(p, row_tile) + TILE - 1) / TILE, 1);
@@ -90,11 +93,21 @@ struct Request {
   }
 };
 
+// Which of 32 keys a row of a tree sees: bit e is key `ahead` + e of those behind its context (below 0: the context, which every
+// row sees).  What is behind the request's last token is for the caller to cut off.
+__device__ __forceinline__ uint32_t tree_bits(const PagedParams& p, const uint32_t* row, int ahead) {
+  if (ahead <= -32) return 0xFFFFFFFFu;
+  const int w = ahead >> 5;
+  auto word = [&](int i) -> uint32_t { return i < 0 ? 0xFFFFFFFFu : i < p.tree_words ? row[i] : 0u; };
+  return __funnelshift_r(word(w), word(w + 1), ahead & 31);
+}
+__device__ __forceinline__ const uint32_t* tree_row(const PagedParams& p, int t) { return p.tree + (int64_t)t * p.tree_words; }
+
 // The rest of a CTA's share, segment by segment: open() gives tiles [from, to) of a unit, close() goes on to the next one.
-template <int ROWS, int TILE>
+template <int ROWS, int TILE, bool TREE>
 struct Walk {
   static constexpr int kUnitCost = unit_cost(ROWS);
-  Request<ROWS, TILE> q;
+  Request<ROWS, TILE, TREE> q;
   int r, head, row_tile, entry, tiles;        // entry: -kUnitCost .. -1 without work, then the unit's tiles
   int from, to;
   int64_t left;                               // entries
@@ -119,7 +132,7 @@ struct Walk {
             left = 0;
             return;
           }
-          q = Request<ROWS, TILE>(p, r);
+          q = Request<ROWS, TILE, TREE>(p, r);
         } while (q.row_tiles == 0);
       }
     }
@@ -129,8 +142,8 @@ struct Walk {
 };
 
 // The share of this CTA; returns the entries of a full share.  All threads; `list` has THREADS / 32 + 2 words of shared memory.
-template <int THREADS, int ROWS, int TILE>
-__device__ __forceinline__ int64_t deal_tiles(const PagedParams& p, int64_t* list, Walk<ROWS, TILE>& at) {
+template <int THREADS, int ROWS, int TILE, bool TREE>
+__device__ __forceinline__ int64_t deal_tiles(const PagedParams& p, int64_t* list, Walk<ROWS, TILE, TREE>& at) {
   constexpr int kW = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   auto block_sum = [&](int64_t x, int64_t& before) -> int64_t {
@@ -153,7 +166,7 @@ __device__ __forceinline__ int64_t deal_tiles(const PagedParams& p, int64_t* lis
     return all;
   };
   auto weight = [&](int r) -> int64_t {
-    return r < p.requests ? p.hk * Request<ROWS, TILE>(p, r).head_entries(p) : 0;
+    return r < p.requests ? p.hk * Request<ROWS, TILE, TREE>(p, r).head_entries(p) : 0;
   };
   constexpr int kUnitCost = unit_cost(ROWS);
   // a thread has `each` requests in a row
@@ -181,7 +194,7 @@ __device__ __forceinline__ int64_t deal_tiles(const PagedParams& p, int64_t* lis
   }
   __syncthreads();
   at.r = (int)list[kW];
-  at.q = Request<ROWS, TILE>(p, at.r);
+  at.q = Request<ROWS, TILE, TREE>(p, at.r);
   int64_t rest = list[kW + 1];
   at.head = 0;
   if (at.q.row_tiles == 1) {                  // the common case without a 64-bit division
@@ -207,8 +220,8 @@ __device__ __forceinline__ int64_t deal_tiles(const PagedParams& p, int64_t* lis
   return share;
 }
 // pieces of a unit whose first tiles are this segment, the CTA's first one or not
-template <int ROWS, int TILE>
-__device__ __forceinline__ int4 cut_unit(const PagedParams& p, const Walk<ROWS, TILE>& u, int64_t share, bool first) {
+template <int ROWS, int TILE, bool TREE>
+__device__ __forceinline__ int4 cut_unit(const PagedParams& p, const Walk<ROWS, TILE, TREE>& u, int64_t share, bool first) {
   return make_int4(u.q.t0 * p.g + u.row_tile * ROWS, u.head, u.q.rows(p, u.row_tile),
                    1 + (int)((u.tiles - u.to + share - 1) / share) + (first ? 1 << 30 : 0));
 }
@@ -249,7 +262,7 @@ __device__ __forceinline__ float lse_of(float top, float sum) { return sum == 0.
 // Rows of no request, and of requests without keys: zeros and -inf.  The rows in front of the first request and behind the
 // last one may be most of a captured step's, so all CTAs take part: a call of 32 single tokens and 8160 such rows
 // of H 32 D 128 (67 MB) takes 66 us, and took 1078 with one.
-template <typename T, int D, int ROWS, int TILE>
+template <typename T, int D, int ROWS, int TILE, bool TREE>
 __device__ __forceinline__ void clear_untouched(const PagedParams& p) {
   const int h = p.hk * p.g;
   auto clear = [&](int64_t t0, int64_t t1, int64_t first, int64_t step) {    // tokens t0 .. t1 - 1 by threads first, first + step, ...
@@ -270,7 +283,7 @@ __device__ __forceinline__ void clear_untouched(const PagedParams& p) {
   }
 #pragma unroll 1
   for (int r = (int)blockIdx.x; r < p.requests; r += gridDim.x) {
-    const Request<ROWS, TILE> q(p, r);
+    const Request<ROWS, TILE, TREE> q(p, r);
     if (q.len == 0) clear(q.t0, q.t0 + q.n, threadIdx.x, blockDim.x);
   }
 }

@@ -787,10 +787,10 @@ void kv8_write(const Tensor& key, const Tensor& value, const Tensor& slot_map, c
          "nvfp4_kv8_write");
 }
 
-// query [Z, H, 1, D] without cu_seqlens, [T, H, D] with
-std::tuple<Tensor, OptTensor> kv8_attention(const Tensor& query, const OptTensor& cu, const Tensor& k_cache,
-                                            const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale,
-                                            const Tensor& table, const Tensor& lengths, double scaling, int64_t g, bool want_lse) {
+// query [Z, H, 1, D] without cu_seqlens, [T, H, D] with; tree: bits [T, W] of what its tokens see of each other
+std::tuple<Tensor, OptTensor> paged_attention(const Tensor& query, const OptTensor& cu, const OptTensor& tree, const Tensor& k_cache,
+                                              const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale,
+                                              const Tensor& table, const Tensor& lengths, double scaling, int64_t g, bool want_lse) {
   require_cuda(query, "query");
   Call c(query);
   const PagedCache p = paged_cache(c, k_cache, v_cache, k_scale, v_scale);
@@ -807,6 +807,10 @@ std::tuple<Tensor, OptTensor> kv8_attention(const Tensor& query, const OptTensor
     require_dims(query, 3, "query must be [T, H, D]");
     require_words(c, *cu, r + 1, at::kInt, "cu_seqlens must be contiguous int32 [requests + 1]");
   }
+  if (tree.has_value()) {
+    require(tree->dim() == 2 && tree->size(1) >= 1, "tree_mask must be contiguous int64 [T, words]");
+    require_words(c, *tree, query.size(0) * tree->size(1), at::kLong, "tree_mask must be contiguous int64 [T, words]");
+  }
   const int64_t t = query.size(0), h = query.size(1), d = query.size(-1);
   require(d == p.d, "query must have the cache's head dim");
   require(g >= 1 && h == p.hk * g, "num_key_value_groups must equal H // Hk");
@@ -818,12 +822,253 @@ std::tuple<Tensor, OptTensor> kv8_attention(const Tensor& query, const OptTensor
   c.done(nvfp4_kv8_attention_plan(dt, t, r, (int)g, (int)d, at::cuda::getDeviceProperties(c.dev.index())->multiProcessorCount, &bytes),
          "nvfp4_kv8_attention_plan");
   Tensor ws = c.empty({(int64_t)bytes}, at::kByte);
+  if (tree.has_value()) {
+    c.done(nvfp4_kv8_tree_attention(q.data_ptr(), dt, q.stride(0), q.stride(1), opt_ptr<int32_t>(cu), t,
+                                    reinterpret_cast<const uint64_t*>(tree->data_ptr<int64_t>()), tree->size(1), p.k, p.k_block, p.v,
+                                    p.v_block, p.ks, p.ks_block, p.vs, p.vs_block, p.blocks, (int)p.bs, table.data_ptr<int32_t>(),
+                                    table.stride(0), table.size(1), lengths.data_ptr<int32_t>(), r, p.hk, (int)g, (int)d, (float)scaling,
+                                    out.data_ptr(), opt_ptr<float>(lse), ws.data_ptr(), bytes, c.status, c.stream),
+           "nvfp4_kv8_tree_attention");
+    return {out, lse};
+  }
   c.done(nvfp4_kv8_attention(q.data_ptr(), dt, q.stride(0), q.stride(1), opt_ptr<int32_t>(cu), t, p.k, p.k_block, p.v, p.v_block,
                              p.ks, p.ks_block, p.vs, p.vs_block, p.blocks, (int)p.bs, table.data_ptr<int32_t>(), table.stride(0),
                              table.size(1), lengths.data_ptr<int32_t>(), r, p.hk, (int)g, (int)d, (float)scaling, out.data_ptr(),
                              opt_ptr<float>(lse), ws.data_ptr(), bytes, c.status, c.stream),
          "nvfp4_kv8_attention");
   return {out, lse};
+}
+
+std::tuple<Tensor, OptTensor> kv8_attention(const Tensor& query, const OptTensor& cu, const Tensor& k_cache, const Tensor& v_cache,
+                                            const Tensor& k_scale, const Tensor& v_scale, const Tensor& table, const Tensor& lengths,
+                                            double scaling, int64_t g, bool want_lse) {
+  return paged_attention(query, cu, std::nullopt, k_cache, v_cache, k_scale, v_scale, table, lengths, scaling, g, want_lse);
+}
+std::tuple<Tensor, OptTensor> kv8_tree_attention(const Tensor& query, const Tensor& cu, const Tensor& tree, const Tensor& k_cache,
+                                                 const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale,
+                                                 const Tensor& table, const Tensor& lengths, double scaling, int64_t g, bool want_lse) {
+  return paged_attention(query, cu, tree, k_cache, v_cache, k_scale, v_scale, table, lengths, scaling, g, want_lse);
+}
+
+// ---------------------------------------------------------------- trees of drafts
+// Requests of a call, from its cu_seqlens.
+int64_t requests_of(const Call& c, const Tensor& cu) {
+  const int64_t r = cu.numel() - 1;
+  require(r >= 1, "cu_seqlens must be contiguous int32 [requests + 1]");
+  require_words(c, cu, r + 1, at::kInt, "cu_seqlens must be contiguous int32 [requests + 1]");
+  return r;
+}
+
+std::tuple<Tensor, Tensor> draft_tree(const Tensor& parents, const Tensor& cu, const Tensor& lengths, int64_t max_tokens) {
+  require_cuda(parents, "parents");
+  Call c(parents);
+  require_dims(parents, 1, "parents must be [T]");
+  const int64_t t = parents.size(0), r = requests_of(c, cu);
+  require_words(c, parents, t, at::kInt, "parents must be contiguous int32 [T]");
+  require_words(c, lengths, r, at::kInt, "lengths must be contiguous int32 [requests]");
+  require(max_tokens >= 1 && max_tokens <= 1024, "max_tokens must be 1 to 1024");
+  Tensor mask = c.empty({t, (max_tokens + 63) / 64}, at::kLong), positions = c.empty({t}, at::kInt);
+  c.done(nvfp4_draft_tree(parents.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), t, r, max_tokens,
+                          reinterpret_cast<uint64_t*>(mask.data_ptr<int64_t>()), positions.data_ptr<int32_t>(), c.stream),
+         "nvfp4_draft_tree");
+  return {mask, positions};
+}
+
+std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor& target_in, const Tensor& tokens, const Tensor& parents, const Tensor& cu,
+                                                 const Tensor& uniforms, const OptTensor& draft_in) {
+  require_cuda(target_in, "target_probs");
+  Call c(target_in);
+  require_dims(target_in, 2, "target_probs must be [T, vocabulary]");
+  const int64_t t = target_in.size(0), v = target_in.size(1), r = requests_of(c, cu);
+  require(v >= 1, "target_probs must have a column");
+  const int dt = dtype_code(target_in.scalar_type());
+  auto rows = [](const Tensor& x) { return x.stride(1) == 1 || x.size(1) == 1 ? x : x.contiguous(); };
+  const Tensor target = rows(target_in);
+  Tensor draft;
+  if (draft_in.has_value()) {
+    c.same(*draft_in);
+    if (draft_in->scalar_type() != target_in.scalar_type()) throw UnsupportedType("draft_probs must have target_probs' dtype");
+    require(draft_in->sizes() == target_in.sizes(), "draft_probs must have target_probs' shape");
+    draft = rows(*draft_in);
+  }
+  if (tokens.scalar_type() != at::kLong && tokens.scalar_type() != at::kInt) throw UnsupportedType("tokens must be int64 or int32 [T]");
+  require_words(c, tokens, t, tokens.scalar_type(), "tokens must be contiguous int64 or int32 [T]");
+  require_words(c, parents, t, at::kInt, "parents must be contiguous int32 [T]");
+  require_words(c, uniforms, t, at::kFloat, "uniforms must be contiguous float32 [T]");
+  Tensor accepted = c.empty({t}, at::kInt), count = c.empty({r}, at::kInt), next = c.empty({r}, at::kLong);
+  c.done(nvfp4_verify_drafts(target.data_ptr(), target.stride(0), draft.defined() ? draft.data_ptr() : nullptr,
+                             draft.defined() ? draft.stride(0) : 0, dt, v, tokens.data_ptr(), tokens.scalar_type() == at::kLong,
+                             parents.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), uniforms.data_ptr<float>(), t, r,
+                             accepted.data_ptr<int32_t>(), count.data_ptr<int32_t>(), next.data_ptr<int64_t>(), c.stream),
+         "nvfp4_verify_drafts");
+  return {accepted, count, next};
+}
+
+// Caches and scales with or without a leading axis of layers, which the kernel writes: no element may be two layers'.
+Tensor paged_keep_path(const Tensor& accepted, const Tensor& count, const Tensor& cu, const Tensor& lengths, const Tensor& table,
+                       const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale) {
+  require_cuda(lengths, "lengths");
+  Call c(lengths);
+  require_table(c, table);
+  const int64_t r = table.size(0), t = accepted.numel();
+  require_words(c, accepted, t, at::kInt, "accepted must be contiguous int32 [T]");
+  require_words(c, count, r, at::kInt, "num_accepted must be contiguous int32 [requests]");
+  require_words(c, cu, r + 1, at::kInt, "cu_seqlens must be contiguous int32 [requests + 1]");
+  require_words(c, lengths, r, at::kInt, "lengths must be contiguous int32 [requests]");
+  const bool many = k_cache.dim() == 5;
+  const int64_t layers = many ? k_cache.size(0) : 1;
+  require(layers >= 1, "k_cache must have a layer");
+  for (const Tensor* x : {&k_cache, &v_cache})
+    if (x->dim() != (many ? 5 : 4)) throw std::invalid_argument("caches must be [layers, blocks, Hk, block_size, D] or [blocks, Hk, block_size, D]");
+  for (const Tensor* x : {&k_scale, &v_scale})
+    if (x->dim() != (many ? 3 : 2)) throw std::invalid_argument("scales must be [layers, blocks, Hk] or [blocks, Hk]");
+  auto first = [&](const Tensor& x) { return many ? x.select(0, 0) : x; };
+  const PagedCache p = paged_cache(c, first(k_cache), first(v_cache), first(k_scale), first(v_scale));
+  auto layer = [&](const Tensor& x, int64_t of_block) -> int64_t {
+    if (layers == 1) return 0;
+    require(x.size(0) == layers, "caches and scales must have the same layers");
+    const int64_t l = x.stride(0), b = x.stride(1), n = x.size(1);
+    require(n == 0 || l >= (n - 1) * b + of_block || (l >= of_block && (n == 1 || b >= (layers - 1) * l + of_block)), "layers must not overlap");
+    return l;
+  };
+  const int64_t block_bytes = p.hk * p.bs * p.d;
+  const int64_t kl = layer(k_cache, block_bytes), vl = layer(v_cache, block_bytes);
+  require(kl % 16 == 0 && vl % 16 == 0, "layers must start on 16 bytes");
+  const int64_t ksl = layer(k_scale, p.hk), vsl = layer(v_scale, p.hk);
+  Tensor keep = c.empty({r}, at::kInt);
+  c.done(nvfp4_paged_keep_path(accepted.data_ptr<int32_t>(), count.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), t,
+                               lengths.data_ptr<int32_t>(), table.data_ptr<int32_t>(), table.stride(0), r, table.size(1), p.k, kl,
+                               p.k_block, p.v, vl, p.v_block, p.ks, ksl, p.ks_block, p.vs, vsl, p.vs_block, layers, p.blocks, p.hk,
+                               (int)p.bs, (int)p.d, keep.data_ptr<int32_t>(), c.stream),
+         "nvfp4_paged_keep_path");
+  return keep;
+}
+
+// ---------------------------------------------------------------- norm of heads and rotation
+// [T, H, D], or [Z, H, S, D], as batch entries, tokens and heads; rows of unit stride on 16 bytes
+struct HeadRows {
+  Tensor keep;
+  int64_t z, s, h, d;
+  int64_t strides[3];
+};
+HeadRows head_rows(const Tensor& x_in) {
+  Tensor x = x_in;
+  const int64_t unit = 16 / x.element_size();
+  bool aligned = x.stride(-1) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) aligned = aligned && (x.size(i) == 1 || x.stride(i) % unit == 0);
+  if (!aligned) x = x.clone(at::MemoryFormat::Contiguous);
+  auto step = [&](int64_t i) { return x.size(i) == 1 ? 0 : x.stride(i); };
+  if (x.dim() == 3) return {x, 1, x.size(0), x.size(1), x.size(2), {0, step(0), step(1)}};
+  return {x, x.size(0), x.size(2), x.size(1), x.size(3), {step(0), step(2), step(1)}};
+}
+// Of x's shape, dense, with heads inside or outside of tokens as in x.
+Tensor empty_rows(const Call& c, const Tensor& x) {
+  if (x.dim() == 4 && x.stride(1) < x.stride(2))
+    return c.empty({x.size(0), x.size(2), x.size(1), x.size(3)}, x.scalar_type()).transpose(1, 2);
+  return c.empty(x.sizes(), x.scalar_type());
+}
+struct NormTables {
+  Tensor cos, sin, wq, wk;
+  OptTensor positions;
+  int64_t rows, pos_batch;
+  int dt, wdt;
+};
+NormTables norm_tables(const Call& c, const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& cos,
+                       const Tensor& sin, const OptTensor& positions, int64_t pos0) {
+  const char* shapes = "query and key must be [T, H, D] and [T, Hk, D], or [Z, H, S, D] and [Z, Hk, S, D]";
+  if (q.dim() != 3 && q.dim() != 4) throw std::invalid_argument(shapes);
+  require_dims(k, q.dim(), shapes);
+  const bool four = q.dim() == 4;
+  const int64_t d = q.size(-1), z = four ? q.size(0) : 1, s = q.size(four ? 2 : 0);
+  require(k.size(-1) == d && (four ? k.size(0) == z && k.size(2) == s : k.size(0) == s), shapes);
+  require(q.size(1) >= 1 && k.size(1) >= 1, "query and key must have a head");
+  require(d == 128 || d == 256, "D must be 128 or 256");
+  c.same(k);
+  if (q.scalar_type() != k.scalar_type()) throw UnsupportedType("query and key must have the same dtype");
+  NormTables t;
+  t.dt = dtype_code(q.scalar_type());
+  for (const Tensor* w : {&wq, &wk}) {
+    c.same(*w);
+    require(w->dim() == 1 && w->size(0) == d, "q_weight and k_weight must be [D]");
+    if (w->scalar_type() != wq.scalar_type() || (w->scalar_type() != q.scalar_type() && w->scalar_type() != at::kFloat))
+      throw UnsupportedType("q_weight and k_weight must both have the operands' dtype, or both float32");
+  }
+  t.wdt = dtype_code(wq.scalar_type());
+  c.same(cos);
+  c.same(sin);
+  require(cos.dim() == 2 && cos.size(1) == d / 2 && sin.sizes() == cos.sizes() && cos.scalar_type() == at::kFloat &&
+              sin.scalar_type() == at::kFloat,
+          "cos / sin must be fp32 [P, D/2]");
+  auto table = [](const Tensor& x) {
+    return x.is_contiguous() && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 ? x : x.clone(at::MemoryFormat::Contiguous);
+  };
+  t.cos = table(cos);
+  t.sin = table(sin);
+  t.wq = wq.contiguous();
+  t.wk = wk.contiguous();
+  t.rows = cos.size(0);
+  t.pos_batch = 0;
+  if (positions.has_value()) {
+    if (positions->scalar_type() != at::kInt && positions->scalar_type() != at::kLong) throw UnsupportedType("positions must be int32 or int64");
+    const bool own = four && positions->dim() == 2;
+    require(own ? positions->size(0) == z && positions->size(1) == s : positions->dim() == 1 && positions->size(0) == s,
+            "positions must be one a token: [T], or [S] or [Z, S]");
+    t.positions = positions->to(q.device(), at::kInt).contiguous();
+    if (own) t.pos_batch = s;
+  } else {
+    require(pos0 >= 0 && (s == 0 || pos0 <= t.rows - s), "positions pos0 .. must lie within cos / sin");
+  }
+  return t;
+}
+
+std::tuple<Tensor, Tensor> norm_rope_forward(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& cos,
+                                             const Tensor& sin, const OptTensor& positions, int64_t pos0, double eps) {
+  require_cuda(q, "query");
+  Call c(q);
+  const NormTables t = norm_tables(c, q, k, wq, wk, cos, sin, positions, pos0);
+  require(eps >= 0.0, "eps must not be negative");
+  const HeadRows a = head_rows(q), b = head_rows(k);
+  Tensor oq = empty_rows(c, q), ok = empty_rows(c, k);
+  const HeadRows ra = head_rows(oq), rb = head_rows(ok);
+  c.done(nvfp4_qk_norm_rope(a.keep.data_ptr(), a.strides, b.keep.data_ptr(), b.strides, t.dt, a.z, a.s, a.h, b.h, (int)a.d,
+                            t.wq.data_ptr(), t.wk.data_ptr(), t.wdt, t.cos.data_ptr<float>(), t.sin.data_ptr<float>(), t.rows,
+                            opt_ptr<int32_t>(t.positions), t.pos_batch, pos0, (float)eps, oq.data_ptr(), ra.strides, ok.data_ptr(),
+                            rb.strides, c.stream),
+         "nvfp4_qk_norm_rope");
+  return {oq, ok};
+}
+
+// gradients of query, key and (where wanted) the weights
+std::array<Tensor, 4> norm_rope_backward(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& cos,
+                                         const Tensor& sin, const OptTensor& positions, int64_t pos0, double eps, const Tensor& gq,
+                                         const Tensor& gk, bool want_wq, bool want_wk) {
+  require_cuda(q, "query");
+  Call c(q);
+  const NormTables t = norm_tables(c, q, k, wq, wk, cos, sin, positions, pos0);
+  auto incoming = [&](const Tensor& g, const Tensor& x) {
+    c.same(g);
+    require(g.sizes() == x.sizes() && g.scalar_type() == x.scalar_type(), "gradients must have their results' shape and dtype");
+    return head_rows(g);
+  };
+  const HeadRows a = head_rows(q), b = head_rows(k), ga = incoming(gq, q), gb = incoming(gk, k);
+  Tensor dq = empty_rows(c, q), dk = empty_rows(c, k), dwq, dwk, ws;
+  const HeadRows ra = head_rows(dq), rb = head_rows(dk);
+  if (want_wq) dwq = c.empty({a.d}, wq.scalar_type());
+  if (want_wk) dwk = c.empty({a.d}, wk.scalar_type());
+  size_t bytes = 0;
+  if (want_wq || want_wk) {
+    c.done(nvfp4_qk_norm_rope_bwd_plan((int)a.d, at::cuda::getDeviceProperties(c.dev.index())->multiProcessorCount, &bytes),
+           "nvfp4_qk_norm_rope_bwd_plan");
+    ws = c.empty({(int64_t)bytes}, at::kByte);
+  }
+  auto ptr = [](const Tensor& x) { return x.defined() ? x.data_ptr() : nullptr; };
+  c.done(nvfp4_qk_norm_rope_bwd(a.keep.data_ptr(), a.strides, b.keep.data_ptr(), b.strides, ga.keep.data_ptr(), ga.strides,
+                                gb.keep.data_ptr(), gb.strides, t.dt, a.z, a.s, a.h, b.h, (int)a.d, t.wq.data_ptr(), t.wk.data_ptr(),
+                                t.wdt, t.cos.data_ptr<float>(), t.sin.data_ptr<float>(), t.rows, opt_ptr<int32_t>(t.positions),
+                                t.pos_batch, pos0, (float)eps, dq.data_ptr(), ra.strides, dk.data_ptr(), rb.strides, ptr(dwq), ptr(dwk),
+                                ptr(ws), bytes, c.stream),
+         "nvfp4_qk_norm_rope_bwd");
+  return {dq, dk, dwq, dwk};
 }
 
 // ---------------------------------------------------------------- backward
@@ -1123,6 +1368,60 @@ Tensor attention(const Tensor& query, const Tensor& key, const Tensor& value, do
   return out;
 }
 
+// As for the attention, a graph node of its own.  It keeps the operands as they were given.
+struct NormRopeBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable saved[7];       // query, key, q_weight, k_weight, cos, sin, positions
+  int64_t pos0 = 0;
+  double eps = 0.0;
+
+  std::string name() const override { return "QkNormRopeBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto& x : saved) x.reset_data();
+  }
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    torch::autograd::variable_list out(4);
+    const bool q = grads[0].defined(), k = grads[1].defined();
+    if (!q && !k) return out;
+    if (c10::GradMode::is_enabled()) throw NotImplemented("qk_norm_rope does not implement a backward of its backward (create_graph)");
+    Tensor t[7];
+    {
+      std::lock_guard<std::mutex> lock(mutex_);
+      for (int i = 0; i < 7; ++i) t[i] = saved[i].unpack();
+    }
+    const Tensor gq = q ? grads[0] : at::zeros_like(t[0]), gk = k ? grads[1] : at::zeros_like(t[1]);
+    auto r = norm_rope_backward(t[0], t[1], t[2], t[3], t[4], t[5], t[6].defined() ? OptTensor(t[6]) : OptTensor(), pos0, eps, gq, gk,
+                                q && task_should_compute_output(2), k && task_should_compute_output(3));
+    for (int i = 0; i < 4; ++i)
+      if (i % 2 == 0 ? q : k) out[i] = r[i];
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& query, const Tensor& key, const Tensor& wq, const Tensor& wk, const Tensor& cos,
+                                        const Tensor& sin, const OptTensor& positions, int64_t pos0, double eps) {
+  const Tensor* all[6] = {&query, &key, &wq, &wk, &cos, &sin};
+  bool record = false;
+  for (int i = 0; i < 6; ++i) {
+    if (all[i]->_fw_grad(0).defined()) throw NotImplemented("qk_norm_rope does not implement forward-mode AD (no jvp)");
+    if (c10::GradMode::is_enabled() && all[i]->requires_grad()) {
+      if (i >= 4) throw NotImplemented("qk_norm_rope has no gradient for cos and sin");
+      record = true;
+    }
+  }
+  c10::AutoGradMode no_grad(false);
+  auto [oq, ok] = norm_rope_forward(query, key, wq, wk, cos, sin, positions, pos0, eps);
+  if (!record) return {oq, ok};
+  std::shared_ptr<NormRopeBackward> node(new NormRopeBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(query, key, wq, wk));
+  for (int i = 0; i < 6; ++i) node->saved[i] = torch::autograd::SavedVariable(*all[i], false);
+  node->saved[6] = torch::autograd::SavedVariable(positions.has_value() ? *positions : Tensor(), false);
+  node->pos0 = pos0;
+  node->eps = eps;
+  torch::autograd::set_history(torch::autograd::variable_list{oq, ok}, node);
+  return {oq, ok};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -1158,6 +1457,12 @@ PYBIND11_MODULE(_native, m) {
   m.def("paged_trim", &paged_trim, nogil());
   m.def("kv8_write", &kv8_write, nogil());
   m.def("kv8_attention", &kv8_attention, nogil());
+  m.def("kv8_tree_attention", &kv8_tree_attention, nogil());
+  m.def("draft_tree", &draft_tree, nogil());
+  m.def("verify_drafts", &verify_drafts, nogil());
+  m.def("paged_keep_path", &paged_keep_path, nogil());
+  m.def("qk_norm_rope", &qk_norm_rope, nogil());
+  m.def("qk_norm_rope_bwd", &norm_rope_backward, nogil());
   m.def("bwd_prep", &bwd_prep, nogil());
   m.def("bf16_rows", &bf16_rows, nogil());
   m.def("bwd_hp", &bwd_hp, nogil());

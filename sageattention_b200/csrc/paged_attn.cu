@@ -91,7 +91,7 @@ struct Smem {
   static constexpr int kBytes = kRing + kShared;
 };
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool kTree>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kernel(PagedParams p) {
   using S = Smem<T, D, NT>;
   constexpr int kSub = Cfg<D>::kSub, kTile = Cfg<D>::kTile, kRows = 8 * NT;
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
   griddep_wait();
   griddep_launch();
 
-  using Place = Walk<kRows, kTile>;
+  using Place = Walk<kRows, kTile, kTree>;
   Place use;
   const int64_t share = deal_tiles<kThreads>(p, list_s, use);
   if (tid == 0) p.cut[cta] = make_int4(0, 0, 0, 0);
@@ -241,16 +241,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
         }
       }
       __syncthreads();
-      // this thread's query rows: 8 nt + 2 c4, + 1.  Rows of no query see all keys (they are not stored).
+      // this thread's query rows: 8 nt + 2 c4, + 1.  Rows of no query see all keys (they are not stored), or what the last one sees.
       float inv[NT][2];
-      int lim[NT][2];
+      int lim[NT][2];                                      // keys that a row sees, or its token in a tree
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int row = nt * 8 + 2 * c4 + k;
           inv[nt][k] = q_inv[row];
-          lim[nt][k] = row < rows ? use.q.seen(p, use.row_tile * kRows + row) : INT_MAX;
+          if (kTree) lim[nt][k] = use.q.t0 + token_of(p, use.row_tile * kRows + min(row, rows - 1));
+          else lim[nt][k] = row < rows ? use.q.seen(p, use.row_tile * kRows + row) : INT_MAX;
         }
       const int lim_first = use.q.seen(p, use.row_tile * kRows);       // the smallest of all rows
 
@@ -351,7 +352,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
                 const float f = scale_product(inv[nt][k], kscale[h]);
                 s[h][nt][k] *= f;
                 s[h][nt][2 + k] *= f;
-                if (masks) {
+                if (kTree && masks) {
+                  const uint32_t bits = tree_bits(p, tree_row(p, lim[nt][k]), key + h * 16 - lim_first) >> krow;
+                  if (krow >= keys[h] || !(bits & 1)) s[h][nt][k] = -INFINITY;
+                  if (krow + 8 >= keys[h] || !(bits >> 8 & 1)) s[h][nt][2 + k] = -INFINITY;
+                } else if (masks) {
                   if (krow >= keys[h] || key + h * 16 + krow >= lim[nt][k]) s[h][nt][k] = -INFINITY;
                   if (krow + 8 >= keys[h] || key + h * 16 + krow + 8 >= lim[nt][k]) s[h][nt][2 + k] = -INFINITY;
                 }
@@ -525,16 +530,20 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kCtas : 2) paged_attn_kern
       first = false;
     }
   }
-  clear_untouched<T, D, kRows, kTile>(p);
+  clear_untouched<T, D, kRows, kTile, kTree>(p);
 }
 
-template <typename T, int D, int NT>
-int run_attention(const PagedParams& p, int sms, cudaStream_t st) {
+template <typename T, int D, int NT, bool kTree>
+int run_kernel(const PagedParams& p, int sms, cudaStream_t st) {
   using S = Smem<T, D, NT>;
   const int grid = (NT == 1 ? kCtas : 2) * sms;
-  if (int rc = allow_smem("nvfp4_kv8_attention", reinterpret_cast<const void*>(paged_attn_kernel<T, D, NT>), S::kBytes)) return rc;
-  if (int rc = launch("nvfp4_kv8_attention", paged_attn_kernel<T, D, NT>, dim3(grid), kThreads, S::kBytes, st, p)) return rc;
+  if (int rc = allow_smem("nvfp4_kv8_attention", reinterpret_cast<const void*>(paged_attn_kernel<T, D, NT, kTree>), S::kBytes)) return rc;
+  if (int rc = launch("nvfp4_kv8_attention", paged_attn_kernel<T, D, NT, kTree>, dim3(grid), kThreads, S::kBytes, st, p)) return rc;
   return launch_combine<T, D, 8 * NT, false>(p, grid, st);
+}
+template <typename T, int D, int NT>
+int run_attention(const PagedParams& p, int sms, cudaStream_t st) {
+  return p.tree != nullptr ? run_kernel<T, D, NT, true>(p, sms, st) : run_kernel<T, D, NT, false>(p, sms, st);
 }
 
 // Which kernel, by query rows a request on average (their numbers are on the device): eight, sixteen or (D = 128) 24 rows of
@@ -563,6 +572,52 @@ int run_rows(const PagedParams& p, int nt, int sms, cudaStream_t st) {
   return run_attention<T, D, 2>(p, sms, st);
 }
 
+// tree_mask: [tokens, tree_words] bits of 64, or null: causal
+int attention(const char* what, const void* q, int q_dtype, int64_t s_qt, int64_t s_qh, const int32_t* cu_seqlens, int64_t tokens,
+              const uint64_t* tree_mask, int64_t tree_words, const uint8_t* k_cache, int64_t k_block, const uint8_t* v_cache,
+              int64_t v_block, const float* k_scale, int64_t ks_block, const float* v_scale, int64_t vs_block, int64_t blocks,
+              int block_size, const int32_t* table, int64_t table_row, int64_t width, const int32_t* lengths, int64_t requests, int64_t hk,
+              int g, int d, float scaling, void* out, float* lse, void* workspace, size_t workspace_bytes, int* status,
+              nvfp4_stream_t stream) {
+  NVFP4_REQUIRE(d == 128 || d == 256, "%s: D must be 128 or 256", what);
+  int lb = 4;
+  while (lb < 7 && (1 << lb) != block_size) ++lb;
+  NVFP4_REQUIRE((1 << lb) == block_size, "%s: block_size must be 16, 32, 64 or 128", what);
+  NVFP4_REQUIRE(requests >= 1 && requests < (1 << 30) && tokens >= 0 && hk >= 1 && g >= 1 && tokens * g < INT32_MAX &&
+                    hk * g < (1 << 20) && blocks >= 0 && blocks < INT32_MAX && width >= 0 && width * block_size < INT32_MAX - 256,
+                "%s: sizes out of range", what);
+  NVFP4_REQUIRE(cu_seqlens != nullptr || tokens == requests, "%s: one token a request without cu_seqlens", what);
+  NVFP4_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)workspace) & 15) == 0 && ((uintptr_t)out & 31) == 0 &&
+                    ((k_block | v_block) & 15) == 0,
+                "%s: cache blocks and workspace must be 16-byte aligned, out 32-byte aligned", what);
+  NVFP4_REQUIRE(((uintptr_t)q & 15) == 0 && ((s_qt | s_qh) * (q_dtype == NVFP4_DT_FP32 ? 4 : 2) & 15) == 0,
+                "%s: query rows must be 16-byte aligned", what);
+  NVFP4_REQUIRE(isfinite(scaling), "%s: scaling must be finite", what);
+  if (tokens == 0) return 0;
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const Choice c = choose(q_dtype, tokens, requests, g, d, sms);
+  const int grid = c.ctas;
+  const int64_t rows = c.rows;
+  NVFP4_REQUIRE(workspace_bytes >= (size_t)(grid * paged_slot_bytes(rows, d)), "%s: workspace too small", what);
+  NVFP4_REQUIRE(q_dtype >= NVFP4_DT_BF16 && q_dtype <= NVFP4_DT_FP32, "%s: unknown dtype %d", what, q_dtype);
+  PagedParams p{q, s_qt, s_qh, cu_seqlens, tokens, k_cache, v_cache, k_block, v_block, k_scale, v_scale, ks_block, vs_block, table,
+                table_row, lengths, (int)requests, (int)width, (int)blocks, lb, (int)hk, g, 0, 0, scaling * kLog2e, out, lse,
+                nullptr, nullptr, nullptr, nullptr, status, reinterpret_cast<const uint32_t*>(tree_mask), (int)(2 * tree_words)};
+  set_group(p, g);
+  p.ws_acc = static_cast<float*>(workspace);
+  p.cut = reinterpret_cast<int4*>(p.ws_acc + 2 * grid * rows * d);
+  p.ws_m = reinterpret_cast<float*>(p.cut + grid);
+  p.ws_l = p.ws_m + 2 * grid * rows;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (c.chunk) return launch_paged_chunk(p, q_dtype, d, grid, st);
+  switch (q_dtype) {
+    case NVFP4_DT_BF16: return d == 128 ? run_rows<__nv_bfloat16, 128>(p, c.nt, sms, st) : run_rows<__nv_bfloat16, 256>(p, c.nt, sms, st);
+    case NVFP4_DT_FP16: return d == 128 ? run_rows<__half, 128>(p, c.nt, sms, st) : run_rows<__half, 256>(p, c.nt, sms, st);
+    default: return d == 128 ? run_rows<float, 128>(p, c.nt, sms, st) : run_rows<float, 256>(p, c.nt, sms, st);
+  }
+}
+
 }  // namespace
 }  // namespace nvfp4
 
@@ -585,41 +640,21 @@ extern "C" int nvfp4_kv8_attention(const void* q, int q_dtype, int64_t s_qt, int
                                    int64_t width, const int32_t* lengths, int64_t requests, int64_t hk, int g, int d,
                                    float scaling, void* out, float* lse, void* workspace, size_t workspace_bytes,
                                    int* status, nvfp4_stream_t stream) {
-  NVFP4_REQUIRE(d == 128 || d == 256, "nvfp4_kv8_attention: D must be 128 or 256");
-  int lb = 4;
-  while (lb < 7 && (1 << lb) != block_size) ++lb;
-  NVFP4_REQUIRE((1 << lb) == block_size, "nvfp4_kv8_attention: block_size must be 16, 32, 64 or 128");
-  NVFP4_REQUIRE(requests >= 1 && requests < (1 << 30) && tokens >= 0 && hk >= 1 && g >= 1 && tokens * g < INT32_MAX &&
-                    hk * g < (1 << 20) && blocks >= 0 && blocks < INT32_MAX && width >= 0 && width * block_size < INT32_MAX - 256,
-                "nvfp4_kv8_attention: sizes out of range");
-  NVFP4_REQUIRE(cu_seqlens != nullptr || tokens == requests, "nvfp4_kv8_attention: one token a request without cu_seqlens");
-  NVFP4_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)workspace) & 15) == 0 && ((uintptr_t)out & 31) == 0 &&
-                    ((k_block | v_block) & 15) == 0,
-                "nvfp4_kv8_attention: cache blocks and workspace must be 16-byte aligned, out 32-byte aligned");
-  NVFP4_REQUIRE(((uintptr_t)q & 15) == 0 && ((s_qt | s_qh) * (q_dtype == NVFP4_DT_FP32 ? 4 : 2) & 15) == 0,
-                "nvfp4_kv8_attention: query rows must be 16-byte aligned");
-  NVFP4_REQUIRE(isfinite(scaling), "nvfp4_kv8_attention: scaling must be finite");
-  if (tokens == 0) return 0;
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const Choice c = choose(q_dtype, tokens, requests, g, d, sms);
-  const int grid = c.ctas;
-  const int64_t rows = c.rows;
-  NVFP4_REQUIRE(workspace_bytes >= (size_t)(grid * paged_slot_bytes(rows, d)), "nvfp4_kv8_attention: workspace too small");
-  NVFP4_REQUIRE(q_dtype >= NVFP4_DT_BF16 && q_dtype <= NVFP4_DT_FP32, "nvfp4_kv8_attention: unknown dtype %d", q_dtype);
-  PagedParams p{q, s_qt, s_qh, cu_seqlens, tokens, k_cache, v_cache, k_block, v_block, k_scale, v_scale, ks_block, vs_block, table,
-                table_row, lengths, (int)requests, (int)width, (int)blocks, lb, (int)hk, g, 0, 0, scaling * kLog2e, out, lse,
-                nullptr, nullptr, nullptr, nullptr, status};
-  set_group(p, g);
-  p.ws_acc = static_cast<float*>(workspace);
-  p.cut = reinterpret_cast<int4*>(p.ws_acc + 2 * grid * rows * d);
-  p.ws_m = reinterpret_cast<float*>(p.cut + grid);
-  p.ws_l = p.ws_m + 2 * grid * rows;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (c.chunk) return launch_paged_chunk(p, q_dtype, d, grid, st);
-  switch (q_dtype) {
-    case NVFP4_DT_BF16: return d == 128 ? run_rows<__nv_bfloat16, 128>(p, c.nt, sms, st) : run_rows<__nv_bfloat16, 256>(p, c.nt, sms, st);
-    case NVFP4_DT_FP16: return d == 128 ? run_rows<__half, 128>(p, c.nt, sms, st) : run_rows<__half, 256>(p, c.nt, sms, st);
-    default: return d == 128 ? run_rows<float, 128>(p, c.nt, sms, st) : run_rows<float, 256>(p, c.nt, sms, st);
-  }
+  return attention("nvfp4_kv8_attention", q, q_dtype, s_qt, s_qh, cu_seqlens, tokens, nullptr, 0, k_cache, k_block, v_cache, v_block, k_scale,
+                   ks_block, v_scale, vs_block, blocks, block_size, table, table_row, width, lengths, requests, hk, g, d, scaling, out, lse,
+                   workspace, workspace_bytes, status, stream);
+}
+
+extern "C" int nvfp4_kv8_tree_attention(const void* q, int q_dtype, int64_t s_qt, int64_t s_qh, const int32_t* cu_seqlens, int64_t tokens,
+                                        const uint64_t* tree_mask, int64_t tree_words, const uint8_t* k_cache, int64_t k_block,
+                                        const uint8_t* v_cache, int64_t v_block, const float* k_scale, int64_t ks_block,
+                                        const float* v_scale, int64_t vs_block, int64_t blocks, int block_size, const int32_t* table,
+                                        int64_t table_row, int64_t width, const int32_t* lengths, int64_t requests, int64_t hk, int g,
+                                        int d, float scaling, void* out, float* lse, void* workspace, size_t workspace_bytes, int* status,
+                                        nvfp4_stream_t stream) {
+  NVFP4_REQUIRE(cu_seqlens != nullptr && tree_mask != nullptr, "nvfp4_kv8_tree_attention: cu_seqlens and tree_mask are needed");
+  NVFP4_REQUIRE(tree_words >= 1 && tree_words < (1 << 20), "nvfp4_kv8_tree_attention: tree_words out of range");
+  return attention("nvfp4_kv8_tree_attention", q, q_dtype, s_qt, s_qh, cu_seqlens, tokens, tree_mask, tree_words, k_cache, k_block, v_cache,
+                   v_block, k_scale, ks_block, v_scale, vs_block, blocks, block_size, table, table_row, width, lengths, requests, hk, g, d,
+                   scaling, out, lse, workspace, workspace_bytes, status, stream);
 }

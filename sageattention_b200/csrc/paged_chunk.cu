@@ -145,12 +145,12 @@ __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint3
 
 // Shared memory behind the tiles.  All of it is dynamic, and within 195 KB: with that the SM's split leaves 60 KB of L1, whose
 // lines hold what the converting warps have asked for, and with more than 195 KB 28.
-template <int D>
+template <int D, bool kTree>
 struct Tail {
   using C = Cfg<D>;
   uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2][2], p_full[2][2], o_full[2], o_free[2], pv_done[2], q_full, q_free;
   int64_t list[C::kThreads / 32 + 2];
-  Walk<C::kRows, kTile> place;
+  Walk<C::kRows, kTile, kTree> place;
   int64_t share;                                           // entries of a full share
   uint32_t tmem_base;
   int expired;
@@ -160,18 +160,18 @@ struct Tail {
   __device__ __forceinline__ float* l() { return c + C::kRows - 128; }       // of rows that a unit of one group's rows does not have
 };
 constexpr int kSmemPercent = 85;
-template <int D>
+template <int D, bool kTree>
 constexpr int smem_bytes() {
-  static_assert(Cfg<D>::kTail + sizeof(Tail<D>) <= 195 * 1024, "L1");
-  return Cfg<D>::kTail + (int)sizeof(Tail<D>);
+  static_assert(Cfg<D>::kTail + sizeof(Tail<D, kTree>) <= 195 * 1024, "L1");
+  return Cfg<D>::kTail + (int)sizeof(Tail<D, kTree>);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kTree>
 __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedParams p) {
   using C = Cfg<D>;
-  using Place = Walk<C::kRows, kTile>;
+  using Place = Walk<C::kRows, kTile, kTree>;
   extern __shared__ __align__(1024) uint8_t smem[];        // at 1024 without static shared memory in front of it, see below
-  Tail<D>& sh = *reinterpret_cast<Tail<D>*>(smem + C::kTail);
+  auto& sh = *reinterpret_cast<Tail<D, kTree>*>(smem + C::kTail);
   auto &k_full = sh.k_full, &k_free = sh.k_free, &v_full = sh.v_full, &v_free = sh.v_free, &pv_done = sh.pv_done, &o_full = sh.o_full,
        &o_free = sh.o_free;
   auto &s_full = sh.s_full, &p_full = sh.p_full;
@@ -628,7 +628,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       const bool merge = C::kGroups == 2 && !both;
       __syncwarp();
       if (!merge && lane == 0) mbar_arrive(&q_free);
-      const int limit = live ? at.q.seen(p, i_row) : 0;    // keys that this row sees
+      const int limit = live || kTree ? at.q.seen(p, i_row) : 0;      // keys that this row sees, or (of a tree) that all rows see
+      // the bits of a tree's row; rows of no query have those of the last one
+      const uint32_t* const bits = kTree ? tree_row(p, at.q.t0 + token_of(p, min(i_row, at.row_tile * C::kRows + rows - 1))) : nullptr;
       float m = -INFINITY, ref = -INFINITY, l = 0.0f;
 
       const int turn = both || C::kGroups == 1 ? 1 : 2, my = turn == 2 ? group : 0;
@@ -649,6 +651,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
         const bool masked = __any_sync(0xffffffffu, live && limit < key0 + C::kN) ||
                             (there & ((1u << (C::kN / 16)) - 1)) != (1u << (C::kN / 16)) - 1;
         const int visible = limit - key0;
+        // columns x .. x + 31 of a tree's row, as far as there are keys
+        auto tree_columns = [&](int x) -> uint32_t {
+          const int left = at.q.len - key0 - x;
+          return left <= 0 ? 0u : tree_bits(p, bits, x - visible) & (left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1);
+        };
         // columns 32 x .. of S: the next ones are on their way while the present ones are used, and the last two stay for
         // the exponentials, which therefore run from the end
         float top = -INFINITY;
@@ -665,11 +672,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
               tmem_ld16(s_at + x * 16, now);
               tmem_ld_wait();
               const int of = sub * kOf + x, left = groups >> of & 1 ? visible - x * 16 : 0;
+              const uint32_t columns = kTree && (groups >> of & 1) ? tree_columns(x * 16) : 0u;
               const float f = scale_product(c_row, exp2_int(info.k_exp[of]));
               float t = -INFINITY;
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
-                now[e] = e < left ? __float_as_uint(__uint_as_float(now[e]) * f) : 0xFF800000u;
+                now[e] = (kTree ? (columns >> e & 1) != 0 : e < left) ? __float_as_uint(__uint_as_float(now[e]) * f) : 0xFF800000u;
                 t = fmaxf(t, __uint_as_float(now[e]));
               }
               top = fmaxf(top, t);
@@ -725,7 +733,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
             tmem_ld32(s_at + x * 32, s[0]);
             tmem_ld_wait();
             const int left = visible - x * 32;
-            uint32_t seen = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1;
+            uint32_t seen = kTree ? tree_columns(x * 32) : left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1;
             seen &= ((there >> (2 * x) & 1) ? 0xFFFFu : 0u) | ((there >> (2 * x + 1) & 1) ? 0xFFFF0000u : 0u);
 #pragma unroll
             for (int e = 0; e < 32; ++e) s[0][e] = (seen >> e & 1) ? s[0][e] : 0xFF800000u;
@@ -924,7 +932,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
       first_segment = false;
     }
   }
-  clear_untouched<T, D, C::kRows, kTile>(p);
+  clear_untouched<T, D, C::kRows, kTile, kTree>(p);
   tc_fence_before();
   __syncthreads();
   report_error(&expired, p.status);
@@ -934,14 +942,19 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1) paged_chunk_kernel(PagedP
   }
 }
 
+template <typename T, int D, bool kTree>
+int run_kernel(const PagedParams& p, int ctas, cudaStream_t st) {
+  using C = Cfg<D>;
+  const void* kern = reinterpret_cast<const void*>(paged_chunk_kernel<T, D, kTree>);
+  constexpr int kBytes = smem_bytes<D, kTree>();
+  if (int rc = allow_smem("nvfp4_kv8_attention", kern, kBytes)) return rc;
+  prefer_l1(kern, kSmemPercent);
+  if (int rc = launch("nvfp4_kv8_attention", paged_chunk_kernel<T, D, kTree>, dim3(ctas), C::kThreads, kBytes, st, p)) return rc;
+  return launch_combine<T, D, C::kRows, true>(p, ctas, st);
+}
 template <typename T, int D>
 int run_chunk(const PagedParams& p, int ctas, cudaStream_t st) {
-  using C = Cfg<D>;
-  const void* kern = reinterpret_cast<const void*>(paged_chunk_kernel<T, D>);
-  if (int rc = allow_smem("nvfp4_kv8_attention", kern, smem_bytes<D>())) return rc;
-  prefer_l1(kern, kSmemPercent);
-  if (int rc = launch("nvfp4_kv8_attention", paged_chunk_kernel<T, D>, dim3(ctas), C::kThreads, smem_bytes<D>(), st, p)) return rc;
-  return launch_combine<T, D, C::kRows, true>(p, ctas, st);
+  return p.tree != nullptr ? run_kernel<T, D, true>(p, ctas, st) : run_kernel<T, D, false>(p, ctas, st);
 }
 
 }  // namespace

@@ -10,6 +10,7 @@ from .flash import (  # noqa: F401
     _run_bwd,
     _run_bwd_hp,
     nvfp4_flash_attn_func,
+    qk_norm_rope,
     rope_quant_nvfp4,
     vproj_quant_nvfp4,
     _next_mult,
@@ -26,13 +27,19 @@ from .flash import (  # noqa: F401
 )
 from .kv_cache import NVFP4KVCache  # noqa: F401
 from .paged_cache import (  # noqa: F401
+    DraftTree,
     FP8PagedKVCache,
     PagedStep,
+    VerifiedDrafts,
+    draft_tree,
     fp8_kv_write,
     fp8_paged_attention,
     fp8_paged_decode,
+    fp8_paged_tree_attention,
+    paged_kv_keep_path,
     paged_kv_reserve,
     paged_kv_trim,
+    verify_drafts,
 )
 
 __all__ = [
@@ -50,4 +57,9 @@ __all__ = [
     "fp8_paged_decode",
     "paged_kv_reserve",
     "paged_kv_trim",
+    "draft_tree",
+    "fp8_paged_tree_attention",
+    "paged_kv_keep_path",
+    "qk_norm_rope",
+    "verify_drafts",
 ]

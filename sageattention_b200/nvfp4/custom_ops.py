@@ -20,6 +20,12 @@ second compute path.
     out, lse = torch.ops.sageattention_b200.fp8_paged_decode(q, k_cache, v_cache, k_scale, v_scale, table, lengths, scaling, groups)
     out, lse = torch.ops.sageattention_b200.fp8_paged_attention(q, cu, k_cache, v_cache, k_scale, v_scale, table, lengths,
                                                                 scaling, groups)
+    mask, positions = torch.ops.sageattention_b200.draft_tree(parents, cu, lengths, max_tokens)
+    out, lse = torch.ops.sageattention_b200.fp8_paged_tree_attention(q, cu, mask, k_cache, v_cache, k_scale, v_scale, table,
+                                                                     lengths, scaling, groups)
+    accepted, num, following = torch.ops.sageattention_b200.verify_drafts(target_probs, tokens, parents, cu, uniforms, draft_probs)
+    keep = torch.ops.sageattention_b200.paged_kv_keep_path(accepted, num, cu, lengths, table, k_cache, v_cache, k_scale, v_scale)
+    q, k = torch.ops.sageattention_b200.qk_norm_rope(q, k, wq, wk, cos, sin, positions, pos0, eps)       # differentiable
 """
 
 from __future__ import annotations
@@ -279,3 +285,103 @@ def fp8_paged_attention(q: torch.Tensor, cu_seqlens: torch.Tensor, k_cache: torc
 @fp8_paged_attention.register_fake
 def _(q, cu_seqlens, k_cache, v_cache, k_scale, v_scale, block_table, lengths, scaling, groups):
     return q.new_empty(q.shape), q.new_empty(q.shape[0], q.shape[1], dtype=torch.float32)
+
+
+# ---------------------------------------------------------------- trees of drafts over the paged cache
+@torch.library.custom_op(f"{_NS}::draft_tree", mutates_args=())
+def draft_tree(parents: torch.Tensor, cu_seqlens: torch.Tensor, lengths: torch.Tensor, max_tokens: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``draft_tree``: (tree_mask, positions)."""
+    return tuple(_paged.draft_tree(parents, cu_seqlens, lengths, max_tokens))
+
+
+@draft_tree.register_fake
+def _(parents, cu_seqlens, lengths, max_tokens):
+    t = parents.shape[0]
+    return parents.new_empty(t, (max_tokens + 63) // 64, dtype=torch.int64), parents.new_empty(t, dtype=torch.int32)
+
+
+@torch.library.custom_op(f"{_NS}::fp8_paged_tree_attention", mutates_args=())
+def fp8_paged_tree_attention(q: torch.Tensor, cu_seqlens: torch.Tensor, tree_mask: torch.Tensor, k_cache: torch.Tensor,
+                             v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_table: torch.Tensor,
+                             lengths: torch.Tensor, scaling: float, groups: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _paged.fp8_paged_tree_attention(q, cu_seqlens, tree_mask, k_cache, v_cache, k_scale, v_scale, block_table, lengths, scaling,
+                                           groups, return_lse=True)
+
+
+@fp8_paged_tree_attention.register_fake
+def _(q, cu_seqlens, tree_mask, k_cache, v_cache, k_scale, v_scale, block_table, lengths, scaling, groups):
+    return q.new_empty(q.shape), q.new_empty(q.shape[0], q.shape[1], dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_NS}::verify_drafts", mutates_args=())
+def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, cu_seqlens: torch.Tensor,
+                  uniforms: torch.Tensor, draft_probs: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``verify_drafts``: (accepted, num_accepted, next_tokens)."""
+    return tuple(_paged.verify_drafts(target_probs, tokens, parents, cu_seqlens, uniforms, draft_probs))
+
+
+@verify_drafts.register_fake
+def _(target_probs, tokens, parents, cu_seqlens, uniforms, draft_probs):
+    r = cu_seqlens.shape[0] - 1
+    return (tokens.new_empty(tokens.shape[0], dtype=torch.int32), tokens.new_empty(r, dtype=torch.int32),
+            tokens.new_empty(r, dtype=torch.int64))
+
+
+@torch.library.custom_op(f"{_NS}::paged_kv_keep_path", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"))
+def paged_kv_keep_path(accepted: torch.Tensor, num_accepted: torch.Tensor, cu_seqlens: torch.Tensor, lengths: torch.Tensor,
+                       block_table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                       v_scale: torch.Tensor) -> torch.Tensor:
+    return _paged.paged_kv_keep_path(accepted, num_accepted, cu_seqlens, lengths, block_table, k_cache, v_cache, k_scale, v_scale)
+
+
+@paged_kv_keep_path.register_fake
+def _(accepted, num_accepted, cu_seqlens, lengths, block_table, k_cache, v_cache, k_scale, v_scale):
+    return lengths.new_empty(lengths.shape)
+
+
+# ---------------------------------------------------------------- norm of queries and keys with their rotation
+def _rows_like(x):
+    """As the operator lays results out: dense, heads inside or outside of tokens as in x."""
+    if x.dim() == 4 and x.stride(1) < x.stride(2):
+        z, h, s, d = x.shape
+        return x.new_empty(z, s, h, d).transpose(1, 2)
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op(f"{_NS}::qk_norm_rope", mutates_args=())
+def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
+                 sin: torch.Tensor, positions: Optional[torch.Tensor], pos0: int, eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    return flash.qk_norm_rope(query, key, q_weight, k_weight, cos, sin, positions, pos0, eps)
+
+
+@qk_norm_rope.register_fake
+def _(query, key, q_weight, k_weight, cos, sin, positions, pos0, eps):
+    return _rows_like(query), _rows_like(key)
+
+
+@torch.library.custom_op(f"{_NS}::qk_norm_rope_bwd", mutates_args=())
+def qk_norm_rope_bwd(query: torch.Tensor, key: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
+                     sin: torch.Tensor, positions: Optional[torch.Tensor], pos0: int, eps: float, grad_q: torch.Tensor,
+                     grad_k: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return flash._qk_norm_rope_backward(query, key, q_weight, k_weight, cos, sin, positions, pos0, eps, grad_q, grad_k)
+
+
+@qk_norm_rope_bwd.register_fake
+def _(query, key, q_weight, k_weight, cos, sin, positions, pos0, eps, grad_q, grad_k):
+    return _rows_like(query), _rows_like(key), q_weight.new_empty(q_weight.shape), k_weight.new_empty(k_weight.shape)
+
+
+def _norm_rope_setup(ctx, inputs, output):
+    query, key, q_weight, k_weight, cos, sin, positions, pos0, eps = inputs
+    ctx.save_for_backward(query, key, q_weight, k_weight, cos, sin, positions)
+    ctx.meta = (pos0, eps)
+
+
+def _norm_rope_backward(ctx, grad_q, grad_k):
+    query, key, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+    grad_q = torch.zeros_like(query) if grad_q is None else grad_q
+    grad_k = torch.zeros_like(key) if grad_k is None else grad_k
+    return (*qk_norm_rope_bwd(query, key, q_weight, k_weight, cos, sin, positions, *ctx.meta, grad_q, grad_k), *[None] * 5)
+
+
+qk_norm_rope.register_autograd(_norm_rope_backward, setup_context=_norm_rope_setup)

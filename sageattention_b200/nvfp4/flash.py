@@ -104,6 +104,26 @@ def rope_quant_nvfp4(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posi
     return _lib.native().rope_quant(x, cos, sin, positions, pos0)
 
 
+def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
+                 sin: torch.Tensor, positions=None, pos0: int = 0, eps: float = 1e-6):
+    """RMS norm of every head's queries and keys and their rotary embedding, in one pass (no counterpart in the reference):
+    ``rope(x / sqrt(mean(x^2) + eps) * weight)`` in fp32, rounded once to the operand's dtype.  Differentiable in operands and weights.
+
+    ``query`` ``[T, H, D]`` and ``key`` ``[T, Hk, D]`` with ``positions`` ``[T]`` (as ``paged_kv_reserve`` and ``draft_tree`` list
+    them), or ``[Z, H, S, D]`` and ``[Z, Hk, S, D]`` with ``[S]`` or ``[Z, S]``; without, token s is at ``pos0 + s``.  Views of a
+    fused projection are taken as they are.  D is 128 or 256; weights ``[D]`` in the operands' dtype or fp32; ``cos`` / ``sin``
+    ``[P, D/2]`` fp32, half-split convention, as for ``rope_quant_nvfp4``.  A position outside the tables makes its rows NaN.  Returns
+    (query, key), heads inside or outside of the tokens as in the operands.  Gradients of weights are summed in an order that
+    depends on sizes and device alone.
+    """
+    return _lib.native().qk_norm_rope(query, key, q_weight, k_weight, cos, sin, positions, pos0, eps)
+
+
+def _qk_norm_rope_backward(query, key, q_weight, k_weight, cos, sin, positions, pos0, eps, grad_q, grad_k):
+    """Gradients of query, key, q_weight and k_weight."""
+    return tuple(_lib.native().qk_norm_rope_bwd(query, key, q_weight, k_weight, cos, sin, positions, pos0, eps, grad_q, grad_k, True, True))
+
+
 def _quant_mxfp8_t(x: torch.Tensor, s_pad: int, _prescale_amax: torch.Tensor | None = None):
     """MXFP8 pack of ``x`` [B, S, D] along S: e4m3 bytes [B, D, s_pad] and e8m0 scale bytes
     [B, D, s_pad/32] (one power-of-two scale per 32 tokens); stands in for ``_pack_mxfp8_along_k`` of

@@ -15,7 +15,9 @@ Layout, shared by every function here:
   lengths            [requests] int32: tokens that a request holds
   free_blocks        [blocks] int32, free_count [1] int32: a stack of block ids, its top at free_count - 1
 
-A step is ``paged_kv_reserve`` (blocks and slots for the new tokens), then in every layer ``fp8_kv_write`` and
+A step of drafted trees is reserve, ``draft_tree``, then in every layer ``fp8_kv_write`` and ``fp8_paged_tree_attention``, then
+``verify_drafts`` of the model's probabilities, ``paged_kv_keep_path`` in all layers and ``paged_kv_trim``.  Any other
+step is ``paged_kv_reserve`` (blocks and slots for the new tokens), then in every layer ``fp8_kv_write`` and
 ``fp8_paged_decode`` or ``fp8_paged_attention``; ``paged_kv_trim`` takes tokens away again (rejected drafts, requests
 that ended).  ``FP8PagedKVCache`` holds the buffers of a model's layers and calls these.
 """
@@ -36,6 +38,21 @@ class PagedStep(NamedTuple):
     positions: torch.Tensor     # [num_slots] int32: position in the request (for the caller's rotary embedding), 0 behind
     cu_seqlens: torch.Tensor    # [requests + 1] int32
     shortage: torch.Tensor      # [1] int32: 1 where nothing was reserved
+
+
+class DraftTree(NamedTuple):
+    """What the tokens of a step's trees see of each other, and where they stand."""
+
+    tree_mask: torch.Tensor     # [T, ceil(max_tokens / 64)] int64: bit j of a token's row: token j of its request is it or above it
+    positions: torch.Tensor     # [T] int32: position in the request along the token's own path
+
+
+class VerifiedDrafts(NamedTuple):
+    """The path that a verification keeps of every request's tree, and the token that follows it."""
+
+    accepted: torch.Tensor      # [T] int32: from cu_seqlens[r] on the path's tokens as numbers within the request, 0 first, then -1
+    num_accepted: torch.Tensor  # [requests] int32
+    next_tokens: torch.Tensor   # [requests] int64, -1 for a request without tokens
 
 
 def paged_kv_reserve(new_lens, lengths, block_table, free_blocks, free_count, num_slots: int, block_size: int) -> PagedStep:
@@ -100,6 +117,61 @@ def fp8_paged_attention(query, cu_seqlens, k_cache, v_cache, k_scale, v_scale, b
     return (out, lse) if return_lse else out
 
 
+def draft_tree(parents, cu_seqlens, lengths, max_tokens: int) -> DraftTree:
+    """Tables of trees of drafted tokens, once a step for all layers.
+
+    Request r's tokens are ``cu_seqlens[r] .. cu_seqlens[r + 1]``, the last ones of its ``lengths[r]`` (reserved before the call); token i
+    hangs on the request's earlier token ``parents[t]`` (int32, counted within the request), and on the context alone where that names
+    none (-1).  ``max_tokens`` (1 to 1024): tokens of the largest tree; what lies behind them sees the context alone.  Tokens of no
+    request have no bits and position 0.
+    """
+    return DraftTree(*_lib.native().draft_tree(parents, cu_seqlens, lengths, max_tokens))
+
+
+def fp8_paged_tree_attention(query, cu_seqlens, tree_mask, k_cache, v_cache, k_scale, v_scale, block_table, lengths, scaling,
+                             num_key_value_groups=1, return_lse=False):
+    """``fp8_paged_attention`` of trees of drafted tokens: token i of a request's n sees the keys in front of them,
+    ``0 .. lengths[r] - n - 1``, and of the n those whose bit its row of ``tree_mask`` has.
+
+    ``tree_mask`` ``[T, words]`` int64, as ``draft_tree`` makes it or any other bits: bit j % 64 of word j / 64 is key
+    ``lengths[r] - n + j``; bits from n on do not count, tokens from 64 * words on are seen by none.  A token that sees no key gets
+    zeros and -inf.  A value that is NaN reaches all tokens of its request's tree (weight 0 times NaN); keys reach those that see them.
+    """
+    out, lse = _lib.native().kv8_tree_attention(query, cu_seqlens, tree_mask, k_cache, v_cache, k_scale, v_scale, block_table, lengths,
+                                                scaling, num_key_value_groups, return_lse)
+    return (out, lse) if return_lse else out
+
+
+def verify_drafts(target_probs, tokens, parents, cu_seqlens, uniforms, draft_probs=None) -> VerifiedDrafts:
+    """Which drafted tokens to keep, so that what is kept and the token behind it are distributed as the target's own draws.
+
+    ``target_probs`` ``[T, vocabulary]`` (bf16 / fp16 / fp32): row t is the target's distribution behind token t.  A request's first
+    token is given (the one that the step before ended with), the others are drafts: ``tokens`` ``[T]`` ids (int64 or int32),
+    ``parents`` as for ``draft_tree`` (a draft that hangs on the context alone is never kept; trees have 1024 tokens at most, what
+    lies behind them is never kept).  ``uniforms`` ``[T]`` float32 in [0, 1): of a draft the number that tests it, of a request's first token
+    the one that draws the next.
+
+    At a token with row p, its children in order, R = p and M = 1.  With ``draft_probs`` (``[T, vocabulary]``, row t: what the children of
+    t were drawn from independently, q) a child c is kept where ``u q(c) M < R(c)``; else R becomes max(R / M - q, 0) and M its sum.
+    Without (drafts that were chosen, such as the likeliest tokens) it is kept where ``u M < R(c)``; else M loses R(c), and R(c) becomes 0.
+    The walk goes on at the first child kept; where none is, the next token is the first v whose running sum of R exceeds w sum(R)
+    (of p, where R is empty).  Sums are in 64 bits.  Entries that are no finite number above zero count as 0, as do ids outside the vocabulary.
+    """
+    return VerifiedDrafts(*_lib.native().verify_drafts(target_probs, tokens, parents, cu_seqlens, uniforms, draft_probs))
+
+
+def paged_kv_keep_path(accepted, num_accepted, cu_seqlens, lengths, block_table, k_cache, v_cache, k_scale, v_scale) -> torch.Tensor:
+    """Move the keys and values of the path that ``verify_drafts`` kept to the front of their request's newest tokens, in place.
+
+    Of the n = ``cu_seqlens[r + 1] - cu_seqlens[r]`` last tokens of request r, token ``accepted[cu_seqlens[r] + j]`` goes to position
+    ``lengths[r] - n + j``, for j below ``num_accepted[r]`` (a path ends in front of an entry that does not ascend).  Caches of one
+    layer, ``[blocks, Hk, block_size, D]``, or of all, ``[layers, blocks, Hk, block_size, D]``, scales likewise.  Where a block receives
+    codes of a larger scale that its own cannot hold, its scale becomes the smallest power of two that can, and its older codes are
+    rounded again to it.  Returns ``keep_lens`` [requests] int32 for ``paged_kv_trim``; the tokens behind them are left as they were.
+    """
+    return _lib.native().paged_keep_path(accepted, num_accepted, cu_seqlens, lengths, block_table, k_cache, v_cache, k_scale, v_scale)
+
+
 class FP8PagedKVCache:
     """The paged 8-bit cache of a model's layers: one table for all of them, codes and scales for each.
 
@@ -147,6 +219,21 @@ class FP8PagedKVCache:
         """``fp8_paged_attention`` of ``[T, H, D]`` over one layer."""
         return fp8_paged_attention(query, cu_seqlens, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
                                    self.block_table, self.lengths, scaling, g, return_lse)
+
+    def attend_tree(self, layer: int, query: torch.Tensor, cu_seqlens: torch.Tensor, tree_mask: torch.Tensor, scaling: float, g: int,
+                    return_lse: bool = False):
+        """``fp8_paged_tree_attention`` of ``[T, H, D]`` over one layer."""
+        return fp8_paged_tree_attention(query, cu_seqlens, tree_mask, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
+                                        self.block_table, self.lengths, scaling, g, return_lse)
+
+    def tree(self, parents: torch.Tensor, cu_seqlens: torch.Tensor, max_tokens: int) -> DraftTree:
+        """``draft_tree`` of the tokens that a step has reserved."""
+        return draft_tree(parents, cu_seqlens, self.lengths, max_tokens)
+
+    def keep_path(self, accepted: torch.Tensor, num_accepted: torch.Tensor, cu_seqlens: torch.Tensor) -> None:
+        """``paged_kv_keep_path`` in all layers, then ``trim`` to what it keeps: the step's other tokens are gone."""
+        self.trim(paged_kv_keep_path(accepted, num_accepted, cu_seqlens, self.lengths, self.block_table, self.k, self.v, self.k_scale,
+                                     self.v_scale))
 
     def cache_bytes(self) -> int:
         """Bytes of codes and scales, all layers and blocks."""
