@@ -532,7 +532,7 @@ int nvfp4_paged_keep_path(const int32_t* accepted, const int32_t* num_accepted, 
  * fp32, rounded once.  (No counterpart in the reference; the rotation is that of nvfp4_rope_pack.)
  *   q [z, s, h, d], k [z, s, hk, d] of `dtype`, d 128 or 256, unit stride along d, rows 16-byte aligned; strides[3]: elements from
  *   batch entry to entry, token to token, head to head (host arrays), the results' likewise
- *   wq, wk [d] of `dtype` or fp32;  cos_tab / sin_tab [table_rows, d/2] fp32
+ *   wq, wk [d] of `dtype` or fp32, 16-byte aligned;  cos_tab / sin_tab [table_rows, d/2] fp32
  *   positions: int32, token s of entry b at positions[b * pos_batch + s], or NULL: pos0 + s.  Rows outside the tables become NaN.
  * nvfp4_qk_norm_rope_bwd: gradients of q and k in their type, and (NULL: not wanted) of the weights in theirs, from operands and
  * incoming gradients; sums in an order that depends on the sizes and the device alone.  workspace: nvfp4_qk_norm_rope_bwd_plan
@@ -550,7 +550,7 @@ int nvfp4_qk_norm_rope_bwd(const void* q, const int64_t* q_strides, const void* 
                            const float* cos_tab, const float* sin_tab, int64_t table_rows, const int32_t* positions,
                            int64_t pos_batch, int64_t pos0, float eps, void* dq, const int64_t* dq_strides, void* dk,
                            const int64_t* dk_strides, void* dwq, void* dwk, void* workspace, size_t workspace_bytes,
-                           nvfp4_stream_t stream);
+                           int* status, nvfp4_stream_t stream);
 
 /*
  * Measured pipe rates (no counterpart in the reference): launches a resident-operand micro-kernel

@@ -94,7 +94,7 @@ SIGNATURES = {
     "nvfp4_qk_norm_rope_bwd_plan": (c_int, [c_int, c_int, POINTER(c_size_t)]),
     "nvfp4_qk_norm_rope_bwd": (c_int, [c_void_p] * 8 + [c_int, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int,
                                        c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_float] + [c_void_p] * 7
-                               + [c_size_t, c_void_p]),
+                               + [c_size_t, c_void_p, c_void_p]),
     "nvfp4_rope_pack": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p,
                                 c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                 c_void_p]),

@@ -999,13 +999,13 @@ NormTables norm_tables(const Call& c, const Tensor& q, const Tensor& k, const Te
   require(cos.dim() == 2 && cos.size(1) == d / 2 && sin.sizes() == cos.sizes() && cos.scalar_type() == at::kFloat &&
               sin.scalar_type() == at::kFloat,
           "cos / sin must be fp32 [P, D/2]");
-  auto table = [](const Tensor& x) {
+  auto on_16 = [](const Tensor& x) {
     return x.is_contiguous() && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 ? x : x.clone(at::MemoryFormat::Contiguous);
   };
-  t.cos = table(cos);
-  t.sin = table(sin);
-  t.wq = wq.contiguous();
-  t.wk = wk.contiguous();
+  t.cos = on_16(cos);
+  t.sin = on_16(sin);
+  t.wq = on_16(wq);
+  t.wk = on_16(wk);
   t.rows = cos.size(0);
   t.pos_batch = 0;
   if (positions.has_value()) {
@@ -1066,7 +1066,7 @@ std::array<Tensor, 4> norm_rope_backward(const Tensor& q, const Tensor& k, const
                                 gb.keep.data_ptr(), gb.strides, t.dt, a.z, a.s, a.h, b.h, (int)a.d, t.wq.data_ptr(), t.wk.data_ptr(),
                                 t.wdt, t.cos.data_ptr<float>(), t.sin.data_ptr<float>(), t.rows, opt_ptr<int32_t>(t.positions),
                                 t.pos_batch, pos0, (float)eps, dq.data_ptr(), ra.strides, dk.data_ptr(), rb.strides, ptr(dwq), ptr(dwk),
-                                ptr(ws), bytes, c.stream),
+                                ptr(ws), bytes, c.status, c.stream),
          "nvfp4_qk_norm_rope_bwd");
   return {dq, dk, dwq, dwk};
 }

@@ -4,18 +4,26 @@
 //   g' = rot_p^-1(dy),  dw = sum over rows g' n,  dx = r (g' w - n mean(g' w n))
 //
 // What bounds it: HBM; a row is read once and written once (backward: two reads, a write).  A row is D/16 lanes, each with eight
-// elements of either half, so that a rotation stays within a lane and every access is 16 bytes wide; a warp has the rows of
-// several heads of a token, whose cos and sin it loads once for all of them.  Statistics, rotation and weight gradients are
-// fp32, rounded once to the type of the operand.
+// elements of either half, so that a rotation stays within a lane and every access is 16 bytes wide; a warp has rows of several
+// heads of a token (a step), STEPS steps together, for which it loads cos and sin once.  Statistics, rotation and weight
+// gradients are fp32, two an instruction, rounded once to the type of the operand.
+//
+// Forward: tasks of queries and keys by turns, so that what is in flight lies together, on the blocks that are resident at once: 16384
+// tokens of H 32 Hk 8 D 128 in bf16 (views of a projection, 336 MB) 57.2 us, a copy of as many bytes 57.6; all
+// queries first 61.8; more blocks than resident 58 to 64; four steps a task 63, as there are fewer warps.
+// Backward: registers hold too few rows for the loads to stay under way (104 us with four steps, 110 with two), so a warp's rows
+// come by bulk copies, the next task's while this one's are used, and a block is of queries or of keys, whose sums it keeps: 85.5
+// us, 503 MB at 0.90 of the copy rate (queries first, then keys, in every block: 90.8; three stages 96, four warps a block
+// 87.5; the forward pass by bulk copies 60.5).
 #include <limits.h>
 #include "common/abi.cuh"
 #include "common/fp4.cuh"
 #include "common/launch.cuh"
+#include "common/pairs.cuh"
+#include "common/sm100.cuh"
 
 namespace nvfp4 {
 namespace {
-
-constexpr int kThreads = 128, kWarps = kThreads / 32;
 
 // One of the two operands: queries or keys.
 struct Operand {
@@ -24,8 +32,8 @@ struct Operand {
   void* y;                                     // result, or gradient of x
   int64_t xz, xs, xh, gz, gs, gh, yz, ys, yh;  // element strides of batch entry, token, head
   const void* w;
-  int heads, log_heads;                        // rows of a warp's step: 2^log_heads heads of a token, the others are further tokens
-  uint32_t chunks;                             // steps times heads of a step cover the heads in so many tasks
+  int heads, log_heads;                        // rows of a step: 2^log_heads heads of a token, the others are further tokens
+  uint32_t chunks;                             // so many tasks have all heads of their tokens
   uint32_t tasks;
 };
 struct NormParams {
@@ -36,253 +44,389 @@ struct NormParams {
   uint32_t tokens, s;                          // z * s, s
   int w_fp32;
   float eps;
-  float* part;                                 // [blocks][2][D] sums of the weights' gradients
+  uint32_t key_blocks;                         // backward: blocks that have keys
+  int stage_bytes;                             // of a task's rows and angles
+  float* part;                                 // [blocks][D] sums of the weights' gradients, the queries' blocks first
+  int* status;
 };
 
 template <typename T, int D>
 struct Shape {
   static constexpr int kLanes = D / 16;        // of a row
-  static constexpr int kRows = 32 / kLanes;    // of a warp
-  static constexpr int kVec = 8 * sizeof(T) / 16;
+  static constexpr int kRows = 32 / kLanes;    // of a step
+  static constexpr int kRowBytes = D * sizeof(T);
 };
 
-template <typename T, int D>
-struct Row {                                   // eight elements of either half, as they lie
-  uint4 v[2][Shape<T, D>::kVec];
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) { return pair(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float low(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float high(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t minus(uint64_t v) { return v ^ 0x8000000080000000ull; }
+template <typename T> __device__ __forceinline__ uint64_t pair_of_16x2(uint32_t w);
+template <> __device__ __forceinline__ uint64_t pair_of_16x2<__nv_bfloat16>(uint32_t w) { return pair(w << 16, w & 0xFFFF0000u); }
+template <> __device__ __forceinline__ uint64_t pair_of_16x2<__half>(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return pair_of(f.x, f.y);
+}
+__device__ __forceinline__ uint4 lds_v4(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+// Eight elements as they lie, and as pairs.
+template <typename T>
+struct Eight {
+  uint4 v[8 * sizeof(T) / 16];
+  __device__ __forceinline__ void zero() {
+    for (uint4& x : v) x = make_uint4(0, 0, 0, 0);
+  }
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < Shape<T, D>::kVec; ++i) v[h][i] = reinterpret_cast<const uint4*>(p + h * (D / 2))[i];
+    for (int i = 0; i < (int)(sizeof(v) / 16); ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
   }
-  __device__ __forceinline__ void values(float (&a)[8], float (&b)[8]) const {
-    const T *pa = reinterpret_cast<const T*>(v[0]), *pb = reinterpret_cast<const T*>(v[1]);
+  __device__ __forceinline__ void load(uint32_t shared) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      a[i] = to_f32<T>(pa[i]);
-      b[i] = to_f32<T>(pb[i]);
-    }
+    for (int i = 0; i < (int)(sizeof(v) / 16); ++i) v[i] = lds_v4(shared + i * 16);
   }
-};
-template <typename T, int D>
-__device__ __forceinline__ void store_row(T* p, const float (&a)[8], const float (&b)[8]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const float(&x)[8] = h == 0 ? a : b;
+  __device__ __forceinline__ void pairs(uint64_t (&x)[4]) const {
     if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(p + h * (D / 2))[0] = make_float4(x[0], x[1], x[2], x[3]);
-      reinterpret_cast<float4*>(p + h * (D / 2))[1] = make_float4(x[4], x[5], x[6], x[7]);
+      x[0] = pair(v[0].x, v[0].y);
+      x[1] = pair(v[0].z, v[0].w);
+      x[2] = pair(v[1].x, v[1].y);
+      x[3] = pair(v[1].z, v[1].w);
     } else {
-      *reinterpret_cast<uint4*>(p + h * (D / 2)) =
-          make_uint4(pack_16x2<T>(x[0], x[1]), pack_16x2<T>(x[2], x[3]), pack_16x2<T>(x[4], x[5]), pack_16x2<T>(x[6], x[7]));
+      x[0] = pair_of_16x2<T>(v[0].x);
+      x[1] = pair_of_16x2<T>(v[0].y);
+      x[2] = pair_of_16x2<T>(v[0].z);
+      x[3] = pair_of_16x2<T>(v[0].w);
     }
+  }
+};
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const uint64_t (&x)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(low(x[0]), high(x[0]), low(x[1]), high(x[1]));
+    reinterpret_cast<float4*>(p)[1] = make_float4(low(x[2]), high(x[2]), low(x[3]), high(x[3]));
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_16x2<T>(low(x[0]), high(x[0])), pack_16x2<T>(low(x[1]), high(x[1])),
+                                              pack_16x2<T>(low(x[2]), high(x[2])), pack_16x2<T>(low(x[3]), high(x[3])));
   }
 }
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+template <typename T>
+__device__ __forceinline__ void load_weights(const NormParams& p, const void* w, int at, uint64_t (&x)[4]) {
+  if (p.w_fp32) {
+    Eight<float> e;
+    e.load(static_cast<const float*>(w) + at);
+    e.pairs(x);
+  } else {
+    Eight<T> e;
+    e.load(static_cast<const T*>(w) + at);
+    e.pairs(x);
+  }
+}
+// sum of a pair's halves over the lanes of a row
+template <int LANES>
+__device__ __forceinline__ float row_sum(uint64_t v) {
+  float x = low(v) + high(v);
+#pragma unroll
+  for (int m = 1; m < LANES; m <<= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
+  return x;
 }
 
-template <typename T, int D>
-struct Task {
-  using S = Shape<T, D>;
-  int lane, group, col;                        // column of this lane's elements of the first half
-  float wa[8], wb[8];
-
-  __device__ __forceinline__ Task() {
-    lane = threadIdx.x & 31;
-    group = lane / S::kLanes;
-    col = lane % S::kLanes * 8;
-  }
-  __device__ __forceinline__ void weights(const NormParams& p, const Operand& o) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      wa[i] = p.w_fp32 ? static_cast<const float*>(o.w)[col + i] : to_f32<T>(static_cast<const T*>(o.w)[col + i]);
-      wb[i] = p.w_fp32 ? static_cast<const float*>(o.w)[D / 2 + col + i] : to_f32<T>(static_cast<const T*>(o.w)[D / 2 + col + i]);
-    }
-  }
-  // where task `t` of an operand lies: this lane's token (or none) and its first head
-  uint32_t token, z, s;
-  int head;
-  bool there;
-  __device__ __forceinline__ void find(const NormParams& p, const Operand& o, uint32_t t, int steps) {
-    const uint32_t chunk = t % o.chunks, first = t / o.chunks * (uint32_t)(S::kRows >> o.log_heads);
-    token = first + (uint32_t)(group >> o.log_heads);
-    there = token < p.tokens;
-    z = token / p.s;
-    s = token - z * p.s;
-    head = (int)(chunk * (uint32_t)steps << o.log_heads) + (group & ((1 << o.log_heads) - 1));
-  }
-  // cos and sin of the token; outside the tables NaN
-  __device__ __forceinline__ void angles(const NormParams& p, float (&c)[8], float (&sn)[8]) const {
-    const int64_t pos = !there ? 0 : p.positions != nullptr ? (int64_t)p.positions[z * p.pos_batch + s] : p.pos0 + s;
-    if (pos >= 0 && pos < p.table_rows) {
-      load8(p.cs + pos * (D / 2) + col, c);
-      load8(p.sn + pos * (D / 2) + col, sn);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = sn[i] = __int_as_float(0x7FC00000);
-    }
-  }
-  // sum over the lanes of a row
-  __device__ __forceinline__ float row_sum(float x) const {
-#pragma unroll
-    for (int m = 1; m < S::kLanes; m <<= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
-    return x;
+// Token `token` of a call, as batch entry and token of it, and its position.
+struct Token {
+  uint32_t z, s;
+  __device__ __forceinline__ Token(const NormParams& p, uint32_t token) : z(token / p.s), s(token - token / p.s * p.s) {}
+  __device__ __forceinline__ int64_t position(const NormParams& p) const {
+    return p.positions != nullptr ? (int64_t)p.positions[z * p.pos_batch + s] : p.pos0 + s;
   }
 };
 
+constexpr int kFwdThreads = 128, kFwdWarps = kFwdThreads / 32, kFwdBlocks = 6;         // blocks of an SM
+
+// Rounds of tasks: each has the same tokens' queries, then their keys.
 template <typename T, int D, int STEPS>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(NormParams p) {
+__global__ void __launch_bounds__(kFwdThreads, kFwdBlocks) qk_norm_rope_kernel(NormParams p, uint32_t round_q, uint32_t round, uint32_t all) {
   using S = Shape<T, D>;
-  Task<T, D> at;
+  const int lane = threadIdx.x & 31, group = lane / S::kLanes, col = lane % S::kLanes * 8;
   griddep_wait();
   griddep_launch();
-  const uint32_t warps = gridDim.x * kWarps, all = p.o[0].tasks + p.o[1].tasks;
-  int had = -1;
-  for (uint32_t i = blockIdx.x * kWarps + (threadIdx.x >> 5); i < all; i += warps) {
-    const int which = i >= p.o[0].tasks;
+  const uint32_t warps = gridDim.x * kFwdWarps;
+  for (uint32_t i = blockIdx.x * kFwdWarps + (threadIdx.x >> 5); i < all; i += warps) {
+    uint32_t sub = i % round;
+    const int which = sub >= round_q;
+    if (which) sub -= round_q;
     const Operand& o = p.o[which];
-    at.find(p, o, which ? i - p.o[0].tasks : i, STEPS);
-    const T* px = static_cast<const T*>(o.x) + at.z * o.xz + at.s * o.xs + at.col;
-    T* py = static_cast<T*>(o.y) + at.z * o.yz + at.s * o.ys + at.col;
-    Row<T, D> x[STEPS];
-#pragma unroll
-    for (int k = 0; k < STEPS; ++k)
-      if (at.there && at.head + (k << o.log_heads) < o.heads) x[k].load(px + (at.head + (k << o.log_heads)) * o.xh);
-    float c[8], s[8];
-    at.angles(p, c, s);
-    if (had != which) at.weights(p, o);
-    had = which;
+    // the task's number among those of its operand
+    const uint32_t t = i / round * (which ? round - round_q : round_q) + sub;
+    const uint32_t chunk = t % o.chunks, token = t / o.chunks * (uint32_t)(S::kRows >> o.log_heads) + (uint32_t)(group >> o.log_heads);
+    const int head = (int)(chunk * STEPS << o.log_heads) + (group & ((1 << o.log_heads) - 1));
+    const int left = token < p.tokens ? (o.heads - head + (1 << o.log_heads) - 1) >> o.log_heads : 0;      // this lane's steps
+    const Token at(p, token < p.tokens ? token : 0);
+    const int64_t x_step = o.xh << o.log_heads, y_step = o.yh << o.log_heads;
+    const T* px = static_cast<const T*>(o.x) + at.z * o.xz + at.s * o.xs + head * o.xh + col;
+    T* py = static_cast<T*>(o.y) + at.z * o.yz + at.s * o.ys + head * o.yh + col;
+    Eight<T> xa[STEPS], xb[STEPS];
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) {
-      const int head = at.head + (k << o.log_heads);
-      const bool mine = at.there && head < o.heads;
-      float a[8], b[8], sum = 0.0f;
-      x[k].values(a, b);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf(a[e], a[e], fmaf(b[e], b[e], sum));
-      const float r = rsqrtf(at.row_sum(sum) * (1.0f / D) + p.eps);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float u = a[e] * r * at.wa[e], v = b[e] * r * at.wb[e];
-        a[e] = u * c[e] - v * s[e];
-        b[e] = v * c[e] + u * s[e];
+      if (k < left) {
+        xa[k].load(px + k * x_step);
+        xb[k].load(px + k * x_step + D / 2);
+      } else {
+        xa[k].zero();
+        xb[k].zero();
       }
-      if (mine) store_row<T, D>(py + head * o.yh, a, b);
+    }
+    const int64_t pos = at.position(p);
+    uint64_t ac[4], as[4], bc[4], bs[4];                   // weights times cos and sin
+    {
+      uint64_t wa[4], wb[4], c[4], s[4];
+      if (pos >= 0 && pos < p.table_rows) {
+        Eight<float> e;
+        e.load(p.cs + pos * (D / 2) + col);
+        e.pairs(c);
+        e.load(p.sn + pos * (D / 2) + col);
+        e.pairs(s);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] = s[e] = pair(0x7FC00000u, 0x7FC00000u);
+      }
+      load_weights<T>(p, o.w, col, wa);
+      load_weights<T>(p, o.w, D / 2 + col, wb);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        ac[e] = mul_pair(wa[e], c[e]);
+        as[e] = mul_pair(wa[e], s[e]);
+        bc[e] = mul_pair(wb[e], c[e]);
+        bs[e] = mul_pair(wb[e], minus(s[e]));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+      uint64_t a[4], b[4];
+      xa[k].pairs(a);
+      xb[k].pairs(b);
+      uint64_t sum = mul_pair(a[0], a[0]), sum_b = mul_pair(b[0], b[0]);
+#pragma unroll
+      for (int e = 1; e < 4; ++e) {
+        sum = fma_pair(a[e], a[e], sum);
+        sum_b = fma_pair(b[e], b[e], sum_b);
+      }
+      const float r = rsqrtf(row_sum<S::kLanes>(add_pair(sum, sum_b)) * (1.0f / D) + p.eps);
+      const uint64_t r2 = pair_of(r, r);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint64_t u = mul_pair(a[e], r2), v = mul_pair(b[e], r2);
+        a[e] = fma_pair(u, ac[e], mul_pair(v, bs[e]));
+        b[e] = fma_pair(v, bc[e], mul_pair(u, as[e]));
+      }
+      if (k < left) {
+        store8<T>(py + k * y_step, a);
+        store8<T>(py + k * y_step + D / 2, b);
+      }
     }
   }
 }
 
-// The rows of an operand after those of the other; sums of a lane's columns stay in registers over all its rows, then go, row
-// group by row group and warp by warp in that order, into the block's own place of `part`.
+constexpr int kBwdWarps = 2, kBwdBlocks = 6, kStages = 2;
+
+// Whether block b of `blocks` has keys, and its number among those of its operand: every blocks / key_blocks-th one.
+struct Share {
+  int which;
+  uint32_t rank, count;
+  __device__ __forceinline__ Share(const NormParams& p, uint32_t b, uint32_t blocks) {
+    const uint32_t before = (uint32_t)((uint64_t)b * p.key_blocks / blocks), behind = (uint32_t)((uint64_t)(b + 1) * p.key_blocks / blocks);
+    which = behind > before;
+    rank = which ? before : b - before;
+    count = which ? p.key_blocks : blocks - p.key_blocks;
+  }
+};
+
+// A stage of a warp: rows of x [tokens][heads][D], of g, cos and sin [tokens][2][D/2].  Sums of a lane's columns stay in registers
+// over all its rows, then go, row group by row group and warp by warp in that order, into the block's place of `part`.
 template <typename T, int D, int STEPS>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_bwd_kernel(NormParams p) {
+__global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks) qk_norm_rope_bwd_kernel(NormParams p) {
   using S = Shape<T, D>;
-  __shared__ float sums[kWarps][D];
-  Task<T, D> at;
+  constexpr int kOperand = S::kRows * STEPS * S::kRowBytes, kAngles = D * 4;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t bars[kBwdWarps][kStages];
+  __shared__ bool inside_s[kBwdWarps][kStages][S::kRows];  // a token's position lies within the tables
+  __shared__ float sums[kBwdWarps][D];
+  __shared__ int expired;
+  const int lane = threadIdx.x & 31, warp = warp_index(), group = lane / S::kLanes, col = lane % S::kLanes * 8;
+  if (threadIdx.x == 0) expired = 0;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&bars[warp][i], 1);
+    mbar_fence_init();
+  }
+  __syncthreads();
   griddep_wait();
   griddep_launch();
-  const uint32_t warps = gridDim.x * kWarps;
-  const int warp = threadIdx.x >> 5;
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const Operand& o = p.o[which];
-    float da[8], db[8];
+  const Share share(p, blockIdx.x, gridDim.x);
+  const Operand& o = p.o[share.which];
+  const uint32_t warps = share.count * kBwdWarps, first = share.rank * kBwdWarps + warp;
+  const int tokens = S::kRows >> o.log_heads, heads = STEPS << o.log_heads;          // of a task
+  const bool dense = o.xh == D && o.gh == D;               // a token's heads are one run
+  const uint32_t stages = smem_u32(smem) + warp * kStages * p.stage_bytes;
+  uint64_t da[4], db[4], wa[4], wb[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) da[e] = db[e] = 0.0f;
-    at.weights(p, o);
-    for (uint32_t i = blockIdx.x * kWarps + warp; i < o.tasks; i += warps) {
-      at.find(p, o, i, STEPS);
-      const T* px = static_cast<const T*>(o.x) + at.z * o.xz + at.s * o.xs + at.col;
-      const T* pg = static_cast<const T*>(o.g) + at.z * o.gz + at.s * o.gs + at.col;
-      T* py = static_cast<T*>(o.y) + at.z * o.yz + at.s * o.ys + at.col;
-      Row<T, D> x[STEPS], g[STEPS];
-#pragma unroll
-      for (int k = 0; k < STEPS; ++k) {
-        const int head = at.head + (k << o.log_heads);
-        if (at.there && head < o.heads) {
-          x[k].load(px + head * o.xh);
-          g[k].load(pg + head * o.gh);
+  for (int e = 0; e < 4; ++e) da[e] = db[e] = 0;
+  load_weights<T>(p, o.w, col, wa);
+  load_weights<T>(p, o.w, D / 2 + col, wb);
+
+  // Lane j asks for token j's rows and angles, or (heads apart) for row j of the task.  The positions of the task behind are on
+  // their way meanwhile.
+  uint32_t next = first, asked = 0;
+  const int of = dense ? lane : lane / heads;              // this lane's token of a task
+  int64_t pos = -1;
+  auto look_up = [&]() {
+    const uint32_t token = next / o.chunks * (uint32_t)tokens + of;
+    pos = next < o.tasks && of < tokens && token < p.tokens ? Token(p, token).position(p) : -1;
+  };
+  auto ask = [&]() {
+    if (next < o.tasks) {
+      const uint32_t stage = asked % kStages, token = next / o.chunks * (uint32_t)tokens + of;
+      const int head0 = next % o.chunks * heads, run = min(o.heads - head0, heads);
+      const int in = dense ? 0 : lane - of * heads;        // first of this lane's heads
+      const bool there = of < tokens && token < p.tokens, rows = there && in < run, angles = there && in == 0;
+      const bool inside = pos >= 0 && pos < p.table_rows;
+      const uint32_t bytes = dense ? run * S::kRowBytes : S::kRowBytes;
+      uint64_t* bar = &bars[warp][stage];
+      const uint32_t total = __reduce_add_sync(0xffffffffu, (rows ? 2 * bytes : 0) + (angles && inside ? kAngles : 0));
+      if (lane == 0) mbar_expect_tx(bar, total);
+      __syncwarp();
+      const uint32_t to = stages + stage * p.stage_bytes;
+      if (rows) {
+        const Token at(p, token);
+        const uint32_t row = to + (of * heads + in) * S::kRowBytes;
+        bulk_load(row, static_cast<const T*>(o.x) + at.z * o.xz + at.s * o.xs + (head0 + in) * o.xh, bytes, bar);
+        bulk_load(row + kOperand, static_cast<const T*>(o.g) + at.z * o.gz + at.s * o.gs + (head0 + in) * o.gh, bytes, bar);
+      }
+      if (angles) {
+        inside_s[warp][stage][of] = inside;
+        if (inside) {
+          bulk_load(to + 2 * kOperand + of * kAngles, p.cs + pos * (D / 2), kAngles / 2, bar);
+          bulk_load(to + 2 * kOperand + of * kAngles + kAngles / 2, p.sn + pos * (D / 2), kAngles / 2, bar);
         }
       }
-      float c[8], s[8];
-      at.angles(p, c, s);
+      next += warps;
+      ++asked;
+    }
+    look_up();
+  };
+  look_up();
+  for (int i = 0; i < kStages - 1; ++i) ask();
+  const int64_t y_step = o.yh << o.log_heads;
+  const int mine = group >> o.log_heads, sub = group & ((1 << o.log_heads) - 1);       // this lane's token and head of a step
+  uint32_t n = 0;
+  for (uint32_t i = first; i < o.tasks; i += warps, ++n) {
+    ask();
+    const uint32_t stage = n % kStages, token = i / o.chunks * (uint32_t)tokens + mine;
+    const int head = (int)(i % o.chunks) * heads + sub;
+    const int left = token < p.tokens ? (o.heads - head + (1 << o.log_heads) - 1) >> o.log_heads : 0;      // this lane's steps
+    const Token at(p, token < p.tokens ? token : 0);
+    T* py = static_cast<T*>(o.y) + at.z * o.yz + at.s * o.ys + head * o.yh + col;
+    mbar_wait_warp(&bars[warp][stage], n / kStages & 1, &expired, 80);
+    const uint32_t from = stages + stage * p.stage_bytes;
+    uint32_t row = from + (mine * heads + sub) * S::kRowBytes + col * sizeof(T);
+    uint64_t c[4], s[4];
+    if (left > 0 && inside_s[warp][stage][mine]) {
+      Eight<float> e;
+      e.load(from + 2 * kOperand + mine * kAngles + col * 4);
+      e.pairs(c);
+      e.load(from + 2 * kOperand + mine * kAngles + kAngles / 2 + col * 4);
+      e.pairs(s);
+    } else {
 #pragma unroll
-      for (int k = 0; k < STEPS; ++k) {
-        const int head = at.head + (k << o.log_heads);
-        const bool mine = at.there && head < o.heads;
-        float a[8], b[8], ga[8], gb[8], sum = 0.0f, dot = 0.0f;
-        x[k].values(a, b);
-        g[k].values(ga, gb);
+      for (int e = 0; e < 4; ++e) c[e] = s[e] = pair(0x7FC00000u, 0x7FC00000u);
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sum = fmaf(a[e], a[e], fmaf(b[e], b[e], sum));
-          const float u = ga[e] * c[e] + gb[e] * s[e], v = gb[e] * c[e] - ga[e] * s[e];
-          ga[e] = u;
-          gb[e] = v;
-          dot = fmaf(u * at.wa[e], a[e], fmaf(v * at.wb[e], b[e], dot));
+    for (int k = 0; k < STEPS; ++k, row += S::kRowBytes << o.log_heads) {
+      if (!__any_sync(0xffffffffu, k < left)) break;
+      // rows of no head are what the stage held, and go nowhere
+      Eight<T> xa, xb, ya, yb;
+      xa.load(row);
+      xb.load(row + S::kRowBytes / 2);
+      ya.load(row + kOperand);
+      yb.load(row + kOperand + S::kRowBytes / 2);
+      uint64_t a[4], b[4], ga[4], gb[4], sum = 0, sum_b = 0, dot = 0, dot_b = 0;
+      xa.pairs(a);
+      xb.pairs(b);
+      ya.pairs(ga);
+      yb.pairs(gb);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sum = fma_pair(a[e], a[e], sum);
+        sum_b = fma_pair(b[e], b[e], sum_b);
+        const uint64_t u = fma_pair(ga[e], c[e], mul_pair(gb[e], s[e])), v = fma_pair(gb[e], c[e], mul_pair(ga[e], minus(s[e])));
+        ga[e] = u;
+        gb[e] = v;
+        dot = fma_pair(mul_pair(u, wa[e]), a[e], dot);
+        dot_b = fma_pair(mul_pair(v, wb[e]), b[e], dot_b);
+      }
+      const float r = rsqrtf(row_sum<S::kLanes>(add_pair(sum, sum_b)) * (1.0f / D) + p.eps);
+      const float m = row_sum<S::kLanes>(add_pair(dot, dot_b)) * r * (1.0f / D);     // mean(g' w n)
+      const uint64_t r2 = pair_of(r, r), m2 = pair_of(-m, -m);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] = mul_pair(a[e], r2);
+        b[e] = mul_pair(b[e], r2);
+        if (k < left) {
+          da[e] = fma_pair(ga[e], a[e], da[e]);
+          db[e] = fma_pair(gb[e], b[e], db[e]);
         }
-        const float r = rsqrtf(at.row_sum(sum) * (1.0f / D) + p.eps);
-        const float m = at.row_sum(dot) * r * (1.0f / D);        // mean(g' w n)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          a[e] *= r;
-          b[e] *= r;
-          if (mine) {
-            da[e] = fmaf(ga[e], a[e], da[e]);
-            db[e] = fmaf(gb[e], b[e], db[e]);
-          }
-          a[e] = r * (ga[e] * at.wa[e] - a[e] * m);
-          b[e] = r * (gb[e] * at.wb[e] - b[e] * m);
-        }
-        if (mine) store_row<T, D>(py + head * o.yh, a, b);
+        a[e] = mul_pair(fma_pair(a[e], m2, mul_pair(ga[e], wa[e])), r2);
+        b[e] = mul_pair(fma_pair(b[e], m2, mul_pair(gb[e], wb[e])), r2);
+      }
+      if (k < left) {
+        store8<T>(py + k * y_step, a);
+        store8<T>(py + k * y_step + D / 2, b);
       }
     }
-    if (p.part == nullptr) continue;
+    __syncwarp();                                          // the stage may be filled again
+  }
+  if (p.part != nullptr) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 4; ++e) {
 #pragma unroll
       for (int m = S::kLanes; m < 32; m <<= 1) {
-        da[e] += __shfl_xor_sync(0xffffffffu, da[e], m);
-        db[e] += __shfl_xor_sync(0xffffffffu, db[e], m);
+        da[e] = add_pair(da[e], __shfl_xor_sync(0xffffffffu, da[e], m));
+        db[e] = add_pair(db[e], __shfl_xor_sync(0xffffffffu, db[e], m));
       }
-      if (at.group == 0) {
-        sums[warp][at.col + e] = da[e];
-        sums[warp][D / 2 + at.col + e] = db[e];
+      if (group == 0) {
+        *reinterpret_cast<uint64_t*>(&sums[warp][col + 2 * e]) = da[e];
+        *reinterpret_cast<uint64_t*>(&sums[warp][D / 2 + col + 2 * e]) = db[e];
       }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < D; i += kThreads) {
+    const uint32_t place = share.which ? gridDim.x - p.key_blocks + share.rank : share.rank;
+    for (int i = threadIdx.x; i < D; i += 32 * kBwdWarps) {
       float t = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) t += sums[w][i];
-      p.part[((int64_t)blockIdx.x * 2 + which) * D + i] = t;
+      for (int w = 0; w < kBwdWarps; ++w) t += sums[w][i];
+      p.part[(int64_t)place * D + i] = t;
     }
-    __syncthreads();
   }
+  __syncthreads();
+  report_error(&expired, p.status);
 }
 
 // Columns of the blocks' sums, in block order: 32 columns a block of threads, 32 threads a column.
 template <typename W>
-__global__ void __launch_bounds__(1024) qk_norm_weights_kernel(const float* part, int blocks, int d, W* dwq, W* dwk) {
+__global__ void __launch_bounds__(1024) qk_norm_weights_kernel(const float* part, int query_blocks, int blocks, int d, W* dwq, W* dwk) {
   __shared__ float sums[32][33];
   griddep_wait();
   griddep_launch();
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, which = (int)blockIdx.x * 32 >= d, col = blockIdx.x * 32 - which * d + lane;
   float t = 0.0f;
-  for (int b = slice; b < blocks; b += 32) t += part[(int64_t)b * 2 * d + col];
+  for (int b = (which ? query_blocks : 0) + slice; b < (which ? blocks : query_blocks); b += 32) t += part[(int64_t)b * d + col];
   sums[slice][lane] = t;
   __syncthreads();
   t = sums[lane][slice];
 #pragma unroll
   for (int m = 16; m > 0; m >>= 1) t += __shfl_xor_sync(0xffffffffu, t, m);
-  if (lane == 0) {
-    const int c = blockIdx.x * 32 + slice;
-    W* to = c < d ? dwq : dwk;
-    if (to != nullptr) to[c < d ? c : c - d] = from_f32<W>(t);
-  }
+  W* to = which ? dwk : dwq;
+  if (lane == 0 && to != nullptr) to[blockIdx.x * 32 - which * d + slice] = from_f32<W>(t);
 }
 
 void plan_operand(Operand& o, int64_t tokens, int rows, int steps) {
@@ -292,12 +436,6 @@ void plan_operand(Operand& o, int64_t tokens, int rows, int steps) {
   o.chunks = (uint32_t)((o.heads + per - 1) / per);
   o.tasks = (uint32_t)((tokens + at_once - 1) / at_once * o.chunks);
 }
-
-constexpr int kBlocksPerSm = 8;
-int blocks_of(const NormParams& p, int sms) {
-  const int64_t want = ((int64_t)p.o[0].tasks + p.o[1].tasks + kWarps - 1) / kWarps, most = (int64_t)kBlocksPerSm * sms;
-  return (int)(want < most ? want : most);
-}
 int sm_count() {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -306,34 +444,51 @@ int sm_count() {
 
 template <typename T, int D>
 int run_forward(NormParams p, cudaStream_t st) {
-  constexpr int kSteps = sizeof(T) == 4 ? 2 : 4;
-  for (Operand& o : p.o) plan_operand(o, p.tokens, Shape<T, D>::kRows, kSteps);
-  return launch("nvfp4_qk_norm_rope", qk_norm_rope_kernel<T, D, kSteps>, dim3((unsigned)blocks_of(p, sm_count())), kThreads, 0, st, p);
+  constexpr int kSteps = sizeof(T) == 4 ? 1 : 2, kRows = Shape<T, D>::kRows;
+  for (Operand& o : p.o) plan_operand(o, p.tokens, kRows, kSteps);
+  // a round has the tokens of the operand that takes more of them at once
+  const int64_t tq = kRows >> p.o[0].log_heads, tk = kRows >> p.o[1].log_heads, tokens = tq > tk ? tq : tk;
+  const uint32_t round_q = (uint32_t)(tokens / tq * p.o[0].chunks), round = round_q + (uint32_t)(tokens / tk * p.o[1].chunks);
+  const int64_t all = (p.tokens + tokens - 1) / tokens * round, most = (int64_t)kFwdBlocks * sm_count(), want = (all + kFwdWarps - 1) / kFwdWarps;
+  NVFP4_REQUIRE(all < (1ll << 31), "nvfp4_qk_norm_rope: too many rows");
+  return launch("nvfp4_qk_norm_rope", qk_norm_rope_kernel<T, D, kSteps>, dim3((unsigned)(want < most ? want : most)), kFwdThreads, 0, st, p,
+                round_q, round, (uint32_t)all);
 }
 template <typename T, int D>
 int run_backward(NormParams p, int w_dtype, void* dwq, void* dwk, cudaStream_t st) {
-  constexpr int kSteps = sizeof(T) == 4 ? 1 : 2;
-  for (Operand& o : p.o) plan_operand(o, p.tokens, Shape<T, D>::kRows, kSteps);
-  const int blocks = blocks_of(p, sm_count());
-  if (int rc = launch("nvfp4_qk_norm_rope_bwd", qk_norm_rope_bwd_kernel<T, D, kSteps>, dim3((unsigned)blocks), kThreads, 0, st, p)) return rc;
+  constexpr int kSteps = sizeof(T) == 4 ? 2 : 4, kRows = Shape<T, D>::kRows;
+  for (Operand& o : p.o) plan_operand(o, p.tokens, kRows, kSteps);
+  const int64_t tq = p.o[0].tasks, tk = p.o[1].tasks, most = (int64_t)kBwdBlocks * sm_count();
+  const int64_t want = (tq + kBwdWarps - 1) / kBwdWarps + (tk + kBwdWarps - 1) / kBwdWarps, blocks = want < most ? want : most;
+  const int64_t keys = blocks * tk / (tq + tk);
+  p.key_blocks = (uint32_t)(keys < 1 ? 1 : keys > blocks - 1 ? blocks - 1 : keys);
+  const int at_once = kRows >> (p.o[0].log_heads < p.o[1].log_heads ? p.o[0].log_heads : p.o[1].log_heads);
+  p.stage_bytes = 2 * kRows * kSteps * Shape<T, D>::kRowBytes + at_once * D * 4;
+  const int smem = kBwdWarps * kStages * p.stage_bytes;
+  // the largest that any call needs: the attribute is set once a kernel
+  constexpr int kMost = kBwdWarps * kStages * (2 * kRows * kSteps * Shape<T, D>::kRowBytes + kRows * D * 4);
+  const auto kern = qk_norm_rope_bwd_kernel<T, D, kSteps>;
+  if (int rc = allow_smem("nvfp4_qk_norm_rope_bwd", reinterpret_cast<const void*>(kern), kMost)) return rc;
+  if (int rc = launch("nvfp4_qk_norm_rope_bwd", kern, dim3((unsigned)blocks), 32 * kBwdWarps, smem, st, p)) return rc;
   if (p.part == nullptr) return 0;
   const dim3 grid(2 * D / 32);
+  const int query_blocks = (int)(blocks - p.key_blocks);
   switch (w_dtype) {
     case NVFP4_DT_BF16:
-      return launch("nvfp4_qk_norm_rope_bwd", qk_norm_weights_kernel<__nv_bfloat16>, grid, 1024, 0, st, p.part, blocks, D,
+      return launch("nvfp4_qk_norm_rope_bwd", qk_norm_weights_kernel<__nv_bfloat16>, grid, 1024, 0, st, p.part, query_blocks, (int)blocks, D,
                     static_cast<__nv_bfloat16*>(dwq), static_cast<__nv_bfloat16*>(dwk));
     case NVFP4_DT_FP16:
-      return launch("nvfp4_qk_norm_rope_bwd", qk_norm_weights_kernel<__half>, grid, 1024, 0, st, p.part, blocks, D,
+      return launch("nvfp4_qk_norm_rope_bwd", qk_norm_weights_kernel<__half>, grid, 1024, 0, st, p.part, query_blocks, (int)blocks, D,
                     static_cast<__half*>(dwq), static_cast<__half*>(dwk));
     default:
-      return launch("nvfp4_qk_norm_rope_bwd", qk_norm_weights_kernel<float>, grid, 1024, 0, st, p.part, blocks, D,
+      return launch("nvfp4_qk_norm_rope_bwd", qk_norm_weights_kernel<float>, grid, 1024, 0, st, p.part, query_blocks, (int)blocks, D,
                     static_cast<float*>(dwq), static_cast<float*>(dwk));
   }
 }
 
 // The arguments that both directions share, checked; 1: there is nothing to do.
-int set_up(const char* what, NormParams& p, int dtype, int64_t z, int64_t s, int64_t h, int64_t hk, int d, int w_dtype, const float* cos_tab,
-           const float* sin_tab, int64_t table_rows, const int32_t* positions, int64_t pos_batch, int64_t pos0, float eps) {
+int set_up(const char* what, NormParams& p, int dtype, int64_t z, int64_t s, int64_t h, int64_t hk, int d, const void* wq,
+           const void* wk, int w_dtype, const float* cos_tab, const float* sin_tab, int64_t table_rows, const int32_t* positions, int64_t pos_batch, int64_t pos0, float eps) {
   NVFP4_REQUIRE(d == 128 || d == 256, "%s: D must be 128 or 256", what);
   NVFP4_REQUIRE(dtype >= NVFP4_DT_BF16 && dtype <= NVFP4_DT_FP32, "%s: unknown dtype %d", what, dtype);
   NVFP4_REQUIRE(w_dtype == dtype || w_dtype == NVFP4_DT_FP32, "%s: weights must be of the operands' type or fp32", what);
@@ -341,6 +496,7 @@ int set_up(const char* what, NormParams& p, int dtype, int64_t z, int64_t s, int
   NVFP4_REQUIRE(s == 0 || z <= (1ll << 30) / s, "%s: too many tokens", what);
   NVFP4_REQUIRE(z * s * (h > hk ? h : hk) < (1ll << 31), "%s: too many rows", what);
   NVFP4_REQUIRE((((uintptr_t)cos_tab | (uintptr_t)sin_tab) & 15) == 0, "%s: cos / sin tables must be 16-byte aligned", what);
+  NVFP4_REQUIRE((((uintptr_t)wq | (uintptr_t)wk) & 15) == 0, "%s: weights must be 16-byte aligned", what);
   NVFP4_REQUIRE(eps >= 0.0f, "%s: eps must not be negative", what);
   p.cs = cos_tab;
   p.sn = sin_tab;
@@ -371,7 +527,7 @@ extern "C" int nvfp4_qk_norm_rope(const void* q, const int64_t* q_strides, const
                                   const int64_t* ok_strides, nvfp4_stream_t stream) {
   const char* what = "nvfp4_qk_norm_rope";
   NormParams p{};
-  const int rc = set_up(what, p, dtype, z, s, h, hk, d, w_dtype, cos_tab, sin_tab, table_rows, positions, pos_batch, pos0, eps);
+  const int rc = set_up(what, p, dtype, z, s, h, hk, d, wq, wk, w_dtype, cos_tab, sin_tab, table_rows, positions, pos_batch, pos0, eps);
   if (rc != 0) return rc < 0 ? rc : 0;
   NVFP4_REQUIRE(rows_aligned(q, q_strides, dtype) && rows_aligned(k, k_strides, dtype) && rows_aligned(out_q, oq_strides, dtype) &&
                     rows_aligned(out_k, ok_strides, dtype),
@@ -389,7 +545,7 @@ extern "C" int nvfp4_qk_norm_rope(const void* q, const int64_t* q_strides, const
 extern "C" int nvfp4_qk_norm_rope_bwd_plan(int d, int sm_count, size_t* workspace_bytes) {
   NVFP4_REQUIRE(d == 128 || d == 256, "nvfp4_qk_norm_rope_bwd_plan: D must be 128 or 256");
   NVFP4_REQUIRE(sm_count >= 1 && workspace_bytes != nullptr, "nvfp4_qk_norm_rope_bwd_plan: bad argument");
-  *workspace_bytes = (size_t)kBlocksPerSm * sm_count * 2 * d * sizeof(float);
+  *workspace_bytes = (size_t)kBwdBlocks * sm_count * d * sizeof(float);
   return 0;
 }
 
@@ -399,10 +555,10 @@ extern "C" int nvfp4_qk_norm_rope_bwd(const void* q, const int64_t* q_strides, c
                                       const float* cos_tab, const float* sin_tab, int64_t table_rows, const int32_t* positions,
                                       int64_t pos_batch, int64_t pos0, float eps, void* dq, const int64_t* dq_strides, void* dk,
                                       const int64_t* dk_strides, void* dwq, void* dwk, void* workspace, size_t workspace_bytes,
-                                      nvfp4_stream_t stream) {
+                                      int* status, nvfp4_stream_t stream) {
   const char* what = "nvfp4_qk_norm_rope_bwd";
   NormParams p{};
-  const int rc = set_up(what, p, dtype, z, s, h, hk, d, w_dtype, cos_tab, sin_tab, table_rows, positions, pos_batch, pos0, eps);
+  const int rc = set_up(what, p, dtype, z, s, h, hk, d, wq, wk, w_dtype, cos_tab, sin_tab, table_rows, positions, pos_batch, pos0, eps);
   if (rc < 0) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (rc == 1) {                               // no rows: the weights' gradients are sums of nothing
@@ -415,9 +571,10 @@ extern "C" int nvfp4_qk_norm_rope_bwd(const void* q, const int64_t* q_strides, c
   NVFP4_REQUIRE(rows_aligned(q, q_strides, dtype) && rows_aligned(k, k_strides, dtype) && rows_aligned(grad_q, gq_strides, dtype) &&
                     rows_aligned(grad_k, gk_strides, dtype) && rows_aligned(dq, dq_strides, dtype) && rows_aligned(dk, dk_strides, dtype),
                 "%s: rows must be 16-byte aligned", what);
+  p.status = status;
   if (dwq != nullptr || dwk != nullptr) {
     NVFP4_REQUIRE(workspace != nullptr && ((uintptr_t)workspace & 3) == 0 &&
-                      workspace_bytes >= (size_t)kBlocksPerSm * sm_count() * 2 * d * sizeof(float),
+                      workspace_bytes >= (size_t)kBwdBlocks * sm_count() * d * sizeof(float),
                   "%s: workspace too small", what);
     p.part = static_cast<float*>(workspace);
   }

@@ -43,7 +43,7 @@ def test_c_entries_refuse_what_they_cannot_do():
     assert L.nvfp4_qk_norm_rope_bwd_plan(256, 148, ctypes.byref(size)) == 0 and size.value > 0
     assert bad(L.nvfp4_qk_norm_rope_bwd_plan(64, 148, ctypes.byref(size)), b"D must")
     assert bad(L.nvfp4_qk_norm_rope_bwd(0, three, 0, three, 0, three, 0, three, 0, 1, 1, 1, 1, 128, n, n, 0, 0, 0, 1, n, 0, 0, 1e-6, 0, three,
-                                        0, three, 16, n, n, 0, n), b"workspace")
+                                        0, three, 16, n, n, 0, n, n), b"workspace")
 
 
 def test_python_entries_refuse_cpu_tensors():
