@@ -33,6 +33,7 @@ struct Operand {
   int64_t xz, xs, xh, gz, gs, gh, yz, ys, yh;  // element strides of batch entry, token, head
   const void* w;
   int heads, log_heads;                        // rows of a step: 2^log_heads heads of a token, the others are further tokens
+  int steps;                                   // of a token in a task; tasks whose tokens take fewer have more of them, one after the other
   uint32_t chunks;                             // so many tasks have all heads of their tokens
   uint32_t tasks;
 };
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdBlocks) qk_norm_rope_kernel(N
     // the task's number among those of its operand
     const uint32_t t = i / round * (which ? round - round_q : round_q) + sub;
     const uint32_t chunk = t % o.chunks, token = t / o.chunks * (uint32_t)(S::kRows >> o.log_heads) + (uint32_t)(group >> o.log_heads);
-    const int head = (int)(chunk * STEPS << o.log_heads) + (group & ((1 << o.log_heads) - 1));
+    const int head = (int)(chunk * o.steps << o.log_heads) + (group & ((1 << o.log_heads) - 1));
     const int left = token < p.tokens ? (o.heads - head + (1 << o.log_heads) - 1) >> o.log_heads : 0;      // this lane's steps
     const Token at(p, token < p.tokens ? token : 0);
     const int64_t x_step = o.xh << o.log_heads, y_step = o.yh << o.log_heads;
@@ -229,6 +230,7 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdBlocks) qk_norm_rope_kernel(N
 }
 
 constexpr int kBwdWarps = 2, kBwdBlocks = 6, kStages = 2;
+constexpr int kBwdStatic = 2048;               // shared memory of a block besides its stages, at most, with what the system reserves
 
 // Whether block b of `blocks` has keys, and its number among those of its operand: every blocks / key_blocks-th one.
 struct Share {
@@ -250,8 +252,8 @@ __global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks) qk_norm_rope_bwd_k
   constexpr int kOperand = S::kRows * STEPS * S::kRowBytes, kAngles = D * 4;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[kBwdWarps][kStages];
-  __shared__ bool inside_s[kBwdWarps][kStages][S::kRows];  // a token's position lies within the tables
-  __shared__ float sums[kBwdWarps][D];
+  __shared__ bool inside_s[kBwdWarps][kStages][S::kRows * STEPS];      // a token's position lies within the tables
+  __shared__ int64_t place_s[kBwdWarps][kStages][S::kRows * STEPS];    // where its gradient's rows are
   __shared__ int expired;
   const int lane = threadIdx.x & 31, warp = warp_index(), group = lane / S::kLanes, col = lane % S::kLanes * 8;
   if (threadIdx.x == 0) expired = 0;
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks) qk_norm_rope_bwd_k
   const Share share(p, blockIdx.x, gridDim.x);
   const Operand& o = p.o[share.which];
   const uint32_t warps = share.count * kBwdWarps, first = share.rank * kBwdWarps + warp;
-  const int tokens = S::kRows >> o.log_heads, heads = STEPS << o.log_heads;          // of a task
+  const int tokens_step = S::kRows >> o.log_heads, tokens = tokens_step * (STEPS / o.steps), heads = o.steps << o.log_heads;       // of a task
   const bool dense = o.xh == D && o.gh == D;               // a token's heads are one run
   const uint32_t stages = smem_u32(smem) + warp * kStages * p.stage_bytes;
   uint64_t da[4], db[4], wa[4], wb[4];
@@ -303,6 +305,8 @@ __global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks) qk_norm_rope_bwd_k
         bulk_load(row + kOperand, static_cast<const T*>(o.g) + at.z * o.gz + at.s * o.gs + (head0 + in) * o.gh, bytes, bar);
       }
       if (angles) {
+        const Token at(p, token);
+        place_s[warp][stage][of] = at.z * o.yz + at.s * o.ys;
         inside_s[warp][stage][of] = inside;
         if (inside) {
           bulk_load(to + 2 * kOperand + of * kAngles, p.cs + pos * (D / 2), kAngles / 2, bar);
@@ -316,33 +320,34 @@ __global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks) qk_norm_rope_bwd_k
   };
   look_up();
   for (int i = 0; i < kStages - 1; ++i) ask();
-  const int64_t y_step = o.yh << o.log_heads;
-  const int mine = group >> o.log_heads, sub = group & ((1 << o.log_heads) - 1);       // this lane's token and head of a step
+  const int shift = o.steps > 2 ? 2 : o.steps - 1;         // steps of a token's place in a task: four, two or one
+  const int sub = group & ((1 << o.log_heads) - 1);        // this lane's head of a step
   uint32_t n = 0;
   for (uint32_t i = first; i < o.tasks; i += warps, ++n) {
     ask();
-    const uint32_t stage = n % kStages, token = i / o.chunks * (uint32_t)tokens + mine;
+    const uint32_t stage = n % kStages, token0 = i / o.chunks * (uint32_t)tokens;
     const int head = (int)(i % o.chunks) * heads + sub;
-    const int left = token < p.tokens ? (o.heads - head + (1 << o.log_heads) - 1) >> o.log_heads : 0;      // this lane's steps
-    const Token at(p, token < p.tokens ? token : 0);
-    T* py = static_cast<T*>(o.y) + at.z * o.yz + at.s * o.ys + head * o.yh + col;
     mbar_wait_warp(&bars[warp][stage], n / kStages & 1, &expired, 80);
     const uint32_t from = stages + stage * p.stage_bytes;
-    uint32_t row = from + (mine * heads + sub) * S::kRowBytes + col * sizeof(T);
-    uint64_t c[4], s[4];
-    if (left > 0 && inside_s[warp][stage][mine]) {
-      Eight<float> e;
-      e.load(from + 2 * kOperand + mine * kAngles + col * 4);
-      e.pairs(c);
-      e.load(from + 2 * kOperand + mine * kAngles + kAngles / 2 + col * 4);
-      e.pairs(s);
-    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) c[e] = s[e] = pair(0x7FC00000u, 0x7FC00000u);
-    }
+    for (int k = 0; k < STEPS; ++k) {                      // straight on: steps of several tokens overlap
+      const int in = (k >> shift) * tokens_step + (group >> o.log_heads), step = k & ((1 << shift) - 1);      // token of the task, its step
+      const int at_head = head + (step << o.log_heads);
+      const bool mine = token0 + in < p.tokens && in < tokens && step < o.steps && at_head < o.heads;
+      if (!__any_sync(0xffffffffu, mine)) break;
+      const uint32_t row = from + (in * heads + sub + (step << o.log_heads)) * S::kRowBytes + col * sizeof(T);
+      const uint32_t angles = from + 2 * kOperand + in * kAngles + col * 4;
+      T* py = static_cast<T*>(o.y) + place_s[warp][stage][in] + at_head * o.yh + col;
+      uint64_t c[4], s[4];
+      Eight<float> cos, sin;
+      cos.load(angles);
+      sin.load(angles + kAngles / 2);
+      cos.pairs(c);
+      sin.pairs(s);
+      if (!inside_s[warp][stage][in]) {
 #pragma unroll
-    for (int k = 0; k < STEPS; ++k, row += S::kRowBytes << o.log_heads) {
-      if (!__any_sync(0xffffffffu, k < left)) break;
+        for (int e = 0; e < 4; ++e) c[e] = s[e] = pair(0x7FC00000u, 0x7FC00000u);
+      }
       // rows of no head are what the stage held, and go nowhere
       Eight<T> xa, xb, ya, yb;
       xa.load(row);
@@ -371,21 +376,23 @@ __global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks) qk_norm_rope_bwd_k
       for (int e = 0; e < 4; ++e) {
         a[e] = mul_pair(a[e], r2);
         b[e] = mul_pair(b[e], r2);
-        if (k < left) {
+        if (mine) {
           da[e] = fma_pair(ga[e], a[e], da[e]);
           db[e] = fma_pair(gb[e], b[e], db[e]);
         }
         a[e] = mul_pair(fma_pair(a[e], m2, mul_pair(ga[e], wa[e])), r2);
         b[e] = mul_pair(fma_pair(b[e], m2, mul_pair(gb[e], wb[e])), r2);
       }
-      if (k < left) {
-        store8<T>(py + k * y_step, a);
-        store8<T>(py + k * y_step + D / 2, b);
+      if (mine) {
+        store8<T>(py, a);
+        store8<T>(py + D / 2, b);
       }
     }
     __syncwarp();                                          // the stage may be filled again
   }
   if (p.part != nullptr) {
+    float* const sums = reinterpret_cast<float*>(smem) + warp * D;       // where the stages were: all of them have been read
+    __syncthreads();
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
 #pragma unroll
@@ -394,8 +401,8 @@ __global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks) qk_norm_rope_bwd_k
         db[e] = add_pair(db[e], __shfl_xor_sync(0xffffffffu, db[e], m));
       }
       if (group == 0) {
-        *reinterpret_cast<uint64_t*>(&sums[warp][col + 2 * e]) = da[e];
-        *reinterpret_cast<uint64_t*>(&sums[warp][D / 2 + col + 2 * e]) = db[e];
+        *reinterpret_cast<uint64_t*>(&sums[col + 2 * e]) = da[e];
+        *reinterpret_cast<uint64_t*>(&sums[D / 2 + col + 2 * e]) = db[e];
       }
     }
     __syncthreads();
@@ -403,7 +410,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, kBwdBlocks) qk_norm_rope_bwd_k
     for (int i = threadIdx.x; i < D; i += 32 * kBwdWarps) {
       float t = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kBwdWarps; ++w) t += sums[w][i];
+      for (int w = 0; w < kBwdWarps; ++w) t += reinterpret_cast<const float*>(smem)[w * D + i];
       p.part[(int64_t)place * D + i] = t;
     }
   }
@@ -429,12 +436,16 @@ __global__ void __launch_bounds__(1024) qk_norm_weights_kernel(const float* part
   if (lane == 0 && to != nullptr) to[blockIdx.x * 32 - which * d + slice] = from_f32<W>(t);
 }
 
-void plan_operand(Operand& o, int64_t tokens, int rows, int steps) {
+// Tasks of at most `steps` steps, of further tokens too where one takes fewer (`fill`).  Returns the tokens of a task.
+int plan_operand(Operand& o, int64_t tokens, int rows, int steps, bool fill) {
   o.log_heads = 0;
   while ((2 << o.log_heads) <= rows && (2 << o.log_heads) <= o.heads) ++o.log_heads;
-  const int64_t per = (int64_t)steps << o.log_heads, at_once = rows >> o.log_heads;
-  o.chunks = (uint32_t)((o.heads + per - 1) / per);
+  const int want = (o.heads + (1 << o.log_heads) - 1) >> o.log_heads;
+  o.steps = want < steps ? want : steps;
+  const int at_once = (rows >> o.log_heads) * (fill ? steps / o.steps : 1);
+  o.chunks = (uint32_t)((want + o.steps - 1) / o.steps);
   o.tasks = (uint32_t)((tokens + at_once - 1) / at_once * o.chunks);
+  return at_once;
 }
 int sm_count() {
   int dev = 0, sms = 148;
@@ -445,9 +456,8 @@ int sm_count() {
 template <typename T, int D>
 int run_forward(NormParams p, cudaStream_t st) {
   constexpr int kSteps = sizeof(T) == 4 ? 1 : 2, kRows = Shape<T, D>::kRows;
-  for (Operand& o : p.o) plan_operand(o, p.tokens, kRows, kSteps);
-  // a round has the tokens of the operand that takes more of them at once
-  const int64_t tq = kRows >> p.o[0].log_heads, tk = kRows >> p.o[1].log_heads, tokens = tq > tk ? tq : tk;
+  const int64_t tq = plan_operand(p.o[0], p.tokens, kRows, kSteps, false), tk = plan_operand(p.o[1], p.tokens, kRows, kSteps, false);
+  const int64_t tokens = tq > tk ? tq : tk;                // a round has those of the operand that takes more of them at once
   const uint32_t round_q = (uint32_t)(tokens / tq * p.o[0].chunks), round = round_q + (uint32_t)(tokens / tk * p.o[1].chunks);
   const int64_t all = (p.tokens + tokens - 1) / tokens * round, most = (int64_t)kFwdBlocks * sm_count(), want = (all + kFwdWarps - 1) / kFwdWarps;
   NVFP4_REQUIRE(all < (1ll << 31), "nvfp4_qk_norm_rope: too many rows");
@@ -457,16 +467,15 @@ int run_forward(NormParams p, cudaStream_t st) {
 template <typename T, int D>
 int run_backward(NormParams p, int w_dtype, void* dwq, void* dwk, cudaStream_t st) {
   constexpr int kSteps = sizeof(T) == 4 ? 2 : 4, kRows = Shape<T, D>::kRows;
-  for (Operand& o : p.o) plan_operand(o, p.tokens, kRows, kSteps);
-  const int64_t tq = p.o[0].tasks, tk = p.o[1].tasks, most = (int64_t)kBwdBlocks * sm_count();
+  const int of_q = plan_operand(p.o[0], p.tokens, kRows, kSteps, true), of_k = plan_operand(p.o[1], p.tokens, kRows, kSteps, true);
+  p.stage_bytes = 2 * kRows * kSteps * Shape<T, D>::kRowBytes + (of_q > of_k ? of_q : of_k) * D * 4;
+  const int smem = kBwdWarps * kStages * p.stage_bytes, fit = kSmemPerSm / (smem + kBwdStatic);
+  const int64_t tq = p.o[0].tasks, tk = p.o[1].tasks, most = (int64_t)(fit < kBwdBlocks ? fit : kBwdBlocks) * sm_count();
   const int64_t want = (tq + kBwdWarps - 1) / kBwdWarps + (tk + kBwdWarps - 1) / kBwdWarps, blocks = want < most ? want : most;
   const int64_t keys = blocks * tk / (tq + tk);
   p.key_blocks = (uint32_t)(keys < 1 ? 1 : keys > blocks - 1 ? blocks - 1 : keys);
-  const int at_once = kRows >> (p.o[0].log_heads < p.o[1].log_heads ? p.o[0].log_heads : p.o[1].log_heads);
-  p.stage_bytes = 2 * kRows * kSteps * Shape<T, D>::kRowBytes + at_once * D * 4;
-  const int smem = kBwdWarps * kStages * p.stage_bytes;
   // the largest that any call needs: the attribute is set once a kernel
-  constexpr int kMost = kBwdWarps * kStages * (2 * kRows * kSteps * Shape<T, D>::kRowBytes + kRows * D * 4);
+  constexpr int kMost = kBwdWarps * kStages * (2 * kRows * kSteps * Shape<T, D>::kRowBytes + kRows * kSteps * D * 4);
   const auto kern = qk_norm_rope_bwd_kernel<T, D, kSteps>;
   if (int rc = allow_smem("nvfp4_qk_norm_rope_bwd", reinterpret_cast<const void*>(kern), kMost)) return rc;
   if (int rc = launch("nvfp4_qk_norm_rope_bwd", kern, dim3((unsigned)blocks), 32 * kBwdWarps, smem, st, p)) return rc;
@@ -532,8 +541,8 @@ extern "C" int nvfp4_qk_norm_rope(const void* q, const int64_t* q_strides, const
   NVFP4_REQUIRE(rows_aligned(q, q_strides, dtype) && rows_aligned(k, k_strides, dtype) && rows_aligned(out_q, oq_strides, dtype) &&
                     rows_aligned(out_k, ok_strides, dtype),
                 "%s: rows must be 16-byte aligned", what);
-  p.o[0] = {q, nullptr, out_q, q_strides[0], q_strides[1], q_strides[2], 0, 0, 0, oq_strides[0], oq_strides[1], oq_strides[2], wq, (int)h, 0, 0, 0};
-  p.o[1] = {k, nullptr, out_k, k_strides[0], k_strides[1], k_strides[2], 0, 0, 0, ok_strides[0], ok_strides[1], ok_strides[2], wk, (int)hk, 0, 0, 0};
+  p.o[0] = {q, nullptr, out_q, q_strides[0], q_strides[1], q_strides[2], 0, 0, 0, oq_strides[0], oq_strides[1], oq_strides[2], wq, (int)h, 0, 0, 0, 0};
+  p.o[1] = {k, nullptr, out_k, k_strides[0], k_strides[1], k_strides[2], 0, 0, 0, ok_strides[0], ok_strides[1], ok_strides[2], wk, (int)hk, 0, 0, 0, 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case NVFP4_DT_BF16: return d == 128 ? run_forward<__nv_bfloat16, 128>(p, st) : run_forward<__nv_bfloat16, 256>(p, st);
@@ -579,9 +588,9 @@ extern "C" int nvfp4_qk_norm_rope_bwd(const void* q, const int64_t* q_strides, c
     p.part = static_cast<float*>(workspace);
   }
   p.o[0] = {q, grad_q, dq, q_strides[0], q_strides[1], q_strides[2], gq_strides[0], gq_strides[1], gq_strides[2], dq_strides[0],
-            dq_strides[1], dq_strides[2], wq, (int)h, 0, 0, 0};
+            dq_strides[1], dq_strides[2], wq, (int)h, 0, 0, 0, 0};
   p.o[1] = {k, grad_k, dk, k_strides[0], k_strides[1], k_strides[2], gk_strides[0], gk_strides[1], gk_strides[2], dk_strides[0],
-            dk_strides[1], dk_strides[2], wk, (int)hk, 0, 0, 0};
+            dk_strides[1], dk_strides[2], wk, (int)hk, 0, 0, 0, 0};
   switch (dtype) {
     case NVFP4_DT_BF16:
       return d == 128 ? run_backward<__nv_bfloat16, 128>(p, w_dtype, dwq, dwk, st) : run_backward<__nv_bfloat16, 256>(p, w_dtype, dwq, dwk, st);
