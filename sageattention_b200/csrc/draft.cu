@@ -12,6 +12,7 @@ namespace nvfp4 {
 namespace {
 
 constexpr int kTree = 1024;                    // nodes of a tree
+constexpr int kPasses = 1 << 30;               // flag of a node that passes its test
 
 // Tokens [t0, t0 + n) of request r, whatever cu holds within the call's tokens.
 struct Span {
@@ -100,7 +101,9 @@ struct VerifyParams {
   int64_t* next;
 };
 
-constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
+// Threads of a block, two of which share an SM: with draft rows 128 registers a thread, in 64 of which (512 threads) they do not
+// fit; without them more warps.  Chains of 32000 tokens 8.5 (13.4) us, the likeliest of 131072 tokens 18.6 (21.2).
+__host__ __device__ constexpr int verify_threads(bool drawn) { return drawn ? 256 : 512; }
 
 __device__ __forceinline__ double ld_cluster_f64(uint32_t saddr, uint32_t rank) {
   uint32_t a;
@@ -117,6 +120,18 @@ __device__ __forceinline__ float mass_of(T v) {
   return f > 0.0f && f < INFINITY ? f : 0.0f;
 }
 
+// 16 bytes, or zeros without a load: predicated, so that a lane's loads stay together
+__device__ __forceinline__ uint4 load_or_zero(const void* src, bool there) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}\n"
+      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+      : "l"(src), "r"((int)there)
+      : "memory");
+  return v;
+}
+
 // The walk down a request's tree.  At node x with the target's row p and children c_1, c_2, ... in order, R_0 = p, M_0 = 1:
 //   with draft rows q:  c_j passes where u q(c_j) M < R(c_j); else R <- max(R / M - q, 0), M <- sum R
 //   without:            c_j passes where u M < R(c_j); else M <- M - R(c_j), R(c_j) <- 0
@@ -124,21 +139,28 @@ __device__ __forceinline__ float mass_of(T v) {
 // w sum R, w the number of node 0.  All of it in 64 bits: a vocabulary's sums in 32 would move the draw by whole tokens.
 //
 // A cluster a request; every block walks for itself over values that all have fetched (a node's p and q at its token, one
-// trip for all nodes), and where a sum over a row is needed the blocks of the cluster share it: a warp has a piece of the
-// row.  What bounds it: the rows (one a rejection, one for the draw) where there are many requests, else the trips to memory and between
-// the blocks, one behind the other.
+// trip for all nodes).  Without draft rows all nodes are tested at once, as a test depends on a node's siblings alone, and the
+// walk follows the first that pass; with them a rejection needs the sum of a row.  The blocks of the cluster share a row, a
+// warp a piece of it.  What bounds it: the rows (one a rejection, one for the draw) where there are many requests, else the trips
+// to memory and between the blocks, one behind the other.
 template <typename T, bool kDrawn>
-__global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(VerifyParams p) {
+__global__ void __launch_bounds__(verify_threads(kDrawn), 2) verify_drafts_kernel(VerifyParams p) {
+  constexpr int kThreads = verify_threads(kDrawn), kWarps = kThreads / 32;
   constexpr int kPer = 16 / sizeof(T);
   constexpr int kStep = 32 * kPer;             // elements of a warp's load
-  __shared__ int16_t up_s[kTree], path_s[kTree], rejected_s[kTree];
+  constexpr int kAhead = 4;                    // loads of a lane under way together, of the draft's row as many again
+  __shared__ int16_t up_s[kTree], path_s[kTree];
   __shared__ int32_t id_s[kTree];
-  __shared__ float px_s[kTree], qx_s[kTree], u_s[kTree];
-  __shared__ double mass_s[kTree];             // of what is left behind j rejections, and one over it
-  __shared__ double block_s[2], warp_s[kVerifyWarps];
+  __shared__ float px_s[kTree], u_s[kTree];
+  __shared__ float qx_s[kDrawn ? kTree : 1];
+  // drawn: first child of a node, next one of its parent; else first child that passes, rejected ones of the path's last node
+  __shared__ int first_s[kTree];
+  __shared__ int16_t next_s[kTree];
+  __shared__ double over_s[kDrawn ? kTree : 1];            // one over what was left behind j rejections
+  __shared__ double block_s[2], warp_s[kWarps];
   __shared__ int node_s, k_s, len_s;
   __shared__ bool done_s;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = warp_index();
   const int rank = blockIdx.z, ranks = gridDim.z, r = blockIdx.x;
   griddep_wait();
   griddep_launch();
@@ -146,271 +168,337 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(VerifyPar
   const int n = (int)min(span.n, (int64_t)kTree);
   const T* const target = static_cast<const T*>(p.p);
   const T* const draft = static_cast<const T*>(p.q);
-  for (int i = tid; i < n; i += kVerifyThreads) {
+  for (int i = tid; i < n; i += kThreads) {
     const int64_t t = span.t0 + i;
     const int a = p.parents[t];
     const int64_t id = p.ids64 ? static_cast<const int64_t*>(p.ids)[t] : (int64_t) static_cast<const int32_t*>(p.ids)[t];
     const bool child = a >= 0 && a < i, known = id >= 0 && id < p.vocab;
-    up_s[i] = (int16_t)(child ? a : -1);
-    id_s[i] = known ? (int32_t)id : -1;
-    u_s[i] = p.u[t];
     float x = 0.0f, y = 0.0f;
     if (child && known) {
       x = mass_of<T>(target[(span.t0 + a) * p.sp + id]);
       if (kDrawn) y = mass_of<T>(draft[(span.t0 + a) * p.sq + id]);
     }
+    up_s[i] = (int16_t)(child ? a : -1);
+    id_s[i] = known ? (int32_t)id : -1;
+    u_s[i] = p.u[t];
     px_s[i] = x;
     if (kDrawn) qx_s[i] = y;
+    first_s[i] = kTree;
+    next_s[i] = kTree;
+  }
+  if (tid == 0) {
+    k_s = 0;
+    path_s[0] = 0;
+  }
+  __syncthreads();
+  if (!kDrawn) {                               // a token again among the siblings is worth nothing
+    uint32_t again = 0;                        // of this thread's nodes, a bit each
+    for (int i = tid, bit = 0; i < n; i += kThreads, ++bit)
+      if (up_s[i] >= 0)
+#pragma unroll 4
+        for (int j = up_s[i] + 1; j < i; ++j)
+          if (up_s[j] == up_s[i] && id_s[j] == id_s[i]) again |= 1u << bit;
+    __syncthreads();
+    for (int i = tid, bit = 0; i < n; i += kThreads, ++bit)
+      if (again >> bit & 1) px_s[i] = 0.0f;
+    __syncthreads();
+  }
+  for (int i = tid; i < n; i += kThreads) {
+    const int up = up_s[i];
+    if (up < 0) continue;
+    int before = -1;
+    double mass = 1.0;
+#pragma unroll 4
+    for (int j = up + 1; j < i; ++j)
+      if (up_s[j] == up) {
+        before = j;
+        if (!kDrawn) mass = fmax(mass - (double)px_s[j], 0.0);
+      }
+    if (kDrawn) {
+      // the first child of a node that has lost none yet: at once known, and marked where it passes
+      if (before < 0) first_s[up] = (double)u_s[i] * (double)qx_s[i] < (double)px_s[i] ? i | kPasses : i;
+      else next_s[before] = (int16_t)i;
+    } else if ((double)u_s[i] * mass < (double)px_s[i]) {
+      atomicMin(&first_s[up], i);
+    }
   }
   __syncthreads();
 
   // what is left of a probability behind k rejections
-  auto left_of = [&](double x, double q, int k) {
-    for (int j = 0; j < k; ++j) x = fmax(x * mass_s[j] - q, 0.0);
-    return x;
-  };
-  // ---- warp 0: on from node_s, behind child `from`, until a row's sum is wanted or no child is left
-  int from = 1, len = 1, node = 0, k = 0;
-  double mass = 1.0;                           // of what is left
-  auto advance = [&]() -> bool {               // true: done
-    for (;;) {
-      int child = -1;
-      for (int i0 = from & ~31; i0 < n && child < 0; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t m = __ballot_sync(0xffffffffu, i >= from && i < n && up_s[i] == node);
-        if (m) child = i0 + __ffs(m) - 1;
-      }
-      if (child < 0) return true;
-      from = child + 1;
-      bool passes;
-      if (kDrawn) {
-        passes = (double)u_s[child] * (double)qx_s[child] * mass < left_of(px_s[child], qx_s[child], k);
-      } else {
-        bool again = false;
-        for (int j = lane; j < k; j += 32) again |= id_s[rejected_s[j]] == id_s[child];
-        again = __any_sync(0xffffffffu, again);
-        const double x = again ? 0.0 : (double)px_s[child];
-        passes = (double)u_s[child] * mass < x;
-        if (!passes) mass = fmax(mass - x, 0.0);
-      }
-      if (passes) {
-        if (lane == 0) path_s[len] = (int16_t)child;
-        ++len;
-        node = child;
-        k = 0;
-        mass = 1.0;
-      } else {
-        if (!kDrawn && lane == 0) rejected_s[k] = (int16_t)child;
-        __syncwarp();
-        ++k;
-        if (kDrawn) return false;
-      }
+  auto left_of = [&](float x, float q, int k) -> double {
+    if (k == 0) return x;
+    double r = x > q ? (double)x - (double)q : 0.0;        // mass 0 is 1
+    for (int j = 1; j < k; ++j) {
+      r = r * over_s[j] - q;
+      if (!(r > 0.0)) r = 0.0;
     }
+    return r;
   };
 
-  // ---- elements of the row of `node`: warp's piece [begin, end) of places, a place being an element behind the 16 bytes that
-  // the row begins in
+  // ---- a row: places are elements behind the 16 bytes that it begins in
   const T *row = nullptr, *row_q = nullptr;
-  int head = 0;
-  bool same = false;
-  auto open_row = [&](int node) {
+  int head = 0, end_row = 0;                   // its places
+  bool same = true;                            // the draft's row begins as the target's does, else it is read one by one
+  int struck = -1;                             // chosen: place of this lane's rejected token, of the first 32
+  auto open_row = [&](int node, int k) {
     row = target + (span.t0 + node) * p.sp;
     head = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    end_row = head + p.vocab;
     row -= head;                               // at 16 bytes; places in front of `head` are never read
     if (kDrawn) {
       const T* q = draft + (span.t0 + node) * p.sq;
       same = (int)((reinterpret_cast<uintptr_t>(q) & 15) / sizeof(T)) == head;
       row_q = q - head;
-    }
-  };
-  auto load = [&](const T* base, int at, bool wide, T (&x)[kPer]) {
-    if (wide && at >= head && at + kPer <= head + p.vocab) {
-      *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(base + at);
     } else {
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) x[e] = at + e >= head && at + e < head + p.vocab ? base[at + e] : from_f32<T>(0.0f);
+      struck = lane < k && id_s[next_s[lane]] >= 0 ? id_s[next_s[lane]] + head : -1;
     }
   };
-  // what is left of elements at .. at + kPer of the row, k rejections behind it; hit: some rejected token may be among them
-  auto rest = [&](int at, int k, bool hit, double (&x)[kPer]) {
-    alignas(16) T a[kPer], b[kPer];
-    load(row, at, true, a);
-    if (kDrawn && k > 0) load(row_q, at, same, b);
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      x[e] = mass_of<T>(a[e]);
-      if (kDrawn && k > 0) x[e] = left_of(x[e], mass_of<T>(b[e]), k);
+  // Chosen: whether rejected tokens lie in places begin .. end; all lanes of the warp.
+  auto touched = [&](int begin, int end, int k) {
+    bool hit = struck >= begin && struck < end;
+    for (int j = 32 + lane; j < k; j += 32) {
+      const int id = id_s[next_s[j]];
+      hit |= id >= 0 && id + head >= begin && id + head < end;
     }
-    if (!kDrawn && hit) {
-      for (int j = 0; j < k; ++j) {
-        const int id = id_s[rejected_s[j]];
-#pragma unroll
-        for (int e = 0; e < kPer; ++e)
-          if (id >= 0 && id + head == at + e) x[e] = 0.0;
-      }
-    }
-  };
-  auto touched = [&](int begin, int end, int k) {          // by a rejected token; all lanes of the warp
-    bool hit = false;
-    if (!kDrawn)
-      for (int j = lane; j < k; j += 32) {
-        const int id = id_s[rejected_s[j]];
-        hit |= id >= 0 && id + head >= begin && id + head < end;
-      }
     return __any_sync(0xffffffffu, hit);
   };
-  // sum of places begin .. end by a warp, in all its lanes
-  auto piece_sum = [&](int begin, int end, int k) {
-    const bool hit = touched(begin, end, k);
-    double sum = 0.0;
-    constexpr int kAhead = 4;
+  // what is left of a lane's elements x (and y) of the step at `base` behind k rejections; all lanes of the warp
+  auto rest = [&](int base, const uint4& raw, const uint4& raw_q, int k, bool hit, double (&left)[kPer]) {
+    const T *x = reinterpret_cast<const T*>(&raw), *y = reinterpret_cast<const T*>(&raw_q);
+    if (!kDrawn || k == 0) {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) left[e] = mass_of<T>(x[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const float a = mass_of<T>(x[e]), b = mass_of<T>(y[e]);
+        left[e] = a > b ? (double)a - (double)b : 0.0;
+      }
 #pragma unroll 1
-    for (int at = begin + lane * kPer; at < end; at += kAhead * kStep) {
+      for (int j = 1; j < k; ++j) {
+        const double over = over_s[j];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const double t = left[e] * over - (double)mass_of<T>(y[e]);
+          left[e] = t > 0.0 ? t : 0.0;
+        }
+      }
+    }
+    if (!kDrawn && hit) {
+      const int at = base + lane * kPer;
+      auto strike = [&](int place) {
+        for (uint32_t m = __ballot_sync(0xffffffffu, place >= base && place < base + kStep); m != 0; m &= m - 1) {
+          const int one = __shfl_sync(0xffffffffu, place, __ffs(m) - 1) - at;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e)
+            if (one == e) left[e] = 0.0;
+        }
+      };
+      strike(struck);
+#pragma unroll 1
+      for (int j = 32 + lane; j - lane < k; j += 32) strike(j < k && id_s[next_s[j]] >= 0 ? id_s[next_s[j]] + head : -1);
+    }
+  };
+  // a lane's elements at place `at` .. (of the row, or of the draft's in its place) where 16 bytes are not all the row's: one by one
+  auto edge = [&](const T* from, int at, uint4& x) {
+    T* one = reinterpret_cast<T*>(&x);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) one[e] = at + e >= head && at + e < end_row ? from[at + e] : from_f32<T>(0.0f);
+  };
+  // sum of places begin .. end by a warp, in all its lanes; begin is a multiple of kStep
+  auto piece_sum = [&](int begin, int end, int k) {
+    const bool both = kDrawn && k > 0, hit = !kDrawn && touched(begin, end, k);
+    double sum = 0.0;
+#pragma unroll 1
+    for (int base = begin; base < end; base += kAhead * kStep) {
+      uint4 x[kAhead], y[kAhead];
+      const int at = base + lane * kPer;
+      auto full = [&](int at) { return at >= head && at + kPer <= end_row; };
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) x[a] = load_or_zero(row + at + a * kStep, full(at + a * kStep) && at + a * kStep < end);
+      if (both) {
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) y[a] = load_or_zero(row_q + at + a * kStep, same && full(at + a * kStep) && at + a * kStep < end);
+      }
+      const bool inside = base >= head && base + kAhead * kStep <= end_row;
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
-        if (at + a * kStep >= end) break;
-        double x[kPer];
-        rest(at + a * kStep, k, hit, x);
+        const int to = at + a * kStep;
+        if (base + a * kStep >= end) break;
+        if (!inside && !full(to)) edge(row, to, x[a]);
+        if (both && (!same || (!inside && !full(to)))) edge(row_q, to, y[a]);
+        double left[kPer];
+        rest(base + a * kStep, x[a], y[a], k, hit, left);
 #pragma unroll
         for (int w = 1; w < kPer; w *= 2)
 #pragma unroll
-          for (int e = 0; e < kPer; e += 2 * w) x[e] += x[e + w];
-        sum += x[0];
+          for (int e = 0; e < kPer; e += 2 * w) left[e] += left[e + w];
+        sum += left[0];
       }
     }
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
     return sum;
   };
-  const int pieces = kVerifyWarps * ranks;
-  auto piece = [&]() { return ((head + p.vocab + pieces - 1) / pieces + kStep - 1) / kStep * kStep; };
-  // first of `n` pieces whose running sum exceeds `at`, or the last with any; `at` becomes relative to it
-  auto pick = [](const auto& of, int n, double& at) {
-    double before = 0.0, start = 0.0;
-    int last = -1;
-    for (int i = 0; i < n; ++i) {
-      const double x = of(i);
-      if (x > 0.0) {
-        last = i;
-        start = before;
-        if (before + x > at) break;
-      }
-      before += x;
+  // sums over the lanes up to this one
+  auto running = [&](double x) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
     }
-    at -= start;
-    return last;
+    return x;
   };
+  // first of the lanes' values whose running sum exceeds `at`, or the last above zero, or -1; `at` becomes relative to it
+  auto pick = [&](double x, double& at) -> int {
+    const double upto = running(x);
+    const uint32_t some = __ballot_sync(0xffffffffu, x > 0.0), above = __ballot_sync(0xffffffffu, x > 0.0 && upto > at);
+    const int who = above ? __ffs(above) - 1 : 31 - __clz(some);
+    if (who >= 0) at -= __shfl_sync(0xffffffffu, upto - x, who);
+    return who;
+  };
+  auto of_warps = [&]() { return lane < kWarps ? warp_s[lane] : 0.0; };
+  double of_blocks = 0.0;                      // this lane's block of the cluster: its sum of the row
   int turn = 0;
-  auto row_sum = [&](int node, int k) {        // all threads of the cluster; the same in all
-    open_row(node);
-    const int size = piece(), begin = (rank * kVerifyWarps + warp) * size;
-    const double mine = piece_sum(begin, min(begin + size, head + p.vocab), k);
-    if (lane == 0) warp_s[warp] = mine;
-    __syncthreads();
-    if (tid == 0) {
-      double t = 0.0;
-      for (int w = 0; w < kVerifyWarps; ++w) t += warp_s[w];
-      block_s[turn] = t;
-    }
-    if (ranks > 1) cluster_sync_all();
-    else __syncthreads();
-    double t = 0.0;
-    for (int c = 0; c < ranks; ++c) t += ranks > 1 ? ld_cluster_f64(smem_u32(&block_s[turn]), c) : block_s[turn];
-    return t;
-  };
-
   if (n > 0) {
-    if (tid == 0) path_s[0] = 0;
+    // thread 0 (drawn): on from node, behind `child`, which was rejected, until a row's sum is wanted or no child is left
+    int node = 0, len = 1, child = kTree;
+    int k = 0;                                 // rejections at the path's last node
     double sum = 0.0;
     int summed = -1, summed_k = 0;             // whose sum it is
-    int at_node = 0, at_k = 0;
+    enum { kWalk, kWhole, kDraw } stage = kWalk;
+    // the draw: its place within what is left, and the places begin .. end that it has been narrowed down to, `whole` of them
+    double at = 0.0;
+    int begin = 0, end = 0, whole = 0;
+    bool mine = true;                          // this block has them
+    // One loop, so that what goes through a row is there once: a kernel that runs its code a few times is as fast as that comes
+    // from memory (three copies of it, the last one's four steps unrolled: chains 23.7 us).
+#pragma unroll 1
     for (;;) {
-      if (warp == 0) {
-        const bool done = advance();
-        if (lane == 0) {
-          node_s = node;
-          k_s = k;
-          len_s = len;
-          done_s = done;
-        }
-      }
-      __syncthreads();
-      at_node = node_s;
-      at_k = k_s;
-      const bool done = done_s;
-      if (done && summed == at_node && summed_k == at_k) break;
-      turn ^= 1;
-      if (kDrawn && !done) {                   // R_k is made of masses 0 .. k - 1
-        if (tid == 0) mass_s[at_k - 1] = at_k == 1 ? 1.0 : sum > 0.0 ? 1.0 / sum : 0.0;
-        __syncthreads();
-      }
-      sum = row_sum(at_node, at_k);
-      summed = at_node;
-      summed_k = at_k;
-      if (done) break;
-      mass = sum;
-    }
-    if (!(sum > 0.0)) {                        // nothing is left: from the row itself
-      turn ^= 1;
-      at_k = 0;
-      sum = row_sum(at_node, 0);
-    }
-    // ---- the draw: block of the cluster, warp's piece, its part, element
-    double at = (double)u_s[0] * sum;
-    const int owner = pick([&](int c) { return ranks > 1 ? ld_cluster_f64(smem_u32(&block_s[turn]), c) : block_s[turn]; }, ranks, at);
-    if (owner < 0) {
-      if (rank == 0 && tid == 0) p.next[r] = 0;            // a row of zeros
-    } else if (owner == rank) {
-      const int size = piece();
-      const int w = max(pick([&](int i) { return warp_s[i]; }, kVerifyWarps, at), 0);
-      int begin = (rank * kVerifyWarps + w) * size, end = min(begin + size, head + p.vocab);
-      if (size > 4 * kStep) {                  // a part a warp
-        const int part = (size / kVerifyWarps + kStep - 1) / kStep * kStep, b = begin + warp * part;
-        const double mine = piece_sum(b, min(b + part, end), at_k);
-        __syncthreads();
-        if (lane == 0) warp_s[warp] = mine;
-        __syncthreads();
-        const int x = max(pick([&](int i) { return warp_s[i]; }, kVerifyWarps, at), 0);
-        begin += x * part;
-        end = min(begin + part, end);
-      }
-      if (warp == 0) {
-        const bool hit = touched(begin, end, at_k);
-        double before = 0.0;
-        int found = -1, last = -1;
-        for (int i = begin; i < end && found < 0; i += kStep) {
-          const int e0 = i + lane * kPer;
-          double x[kPer], sums = 0.0;
-          rest(e0, at_k, hit, x);
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) sums += x[e];
-          double upto = sums;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
-          }
-          double run = before + (upto - sums);
-          int mine = INT_MAX, top = -1;
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) {
-            run += x[e];
-            if (x[e] > 0.0 && e0 + e < end) {
-              if (run > at && mine == INT_MAX) mine = e0 + e;
-              top = e0 + e;
+      if (stage == kWalk) {
+        if (tid == 0) {
+          if (!kDrawn) {
+            for (int c; (c = first_s[node]) < kTree; node = c) path_s[len++] = (int16_t)c;
+          } else {
+            // `child` has been rejected k - 1 times over: its next one is tested against what is left
+            bool passes = false;
+            if (k > 0) {
+              child = next_s[child];
+              passes = child < kTree && (double)u_s[child] * (double)qx_s[child] * sum < left_of(px_s[child], qx_s[child], k);
             }
+            if (k == 0 || passes) {
+              if (passes) {
+                path_s[len++] = (int16_t)child;
+                node = child;
+                k = 0;
+              }
+              while ((child = first_s[node]) & kPasses) path_s[len++] = (int16_t)(node = child & ~kPasses);
+            }
+            done_s = child >= kTree;
+            if (child < kTree) {
+              if (k > 0) over_s[k] = sum > 0.0 ? 1.0 / sum : 0.0;
+              ++k;
+            }
+            k_s = k;
           }
-          before += __shfl_sync(0xffffffffu, upto, 31);
-          const int first = __reduce_min_sync(0xffffffffu, mine);
-          last = max(last, __reduce_max_sync(0xffffffffu, top));
-          if (first != INT_MAX) found = first;
+          node_s = node;
+          len_s = len;
         }
-        if (lane == 0) p.next[r] = max((found >= 0 ? found : last) - head, 0);
+        __syncthreads();
+        const int last = node_s;
+        if (!kDrawn) {
+          for (int i = tid; i < n; i += kThreads)
+            if (up_s[i] == last) next_s[atomicAdd(&k_s, 1)] = (int16_t)i;      // in any order
+          __syncthreads();
+        }
+        k = k_s;
+        if (!kDrawn || done_s) {
+          const bool known = summed == last && summed_k == k;
+          stage = known && sum > 0.0 ? kDraw : kWhole;
+          if (known && stage == kWhole) k = 0;             // nothing is left: from the row itself
+        }
+        if (stage != kDraw) open_row(last, k);
+        summed = last;
+        summed_k = k;
       }
+      const bool parts = stage == kDraw && whole != 0;     // of a piece, else pieces of the row
+      if (stage != kDraw || parts) {
+        const int size = parts ? (whole / kWarps + kStep - 1) / kStep * kStep
+                               : ((end_row + kWarps * ranks - 1) / (kWarps * ranks) + kStep - 1) / kStep * kStep;
+        const int b = parts ? begin + warp * size : (rank * kWarps + warp) * size;
+        const double x = piece_sum(b, min(b + size, parts ? end : end_row), k);
+        if (parts) __syncthreads();                        // the sums before have been read
+        if (lane == 0) warp_s[warp] = x;
+        __syncthreads();
+        if (!parts) {
+          turn ^= 1;
+          double t = of_warps();
+#pragma unroll
+          for (int m = 16; m > 0; m >>= 1) t += __shfl_xor_sync(0xffffffffu, t, m);
+          of_blocks = lane == 0 ? t : 0.0;
+          if (ranks > 1) {
+            if (tid == 0) block_s[turn] = t;
+            cluster_sync_all();
+            of_blocks = lane < ranks ? ld_cluster_f64(smem_u32(&block_s[turn]), lane) : 0.0;
+            t = of_blocks;
+#pragma unroll
+            for (int m = 4; m > 0; m >>= 1) t += __shfl_xor_sync(0xffffffffu, t, m);
+            t = __shfl_sync(0xffffffffu, t, 0);
+          }
+          sum = t;
+          if (stage == kWalk) continue;
+          if (!(sum > 0.0) && k > 0) {                     // nothing is left: from the row itself
+            k = 0;
+            __syncthreads();
+            continue;
+          }
+          stage = kDraw;
+        } else {
+          begin += max(pick(of_warps(), at), 0) * size;
+          end = min(begin + size, end);
+          whole = size;
+        }
+      }
+      if (whole == 0) {                                    // the cluster's block, its warp's piece
+        at = (double)u_s[0] * sum;
+        const int owner = pick(of_blocks, at);
+        if (owner < 0 && rank == 0 && tid == 0) p.next[r] = 0;                 // a row of zeros
+        mine = owner == rank;
+        if (!mine) break;
+        whole = ((end_row + kWarps * ranks - 1) / (kWarps * ranks) + kStep - 1) / kStep * kStep;
+        begin = (rank * kWarps + max(pick(of_warps(), at), 0)) * whole;
+        end = min(begin + whole, end_row);
+      }
+      if (whole == kStep) break;
+    }
+    if (mine && warp == 0) {                               // a warp's load of places: which one
+      const bool both = kDrawn && k > 0;
+      const int to = begin + lane * kPer;
+      const bool full = to >= head && to + kPer <= end_row;
+      uint4 x = load_or_zero(row + to, full && to < end), y = load_or_zero(row_q + to, both && same && full && to < end);
+      if (!full && to < end) edge(row, to, x);
+      if (both && to < end && (!same || !full)) edge(row_q, to, y);
+      double left[kPer], own = 0.0;
+      rest(begin, x, y, k, !kDrawn, left);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) own += left[e];
+      double run = running(own) - own;
+      int first = INT_MAX, last = 0;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        run += left[e];
+        if (left[e] > 0.0) {
+          if (run > at) first = min(first, to + e);
+          last = max(last, to + e);
+        }
+      }
+      first = __reduce_min_sync(0xffffffffu, first);
+      last = __reduce_max_sync(0xffffffffu, last);
+      if (lane == 0) p.next[r] = max((first < INT_MAX ? first : last) - head, 0);
     }
     if (rank == 0) {
       const int kept = len_s;
-      for (int64_t i = tid; i < span.n; i += kVerifyThreads) p.accepted[span.t0 + i] = i < kept ? path_s[i] : -1;
+      for (int64_t i = tid; i < span.n; i += kThreads) p.accepted[span.t0 + i] = i < kept ? path_s[i] : -1;
       if (tid == 0) p.count[r] = kept;
     }
   } else if (rank == 0 && tid == 0) {
@@ -424,7 +512,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(VerifyPar
 template <typename T>
 int run_verify(const VerifyParams& p, int ranks, cudaStream_t st) {
   const auto kern = p.q != nullptr ? verify_drafts_kernel<T, true> : verify_drafts_kernel<T, false>;
-  return launch_cluster("nvfp4_verify_drafts", kern, dim3((unsigned)p.requests, 1, (unsigned)ranks), (unsigned)ranks, kVerifyThreads, 0, st, p);
+  return launch_cluster("nvfp4_verify_drafts", kern, dim3((unsigned)p.requests, 1, (unsigned)ranks), (unsigned)ranks,
+                        verify_threads(p.q != nullptr), 0, st, p);
 }
 
 }  // namespace
@@ -453,7 +542,7 @@ extern "C" int nvfp4_verify_drafts(const void* target_probs, int64_t target_row,
                        (int)requests, (int)vocab, accepted, num_accepted, next_tokens};
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  int ranks = 8;                               // as many blocks as are resident twice over
+  int ranks = 8;                               // as many blocks as are resident at once
   while (ranks > 1 && requests * ranks > 2 * sms) ranks >>= 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (dtype) {

@@ -6,8 +6,8 @@
 // the one rounding of the value it stood for to the receiving block's scale, which becomes the smallest power of two that holds
 // what came from blocks of larger scales where that is more than it was, and older codes are rounded again to it.
 //
-// A warp has one head's keys or values of a layer, a block of threads eight such of one request, which share what the tables say of
-// the tokens that move to a block.  What bounds it: trips to memory one behind the other (count, path, tables, scales, codes); a
+// A warp has a head's keys or values of a layer (a unit) after the other, a block of threads those of one request, which share
+// what the tables say of the tokens that move to a block.  What bounds it: trips to memory one behind the other (count, path, tables, scales, codes); a
 // call moves a few tokens of a request.
 #include <limits.h>
 #include "common/abi.cuh"
@@ -31,6 +31,36 @@ struct KeepParams {
   int64_t scale_block[2], scale_layer[2];
   int32_t* keep;
 };
+
+// Codes of scale s as codes of scale `now`, each the one rounding of its value.  Between powers of two a code times their quotient
+// is exact; other scales are divided by (a call of its own, which hardly any makes: in place it costs 40 registers).
+__device__ __noinline__ uint4 codes_divided(uint4 v, float s, float now) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint32_t lo, hi;
+    half4_of_e4m3x4(w[k], lo, hi);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    w[k] = e4m3x4(__fdiv_rn(a.x * s, now), __fdiv_rn(a.y * s, now), __fdiv_rn(b.x * s, now), __fdiv_rn(b.y * s, now));
+  }
+  return v;
+}
+__device__ __forceinline__ uint4 codes_again(uint4 v, float s, float now) {
+  const uint32_t a = __float_as_uint(s), b = __float_as_uint(now);
+  const int e = (int)(a >> 23) - (int)(b >> 23);           // of the quotient, where both are normal powers of two
+  const bool powers = ((a | b) & 0x807FFFFFu) == 0 && a != 0 && b != 0 && a < 0x7F800000u && b < 0x7F800000u && e > -126 && e < 127;
+  if (!powers) return codes_divided(v, s, now);
+  const float f = __uint_as_float((uint32_t)(e + 127) << 23);
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint32_t lo, hi;
+    half4_of_e4m3x4(w[k], lo, hi);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo)), y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    w[k] = e4m3x4(x.x * f, x.y * f, y.x * f, y.y * f);
+  }
+  return v;
+}
 
 template <int D>
 __global__ void __launch_bounds__(kThreads) keep_path_kernel(KeepParams p) {
@@ -60,16 +90,13 @@ __global__ void __launch_bounds__(kThreads) keep_path_kernel(KeepParams p) {
   if (tid == 0 && blockIdx.y == 0) p.keep[r] = max(base + end, 0);
   if (first >= end || base < 0) return;
   const int bs = 1 << p.log_block, mask = bs - 1;
-  const int unit = blockIdx.y * kWarps + warp;
-  const int head = unit % p.hk, operand = unit / p.hk & 1, layer = unit / (2 * p.hk);
-  uint8_t* const codes = unit < p.units ? p.cache[operand] + layer * p.layer[operand] + ((int64_t)head << p.log_block) * D : nullptr;
-  float* const scales = unit < p.units ? p.scale[operand] + layer * p.scale_layer[operand] + head : nullptr;
   const int32_t* const row = p.table + r * p.table_row;
   auto block_at = [&](int64_t pos) -> int {
     const int64_t e = pos >> p.log_block;
     const int b = e < p.width ? row[e] : -1;
     return (unsigned)b < (unsigned)p.blocks ? b : -1;
   };
+  const int sub = lane / kLanes, piece = lane % kLanes * 16;           // this lane's token of a load, its bytes
   for (int j0 = first; j0 < end;) {
     const int to = base + j0, offset = to & mask, count = min(end - j0, bs - offset);      // tokens j0 .. of one block
     __syncthreads();
@@ -81,79 +108,99 @@ __global__ void __launch_bounds__(kThreads) keep_path_kernel(KeepParams p) {
     const int into = block_at(to);
     __syncthreads();
     j0 += count;
-    if (into < 0 || codes == nullptr) continue;
-    uint8_t* const dst = codes + into * p.block[operand];
-    const float was = scales[into * p.scale_block[operand]];
-    auto scale_of = [&](int i) { return scales[(from_s[i] >> p.log_block) * p.scale_block[operand]]; };
-    auto source = [&](int i) { return codes + (from_s[i] >> p.log_block) * p.block[operand] + (from_s[i] & mask) * D + lane % kLanes * 16; };
-    bool larger = false, other = false;
-    for (int i = lane; i < count; i += 32)
-      if (from_s[i] >= 0) {
-        const float s = scale_of(i);
-        larger |= s > was;
-        other |= s != was;
-      }
-    larger = __any_sync(0xffffffffu, larger);
-    other = __any_sync(0xffffffffu, other);
-    float now = was;
-    if (larger) {
+    if (into < 0) continue;
+    // keys or values of one head of a layer
+    struct Unit {
+      uint8_t* codes;
+      float* scales;
+      int64_t block, scale_block;
+    };
+    auto unit_of = [&](int u) -> Unit {
+      const int head = u % p.hk, operand = u / p.hk & 1, layer = u / (2 * p.hk);
+      return {p.cache[operand] + layer * p.layer[operand] + ((int64_t)head << p.log_block) * D,
+              p.scale[operand] + layer * p.scale_layer[operand] + head, p.block[operand], p.scale_block[operand]};
+    };
+    auto scale_of = [&](const Unit& x, int i) { return x.scales[(from_s[i] >> p.log_block) * x.scale_block]; };
+    auto source = [&](const Unit& x, int i) {
+      return reinterpret_cast<const uint4*>(x.codes + (from_s[i] >> p.log_block) * x.block + (from_s[i] & mask) * D + piece);
+    };
+    auto magnitude = [](const uint4& v, float s) -> uint32_t {           // the largest, as float bits
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
       uint32_t top = 0;
-      for (int i = lane / kLanes; i < count; i += kRows) {
-        if (from_s[i] < 0) continue;
-        const float s = scale_of(i);
-        if (!(s > was)) continue;
-        const uint4 v = *reinterpret_cast<const uint4*>(source(i));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t lo, hi;
-          half4_of_e4m3x4(w[k], lo, hi);
-          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-          top = max(max(top, max(kv8_magnitude(a.x * s), kv8_magnitude(a.y * s))), max(kv8_magnitude(b.x * s), kv8_magnitude(b.y * s)));
-        }
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (top != 0) now = fmaxf(was, kv8_scale(top));
-    }
-    auto again = [&](uint4& v, float s) {                  // codes of scale s to codes of `now`
-      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t lo, hi;
         half4_of_e4m3x4(w[k], lo, hi);
         const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-        w[k] = e4m3x4(__fdiv_rn(a.x * s, now), __fdiv_rn(a.y * s, now), __fdiv_rn(b.x * s, now), __fdiv_rn(b.y * s, now));
+        top = max(max(top, max(kv8_magnitude(a.x * s), kv8_magnitude(a.y * s))), max(kv8_magnitude(b.x * s), kv8_magnitude(b.y * s)));
       }
+      return top;
     };
-    if (now != was) {
-      for (int x = lane; x < offset * kLanes; x += 32) {
-        uint4 v = reinterpret_cast<const uint4*>(dst)[x];
-        again(v, was);
-        reinterpret_cast<uint4*>(dst)[x] = v;
-      }
-      if (lane == 0) scales[into * p.scale_block[operand]] = now;
-    }
-    // all of a round's tokens are read before any is written; those of later rounds lie behind what is written
-    for (int i0 = lane / kLanes; i0 - lane / kLanes < count; i0 += kAhead * kRows) {
-      uint4 v[kAhead];
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        const int i = i0 + a * kRows;
-        if (i < count && from_s[i] >= 0) v[a] = *reinterpret_cast<const uint4*>(source(i));
-      }
-      __syncwarp();
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        const int i = i0 + a * kRows;
-        if (i >= count || from_s[i] < 0) continue;
-        if (other) {
-          // a block that receives keeps its scale in `now`, but its own tokens were of the one before
-          const float s = (from_s[i] >> p.log_block) == into ? was : scale_of(i);
-          if (s != now) again(v[a], s);
+    // the block's scale once the largest value that comes from larger scales is known; older codes follow it
+    auto grow = [&](const Unit& x, float was, uint32_t top) -> float {
+      top = __reduce_max_sync(0xffffffffu, top);
+      const float now = top != 0 ? fmaxf(was, kv8_scale(top)) : was;
+      if (now != was) {
+        uint4* old = reinterpret_cast<uint4*>(x.codes + into * x.block);
+        for (int i = lane; i < offset * kLanes; i += 32) {
+          const uint4 v = old[i];
+          old[i] = codes_again(v, was, now);
         }
-        *reinterpret_cast<uint4*>(dst + (offset + i) * D + lane % kLanes * 16) = v[a];
+        if (lane == 0) x.scales[into * x.scale_block] = now;
       }
-      __syncwarp();
+      return now;
+    };
+    for (int u = blockIdx.y * kWarps + warp; u < p.units; u += gridDim.y * kWarps) {
+      const Unit x = unit_of(u);
+      // Rounds of tokens, each read before any of it is written; those of later rounds lie behind what is written.  The first
+      // one's codes come with the scales, whatever those turn out to be.
+      uint4 v[kAhead];
+      float s[kAhead];
+      auto read = [&](int i0) {
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const int i = i0 + sub + a * kRows;
+          s[a] = 0.0f;
+          if (i < count && from_s[i] >= 0) {
+            v[a] = *source(x, i);
+            s[a] = scale_of(x, i);
+          }
+        }
+      };
+      const float was = x.scales[into * x.scale_block];
+      read(0);
+      bool larger = false;
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) larger |= s[a] > was;
+      for (int i = kAhead * kRows + lane; i < count; i += 32) larger |= from_s[i] >= 0 && scale_of(x, i) > was;
+      float now = was;
+      if (__any_sync(0xffffffffu, larger)) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+          if (s[a] > was) top = max(top, magnitude(v[a], s[a]));
+        for (int i = kAhead * kRows + sub; i < count; i += kRows) {
+          if (from_s[i] < 0) continue;
+          const float t = scale_of(x, i);
+          if (t > was) top = max(top, magnitude(*source(x, i), t));
+        }
+        now = grow(x, was, top);
+      }
+      for (int i0 = 0;;) {
+        __syncwarp();
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const int i = i0 + sub + a * kRows;
+          if (i >= count || from_s[i] < 0) continue;
+          // the block that receives has its new scale by now, but its own tokens were of the one before
+          const float t = (from_s[i] >> p.log_block) == into ? was : s[a];
+          if (t != now) v[a] = codes_again(v[a], t, now);
+          *reinterpret_cast<uint4*>(x.codes + into * x.block + (offset + i) * D + piece) = v[a];
+        }
+        if ((i0 += kAhead * kRows) >= count) break;
+        __syncwarp();
+        read(i0);
+      }
     }
   }
 }
@@ -176,15 +223,15 @@ extern "C" int nvfp4_paged_keep_path(const int32_t* accepted, const int32_t* num
   NVFP4_REQUIRE(requests >= 1 && requests < (1 << 30) && width >= 1 && width < (1 << 30) && blocks >= 0 && blocks < INT32_MAX &&
                     tokens >= 0 && tokens < INT32_MAX && hk >= 1 && layers >= 0,
                 "nvfp4_paged_keep_path: sizes out of range");
-  const int64_t most = 65535 * kWarps;         // units of a grid
-  NVFP4_REQUIRE(hk <= most && layers <= most / (2 * hk), "nvfp4_paged_keep_path: too many layers and heads");
+  NVFP4_REQUIRE(hk <= (1 << 20) && layers <= (1 << 28) / (2 * hk), "nvfp4_paged_keep_path: too many layers and heads");
   NVFP4_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0 && ((k_block | v_block | k_layer | v_layer) & 15) == 0,
                 "nvfp4_paged_keep_path: cache blocks must be 16-byte aligned");
   const int units = (int)(layers * 2 * hk);
+  const int64_t want = ((int64_t)units + kWarps - 1) / kWarps, y = want < 65535 ? want : 65535;
   const KeepParams p{accepted, num_accepted, cu_seqlens, lengths, table, table_row, tokens, (int)requests, (int)width, (int)blocks, lb,
                      (int)hk, units, {k_cache, v_cache}, {k_block, v_block}, {k_layer, v_layer}, {k_scale, v_scale},
                      {ks_block, vs_block}, {ks_layer, vs_layer}, keep_lens};
-  const dim3 grid((unsigned)requests, (unsigned)((units + kWarps - 1) / kWarps > 0 ? (units + kWarps - 1) / kWarps : 1));
+  const dim3 grid((unsigned)requests, (unsigned)(y > 1 ? y : 1));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return d == 128 ? launch("nvfp4_paged_keep_path", keep_path_kernel<128>, grid, kThreads, 0, st, p)
                   : launch("nvfp4_paged_keep_path", keep_path_kernel<256>, grid, kThreads, 0, st, p);

@@ -30,7 +30,7 @@ def test_c_entries_refuse_what_they_cannot_do():
     keep = lambda d=128, bs=16, layers=1, hk=1, k=0, kb=2048, kl=0: L.nvfp4_paged_keep_path(
         n, n, n, 4, n, n, 1, 1, 1, k, kl, kb, 0, 0, 2048, n, 0, 1, n, 0, 1, layers, 1, hk, bs, d, n, n)
     assert bad(keep(d=64), b"D must") and bad(keep(bs=8), b"block_size") and bad(keep(k=8), b"aligned") and bad(keep(kb=2056), b"aligned")
-    assert bad(keep(kl=4), b"aligned") and bad(keep(layers=-1), b"sizes") and bad(keep(layers=1 << 20), b"layers")
+    assert bad(keep(kl=4), b"aligned") and bad(keep(layers=-1), b"sizes") and bad(keep(layers=1 << 28), b"layers")
     import ctypes
     three = (ctypes.c_int64 * 3)(0, 128, 128)
     odd = (ctypes.c_int64 * 3)(0, 128, 129)
