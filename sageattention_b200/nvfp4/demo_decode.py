@@ -5,7 +5,7 @@
 Stands in for the reference's ``example/nvfp4_decode_demo.py`` (which patches a pretrained Qwen2):
 no checkpoint is assumed here, so the model is a randomly initialised pre-norm decoder with
 rotary embeddings and grouped-query attention (default 8 query heads on 2 KV heads, head dim
-128).  The prompt is prefilled once with plain bf16 attention; decoding then runs four ways from
+128).  The prompt is prefilled once with plain bf16 attention; decoding then runs five ways from
 the same prompt state --
 
   bf16    keys and values kept in bf16, ``scaled_dot_product_attention`` per step (the baseline);
@@ -13,7 +13,9 @@ the same prompt state --
           ``nvfp4_flash_decode_prequant`` over the packed cache;
   hybrid  ``NVFP4KVCache.hybrid_decode``: recent tokens in bf16, older prefix in NVFP4;
   fp8     one ``FP8PagedKVCache`` for all layers: blocks and slots of the step's tokens reserved on the GPU, keys and
-          values in e4m3 with a scale for each block and head --
+          values in e4m3 with a scale for each block and head;
+  tree    the same cache, several tokens a step: small trees of tokens that followed the last one before, attended at once,
+          verified against the model's own choice, the accepted path moved together in the cache --
 
 and the demo reports what the reference's demo reports: greedy top-1 agreement with the bf16 run,
 the teacher-forced logit cosine per step, cache memory per mode, and the per-step latency.
@@ -28,7 +30,7 @@ import time
 import torch
 import torch.nn.functional as F
 
-from . import FP8PagedKVCache, NVFP4KVCache, nvfp4_flash_decode_prequant
+from . import FP8PagedKVCache, NVFP4KVCache, nvfp4_flash_decode_prequant, verify_drafts
 
 
 class TinyGQADecoder(torch.nn.Module):
@@ -174,6 +176,71 @@ def generate(model, kv, first_logits, n_new, mode, capacity, window, forced=None
     return torch.stack(toks, 1), torch.stack(logs, 1), ms, state
 
 
+def lookup_tree(tokens, branches=3, depth=4):
+    """A tree of drafts below the last of ``tokens``: what followed its latest earlier occurrences.  (tokens, parents), the last
+    token itself first; siblings are distinct."""
+    out, parents = [tokens[-1]], [-1]
+    found = [i for i in range(len(tokens) - 2, -1, -1) if tokens[i] == tokens[-1]][:branches]
+    for i in found:
+        at = 0
+        for t in tokens[i + 1:i + 1 + depth]:
+            known = [j for j, (x, a) in enumerate(zip(out, parents)) if x == t and a == at]
+            if not known:
+                out.append(t)
+                parents.append(at)
+            at = known[0] if known else len(out) - 1
+    return out, parents
+
+
+@torch.no_grad()
+def tree_step(model, cache, tokens, parents, lens, most, uniforms, temperature=0.0):
+    """One step of every request's tree (``tokens`` and ``parents`` request by request, ``lens`` of them): the cache keeps the
+    accepted paths.  Returns the verification."""
+    step = cache.reserve(lens, tokens.shape[0])
+    tree = cache.tree(parents, step.cu_seqlens, most)
+    x = model.emb[tokens][None]
+    for li, blk in enumerate(model.blocks):
+        q, k, v = (t[0].transpose(0, 1) for t in model.qkv(blk, x, tree.positions))
+        cache.write(li, k, v, step.slot_map)
+        attn = cache.attend_tree(li, q, step.cu_seqlens, tree.tree_mask, model.d ** -0.5, model.h // model.hk)
+        x = model.finish(blk, x, attn.transpose(0, 1)[None])
+    logits = model.logits(x.transpose(0, 1))
+    probs = torch.softmax(logits / temperature, -1) if temperature > 0 else F.one_hot(logits.argmax(-1), logits.shape[-1]).float()
+    got = verify_drafts(probs, tokens, parents, step.cu_seqlens, uniforms)
+    cache.keep_path(got.accepted, got.num_accepted, step.cu_seqlens)
+    return got
+
+
+@torch.no_grad()
+def generate_trees(model, prompt, kv, first_logits, n_new, capacity, temperature=0.0):
+    """Generation with drafted trees; returns tokens [Z, n_new + 1], steps, ms/step, the cache."""
+    cache = fresh_state(model, kv, "fp8", capacity + 64, 0)
+    dev = first_logits.device
+    gen = torch.Generator(device=dev).manual_seed(0)
+    texts = [list(row) + [int(t)] for row, t in zip(prompt.tolist(), first_logits.argmax(-1))]
+    goal, steps, t0 = prompt.shape[1] + 1 + n_new, 0, None
+    while min(len(t) for t in texts) < goal:
+        if steps == 1:
+            torch.cuda.synchronize()
+            t0 = time.perf_counter()
+        trees = [lookup_tree(t) if len(t) < goal else ([], []) for t in texts]           # a finished request has no tokens
+        flat = lambda i, dtype: torch.tensor([x for tree in trees for x in tree[i]], dtype=dtype, device=dev)
+        tokens, parents = flat(0, torch.int64), flat(1, torch.int32)
+        lens = torch.tensor([len(t) for t, _ in trees], dtype=torch.int32, device=dev)
+        got = tree_step(model, cache, tokens, parents, lens, int(max(len(t) for t, _ in trees)),
+                        torch.rand(tokens.shape[0], generator=gen, device=dev), temperature)
+        accepted, count, after = got.accepted.tolist(), got.num_accepted.tolist(), got.next_tokens.tolist()
+        at = 0
+        for text, (ids, _), n, x in zip(texts, trees, count, after):
+            if ids:
+                text += [ids[i] for i in accepted[at + 1:at + n]] + [x]
+            at += len(ids)
+        steps += 1
+    torch.cuda.synchronize()
+    ms = (time.perf_counter() - t0) * 1e3 / (steps - 1) if steps > 1 else float("nan")
+    return torch.tensor([t[prompt.shape[1]:goal] for t in texts], device=dev), steps, ms, cache
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     ap.add_argument("--layers", type=int, default=4)
@@ -215,6 +282,10 @@ def main(argv=None):
         print(f"  {mode:<6} cache: {ms:.3f} ms/step; free-running top-1 agreement with bf16 {agree * 100:.1f} %; "
               f"teacher-forced logit cosine {cos:.4f}; cache {mem / 1e6:.2f} MB vs bf16 {bf / 1e6:.2f} MB "
               f"({bf / mem:.2f}x)")
+    toks, steps, ms, state = generate_trees(model, tokens, kv, first, a.new, cap)
+    agree = float((toks == ref_toks).float().mean())
+    report["tree"] = {"agreement": agree, "ms_per_step": ms, "steps": steps, "tokens_per_step": a.new / steps, "bytes": state.held_bytes()}
+    print(f"  tree   cache: {ms:.3f} ms/step of {a.new / steps:.2f} tokens a request or more; free-running top-1 agreement with bf16 {agree * 100:.1f} %")
     return report
 
 

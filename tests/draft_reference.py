@@ -108,7 +108,7 @@ def keep_path(path, n, length, row, codes, scale, block):
             if bool(grown.any()):
                 codes[b, grown, :first] = R.nearest_e4m3(codes[b, grown, :first] * (was[grown] / now[grown])[:, None, None])
             for o, x, s in moves:
-                codes[b, :, o] = torch.where((s == now)[:, None], x, R.nearest_e4m3(x * (s / now)[:, None]))
+                codes[b, :, o] = torch.where(((s == now) | (now == 0))[:, None], x, R.nearest_e4m3(x * (s / now)[:, None]))
             scale[b] = now
     return max(base + len(path), 0)
 

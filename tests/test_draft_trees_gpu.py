@@ -409,6 +409,29 @@ def test_blocks_that_are_none():
     _check_keep(new, held, [[0, 5, 9, 13, 15, 33, 39], [1, 4, 20, 29]], 1, 256, 16, 1, seed=1, table=table[:, :2].contiguous())
 
 
+def test_blocks_of_scale_zero():
+    """Zeros that move to a block which was never written, and to one with a scale."""
+    block, d = 16, 128
+    k, ks, _ = _empty_cache(4, 2, block, d, 1)
+    v, vs, _ = _empty_cache(4, 2, block, d, 2)
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32)
+    for c, s in ((k, ks), (v, vs)):
+        s[0] = 0.0
+        c.view(torch.uint8)[1] = 0                                             # 0 times any scale
+        s[1] = 4.0
+        s[3] = 0.0                                                             # and any codes times 0
+    want = []
+    for c, s in ((k, ks), (v, vs)):
+        x, y = _as_values(c), s.cpu().double()
+        for r in range(2):
+            T.keep_path([0, 4, 7, 20], 24, 30, table[r], x, y, block)
+        want.append((x, y))
+    keep = _nv().paged_kv_keep_path(_i32(([0, 4, 7, 20] + [-1] * 20) * 2), _i32([4, 4]), _i32([0, 24, 48]), _i32([30, 30]), table.cuda(), k, v, ks, vs)
+    assert keep.tolist() == [10, 10]
+    for (x, y), c, s in zip(want, (k, v), (ks, vs)):
+        assert torch.equal(_as_values(c), x) and torch.equal(s.cpu().double(), y)
+
+
 def test_layers_inside_blocks():
     """[blocks, layers, ...] in memory: layers closer together than blocks."""
     k, ks, _ = _empty_cache(6 * 3, 2, 16, 128, 1)
