@@ -6,7 +6,8 @@
 // and CTA c takes entries [c, c + 1) * ceil(total / CTAs) of it, so ragged lengths need no plan on the host.  In front of a
 // unit's tiles the list has unit_cost() entries without work, for what a unit costs besides (its query, its merge).  With one, two,
 // three and four of them: decode of 160 requests of 1 to 4100 keys 23.1, 22.7, 24.2, 24.3 us; drafts of 32 requests 79.5, 70.0,
-// 67.7, 69.4; chunks and single tokens in one batch at D 256 87.6, 82.7, 79.0, 79.4.  A CTA can hold
+// 67.7, 69.4; chunks and single tokens in one batch at D 256 87.6, 82.7, 79.0, 79.4.  Trees of many rows, whose units go through all
+// keys: 32 of 16 to 64 nodes, none to four of them 122.5, 104.7, 96.6, 100.8, 104.8.  A CTA can hold
 // the end of one unit and the beginning of another, each a partial result of its own (slots 2 c and 2 c + 1).
 #pragma once
 #include <cuda_runtime.h>
@@ -54,7 +55,7 @@ __device__ __forceinline__ int token_of(const PagedParams& p, int i) {
   return (int)((__umulhi((uint32_t)i, p.g_mul) + (uint32_t)i) >> p.g_shift);
 }
 
-__host__ __device__ constexpr int unit_cost(int rows) { return rows <= 8 ? 2 : 3; }
+__host__ __device__ constexpr int unit_cost(int rows, bool tree) { return rows <= 8 || (tree && rows >= 128) ? 2 : 3; }
 
 // What a request asks for: its query tokens [t0, t0 + n), its keys, its units.  TREE: what its tokens see of each other is in
 // bits, so that all of them go through all keys.
@@ -86,7 +87,7 @@ struct Request {
     return max((limit(p, row_tile) + TILE - 1) / TILE, 1);
   }
   __device__ __forceinline__ int64_t head_entries(const PagedParams& p) const {
-    int64_t sum = (int64_t)unit_cost(ROWS) * row_tiles;
+    int64_t sum = (int64_t)unit_cost(ROWS, TREE) * row_tiles;
 #pragma unroll 1
     for (int j = 0; j < row_tiles; ++j) sum += tiles(p, j);
     return sum;
@@ -106,7 +107,7 @@ __device__ __forceinline__ const uint32_t* tree_row(const PagedParams& p, int t)
 // The rest of a CTA's share, segment by segment: open() gives tiles [from, to) of a unit, close() goes on to the next one.
 template <int ROWS, int TILE, bool TREE>
 struct Walk {
-  static constexpr int kUnitCost = unit_cost(ROWS);
+  static constexpr int kUnitCost = unit_cost(ROWS, TREE);
   Request<ROWS, TILE, TREE> q;
   int r, head, row_tile, entry, tiles;        // entry: -kUnitCost .. -1 without work, then the unit's tiles
   int from, to;
@@ -168,7 +169,7 @@ __device__ __forceinline__ int64_t deal_tiles(const PagedParams& p, int64_t* lis
   auto weight = [&](int r) -> int64_t {
     return r < p.requests ? p.hk * Request<ROWS, TILE, TREE>(p, r).head_entries(p) : 0;
   };
-  constexpr int kUnitCost = unit_cost(ROWS);
+  constexpr int kUnitCost = unit_cost(ROWS, TREE);
   // a thread has `each` requests in a row
   const int each = (p.requests + THREADS - 1) / THREADS, r0 = tid * each;
   int64_t mine = 0, before;

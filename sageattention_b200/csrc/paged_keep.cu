@@ -9,7 +9,7 @@
 // A warp has a head's keys or values of a layer (a unit) after the other, a block of threads those of one request, which share
 // what the tables say of the tokens that move to a block.  What bounds it: trips to memory one behind the other (count, path,
 // table, codes with their scales); a call moves a few tokens of a request.  Paths of 64 requests in 16 layers of Hk 8 D 128, blocks of
-// 16: 11.2 us, 12.0 with the scales in a trip of their own; units of a request on the blocks that are resident at once, several a
+// 16: 9.5 us, one more with the scales in a trip of their own; units of a request on the blocks that are resident at once, several a
 // warp, 15 to 18.
 #include <limits.h>
 #include "common/abi.cuh"
@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kMaxBlock = 128;
+constexpr int kResident = 5;                   // blocks of an SM: four loads ahead, at 80 registers and three blocks, took 11.6 us instead of 9.5
 
 struct KeepParams {
   const int32_t *accepted, *count, *cu, *lengths, *table;
@@ -66,9 +67,9 @@ __device__ __forceinline__ uint4 codes_again(uint4 v, float s, float now) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads) keep_path_kernel(KeepParams p) {
+__global__ void __launch_bounds__(kThreads, kResident) keep_path_kernel(KeepParams p) {
   constexpr int kLanes = D / 16, kRows = 32 / kLanes;      // lanes of a token, tokens of a warp's load
-  constexpr int kAhead = 4;                                // loads of a lane under way together
+  constexpr int kAhead = 2;                                // loads of a lane under way together
   __shared__ int first_s, end_s;                           // the path's tail that moves: [first_s, end_s)
   __shared__ int64_t from_s[kMaxBlock];                    // of a receiving block's tokens: block * block size + offset, or -1
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x;

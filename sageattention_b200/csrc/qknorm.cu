@@ -426,6 +426,7 @@ __global__ void __launch_bounds__(1024) qk_norm_weights_kernel(const float* part
   griddep_launch();
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, which = (int)blockIdx.x * 32 >= d, col = blockIdx.x * 32 - which * d + lane;
   float t = 0.0f;
+#pragma unroll 8
   for (int b = (which ? query_blocks : 0) + slice; b < (which ? blocks : query_blocks); b += 32) t += part[(int64_t)b * d + col];
   sums[slice][lane] = t;
   __syncthreads();

@@ -15,11 +15,10 @@ Layout, shared by every function here:
   lengths            [requests] int32: tokens that a request holds
   free_blocks        [blocks] int32, free_count [1] int32: a stack of block ids, its top at free_count - 1
 
-A step of drafted trees is reserve, ``draft_tree``, then in every layer ``fp8_kv_write`` and ``fp8_paged_tree_attention``, then
-``verify_drafts`` of the model's probabilities, ``paged_kv_keep_path`` in all layers and ``paged_kv_trim``.  Any other
-step is ``paged_kv_reserve`` (blocks and slots for the new tokens), then in every layer ``fp8_kv_write`` and
+A step is ``paged_kv_reserve`` (blocks and slots for the new tokens), then in every layer ``fp8_kv_write`` and
 ``fp8_paged_decode`` or ``fp8_paged_attention``; ``paged_kv_trim`` takes tokens away again (rejected drafts, requests
-that ended).  ``FP8PagedKVCache`` holds the buffers of a model's layers and calls these.
+that ended).  With trees of drafted tokens: ``draft_tree`` once, ``fp8_paged_tree_attention`` in every layer, ``verify_drafts``,
+then ``paged_kv_keep_path`` for all layers in front of the trim.  ``FP8PagedKVCache`` holds the buffers of a model's layers and calls these.
 """
 
 from __future__ import annotations

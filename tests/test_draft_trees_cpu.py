@@ -82,3 +82,16 @@ def test_custom_ops_infer_shapes():
         x = torch.empty(2, 30, 4, 128).transpose(1, 2)
         a, _ = ns.qk_norm_rope(x, x, torch.empty(128), torch.empty(128), t, t, None, 0, 1e-6)
         assert a.shape == x.shape and a.stride() == x.stride()
+
+
+def test_waits_of_the_gradient_kernel_are_bounded_and_reported():
+    """Its copies arrive on barriers: every wait is of the whole warp and gives up, and what gave up is told at the end."""
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sageattention_b200", "csrc")
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, "qknorm.cu")).read())
+    start = text.index("qk_norm_rope_bwd_kernel(NormParams p)")
+    body = text[start:re.compile(r"^}", re.M).search(text, start).start()]
+    assert set(re.findall(r"\bmbar_\w*wait\w*", body)) == {"mbar_wait_warp"} and len(re.findall(r"&expired, \d+\)", body)) == 1
+    assert re.search(r"__syncthreads\(\);\s*report_error\(&expired, p\.status\);\s*$", body)
+    # copies into a stage are asked for when all lanes have read it
+    assert body.rindex("__syncwarp();") < body.index("if (p.part != nullptr)")

@@ -528,6 +528,17 @@ def test_steps_of_trees_one_after_the_other():
         assert int(cache.free_count) == ref["count"] and cache.free_blocks[:ref["count"]].tolist() == ref["free"][:ref["count"]].tolist()
 
 
+def test_a_step_that_does_not_fit_keeps_everything():
+    cache = _filled(2, [40, 3, 15, 100], 1)
+    before = _state(cache)
+    model, parents, tokens, u = _inputs(2, [150, 150, 150, 90], 3)             # more blocks than there are
+    step, tree, outs, got = _step(cache, 2, model, parents, tokens, u, _i32([150, 150, 150, 90]), 150, 4, 0.1)
+    assert int(step.shortage) == 1 and not tree.tree_mask.any() and not tree.positions.any()
+    assert all(not o.any() for o in outs)
+    assert bool((got.accepted == -1).all()) and got.num_accepted.tolist() == [0] * 4 and got.next_tokens.tolist() == [-1] * 4
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(_state(cache), before))
+
+
 def test_a_captured_step_of_trees():
     layers, new = 2, [9, 12, 0, 30]
     model, parents, tokens, u = _inputs(layers, new, 3)
