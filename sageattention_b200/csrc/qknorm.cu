@@ -8,13 +8,15 @@
 // heads of a token (a step), STEPS steps together, for which it loads cos and sin once.  Statistics, rotation and weight
 // gradients are fp32, two an instruction, rounded once to the type of the operand.
 //
-// Forward: tasks of queries and keys by turns, so that what is in flight lies together, on the blocks that are resident at once: 16384
-// tokens of H 32 Hk 8 D 128 in bf16 (views of a projection, 336 MB) 57.2 us, a copy of as many bytes 57.6; all
-// queries first 61.8; more blocks than resident 58 to 64; four steps a task 63, as there are fewer warps.
+// Forward: tasks of queries and keys by turns, so that what is in flight lies together, on the blocks that are resident at once: 16001
+// tokens of H 32 Hk 8 D 128 in bf16 (views of a projection, 328 MB) 61.6 us, a copy of as many bytes 51.  On the same buffers
+// again and again (16384 tokens) 57.2; all queries first 61.8; more blocks than resident 58 to 64; four steps a task 63, as there
+// are fewer warps.  More under way does not help (rows asked into L2 a task ahead 63.6 instead of 61.6, two ahead 64.2), nor do
+// loads past L1 (63.3) or stores that L2 gives up first (62.4).
 // Backward: registers hold too few rows for the loads to stay under way (104 us with four steps, 110 with two), so a warp's rows
-// come by bulk copies, the next task's while this one's are used, and a block is of queries or of keys, whose sums it keeps: 85.5
-// us, 503 MB at 0.90 of the copy rate (queries first, then keys, in every block: 90.8; three stages 96, four warps a block
-// 87.5; the forward pass by bulk copies 60.5).
+// come by bulk copies, the next task's while this one's are used, and a block is of queries or of keys, whose sums it keeps: 16384
+// tokens, 503 MB, 84.9 us, an addition of two tensors of that size 73 (queries first, then keys, in every block: 90.8; three stages
+// 96, four warps a block 87.5; tasks of keys that do not fill a stage 88.8; the forward pass by bulk copies 60.5 instead of 57.2).
 #include <limits.h>
 #include "common/abi.cuh"
 #include "common/fp4.cuh"
