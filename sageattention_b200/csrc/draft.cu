@@ -449,6 +449,7 @@ __global__ void __launch_bounds__(verify_threads(kDrawn), 2) verify_drafts_kerne
           if (stage == kWalk) continue;
           if (!(sum > 0.0) && k > 0) {                     // nothing is left: from the row itself
             k = 0;
+            struck = -1;
             __syncthreads();
             continue;
           }

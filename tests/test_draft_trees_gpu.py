@@ -308,6 +308,22 @@ def test_rows_that_are_no_distribution_and_borders():
             assert 0 <= int(out.next_tokens) < 5 and 1 <= int(out.num_accepted) <= 4
 
 
+@pytest.mark.parametrize("v", [2, 40, 3000])
+def test_drafts_that_leave_nothing(v):
+    """Rows that sum to less than one, all of whose tokens are drafts and rejected: the next token is drawn from the row itself."""
+    n = min(v, 60) + 1
+    p = torch.zeros(n, v)
+    p[:, :n - 1] = 0.01 + 0.3 * torch.rand(n, n - 1, generator=torch.Generator().manual_seed(v)) / n
+    tokens = torch.arange(n) - 1
+    for parents in ([-1] + [0] * (n - 1), [-1] + [0] * (n - 1 - n // 3) + [1] * (n // 3)):
+        for w in (0.0, 0.3, 0.99):
+            u = torch.full((n,), 1 - 2.0 ** -24)
+            u[0] = w
+            assert _check_verify(p, tokens, parents, [0, n], u) == [1]
+            q = torch.full((n, v), 1.0)                                        # more than the target has, everywhere
+            assert _check_verify(p, tokens, parents, [0, n], u, q) == [1]
+
+
 def test_strided_rows_and_offsets_that_are_none():
     wide, other = _rows(9, 300, 1).cuda(), _rows(9, 300, 2).cuda()
     parents, starts = [-1, 0, 0, 1, -1, 0, 1, 1], [0, 4, 8]
