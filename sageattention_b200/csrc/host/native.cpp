@@ -1013,7 +1013,9 @@ NormTables norm_tables(const Call& c, const Tensor& q, const Tensor& k, const Te
     const bool own = four && positions->dim() == 2;
     require(own ? positions->size(0) == z && positions->size(1) == s : positions->dim() == 1 && positions->size(0) == s,
             "positions must be one a token: [T], or [S] or [Z, S]");
-    t.positions = positions->to(q.device(), at::kInt).contiguous();
+    // what 32 bits do not hold lies outside the tables as well
+    const Tensor near = positions->scalar_type() == at::kLong ? positions->clamp(-1, INT32_MAX) : *positions;
+    t.positions = near.to(q.device(), at::kInt).contiguous();
     if (own) t.pos_batch = s;
   } else {
     require(pos0 >= 0 && (s == 0 || pos0 <= t.rows - s), "positions pos0 .. must lie within cos / sin");

@@ -161,6 +161,8 @@ def test_rows_of_zeros_infinities_and_positions_outside():
     q, k = nv.qk_norm_rope(a, x, w, w, cos, sin, pos)
     assert bool((q[1] == 0).all()) and bool(torch.isnan(q[2, 1:3]).any(1).all()) and bool(torch.isfinite(q[2, [0, 3]]).all())
     assert bool(torch.isfinite(q[3]).all()) and bool(torch.isnan(q[4:]).all()) and torch.equal(torch.nan_to_num(q), torch.nan_to_num(k))
+    far, _ = nv.qk_norm_rope(x, x, w, w, cos, sin, torch.tensor([0, 3, 9, 5, -1 - 2 ** 32, 2 ** 32], device="cuda"))
+    assert torch.equal(torch.nan_to_num(far), torch.nan_to_num(q.detach()))
     (grad,) = torch.autograd.grad(q, a, torch.ones_like(q))
     assert bool(torch.isfinite(grad[[0, 1, 3]]).all()) and bool(torch.isfinite(grad[2, [0, 3]]).all()) and bool(torch.isnan(grad[4:]).all())
 
