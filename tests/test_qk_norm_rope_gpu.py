@@ -118,6 +118,44 @@ def test_batches(z, h, hk, s, d, dtype, inside):
             _check_backward(res[i], res[2 + i], x.detach(), w, c, sn, 1e-6, grads[i])
 
 
+@pytest.mark.parametrize("seed", range(40))
+def test_any_heads_lengths_and_strides(seed):
+    """Heads that fill a step and a task or do not, tokens apart, heads apart, gradients laid out otherwise than results."""
+    g = torch.Generator().manual_seed(1000 + seed)
+    pick = lambda *x: x[int(torch.randint(len(x), (1,), generator=g))]
+    d, dtype, four = pick(128, 256), pick(torch.bfloat16, torch.float16, torch.float32), pick(True, False)
+    hk, h = pick(1, 2, 3, 4, 5, 8), pick(1, 2, 3, 6, 7, 12, 17, 20, 33)
+    z, s = (pick(1, 2, 3) if four else 1), pick(1, 2, 3, 15, 16, 17, 31, 64, 129, 300)
+    w = pick(dtype, torch.float32)
+    gap, lead = pick(0, 0, 1, 2), pick(0, 3)                                   # heads between heads, tokens in front
+
+    def laid(x):                                                               # [Z, H, S, D]
+        n = x.shape[1]
+        if pick(True, False):                                                  # tokens outside
+            buf = torch.zeros(z, s + lead, n * (1 + gap), d, dtype=dtype, device="cuda")
+            view = buf[:, lead:, ::1 + gap].transpose(1, 2)
+        else:
+            buf = torch.zeros(z, n * (1 + gap), s + lead, d, dtype=dtype, device="cuda")
+            view = buf[:, ::1 + gap, lead:]
+        view.copy_(x)
+        return view
+
+    q, k, wq, wk = _operands((z, h, s, d), (z, hk, s, d), dtype, w, seed)
+    cos, sin = _tables(400, d, seed=seed)
+    pos = torch.randint(400, (z, s) if four else (s,), generator=g).int()
+    c, sn = _at(cos, pos if four else pos[None], 4), _at(sin, pos if four else pos[None], 4)
+    flat = (lambda x: x) if four else (lambda x: x[0].transpose(0, 1))         # [T, H, D]
+    back = (lambda x: x) if four else (lambda x: x.transpose(0, 1)[None])
+    leaves = [flat(laid(q)).detach().requires_grad_(True), flat(laid(k)).detach().requires_grad_(True),
+              wq.cuda().requires_grad_(True), wk.cuda().requires_grad_(True)]
+    out = _nv().qk_norm_rope(*leaves, cos.cuda(), sin.cuda(), pos.cuda())
+    grads = [torch.randn(x.shape, generator=g).to(dtype) for x in (q, k)]
+    res = torch.autograd.grad(out, leaves, [flat(laid(x)) for x in grads])
+    for i, (x, wt) in enumerate(((q, wq), (k, wk))):
+        _check_forward(back(out[i].detach()), x, wt, c, sn, 1e-6)
+        _check_backward(back(res[i]), res[2 + i], x, wt, c, sn, 1e-6, grads[i])
+
+
 def test_views_of_a_projection_unaligned_and_broadcast_operands():
     nv = _nv()
     g = torch.Generator().manual_seed(1)
