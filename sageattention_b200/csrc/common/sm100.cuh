@@ -314,6 +314,18 @@ __device__ __forceinline__ void prefetch_l2(const void* p) {
   asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
 
+// 16 bytes, or zeros without a load: predicated, so that a lane's loads stay together
+__device__ __forceinline__ uint4 load_or_zero(const void* src, bool there) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}\n"
+      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+      : "l"(src), "r"((int)there)
+      : "memory");
+  return v;
+}
+
 // Per-thread asynchronous 4-byte global -> shared copy; src_bytes = 0 zero-fills.
 __device__ __forceinline__ void cp_async_4(uint32_t saddr, const void* gptr, uint32_t src_bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(saddr), "l"(gptr), "r"(src_bytes)

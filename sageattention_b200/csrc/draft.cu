@@ -120,18 +120,6 @@ __device__ __forceinline__ float mass_of(T v) {
   return f > 0.0f && f < INFINITY ? f : 0.0f;
 }
 
-// 16 bytes, or zeros without a load: predicated, so that a lane's loads stay together
-__device__ __forceinline__ uint4 load_or_zero(const void* src, bool there) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-      "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}\n"
-      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
-      : "l"(src), "r"((int)there)
-      : "memory");
-  return v;
-}
-
 // The walk down a request's tree.  At node x with the target's row p and children c_1, c_2, ... in order, R_0 = p, M_0 = 1:
 //   with draft rows q:  c_j passes where u q(c_j) M < R(c_j); else R <- max(R / M - q, 0), M <- sum R
 //   without:            c_j passes where u M < R(c_j); else M <- M - R(c_j), R(c_j) <- 0
@@ -224,9 +212,8 @@ __global__ void __launch_bounds__(verify_threads(kDrawn), 2) verify_drafts_kerne
   }
   __syncthreads();
 
-  // what is left of a probability behind k rejections
+  // what is left of a probability behind k rejections, one at least
   auto left_of = [&](float x, float q, int k) -> double {
-    if (k == 0) return x;
     double r = x > q ? (double)x - (double)q : 0.0;        // mass 0 is 1
     for (int j = 1; j < k; ++j) {
       r = r * over_s[j] - q;

@@ -103,18 +103,6 @@ __device__ __forceinline__ void fewer_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// 16 bytes, or zeros without a load: predicated, so that the loads of a thread stay together
-__device__ __forceinline__ uint4 load_or_zero(const uint8_t* src, bool there) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-      "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}\n"
-      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
-      : "l"(src), "r"((int)there)
-      : "memory");
-  return v;
-}
-
 // What a tile's softmax has to know: factor of its scores, log2 of what its values were divided by, which 16-key groups are there
 // (a bit each).  Where the scales lie apart `there` is 0, `apart` says which groups are there, and each has exponents of its own.
 struct TileInfo {

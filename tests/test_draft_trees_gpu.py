@@ -462,6 +462,42 @@ def test_layers_inside_blocks():
         assert torch.equal(a.contiguous().view(torch.uint8), b.view(torch.uint8))
 
 
+def test_layers_blocks_and_rows_past_32_bits():
+    """Blocks half a gigabyte apart, layers 2.5: a path moved in both; rows of probabilities two gigabytes apart."""
+    hk, block, d, apart, layer = 2, 16, 128, (1 << 29) + 4096, 5 << 29
+    flat = torch.empty(layer + 5 * apart, dtype=torch.uint8, device="cuda")
+    view = lambda at: flat.as_strided((2, 5, hk, block, d), (layer, apart, block * d, d, 1), at)
+    small = [_empty_cache(2 * 5, hk, block, d, x) for x in (1, 2)]
+    caches, scales = [view(0), view(1 << 20)], [x[1].view(2, 5, hk) for x in small]
+    want = []
+    for c, (codes, scale, _) in zip(caches, small):
+        c.copy_(codes.view(torch.uint8).view(2, 5, hk, block, d))
+        want.append([(_as_values(codes.view(2, 5, hk, block, d)[i]), scale.view(2, 5, hk)[i].cpu().double()) for i in (0, 1)])
+    table = torch.tensor([[4, 0, 3], [2, 1, -1]], dtype=torch.int32)
+    path, new, total = [0, 3, 20, 21, 29], [30, 25], [45, 32]
+    for values in want:
+        for x, y in values:
+            for r in (0, 1):
+                T.keep_path([a for a in path if a < new[r]], new[r], total[r], table[r], x, y, block)
+    keep = _nv().paged_kv_keep_path(_i32(path + [-1] * 25 + path[:4] + [-1] * 21), _i32([5, 4]), _i32([0, 30, 55]), _i32(total), table.cuda(), *caches, *scales)
+    assert keep.tolist() == [20, 11]
+    for c, s, values in zip(caches, scales, want):
+        for i, (x, y) in enumerate(values):
+            assert torch.equal(c[i].contiguous().cpu().view(torch.float8_e4m3fn).double(), x) and torch.equal(s[i].cpu().double(), y)
+    del flat, caches, view
+    v, stride = 700, (1 << 29) + 5
+    wide = torch.empty(5 * stride, device="cuda")
+    p = wide.as_strided((5, v), (stride, 1), 3)
+    p.copy_(_rows(5, v, 1).cuda())
+    parents, u = [-1, 0, 1, 2, 3], torch.tensor([0.7, 1e-6, 1e-6, 1e-6, 1e-6])
+    tokens = p.argmax(1).roll(1).cpu()
+    got = _nv().verify_drafts(p, tokens.cuda(), _i32(parents), _i32([0, 5]), u.cuda())
+    assert got.accepted.tolist() == [0, 1, 2, 3, 4]
+    assert int(got.next_tokens) == T.verify(p.cpu().double().numpy(), tokens.tolist(), parents, u.double().numpy())[1]
+    got = _nv().verify_drafts(p, tokens.cuda(), _i32(parents), _i32([0, 5]), u.cuda(), p)
+    assert got.accepted.tolist() == [0, 1, 2, 3, 4]
+
+
 # ------------------------------------------------------------------------------------------------ together
 def _step(cache, layers, model, parents, tokens, u, cu_lens, most, g, scaling):
     """A step of drafted trees, as a server runs it; `model`: (query, key, value) of every layer, and the target's rows."""

@@ -205,6 +205,28 @@ def test_rows_of_zeros_infinities_and_positions_outside():
     assert bool(torch.isfinite(grad[[0, 1, 3]]).all()) and bool(torch.isfinite(grad[2, [0, 3]]).all()) and bool(torch.isnan(grad[4:]).all())
 
 
+def test_rows_past_32_bits():
+    """Tokens half a gigabyte apart, operands and gradients: the results of the same rows side by side."""
+    nv = _nv()
+    t, h, d, apart = 20, 5, 128, (1 << 28) + 8
+    flat = torch.empty(t * apart, dtype=torch.bfloat16, device="cuda")
+    view = lambda heads, at: flat.as_strided((t, heads, d), (apart, d, 1), at)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    near = [torch.randn(t, n, d, generator=g, device="cuda").bfloat16() for n in (h, 2, h, 2)]
+    far = [view(n, at) for n, at in ((h, 0), (2, 1024), (h, 4096), (2, 8192))]
+    for a, b in zip(far, near):
+        a.copy_(b)
+    assert (t - 1) * apart > 1 << 32
+    w = torch.ones(d, device="cuda")
+    cos, sin = (x.cuda() for x in _tables(t, d))
+    res = []
+    for q, k, gq, gk in (near, far):
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, w, w)]
+        out = nv.qk_norm_rope(*leaves, cos, sin)
+        res.append([*(x.detach() for x in out), *torch.autograd.grad(out, leaves, (gq, gk))])
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
 def test_no_tokens():
     nv = _nv()
     cos, sin = (x.cuda() for x in _tables(10, 128))
