@@ -179,38 +179,66 @@ __global__ void __launch_bounds__(verify_threads(kDrawn), 2) verify_drafts_kerne
     path_s[0] = 0;
   }
   __syncthreads();
-  if (!kDrawn) {                               // a token again among the siblings is worth nothing
-    uint32_t again = 0;                        // of this thread's nodes, a bit each
-    for (int i = tid, bit = 0; i < n; i += kThreads, ++bit)
-      if (up_s[i] >= 0)
-#pragma unroll 4
-        for (int j = up_s[i] + 1; j < i; ++j)
-          if (up_s[j] == up_s[i] && id_s[j] == id_s[i]) again |= 1u << bit;
-    __syncthreads();
-    for (int i = tid, bit = 0; i < n; i += kThreads, ++bit)
-      if (again >> bit & 1) px_s[i] = 0.0f;
-    __syncthreads();
-  }
-  for (int i = tid; i < n; i += kThreads) {
-    const int up = up_s[i];
-    if (up < 0) continue;
-    int before = -1;
-    double mass = 1.0;
-#pragma unroll 4
-    for (int j = up + 1; j < i; ++j)
-      if (up_s[j] == up) {
-        before = j;
-        if (!kDrawn) mass = fmax(mass - (double)px_s[j], 0.0);
+  // Where a node stands among its siblings.  A token again among them is worth nothing.
+  if (n <= 32) {                               // a warp knows it by itself: 26 nodes of 64 requests 18.9 -> 18.0 us
+    if (warp == 0) {
+      const int up = lane < n ? up_s[lane] : -1;
+      const uint32_t in_front = (1u << lane) - 1, siblings = __match_any_sync(0xffffffffu, up >= 0 ? up : kTree + lane);
+      if (kDrawn) {
+        const uint32_t before = siblings & in_front;
+        if (up >= 0) {
+          if (before == 0) first_s[up] = (double)u_s[lane] * (double)qx_s[lane] < (double)px_s[lane] ? lane | kPasses : lane;
+          else next_s[31 - __clz(before)] = (int16_t)lane;
+        }
+      } else {
+        const int id = lane < n ? id_s[lane] : -1;
+        const bool again = (__match_any_sync(0xffffffffu, id) & siblings & in_front) != 0;
+        const float x = up >= 0 && !again ? px_s[lane] : 0.0f;
+        double mass = 1.0;
+        for (uint32_t m = siblings & in_front; __any_sync(0xffffffffu, m != 0); m &= m - 1) {
+          const float other = __shfl_sync(0xffffffffu, x, m != 0 ? __ffs(m) - 1 : lane);
+          if (m != 0) mass = fmax(mass - (double)other, 0.0);
+        }
+        const bool passes = up >= 0 && (double)u_s[lane] * mass < (double)x;
+        const uint32_t all = __ballot_sync(0xffffffffu, passes) & siblings;
+        if (passes && __ffs(all) - 1 == lane) first_s[up] = lane;
       }
-    if (kDrawn) {
-      // the first child of a node that has lost none yet: at once known, and marked where it passes
-      if (before < 0) first_s[up] = (double)u_s[i] * (double)qx_s[i] < (double)px_s[i] ? i | kPasses : i;
-      else next_s[before] = (int16_t)i;
-    } else if ((double)u_s[i] * mass < (double)px_s[i]) {
-      atomicMin(&first_s[up], i);
     }
+    __syncthreads();
+  } else {
+    if (!kDrawn) {
+      uint32_t again = 0;                      // of this thread's nodes, a bit each
+      for (int i = tid, bit = 0; i < n; i += kThreads, ++bit)
+        if (up_s[i] >= 0)
+#pragma unroll 4
+          for (int j = up_s[i] + 1; j < i; ++j)
+            if (up_s[j] == up_s[i] && id_s[j] == id_s[i]) again |= 1u << bit;
+      __syncthreads();
+      for (int i = tid, bit = 0; i < n; i += kThreads, ++bit)
+        if (again >> bit & 1) px_s[i] = 0.0f;
+      __syncthreads();
+    }
+    for (int i = tid; i < n; i += kThreads) {
+      const int up = up_s[i];
+      if (up < 0) continue;
+      int before = -1;
+      double mass = 1.0;
+#pragma unroll 4
+      for (int j = up + 1; j < i; ++j)
+        if (up_s[j] == up) {
+          before = j;
+          if (!kDrawn) mass = fmax(mass - (double)px_s[j], 0.0);
+        }
+      if (kDrawn) {
+        // the first child of a node that has lost none yet: at once known, and marked where it passes
+        if (before < 0) first_s[up] = (double)u_s[i] * (double)qx_s[i] < (double)px_s[i] ? i | kPasses : i;
+        else next_s[before] = (int16_t)i;
+      } else if ((double)u_s[i] * mass < (double)px_s[i]) {
+        atomicMin(&first_s[up], i);
+      }
+    }
+    __syncthreads();
   }
-  __syncthreads();
 
   // what is left of a probability behind k rejections, one at least
   auto left_of = [&](float x, float q, int k) -> double {

@@ -271,6 +271,21 @@ def test_clusters_of_every_size(requests, drawn):
     _check_verify(p, _drafts(p, q, parents, starts, 4, likeliest=not drawn).int(), parents, starts, u, q)
 
 
+@pytest.mark.parametrize("drawn", [True, False])
+def test_trees_of_about_a_warp(drawn):
+    """One warp finds the siblings of up to 32 nodes, each thread those of its own behind that; tokens come again among them."""
+    new = [31, 32, 33, 34, 32, 33, 32]
+    g = torch.Generator().manual_seed(8)
+    starts, total, v = _starts(new), sum(new), 11
+    p, q = _rows(total, v, 3, peak=2.0), _rows(total, v, 4, peak=2.0) if drawn else None
+    for near in (1, 2, 40):                                                    # chains, trees and shallow ones
+        parents = [-1 if i == 0 else int(torch.randint(min(i, near), (1,), generator=g)) + max(0, i - near) * (near < 40)
+                   for n in new for i in range(n)]
+        for seed in range(4):
+            tokens = torch.randint(-1, v, (total,), generator=g) if seed else _drafts(p, q, parents, starts, seed)
+            _check_verify(p, tokens, parents, starts, torch.rand(total, generator=g) * (1.0 if seed < 3 else 0.2), q)
+
+
 def test_long_chains_and_wide_trees():
     """Trees end with their 1024th token; children of one node in the hundreds, all of them rejected."""
     p = _rows(1100, 50, 1)
