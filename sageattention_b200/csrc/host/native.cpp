@@ -20,6 +20,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <array>
 #include <cstdlib>
 #include <cstring>
@@ -961,11 +962,13 @@ HeadRows head_rows(const Tensor& x_in) {
   if (x.dim() == 3) return {x, 1, x.size(0), x.size(1), x.size(2), {0, step(0), step(1)}};
   return {x, x.size(0), x.size(2), x.size(1), x.size(3), {step(0), step(2), step(1)}};
 }
-// Of x's shape, dense, with heads inside or outside of tokens as in x.
+// Of x's shape, dense, with heads inside or outside of tokens as in x.  No view of another tensor: one that is made without
+// gradients cannot be changed in place in a graph.
 Tensor empty_rows(const Call& c, const Tensor& x) {
-  if (x.dim() == 4 && x.stride(1) < x.stride(2))
-    return c.empty({x.size(0), x.size(2), x.size(1), x.size(3)}, x.scalar_type()).transpose(1, 2);
-  return c.empty(x.sizes(), x.scalar_type());
+  if (x.dim() != 4 || x.stride(1) >= x.stride(2)) return c.empty(x.sizes(), x.scalar_type());
+  // as a dense [Z, S, H, D] lies
+  const int64_t z = x.size(0), h = std::max<int64_t>(x.size(1), 1), s = std::max<int64_t>(x.size(2), 1), d = x.size(3);
+  return at::detail::empty_strided_cuda({z, x.size(1), x.size(2), d}, {s * h * d, d, h * d, 1}, x.scalar_type(), c.dev);
 }
 struct NormTables {
   Tensor cos, sin, wq, wk;
