@@ -512,6 +512,12 @@ int nvfp4_verify_drafts(const void* target_probs, int64_t target_row, const void
                         int64_t vocab, const void* tokens, int tokens_int64, const int32_t* parents, const int32_t* cu_seqlens,
                         const float* uniforms, int64_t num_tokens, int64_t requests, int32_t* accepted, int32_t* num_accepted,
                         int64_t* next_tokens, nvfp4_stream_t stream);
+/* The same where a tree's nodes from max_tokens (1 to 1024) on are never kept: with the max_tokens of nvfp4_draft_tree, which leaves such
+ * nodes without their ancestors, a tree larger than it is verified as far as it was attended. */
+int nvfp4_verify_drafts_within(const void* target_probs, int64_t target_row, const void* draft_probs, int64_t draft_row, int dtype,
+                               int64_t vocab, const void* tokens, int tokens_int64, const int32_t* parents, const int32_t* cu_seqlens,
+                               const float* uniforms, int64_t num_tokens, int64_t requests, int64_t max_tokens, int32_t* accepted,
+                               int32_t* num_accepted, int64_t* next_tokens, nvfp4_stream_t stream);
 
 /*
  * The tokens of an accepted path moved together: of a request's n newest tokens, token accepted[cu[r] + j] (ascending in j <

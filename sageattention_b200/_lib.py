@@ -86,6 +86,8 @@ SIGNATURES = {
                                          c_size_t, c_void_p, c_void_p]),
     "nvfp4_verify_drafts": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                     c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nvfp4_verify_drafts_within": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_void_p, c_int, c_void_p, c_void_p,
+                                           c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
     "nvfp4_paged_keep_path": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64]
                               + [c_void_p, c_int64, c_int64] * 4 + [c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p]),
     "nvfp4_qk_norm_rope": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p,

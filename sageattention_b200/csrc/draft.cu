@@ -1,7 +1,7 @@
 // Trees of drafted tokens: what every node sees and where it stands, and which of them the target's probabilities keep.
 //
 // A request's tokens cu[r] .. cu[r + 1] are a tree: its node 0 is the token that the step before ended with, node i hangs on the
-// earlier node that parents[] names.  Nodes behind the 1024th are not part of it.
+// earlier node that parents[] names.  Nodes from max_tokens (1024 at most) on are not part of it: they see none of it, and none is kept.
 #include <limits.h>
 #include "common/abi.cuh"
 #include "common/fp4.cuh"
@@ -96,7 +96,7 @@ struct VerifyParams {
   const int32_t *parents, *cu;
   const float* u;
   int64_t tokens;
-  int requests, vocab;
+  int requests, vocab, most;                   // most: nodes of a tree that may be kept
   int32_t *accepted, *count;
   int64_t* next;
 };
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(verify_threads(kDrawn), 2) verify_drafts_kerne
   griddep_wait();
   griddep_launch();
   const Span span(p.cu, r, p.tokens);
-  const int n = (int)min(span.n, (int64_t)kTree);
+  const int n = (int)min(span.n, (int64_t)p.most);
   const T* const target = static_cast<const T*>(p.p);
   const T* const draft = static_cast<const T*>(p.q);
   for (int i = tid; i < n; i += kThreads) {
@@ -546,16 +546,18 @@ extern "C" int nvfp4_draft_tree(const int32_t* parents, const int32_t* cu_seqlen
   return launch("nvfp4_draft_tree", draft_tree_kernel, dim3((unsigned)requests), kTreeThreads, 0, static_cast<cudaStream_t>(stream), p);
 }
 
-extern "C" int nvfp4_verify_drafts(const void* target_probs, int64_t target_row, const void* draft_probs, int64_t draft_row, int dtype,
-                                   int64_t vocab, const void* tokens, int tokens_int64, const int32_t* parents, const int32_t* cu_seqlens,
-                                   const float* uniforms, int64_t num_tokens, int64_t requests, int32_t* accepted, int32_t* num_accepted,
-                                   int64_t* next_tokens, nvfp4_stream_t stream) {
+extern "C" int nvfp4_verify_drafts_within(const void* target_probs, int64_t target_row, const void* draft_probs, int64_t draft_row,
+                                          int dtype, int64_t vocab, const void* tokens, int tokens_int64, const int32_t* parents,
+                                          const int32_t* cu_seqlens, const float* uniforms, int64_t num_tokens, int64_t requests,
+                                          int64_t max_tokens, int32_t* accepted, int32_t* num_accepted, int64_t* next_tokens,
+                                          nvfp4_stream_t stream) {
+  NVFP4_REQUIRE(max_tokens >= 1 && max_tokens <= kTree, "nvfp4_verify_drafts: max_tokens must be 1 to 1024");
   NVFP4_REQUIRE(vocab >= 1 && vocab < (1 << 30), "nvfp4_verify_drafts: vocabulary out of range");
   NVFP4_REQUIRE(requests >= 1 && requests < (1 << 30) && num_tokens >= 0 && num_tokens < (1ll << 31), "nvfp4_verify_drafts: sizes out of range");
   const int64_t size = dtype == NVFP4_DT_FP32 ? 4 : 2;
   NVFP4_REQUIRE((((uintptr_t)target_probs | (uintptr_t)draft_probs) & (uintptr_t)(size - 1)) == 0, "nvfp4_verify_drafts: unaligned rows");
   const VerifyParams p{target_probs, draft_probs, target_row, draft_row, tokens, tokens_int64, parents, cu_seqlens, uniforms, num_tokens,
-                       (int)requests, (int)vocab, accepted, num_accepted, next_tokens};
+                       (int)requests, (int)vocab, (int)max_tokens, accepted, num_accepted, next_tokens};
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   int ranks = 8;                               // as many blocks as are resident at once
@@ -567,4 +569,12 @@ extern "C" int nvfp4_verify_drafts(const void* target_probs, int64_t target_row,
     case NVFP4_DT_FP32: return run_verify<float>(p, ranks, st);
   }
   return fail(-1, "nvfp4_verify_drafts: unknown dtype %d", dtype);
+}
+
+extern "C" int nvfp4_verify_drafts(const void* target_probs, int64_t target_row, const void* draft_probs, int64_t draft_row, int dtype,
+                                   int64_t vocab, const void* tokens, int tokens_int64, const int32_t* parents, const int32_t* cu_seqlens,
+                                   const float* uniforms, int64_t num_tokens, int64_t requests, int32_t* accepted, int32_t* num_accepted,
+                                   int64_t* next_tokens, nvfp4_stream_t stream) {
+  return nvfp4_verify_drafts_within(target_probs, target_row, draft_probs, draft_row, dtype, vocab, tokens, tokens_int64, parents, cu_seqlens,
+                                    uniforms, num_tokens, requests, kTree, accepted, num_accepted, next_tokens, stream);
 }

@@ -876,12 +876,13 @@ std::tuple<Tensor, Tensor> draft_tree(const Tensor& parents, const Tensor& cu, c
 }
 
 std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor& target_in, const Tensor& tokens, const Tensor& parents, const Tensor& cu,
-                                                 const Tensor& uniforms, const OptTensor& draft_in) {
+                                                 const Tensor& uniforms, const OptTensor& draft_in, int64_t max_tokens) {
   require_cuda(target_in, "target_probs");
   Call c(target_in);
   require_dims(target_in, 2, "target_probs must be [T, vocabulary]");
   const int64_t t = target_in.size(0), v = target_in.size(1), r = requests_of(c, cu);
   require(v >= 1, "target_probs must have a column");
+  require(max_tokens >= 1 && max_tokens <= 1024, "max_tokens must be 1 to 1024");
   const int dt = dtype_code(target_in.scalar_type());
   auto rows = [](const Tensor& x) { return x.stride(1) == 1 || x.size(1) == 1 ? x : x.contiguous(); };
   const Tensor target = rows(target_in);
@@ -897,10 +898,10 @@ std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor& target_in, const 
   require_words(c, parents, t, at::kInt, "parents must be contiguous int32 [T]");
   require_words(c, uniforms, t, at::kFloat, "uniforms must be contiguous float32 [T]");
   Tensor accepted = c.empty({t}, at::kInt), count = c.empty({r}, at::kInt), next = c.empty({r}, at::kLong);
-  c.done(nvfp4_verify_drafts(target.data_ptr(), target.stride(0), draft.defined() ? draft.data_ptr() : nullptr,
-                             draft.defined() ? draft.stride(0) : 0, dt, v, tokens.data_ptr(), tokens.scalar_type() == at::kLong,
-                             parents.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), uniforms.data_ptr<float>(), t, r,
-                             accepted.data_ptr<int32_t>(), count.data_ptr<int32_t>(), next.data_ptr<int64_t>(), c.stream),
+  c.done(nvfp4_verify_drafts_within(target.data_ptr(), target.stride(0), draft.defined() ? draft.data_ptr() : nullptr,
+                                    draft.defined() ? draft.stride(0) : 0, dt, v, tokens.data_ptr(), tokens.scalar_type() == at::kLong,
+                                    parents.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), uniforms.data_ptr<float>(), t, r, max_tokens,
+                                    accepted.data_ptr<int32_t>(), count.data_ptr<int32_t>(), next.data_ptr<int64_t>(), c.stream),
          "nvfp4_verify_drafts");
   return {accepted, count, next};
 }

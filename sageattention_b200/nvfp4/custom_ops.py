@@ -23,7 +23,8 @@ second compute path.
     mask, positions = torch.ops.sageattention_b200.draft_tree(parents, cu, lengths, max_tokens)
     out, lse = torch.ops.sageattention_b200.fp8_paged_tree_attention(q, cu, mask, k_cache, v_cache, k_scale, v_scale, table,
                                                                      lengths, scaling, groups)
-    accepted, num, following = torch.ops.sageattention_b200.verify_drafts(target_probs, tokens, parents, cu, uniforms, draft_probs)
+    accepted, num, following = torch.ops.sageattention_b200.verify_drafts(target_probs, tokens, parents, cu, uniforms, draft_probs,
+                                                                                 max_tokens)
     keep = torch.ops.sageattention_b200.paged_kv_keep_path(accepted, num, cu, lengths, table, k_cache, v_cache, k_scale, v_scale)
     q, k = torch.ops.sageattention_b200.qk_norm_rope(q, k, wq, wk, cos, sin, positions, pos0, eps)       # differentiable
 """
@@ -315,13 +316,13 @@ def _(q, cu_seqlens, tree_mask, k_cache, v_cache, k_scale, v_scale, block_table,
 
 @torch.library.custom_op(f"{_NS}::verify_drafts", mutates_args=())
 def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, cu_seqlens: torch.Tensor,
-                  uniforms: torch.Tensor, draft_probs: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                  uniforms: torch.Tensor, draft_probs: Optional[torch.Tensor], max_tokens: int = 1024) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``verify_drafts``: (accepted, num_accepted, next_tokens)."""
-    return tuple(_paged.verify_drafts(target_probs, tokens, parents, cu_seqlens, uniforms, draft_probs))
+    return tuple(_paged.verify_drafts(target_probs, tokens, parents, cu_seqlens, uniforms, draft_probs, max_tokens))
 
 
 @verify_drafts.register_fake
-def _(target_probs, tokens, parents, cu_seqlens, uniforms, draft_probs):
+def _(target_probs, tokens, parents, cu_seqlens, uniforms, draft_probs, max_tokens=1024):
     r = cu_seqlens.shape[0] - 1
     return (tokens.new_empty(tokens.shape[0], dtype=torch.int32), tokens.new_empty(r, dtype=torch.int32),
             tokens.new_empty(r, dtype=torch.int64))

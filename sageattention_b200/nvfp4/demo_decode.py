@@ -206,7 +206,7 @@ def tree_step(model, cache, tokens, parents, lens, most, uniforms, temperature=0
         x = model.finish(blk, x, attn.transpose(0, 1)[None])
     logits = model.logits(x.transpose(0, 1))
     probs = torch.softmax(logits / temperature, -1) if temperature > 0 else F.one_hot(logits.argmax(-1), logits.shape[-1]).float()
-    got = verify_drafts(probs, tokens, parents, step.cu_seqlens, uniforms)
+    got = verify_drafts(probs, tokens, parents, step.cu_seqlens, uniforms, max_tokens=most)
     cache.keep_path(got.accepted, got.num_accepted, step.cu_seqlens)
     return got
 

@@ -121,8 +121,8 @@ def draft_tree(parents, cu_seqlens, lengths, max_tokens: int) -> DraftTree:
 
     Request r's tokens are ``cu_seqlens[r] .. cu_seqlens[r + 1]``, the last ones of its ``lengths[r]`` (reserved before the call); token i
     hangs on the request's earlier token ``parents[t]`` (int32, counted within the request), and on the context alone where that names
-    none (-1).  ``max_tokens`` (1 to 1024): tokens of the largest tree; what lies behind them sees the context alone.  Tokens of no
-    request have no bits and position 0.
+    none (-1).  ``max_tokens`` (1 to 1024): tokens of the largest tree; what lies behind them sees the context alone, and
+    ``verify_drafts`` with the same ``max_tokens`` never keeps it.  Tokens of no request have no bits and position 0.
     """
     return DraftTree(*_lib.native().draft_tree(parents, cu_seqlens, lengths, max_tokens))
 
@@ -141,13 +141,14 @@ def fp8_paged_tree_attention(query, cu_seqlens, tree_mask, k_cache, v_cache, k_s
     return (out, lse) if return_lse else out
 
 
-def verify_drafts(target_probs, tokens, parents, cu_seqlens, uniforms, draft_probs=None) -> VerifiedDrafts:
+def verify_drafts(target_probs, tokens, parents, cu_seqlens, uniforms, draft_probs=None, max_tokens: int = 1024) -> VerifiedDrafts:
     """Which drafted tokens to keep, so that what is kept and the token behind it are distributed as the target's own draws.
 
     ``target_probs`` ``[T, vocabulary]`` (bf16 / fp16 / fp32): row t is the target's distribution behind token t.  A request's first
     token is given (the one that the step before ended with), the others are drafts: ``tokens`` ``[T]`` ids (int64 or int32),
-    ``parents`` as for ``draft_tree`` (a draft that hangs on the context alone is never kept; trees have 1024 tokens at most, what
-    lies behind them is never kept).  ``uniforms`` ``[T]`` float32 in [0, 1): of a draft the number that tests it, of a request's first token
+    ``parents`` as for ``draft_tree`` (a draft that hangs on the context alone is never kept).  ``max_tokens`` (1 to 1024): what lies
+    behind them in a tree is never kept; where trees may be larger than what ``draft_tree`` was told (a captured step, whose
+    ``max_tokens`` stays as it was), the same number, as drafts behind it were attended without their ancestors.  ``uniforms`` ``[T]`` float32 in [0, 1): of a draft the number that tests it, of a request's first token
     the one that draws the next.
 
     At a token with row p, its children in order, R = p and M = 1.  With ``draft_probs`` (``[T, vocabulary]``, row t: what the children of
@@ -156,7 +157,7 @@ def verify_drafts(target_probs, tokens, parents, cu_seqlens, uniforms, draft_pro
     The walk goes on at the first child kept; where none is, the next token is the first v whose running sum of R exceeds w sum(R)
     (of p, where R is empty).  Sums are in 64 bits.  Entries that are no finite number above zero count as 0, as do ids outside the vocabulary.
     """
-    return VerifiedDrafts(*_lib.native().verify_drafts(target_probs, tokens, parents, cu_seqlens, uniforms, draft_probs))
+    return VerifiedDrafts(*_lib.native().verify_drafts(target_probs, tokens, parents, cu_seqlens, uniforms, draft_probs, max_tokens))
 
 
 def paged_kv_keep_path(accepted, num_accepted, cu_seqlens, lengths, block_table, k_cache, v_cache, k_scale, v_scale) -> torch.Tensor:
