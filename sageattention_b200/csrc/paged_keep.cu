@@ -11,6 +11,7 @@
 // table, codes with their scales); a call moves a few tokens of a request.  Paths of 64 requests in 16 layers of Hk 8 D 128, blocks of
 // 16: 9.5 us, one more with the scales in a trip of their own; units of a request on the blocks that are resident at once, several a
 // warp, 15 to 18.
+#include <float.h>
 #include <limits.h>
 #include "common/abi.cuh"
 #include "common/fp4.cuh"
@@ -35,16 +36,27 @@ struct KeepParams {
   int32_t* keep;
 };
 
+// x s / now, of which `about` is an approximation to 2^-22, as a float that is rounded to the code that the quotient itself would be:
+// on the right side of the border between codes that it lies at.  Borders have five significant bits at most, so both sides of the
+// comparison are exact in 64 bits.
+__device__ __forceinline__ float beside(float about, float x, float s, float now) {
+  const uint32_t u = __float_as_uint(about) & 0x7FFFFFFFu, border = (u + 0x40000u) & 0x7FF80000u;
+  const double d = fabs((double)x * (double)s) - (double)__uint_as_float(border) * fabs((double)now);
+  const uint32_t v = d > 0.0 ? max(u, border + 1) : d < 0.0 ? min(u, border - 1) : d == 0.0 ? border : u;
+  return copysignf(__uint_as_float(v), about);
+}
 // Codes of scale s as codes of scale `now`, each the one rounding of its value.  Between powers of two a code times their quotient
-// is exact; other scales are divided by (a call of its own, which hardly any makes: in place it costs 40 registers).
+// is exact; other scales take a call of their own, which hardly any makes: in place it costs 40 registers.
 __device__ __noinline__ uint4 codes_divided(uint4 v, float s, float now) {
+  float f = __fdiv_rn(s, now);
+  if (f > FLT_MAX) f = FLT_MAX;                            // 0 stays 0
   uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     uint32_t lo, hi;
     half4_of_e4m3x4(w[k], lo, hi);
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    w[k] = e4m3x4(__fdiv_rn(a.x * s, now), __fdiv_rn(a.y * s, now), __fdiv_rn(b.x * s, now), __fdiv_rn(b.y * s, now));
+    w[k] = e4m3x4(beside(a.x * f, a.x, s, now), beside(a.y * f, a.y, s, now), beside(b.x * f, b.x, s, now), beside(b.y * f, b.y, s, now));
   }
   return v;
 }
