@@ -523,7 +523,8 @@ int nvfp4_verify_drafts_within(const void* target_probs, int64_t target_row, con
  * The tokens of an accepted path moved together: of a request's n newest tokens, token accepted[cu[r] + j] (ascending in j <
  * num_accepted[r]; the path ends in front of an entry that is not) goes to position lengths[r] - n + j, keys and values of all layers
  * and heads.  A block that receives codes of larger scales takes the smallest power of two that holds them, and its older codes are
- * rounded again to it.  keep_lens [requests]: what nvfp4_paged_trim is to keep.  Caches [layers, blocks, Hk, block_size, D] in bytes,
+ * rounded again to it, each once from the value it stood for; codes behind the path stay, under the scale that their block has then,
+ * and are no tokens any more.  keep_lens [requests]: what nvfp4_paged_trim is to keep.  Caches [layers, blocks, Hk, block_size, D] in bytes,
  * scales [layers, blocks, Hk], strides of layer and block in elements.
  */
 int nvfp4_paged_keep_path(const int32_t* accepted, const int32_t* num_accepted, const int32_t* cu_seqlens, int64_t tokens,

@@ -7,7 +7,10 @@
 // unit's tiles the list has unit_cost() entries without work, for what a unit costs besides (its query, its merge).  With one, two,
 // three and four of them: decode of 160 requests of 1 to 4100 keys 23.1, 22.7, 24.2, 24.3 us; drafts of 32 requests 79.5, 70.0,
 // 67.7, 69.4; chunks and single tokens in one batch at D 256 87.6, 82.7, 79.0, 79.4.  Trees of many rows, whose units go through all
-// keys: 32 of 16 to 64 nodes, none to four of them 122.5, 104.7, 96.6, 100.8, 104.8.  A CTA can hold
+// keys: 32 of 16 to 64 nodes, none to four of them 122.5, 104.7, 96.6, 100.8, 104.8.  Two against three of them in twelve other batches:
+// 0.4 to 3.3 % faster in nine (D 128: 24 trees of 10 to 30 nodes 104.2, 106.8; 16 of 60 to 100 60.3, 62.3; 64 of 40 170.0, 171.3; D 256: 32 of 8 to 64
+// 73.6, 74.7; 16 of 60 70.4, 70.9), slower where a few large trees are all there is (8 of 64 to 200, D 128 205.1, 204.3; 8 of 60 to 130, D 256 70.1, 68.1).
+// A CTA can hold
 // the end of one unit and the beginning of another, each a partial result of its own (slots 2 c and 2 c + 1).
 #pragma once
 #include <cuda_runtime.h>

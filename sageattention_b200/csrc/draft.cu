@@ -102,7 +102,8 @@ struct VerifyParams {
 };
 
 // Threads of a block, two of which share an SM: with draft rows 128 registers a thread, in 64 of which (512 threads) they do not
-// fit; without them more warps.  Chains of 32000 tokens 8.5 (13.4) us, the likeliest of 131072 tokens 18.6 (21.2).
+// fit; without them more warps.  Chains of 32000 tokens 8.5 (13.4) us, the likeliest of 131072 tokens 18.6 (21.2).  Chosen drafts of 16-bit
+// rows, eight elements a load, spill 84 bytes in 64 registers: 131072 tokens in bf16 17.4 us where fp32 takes 18.0.
 __host__ __device__ constexpr int verify_threads(bool drawn) { return drawn ? 256 : 512; }
 
 __device__ __forceinline__ double ld_cluster_f64(uint32_t saddr, uint32_t rank) {
@@ -180,7 +181,10 @@ __global__ void __launch_bounds__(verify_threads(kDrawn), 2) verify_drafts_kerne
   }
   __syncthreads();
   // Where a node stands among its siblings.  A token again among them is worth nothing.
-  if (n <= 32) {                               // a warp knows it by itself: 26 nodes of 64 requests 18.9 -> 18.0 us
+  // Of up to 32 nodes a warp knows it by itself.  Chosen, instead of the search below: 64 requests of 26 nodes over 131072 tokens 18.0 us (18.9), over
+  // 32000 10.0 (11.2), 256 of 32 16.4 (17.8), one of 16 9.2 (10.0), a chain of eight 7.0 (7.1); drawn, whose search does less, it is as
+  // fast: 64 of 20 30.6 (30.8), 16 of 32 23.5 (23.7), chains of six 10.5 (10.4).
+  if (n <= 32) {
     if (warp == 0) {
       const int up = lane < n ? up_s[lane] : -1;
       const uint32_t in_front = (1u << lane) - 1, siblings = __match_any_sync(0xffffffffu, up >= 0 ? up : kTree + lane);

@@ -4,7 +4,8 @@
 // Once a_j is not j it is above j from there on, so what moves is the path's tail, to places in front of where it lies, and a
 // block that receives tokens receives all behind its first one.  Within blocks of equal scales codes are copied; else a code is
 // the one rounding of the value it stood for to the receiving block's scale, which becomes the smallest power of two that holds
-// what came from blocks of larger scales where that is more than it was, and older codes are rounded again to it.
+// what came from blocks of larger scales where that is more than it was, and older codes are rounded again to it.  Codes behind the
+// path stay, and are no tokens any more: their block's scale may have grown.
 //
 // A warp has a head's keys or values of a layer (a unit) after the other, a block of threads those of one request, which share
 // what the tables say of the tokens that move to a block.  What bounds it: trips to memory one behind the other (count, path,
@@ -23,7 +24,9 @@ namespace {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kMaxBlock = 128;
-constexpr int kResident = 5;                   // blocks of an SM: four loads ahead, at 80 registers and three blocks, took 11.6 us instead of 9.5
+// Blocks of an SM, with 48 registers a thread, out of which 96 bytes are spilled: four loads ahead, at 80
+// registers and three blocks, took 11.6 us instead of 9.5.
+constexpr int kResident = 5;
 
 struct KeepParams {
   const int32_t *accepted, *count, *cu, *lengths, *table;

@@ -6,12 +6,14 @@
 // What bounds it: HBM; a row is read once and written once (backward: two reads, a write).  A row is D/16 lanes, each with eight
 // elements of either half, so that a rotation stays within a lane and every access is 16 bytes wide; a warp has rows of several
 // heads of a token (a step), STEPS steps together, for which it loads cos and sin once.  Statistics, rotation and weight
-// gradients are fp32, two an instruction, rounded once to the type of the operand.
+// gradients are fp32, two an instruction, rounded once to the type of the operand.  Squares are fp32 too: a row whose mean square is
+// beyond it (values of 2^60) becomes 0, one whose squares vanish in it (below 2^-74) has eps alone.
 //
 // Forward: tasks of queries and keys by turns, so that what is in flight lies together, on the blocks that are resident at once: 16001
 // tokens of H 32 Hk 8 D 128 in bf16 (views of a projection, 328 MB) 61.6 us, a copy of as many bytes 51.  On the same buffers
 // again and again (16384 tokens) 57.2; all queries first 61.8; more blocks than resident 58 to 64; four steps a task 63, as there
-// are fewer warps.  More under way does not help (rows asked into L2 a task ahead 63.6 instead of 61.6, two ahead 64.2), nor do
+// are fewer warps.  fp32 rows are twice as many registers, so a task is one step (8000 tokens 61.9 us, with two steps and 216 bytes of spills
+// 76.8; 4000 of H 16 Hk 4 D 256 41.6, 46.8; 32 tokens 2.5, 3.4).  More under way does not help (rows asked into L2 a task ahead 63.6 instead of 61.6, two ahead 64.2), nor do
 // loads past L1 (63.3) or stores that L2 gives up first (62.4).
 // Backward: registers hold too few rows for the loads to stay under way (104 us with four steps, 110 with two), so a warp's rows
 // come by bulk copies, the next task's while this one's are used, and a block is of queries or of keys, whose sums it keeps: 16384

@@ -112,9 +112,10 @@ def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, q_weight: torch.Tensor,
     ``query`` ``[T, H, D]`` and ``key`` ``[T, Hk, D]`` with ``positions`` ``[T]`` (as ``paged_kv_reserve`` and ``draft_tree`` list
     them), or ``[Z, H, S, D]`` and ``[Z, Hk, S, D]`` with ``[S]`` or ``[Z, S]``; without, token s is at ``pos0 + s``.  Views of a
     fused projection are taken as they are.  D is 128 or 256; weights ``[D]`` in the operands' dtype or fp32; ``cos`` / ``sin``
-    ``[P, D/2]`` fp32, half-split convention, as for ``rope_quant_nvfp4``.  A position outside the tables makes its rows NaN.  Returns
-    (query, key), heads inside or outside of the tokens as in the operands.  Gradients of weights are summed in an order that
-    depends on sizes and device alone.
+    ``[P, D/2]`` fp32, half-split convention, as for ``rope_quant_nvfp4``.  A position outside the tables makes its rows NaN, and the
+    gradients of the weights with them.  Returns (query, key), heads inside or outside of the tokens as in the operands, tensors of
+    their own that may be changed in place.  Squares are summed in fp32: values of 2^60 and more are outside of what it norms.  Gradients of
+    weights are summed in an order that depends on sizes and device alone.
     """
     return _lib.native().qk_norm_rope(query, key, q_weight, k_weight, cos, sin, positions, pos0, eps)
 

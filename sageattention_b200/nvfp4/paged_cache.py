@@ -167,7 +167,8 @@ def paged_kv_keep_path(accepted, num_accepted, cu_seqlens, lengths, block_table,
     ``lengths[r] - n + j``, for j below ``num_accepted[r]`` (a path ends in front of an entry that does not ascend).  Caches of one
     layer, ``[blocks, Hk, block_size, D]``, or of all, ``[layers, blocks, Hk, block_size, D]``, scales likewise.  Where a block receives
     codes of a larger scale that its own cannot hold, its scale becomes the smallest power of two that can, and its older codes are
-    rounded again to it.  Returns ``keep_lens`` [requests] int32 for ``paged_kv_trim``; the tokens behind them are left as they were.
+    rounded again to it.  Returns ``keep_lens`` [requests] int32 for ``paged_kv_trim``.  The codes behind those tokens are left as they were,
+    but the scale of the path's last block may have grown over them: what lies there is no token any more, with or without the trim.
     """
     return _lib.native().paged_keep_path(accepted, num_accepted, cu_seqlens, lengths, block_table, k_cache, v_cache, k_scale, v_scale)
 
